@@ -41,6 +41,8 @@ KERNEL_QUANT_GEMV = 33
 KERNEL_MOE_DECODE = 34
 KERNEL_FP8_BLOCK_GEMM = 35
 KERNEL_DENSE_FFN_DECODE = 36
+KERNEL_KV_CACHE = 37
+KERNEL_KV_ATTENTION = 38
 
 LINEAR_FP8_E4M3_E8M0 = 4
 LINEAR_FP8_E4M3_E8M0_PACKED = 5
@@ -250,6 +252,30 @@ class SharedFfnArgs(C.Structure):
                 ("swiglu_limit", f32), ("flags", u32), ("stream", u64)]
 
 
+class KvCacheArgs(C.Structure):
+    """FerruleHipKvCacheArgs (160 bytes); no reference counterpart."""
+    _fields_ = [("batch", u32), ("rows", u32), ("kv_heads", u32), ("head_dim", u32), ("page_tokens", u32),
+                ("page_count", u32), ("max_pages", u32), ("max_query_length", u32), ("value_type", u32),
+                ("reserved", u32), ("key_row_stride", u64), ("key_head_stride", u64), ("value_row_stride", u64),
+                ("value_head_stride", u64), ("keys", u64), ("values", u64), ("k_payload", u64), ("k_scales", u64),
+                ("v_payload", u64), ("v_scales", u64), ("query_indptr", u64), ("sequence_lengths", u64),
+                ("page_table", u64), ("error", u64), ("stream", u64)]
+
+
+class KvAttentionArgs(C.Structure):
+    """FerruleHipKvAttentionArgs (192 bytes); no reference counterpart."""
+    _fields_ = [("batch", u32), ("rows", u32), ("q_heads", u32), ("kv_heads", u32), ("head_dim", u32),
+                ("page_tokens", u32), ("page_count", u32), ("max_pages", u32), ("max_query_length", u32),
+                ("max_sequence_length", u32), ("window", u32), ("sinks", u32), ("flags", u32), ("softmax_scale", f32),
+                ("q_row_stride", u64), ("q_head_stride", u64), ("output_row_stride", u64), ("output_head_stride", u64),
+                ("q", u64), ("output", u64), ("k_payload", u64), ("k_scales", u64), ("v_payload", u64),
+                ("v_scales", u64), ("query_indptr", u64), ("sequence_lengths", u64), ("page_table", u64),
+                ("error", u64), ("workspace", u64), ("workspace_bytes", u64), ("stream", u64)]
+
+
+KV_F32, KV_BF16 = 0, 1
+KV_ATTENTION_QUERY_F32, KV_ATTENTION_OUTPUT_F32 = 1, 2
+KV_HEAD_DIMS = (64, 128, 256, 512)
 SHARED_FFN_ACCUMULATE = 1
 SHARED_FFN_TILE_SCHEDULE = 2
 GEMM_OUTPUT_BF16 = 1
@@ -298,6 +324,13 @@ PROTOTYPES = {
     "ferrule_hip_prepare_mxfp4_sfb": (C.c_int32, [C.POINTER(PrepareMxfp4SfbArgs)]),
     "ferrule_hip_prepare_mxfp4_block_major": (C.c_int32, [C.POINTER(PrepareMxfp4BlockMajorArgs)]),
     "ferrule_hip_prepare_fp8_block_major": (C.c_int32, [C.POINTER(PrepareFp8BlockMajorArgs)]),
+    "ferrule_hip_kv_cache_append_can_implement": (C.c_int32, [C.POINTER(KvCacheArgs)]),
+    "ferrule_hip_kv_cache_append_launch": (C.c_int32, [C.POINTER(KvCacheArgs)]),
+    "ferrule_hip_kv_cache_read_can_implement": (C.c_int32, [C.POINTER(KvCacheArgs)]),
+    "ferrule_hip_kv_cache_read_launch": (C.c_int32, [C.POINTER(KvCacheArgs)]),
+    "ferrule_hip_kv_attention_workspace_size": (C.c_uint64, [C.POINTER(KvAttentionArgs)]),
+    "ferrule_hip_kv_attention_can_implement": (C.c_int32, [C.POINTER(KvAttentionArgs)]),
+    "ferrule_hip_kv_attention_launch": (C.c_int32, [C.POINTER(KvAttentionArgs)]),
 }
 
 _lib = None

@@ -1,0 +1,315 @@
+// Writing the MXFP4 key/value cache and reading it back (no reference symbol; formats, layout and
+// batch description: include/ferrule_hip_provider.h).
+//
+// A wave owns one head of eight neighbouring tokens, the unit of the value layout: lane = (token
+// lane / 8, piece lane % 8), a piece being 16 values, so a scale block is two adjacent lanes and
+// its maximum one exchange.  Both kernels move a row's bytes once and are bound by memory for
+// whole prompts, by launch and latency for a decode step's rows.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "../../include/ferrule_hip_provider.h"
+#include "kv_cache.cuh"
+
+namespace ferrule_hip {
+namespace {
+
+constexpr uint32_t kWaves = 4;
+
+// Where a wave works: eight tokens of one head.
+struct KvTile {
+  KvSequence sequence;
+  uint32_t head;
+  uint32_t page_token;  // of the tile's first token
+  uint64_t page_head;   // page * kv_heads + head
+  bool page_valid;      // false: no token of the tile has a place
+  int32_t first;        // position of the tile's first token, a multiple of 8
+};
+
+__device__ __forceinline__ bool kv_tile(const FerruleHipKvCacheArgs &a, KvTile &tile) {
+  const uint32_t b = blockIdx.y;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(blockIdx.x * kWaves + (threadIdx.x >> 6));
+  tile.head = wave % a.kv_heads;
+  const uint32_t group = wave / a.kv_heads;
+  tile.sequence = kv_sequence(a.query_indptr, a.sequence_lengths, b, a.rows, a.max_query_length);
+  if (tile.sequence.bad && wave == 0u && (threadIdx.x & 63u) == 0u) kv_report(a.error);
+  // groups of eight are counted from the one that holds the first row; position may be negative
+  const int32_t base = tile.sequence.position & ~7;
+  tile.first = base + static_cast<int32_t>(group * 8u);
+  if (tile.first >= tile.sequence.position + static_cast<int32_t>(tile.sequence.rows)) return false;
+  tile.page_valid = false;
+  tile.page_head = 0;
+  tile.page_token = 0;
+  const uint32_t slot = static_cast<uint32_t>(tile.first) / a.page_tokens;
+  if (tile.first >= 0 && slot < a.max_pages) {
+    const int32_t page = global_ptr<const int32_t>(a.page_table)[static_cast<uint64_t>(b) * a.max_pages + slot];
+    tile.page_token = static_cast<uint32_t>(tile.first) % a.page_tokens;
+    tile.page_valid = static_cast<uint32_t>(page) < a.page_count;
+    if (tile.page_valid) tile.page_head = static_cast<uint64_t>(page) * a.kv_heads + tile.head;
+  }
+  if (!tile.page_valid && (threadIdx.x & 63u) == 0u) kv_report(a.error);
+  return true;
+}
+
+// Sixteen consecutive values of a row as f32.
+template <typename T>
+__device__ __forceinline__ void load16(const T *src, float (&x)[16]) {
+  if constexpr (sizeof(T) == 2) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const i32x4_t w = reinterpret_cast<const i32x4_t *>(src)[i];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        x[8 * i + 2 * e] = __uint_as_float(static_cast<uint32_t>(w[e]) << 16);
+        x[8 * i + 2 * e + 1] = __uint_as_float(static_cast<uint32_t>(w[e]) & 0xffff0000u);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const f32x4_t w = reinterpret_cast<const f32x4_t *>(src)[i];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[4 * i + e] = w[e];
+    }
+  }
+}
+
+// Half a scale block (16 values; the other half is in lane ^ 1) -> its eight payload bytes and the
+// block's scale byte.  All in bits: with amax = 1.f * 2^e the smallest n with 6 * 2^n >= amax is
+// e - 2 while 1.f <= 1.5, else e - 1; and |x| / 2^n rounds to the one-mantissa-bit grid by adding
+// just under half a step, which sends a tie down.
+__device__ __forceinline__ uint32_t quantise16(const float (&x)[16], uint32_t (&packed)[2]) {
+  uint32_t top = 0u;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
+  top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 1, 64)));
+  packed[0] = packed[1] = 0u;
+  if (top >= 0x7f800000u) return kNanBlock;
+  const int32_t exponent = static_cast<int32_t>(top >> 23) - 127;
+  int32_t n = exponent - 2 + ((top & 0x7fffffu) > 0x400000u ? 1 : 0);
+  n = max(n, -126);
+  const float inverse = __uint_as_float(static_cast<uint32_t>(127 - n) << 23);  // n <= 126: normal
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const float q = x[i] * inverse;  // exact, |q| <= 6, or below every threshold
+    const uint32_t bits = __float_as_uint(q) & 0x7fffffffu;
+    const float m = __uint_as_float(bits);
+    const uint32_t large = ((bits + 0x1fffffu) >> 22) - 252u;            // m >= 1: 2..7
+    const uint32_t small = (m > 0.25f ? 1u : 0u) + (m > 0.75f ? 1u : 0u);  // m < 1: 0..2
+    const uint32_t code = (m >= 1.0f ? large : small) | ((__float_as_uint(q) >> 28) & 8u);
+    packed[i >> 3] |= code << (4 * (i & 7));
+  }
+  return static_cast<uint32_t>(n + 127);
+}
+
+template <typename T, uint32_t D>
+__global__ __launch_bounds__(256) void kv_append_kernel(FerruleHipKvCacheArgs a) {
+  using Layout = KvLayout<D>;
+  // the value bytes of 128 values of eight tokens, turned in LDS: [value pair][token]
+  __shared__ __align__(16) uint8_t turned[kWaves][64][8];
+  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+  KvTile tile;
+  if (!kv_tile(a, tile) || !tile.page_valid) return;
+  const uint32_t t = lane >> 3, piece = lane & 7u;
+  const int32_t index = tile.first + static_cast<int32_t>(t) - tile.sequence.position;  // row of the sequence
+  const bool live = index >= 0 && index < static_cast<int32_t>(tile.sequence.rows);
+  const bool whole = __ballot(live) == ~0ull;
+  const uint64_t row = tile.sequence.row + static_cast<uint64_t>(live ? index : 0);
+  const T *keys = global_ptr<const T>(a.keys) + row * a.key_row_stride + tile.head * a.key_head_stride;
+  const T *values = global_ptr<const T>(a.values) + row * a.value_row_stride + tile.head * a.value_head_stride;
+  uint8_t *k_payload = global_ptr<uint8_t>(a.k_payload) + Layout::payload(tile.page_head, a.page_tokens);
+  uint8_t *k_scales = global_ptr<uint8_t>(a.k_scales) + Layout::scales(tile.page_head, a.page_tokens);
+  uint8_t *v_payload = global_ptr<uint8_t>(a.v_payload) + Layout::payload(tile.page_head, a.page_tokens);
+  uint8_t *v_scales = global_ptr<uint8_t>(a.v_scales) + Layout::scales(tile.page_head, a.page_tokens);
+  const uint32_t token = tile.page_token + t;
+#pragma unroll
+  for (uint32_t c = 0; c < Layout::kKeyChunks; ++c) {
+    const uint32_t d = c * 128u + piece * 16u;
+    const bool inside = live && d < D;
+    float k[16], v[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) k[i] = v[i] = 0.0f;
+    if (inside) {
+      load16(keys + d, k);
+      load16(values + d, v);
+    }
+    uint32_t kq[2], vq[2];
+    const uint32_t ks = quantise16(k, kq);
+    const uint32_t vs = quantise16(v, vq);
+    if (inside) {
+      *reinterpret_cast<uint2 *>(k_payload + Layout::key_byte(token, c) + piece * 8u) = make_uint2(kq[0], kq[1]);
+      if ((piece & 1u) == 0u) {
+        k_scales[Layout::key_scale(token, d / 32u)] = static_cast<uint8_t>(ks);
+        v_scales[Layout::value_scale(token, d / 32u)] = static_cast<uint8_t>(vs);
+      }
+    }
+    if (whole) {  // wave-uniform
+#pragma unroll
+      for (uint32_t i = 0; i < 8u; ++i) turned[wave][piece * 8u + i][t] = static_cast<uint8_t>(vq[i >> 2] >> (8u * (i & 3u)));
+      wave_lds_fence();
+      const uint2 pair = *reinterpret_cast<const uint2 *>(&turned[wave][lane][0]);
+      if (c * 64u + lane < D / 2u) {
+        *reinterpret_cast<uint2 *>(v_payload + Layout::value_byte(tile.page_token, c * 64u + lane)) = pair;
+      }
+      wave_lds_fence();
+    } else if (inside) {
+#pragma unroll
+      for (uint32_t i = 0; i < 8u; ++i) {
+        v_payload[Layout::value_byte(token, d / 2u + i)] = static_cast<uint8_t>(vq[i >> 2] >> (8u * (i & 3u)));
+      }
+    }
+  }
+}
+
+// A pair of values as stored in the output row.
+__device__ __forceinline__ void store_pair(float *dst, float x, float y) {
+  *reinterpret_cast<float2 *>(dst) = make_float2(x, y);
+}
+__device__ __forceinline__ void store_pair(uint16_t *dst, float x, float y) {  // exact in BF16
+  *reinterpret_cast<uint32_t *>(dst) = (__float_as_uint(x) >> 16) | (__float_as_uint(y) & 0xffff0000u);
+}
+
+__device__ __forceinline__ float block_scale(uint32_t byte) {
+  return byte == kNanBlock ? __uint_as_float(0x7fc00000u) : e8m0_to_f32(byte);
+}
+
+template <typename T, uint32_t D>
+__global__ __launch_bounds__(256) void kv_read_kernel(FerruleHipKvCacheArgs a) {
+  using Layout = KvLayout<D>;
+  const uint32_t lane = threadIdx.x & 63u;
+  KvTile tile;
+  if (!kv_tile(a, tile)) return;
+  const uint8_t *k_payload = global_ptr<const uint8_t>(a.k_payload) + Layout::payload(tile.page_head, a.page_tokens);
+  const uint8_t *k_scales = global_ptr<const uint8_t>(a.k_scales) + Layout::scales(tile.page_head, a.page_tokens);
+  const uint8_t *v_payload = global_ptr<const uint8_t>(a.v_payload) + Layout::payload(tile.page_head, a.page_tokens);
+  const uint8_t *v_scales = global_ptr<const uint8_t>(a.v_scales) + Layout::scales(tile.page_head, a.page_tokens);
+  const int32_t offset = tile.first - tile.sequence.position;  // row of the sequence of the tile's first token
+  const int32_t rows = static_cast<int32_t>(tile.sequence.rows);
+  // keys: lane = (token, piece) as in the writer
+  {
+    const uint32_t t = lane >> 3, piece = lane & 7u;
+    const int32_t index = offset + static_cast<int32_t>(t);
+    if (index >= 0 && index < rows) {
+      T *out = global_ptr<T>(a.keys) + (tile.sequence.row + static_cast<uint64_t>(index)) * a.key_row_stride +
+               tile.head * a.key_head_stride;
+      const uint32_t token = tile.page_token + t;
+#pragma unroll
+      for (uint32_t c = 0; c < Layout::kKeyChunks; ++c) {
+        const uint32_t d = c * 128u + piece * 16u;
+        if (d >= D) break;
+        uint2 bytes = make_uint2(0u, 0u);
+        float scale = 0.0f;
+        if (tile.page_valid) {
+          bytes = *reinterpret_cast<const uint2 *>(k_payload + Layout::key_byte(token, c) + piece * 8u);
+          scale = block_scale(k_scales[Layout::key_scale(token, d / 32u)]);
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < 8u; ++i) {
+          const uint32_t byte = (i < 4u ? bytes.x : bytes.y) >> (8u * (i & 3u));
+          store_pair(out + d + 2u * i, fp4_e2m1_decode(byte & 15u) * scale, fp4_e2m1_decode((byte >> 4) & 15u) * scale);
+        }
+      }
+    }
+  }
+  // values: a lane has one pair of values of all eight tokens, a token's row is 64 lanes side by side
+#pragma unroll
+  for (uint32_t c = 0; c < Layout::kKeyChunks; ++c) {
+    const uint32_t pair = c * 64u + lane;
+    if (pair >= D / 2u) break;
+    uint2 bytes = make_uint2(0u, 0u), scales = make_uint2(0u, 0u);
+    if (tile.page_valid) {
+      bytes = *reinterpret_cast<const uint2 *>(v_payload + Layout::value_byte(tile.page_token, pair));
+      scales = *reinterpret_cast<const uint2 *>(v_scales + Layout::value_scale(tile.page_token, pair / 16u));
+    }
+#pragma unroll
+    for (uint32_t t = 0; t < 8u; ++t) {
+      const int32_t index = offset + static_cast<int32_t>(t);
+      if (index < 0 || index >= rows) continue;
+      const uint32_t byte = (t < 4u ? bytes.x : bytes.y) >> (8u * (t & 3u));
+      const float scale = tile.page_valid ? block_scale(((t < 4u ? scales.x : scales.y) >> (8u * (t & 3u))) & 255u) : 0.0f;
+      T *out = global_ptr<T>(a.values) + (tile.sequence.row + static_cast<uint64_t>(index)) * a.value_row_stride +
+               tile.head * a.value_head_stride;
+      store_pair(out + 2u * pair, fp4_e2m1_decode(byte & 15u) * scale, fp4_e2m1_decode((byte >> 4) & 15u) * scale);
+    }
+  }
+}
+
+FerruleHipStatus validate(const FerruleHipKvCacheArgs &a) {
+  if (a.batch == 0u || a.rows == 0u) return FERRULE_HIP_SUCCESS;  // nothing to do
+  if (a.reserved != 0u || a.value_type > FERRULE_HIP_KV_BF16) return FERRULE_HIP_INVALID_ARGUMENT;
+  if (a.kv_heads == 0u || a.head_dim == 0u || a.page_count == 0u || a.max_pages == 0u || a.max_query_length == 0u ||
+      !kv_page_tokens_valid(a.page_tokens) || a.page_count > 0x7fffffffu || a.rows > 0x7fffffffu) {
+    return FERRULE_HIP_INVALID_ARGUMENT;
+  }
+  const uint32_t bytes = a.value_type == FERRULE_HIP_KV_BF16 ? 2u : 4u;
+  if (!kv_rows_aligned(a.keys, a.key_row_stride, a.key_head_stride, bytes) ||
+      !kv_rows_aligned(a.values, a.value_row_stride, a.value_head_stride, bytes) || !kv_aligned16(a.k_payload) ||
+      !kv_aligned16(a.k_scales) || !kv_aligned16(a.v_payload) || !kv_aligned16(a.v_scales) || a.query_indptr == 0u ||
+      a.sequence_lengths == 0u || a.page_table == 0u || ((a.query_indptr | a.sequence_lengths | a.page_table | a.error) & 3u)) {
+    return FERRULE_HIP_INVALID_ARGUMENT;
+  }
+  if (!kv_head_dim_supported(a.head_dim)) return FERRULE_HIP_UNSUPPORTED;
+  // the grid: batch in y, eight-token groups times heads in x
+  const uint64_t groups = (static_cast<uint64_t>(a.max_query_length) + 7u) / 8u + 1u;
+  if (a.batch > 65535u || groups * a.kv_heads > 0x7fffffffull) return FERRULE_HIP_UNSUPPORTED;
+  return FERRULE_HIP_SUCCESS;
+}
+
+template <template <typename, uint32_t> class Launch>
+FerruleHipStatus dispatch(const FerruleHipKvCacheArgs *args) {
+  if (args == nullptr) return FERRULE_HIP_INVALID_ARGUMENT;
+  const FerruleHipStatus status = validate(*args);
+  if (status != FERRULE_HIP_SUCCESS || args->batch == 0u || args->rows == 0u) return status;
+  const FerruleHipKvCacheArgs &a = *args;
+  hipStream_t stream = reinterpret_cast<hipStream_t>(static_cast<uintptr_t>(a.stream));
+  // rows that start inside a group of eight touch one group more
+  const uint32_t rows = a.max_query_length < a.rows ? a.max_query_length : a.rows;
+  const uint32_t groups = rows == 1u ? 1u : (rows + 7u) / 8u + 1u;
+  const dim3 grid((groups * a.kv_heads + kWaves - 1u) / kWaves, a.batch);
+  clear_launch_error();
+  if (a.value_type == FERRULE_HIP_KV_BF16) {
+    switch (a.head_dim) {
+      case 64: Launch<uint16_t, 64>::run(a, grid, stream); break;
+      case 128: Launch<uint16_t, 128>::run(a, grid, stream); break;
+      case 256: Launch<uint16_t, 256>::run(a, grid, stream); break;
+      default: Launch<uint16_t, 512>::run(a, grid, stream); break;
+    }
+  } else {
+    switch (a.head_dim) {
+      case 64: Launch<float, 64>::run(a, grid, stream); break;
+      case 128: Launch<float, 128>::run(a, grid, stream); break;
+      case 256: Launch<float, 256>::run(a, grid, stream); break;
+      default: Launch<float, 512>::run(a, grid, stream); break;
+    }
+  }
+  return take_launch_error() == hipSuccess ? FERRULE_HIP_SUCCESS : FERRULE_HIP_LAUNCH_FAILED;
+}
+
+template <typename T, uint32_t D>
+struct Append {
+  static void run(const FerruleHipKvCacheArgs &a, dim3 grid, hipStream_t stream) {
+    kv_append_kernel<T, D><<<grid, 256, 0, stream>>>(a);
+  }
+};
+template <typename T, uint32_t D>
+struct Read {
+  static void run(const FerruleHipKvCacheArgs &a, dim3 grid, hipStream_t stream) {
+    kv_read_kernel<T, D><<<grid, 256, 0, stream>>>(a);
+  }
+};
+
+}  // namespace
+}  // namespace ferrule_hip
+
+extern "C" int32_t ferrule_hip_kv_cache_append_can_implement(const FerruleHipKvCacheArgs *args) {
+  return args == nullptr ? FERRULE_HIP_INVALID_ARGUMENT : ferrule_hip::validate(*args);
+}
+extern "C" int32_t ferrule_hip_kv_cache_append_launch(const FerruleHipKvCacheArgs *args) {
+  return ferrule_hip::dispatch<ferrule_hip::Append>(args);
+}
+extern "C" int32_t ferrule_hip_kv_cache_read_can_implement(const FerruleHipKvCacheArgs *args) {
+  return args == nullptr ? FERRULE_HIP_INVALID_ARGUMENT : ferrule_hip::validate(*args);
+}
+extern "C" int32_t ferrule_hip_kv_cache_read_launch(const FerruleHipKvCacheArgs *args) {
+  return ferrule_hip::dispatch<ferrule_hip::Read>(args);
+}

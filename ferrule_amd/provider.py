@@ -99,6 +99,63 @@ def _ptr(t: torch.Tensor | None) -> int:
     return 0 if t is None else t.data_ptr()
 
 
+def kv_cache_shapes(page_count: int, page_tokens: int, kv_heads: int, head_dim: int) -> tuple[tuple[int, ...], ...]:
+    """Shapes of the four byte arrays of an MXFP4 key/value cache (``FerruleHipKvCacheArgs``):
+    key payload, key scales, value payload, value scales."""
+    p, h, t, d = page_count, kv_heads, page_tokens, head_dim
+    return ((p, h, t // 32, -(-d // 128), 32, min(d, 128) // 2), (p, h, t // 32, d // 32, 32),
+            (p, h, t // 8, d // 2, 8), (p, h, t // 8, d // 32, 8))
+
+
+class HipKvCache:
+    """One layer's keys and values in pages, E2M1 nibbles with one E8M0 scale byte per 32 values of
+    a row (17/32 byte a value).  Holds the caller's four ``uint8`` device tensors."""
+
+    def __init__(self, page_tokens: int, kv_heads: int, head_dim: int, k_payload: torch.Tensor,
+                 k_scales: torch.Tensor, v_payload: torch.Tensor, v_scales: torch.Tensor):
+        if page_tokens < 32 or page_tokens > 1024 or page_tokens & (page_tokens - 1):
+            raise ValueError(f"HIP KV cache pages hold a power of two of 32..1024 tokens, got {page_tokens}")
+        if head_dim not in abi.KV_HEAD_DIMS or kv_heads < 1:
+            raise ValueError(f"HIP KV cache needs a head size of {abi.KV_HEAD_DIMS} and at least one head, got "
+                             f"{head_dim} and {kv_heads}")
+        self.page_tokens, self.kv_heads, self.head_dim = page_tokens, kv_heads, head_dim
+        self.k_payload, self.k_scales, self.v_payload, self.v_scales = k_payload, k_scales, v_payload, v_scales
+        self.page_count = k_payload.shape[0]
+        arrays = (k_payload, k_scales, v_payload, v_scales)
+        for t, shape in zip(arrays, kv_cache_shapes(self.page_count, page_tokens, kv_heads, head_dim)):
+            if t.dtype != torch.uint8 or tuple(t.shape) != shape or not t.is_contiguous() or \
+                    t.device != k_payload.device:
+                raise ValueError(f"HIP KV cache array must be contiguous uint8 {shape}, got {t.dtype} {tuple(t.shape)}")
+        if self.page_count < 1:
+            raise ValueError("HIP KV cache needs at least one page")
+
+
+class HipKvBatch:
+    """What one step's rows are: ``query_indptr`` [batch + 1], ``sequence_lengths`` [batch] and
+    ``page_table`` [batch, max_pages], int32 on the device, read when the kernels run.  Sequence b has
+    the rows ``query_indptr[b] .. query_indptr[b + 1]`` and ``sequence_lengths[b]`` tokens with them; its
+    row i stands at position ``sequence_lengths[b] - n_b + i``.  ``rows`` is the length of the row
+    tensors, ``max_query_length`` a bound of the n_b and ``max_sequence_length`` one of the lengths
+    (by default what the page table can hold; a closer one splits long sequences better)."""
+
+    def __init__(self, query_indptr: torch.Tensor, sequence_lengths: torch.Tensor, page_table: torch.Tensor,
+                 rows: int, max_query_length: int | None = None, max_sequence_length: int | None = None):
+        batch = sequence_lengths.shape[0] if sequence_lengths.dim() == 1 else -1
+        for name, t, shape in (("query_indptr", query_indptr, (batch + 1,)),
+                               ("sequence_lengths", sequence_lengths, (batch,)),
+                               ("page_table", page_table, (batch, page_table.shape[-1]))):
+            if t.dtype != torch.int32 or tuple(t.shape) != shape or not t.is_contiguous() or \
+                    t.device != query_indptr.device:
+                raise ValueError(f"HIP KV batch {name} must be contiguous int32 {shape}, got {t.dtype} {tuple(t.shape)}")
+        self.query_indptr, self.sequence_lengths, self.page_table = query_indptr, sequence_lengths, page_table
+        self.batch, self.max_pages, self.rows = batch, page_table.shape[1], int(rows)
+        self.max_query_length = self.rows if max_query_length is None else int(max_query_length)
+        self.max_sequence_length = max_sequence_length if max_sequence_length is None else int(max_sequence_length)
+        if self.rows < 0 or self.max_query_length < min(self.rows, 1) or \
+                (self.max_sequence_length is not None and self.max_sequence_length < 0):
+            raise ValueError("HIP KV batch needs rows >= 0 and bounds of at least one row")
+
+
 def validate_dsv4_router_token_ids(token_ids, hash_rows: int) -> list[int]:
     """context.rs:1861-1891: every id must address a row of the hash table."""
     token_ids = [int(t) for t in token_ids]
@@ -1026,6 +1083,137 @@ class HipArtifactOperatorContext:
             split_pre_f32=_ptr(out["pre"]), split_post_f32=_ptr(out["post"]), split_comb_f32=_ptr(out["comb"]))
         self._two_phase("HC producer", self.lib.ferrule_hip_hc_producer_can_implement,
                         self.lib.ferrule_hip_hc_producer_launch, a)
+        return out
+
+    # -- MXFP4 key/value cache ------------------------------------------------------
+    def kv_cache(self, page_count: int, page_tokens: int, kv_heads: int, head_dim: int) -> HipKvCache:
+        """A new cache on this context's device; every byte zero."""
+        arrays = (torch.zeros(shape, dtype=torch.uint8, device=self.device)
+                  for shape in kv_cache_shapes(page_count, page_tokens, kv_heads, head_dim))
+        return HipKvCache(page_tokens, kv_heads, head_dim, *arrays)
+
+    def _check_kv(self, cache: HipKvCache, batch: HipKvBatch, error: torch.Tensor | None, *tensors) -> None:
+        device = cache.k_payload.device
+        if device.type != "cuda" or device.index != (torch.cuda.current_device() if self.device.index is None
+                                                     else self.device.index):
+            raise ValueError(f"HIP KV operators run on {self.device}, the cache is on {device}")
+        if batch.page_table.device != device or any(t.device != device for t in tensors):
+            raise ValueError(f"HIP KV operators need every tensor on the cache's device {device}")
+        if error is not None and (error.dtype != torch.int32 or error.numel() != 1 or error.device != device):
+            raise ValueError("HIP KV error flag must be one int32 on the device")
+
+    def _kv_launch(self, what: str, can_implement, launch, args) -> None:
+        """``_two_phase`` with this context's device current, which a launch on its stream needs."""
+        if self.device.index is None or torch.cuda.current_device() == self.device.index:
+            self._two_phase(what, can_implement, launch, args)
+        else:
+            with torch.cuda.device(self.device):
+                self._two_phase(what, can_implement, launch, args)
+
+    @staticmethod
+    def _check_kv_rows(what: str, t: torch.Tensor, rows: int, heads: int, head_dim: int) -> None:
+        if t.dtype not in (torch.bfloat16, torch.float32) or tuple(t.shape) != (rows, heads, head_dim) or \
+                (t.stride(2) != 1 and t.numel() > 0):
+            raise ValueError(f"HIP KV {what} must be bf16 or f32 {(rows, heads, head_dim)} with consecutive values, "
+                             f"got {t.dtype} {tuple(t.shape)} strides {t.stride()}")
+
+    def _kv_cache_args(self, cache: HipKvCache, batch: HipKvBatch, k: torch.Tensor, v: torch.Tensor,
+                       error: torch.Tensor | None) -> abi.KvCacheArgs:
+        self._check_kv(cache, batch, error, k, v)
+        self._check_kv_rows("keys", k, batch.rows, cache.kv_heads, cache.head_dim)
+        self._check_kv_rows("values", v, batch.rows, cache.kv_heads, cache.head_dim)
+        if k.dtype != v.dtype:
+            raise ValueError("HIP KV keys and values share one type")
+        return abi.KvCacheArgs(
+            batch=batch.batch, rows=batch.rows, kv_heads=cache.kv_heads, head_dim=cache.head_dim,
+            page_tokens=cache.page_tokens, page_count=cache.page_count, max_pages=batch.max_pages,
+            max_query_length=batch.max_query_length,
+            value_type=abi.KV_BF16 if k.dtype == torch.bfloat16 else abi.KV_F32,
+            key_row_stride=k.stride(0), key_head_stride=k.stride(1), value_row_stride=v.stride(0),
+            value_head_stride=v.stride(1), keys=_ptr(k), values=_ptr(v), k_payload=_ptr(cache.k_payload),
+            k_scales=_ptr(cache.k_scales), v_payload=_ptr(cache.v_payload), v_scales=_ptr(cache.v_scales),
+            query_indptr=_ptr(batch.query_indptr), sequence_lengths=_ptr(batch.sequence_lengths),
+            page_table=_ptr(batch.page_table), error=_ptr(error))
+
+    def kv_cache_append(self, cache: HipKvCache, batch: HipKvBatch, k: torch.Tensor, v: torch.Tensor,
+                        error: torch.Tensor | None = None) -> None:
+        """Quantise the batch's key and value rows (BF16 or f32 [rows, kv_heads, head_dim], rows and
+        heads strided as they like) and write them at their positions.  The bytes are those of
+        ``pack_fp4_rows_from_f32`` (its default rounding), except that a block holding an infinity or
+        a NaN is written as a block of NaN.  ``error`` (int32 [1], cleared by the caller) becomes 1 when
+        a row has no valid place; such rows are dropped.  The pages written belong to one sequence each."""
+        if batch.rows == 0 or batch.batch == 0:
+            return
+        self._kv_launch("KV cache append", self.lib.ferrule_hip_kv_cache_append_can_implement,
+                        self.lib.ferrule_hip_kv_cache_append_launch, self._kv_cache_args(cache, batch, k, v, error))
+
+    def kv_cache_read_into(self, cache: HipKvCache, batch: HipKvBatch, k: torch.Tensor, v: torch.Tensor,
+                           error: torch.Tensor | None = None) -> None:
+        """The cache's values at the batch's positions into BF16 or f32 [rows, kv_heads, head_dim], exact
+        in either type.  To read positions s..e of a sequence give it e - s rows and length e.  A row
+        without a valid place reads as zeros and sets ``error``."""
+        if batch.rows == 0 or batch.batch == 0:
+            return
+        self._kv_launch("KV cache read", self.lib.ferrule_hip_kv_cache_read_can_implement,
+                        self.lib.ferrule_hip_kv_cache_read_launch, self._kv_cache_args(cache, batch, k, v, error))
+
+    def _kv_attention_args(self, cache: HipKvCache, batch: HipKvBatch, q_heads: int, window: int,
+                           sinks: int) -> abi.KvAttentionArgs:
+        if q_heads < 1 or q_heads % cache.kv_heads:
+            raise ValueError(f"HIP KV attention needs a multiple of {cache.kv_heads} query heads, got {q_heads}")
+        if window < 0 or sinks < 0:
+            raise ValueError("HIP KV attention window and sinks must not be negative")
+        limit = batch.max_pages * cache.page_tokens
+        return abi.KvAttentionArgs(
+            batch=batch.batch, rows=batch.rows, q_heads=q_heads, kv_heads=cache.kv_heads, head_dim=cache.head_dim,
+            page_tokens=cache.page_tokens, page_count=cache.page_count, max_pages=batch.max_pages,
+            max_query_length=batch.max_query_length,
+            max_sequence_length=min(limit, 0x7fffffff) if batch.max_sequence_length is None else batch.max_sequence_length,
+            window=window, sinks=sinks, softmax_scale=1.0)
+
+    def kv_cache_attention_workspace(self, cache: HipKvCache, batch: HipKvBatch, q_heads: int, window: int = 0,
+                                     sinks: int = 0) -> torch.Tensor:
+        """The scratch that ``kv_cache_attention_into`` needs for batches of this shape (uint8, possibly
+        empty).  It belongs to one call at a time: keep one per stream, and one per captured graph that
+        may replay while another runs."""
+        args = self._kv_attention_args(cache, batch, q_heads, window, sinks)
+        size = self.lib.ferrule_hip_kv_attention_workspace_size(C.byref(args))
+        return torch.empty(size, dtype=torch.uint8, device=self.device)
+
+    def kv_cache_attention_into(self, cache: HipKvCache, batch: HipKvBatch, q: torch.Tensor, out: torch.Tensor,
+                                softmax_scale: float, window: int = 0, sinks: int = 0,
+                                workspace: torch.Tensor | None = None,
+                                error: torch.Tensor | None = None) -> torch.Tensor:
+        """Attention of the batch's rows over the cache, their own keys and values appended before:
+        ``q`` and ``out`` are BF16 or f32 [rows, q_heads, head_dim] (f32 queries are rounded to BF16), head h
+        reads key/value head h // (q_heads // kv_heads), and the row at position p sees position j when
+        ``j <= p and (window == 0 or p - j < window or j < sinks)``.  A row that sees nothing writes
+        zeros.  Without ``workspace`` one is taken from torch's allocator for the call."""
+        self._check_kv(cache, batch, error, q, out)
+        q_heads = q.shape[1] if q.dim() == 3 else 0
+        self._check_kv_rows("queries", q, batch.rows, q_heads, cache.head_dim)
+        self._check_kv_rows("output", out, batch.rows, q_heads, cache.head_dim)
+        if batch.rows == 0 or batch.batch == 0:
+            return out
+        a = self._kv_attention_args(cache, batch, q_heads, window, sinks)
+        a.flags = (abi.KV_ATTENTION_QUERY_F32 if q.dtype == torch.float32 else 0) | \
+            (abi.KV_ATTENTION_OUTPUT_F32 if out.dtype == torch.float32 else 0)
+        a.softmax_scale = softmax_scale
+        a.q_row_stride, a.q_head_stride, a.output_row_stride, a.output_head_stride = *q.stride()[:2], *out.stride()[:2]
+        a.q, a.output = _ptr(q), _ptr(out)
+        a.k_payload, a.k_scales = _ptr(cache.k_payload), _ptr(cache.k_scales)
+        a.v_payload, a.v_scales = _ptr(cache.v_payload), _ptr(cache.v_scales)
+        a.query_indptr, a.sequence_lengths = _ptr(batch.query_indptr), _ptr(batch.sequence_lengths)
+        a.page_table, a.error = _ptr(batch.page_table), _ptr(error)
+        if workspace is None:
+            size = self.lib.ferrule_hip_kv_attention_workspace_size(C.byref(a))
+            with torch.cuda.stream(self.stream):       # the block is reused in this stream's order
+                workspace = torch.empty(size, dtype=torch.uint8, device=self.device)
+        elif workspace.dtype != torch.uint8 or workspace.device != self.device or not workspace.is_contiguous():
+            raise ValueError("HIP KV attention workspace must be contiguous uint8 on the device")
+        a.workspace, a.workspace_bytes = _ptr(workspace), workspace.numel()
+        self._kv_launch("KV attention", self.lib.ferrule_hip_kv_attention_can_implement,
+                        self.lib.ferrule_hip_kv_attention_launch, a)
         return out
 
     # -- routed MoE ---------------------------------------------------------------

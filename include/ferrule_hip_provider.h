@@ -52,6 +52,8 @@ typedef enum FerruleHipStatus {
 #define FERRULE_HIP_KERNEL_MOE_DECODE 34u
 #define FERRULE_HIP_KERNEL_FP8_BLOCK_GEMM 35u
 #define FERRULE_HIP_KERNEL_DENSE_FFN_DECODE 36u
+#define FERRULE_HIP_KERNEL_KV_CACHE 37u
+#define FERRULE_HIP_KERNEL_KV_ATTENTION 38u
 #define FERRULE_HIP_KERNEL_BIT(id) (1ull << ((id) - 1u))
 
 typedef struct FerruleHipProviderManifest {
@@ -867,6 +869,133 @@ typedef struct FerruleHipHcProducerArgs {
 int32_t ferrule_hip_hc_producer_can_implement(const FerruleHipHcProducerArgs *args);
 int32_t ferrule_hip_hc_producer_launch(const FerruleHipHcProducerArgs *args);
 
+/* ------------------------------------------------------------------------ */
+/* (4) MXFP4 key/value cache: no reference symbol                             */
+/* ------------------------------------------------------------------------ */
+
+/* A layer's keys and values in pages of `page_tokens` tokens (a power of two, 32..1024), each row of
+ * head_dim (64, 128, 256 or 512) values as E2M1 nibbles with one E8M0 scale byte per 32 values:
+ * 17/32 byte a value.  For `page_count` pages and `kv_heads` heads, row-major byte arrays:
+ *   k_payload [page_count][kv_heads][page_tokens/32][ceil(D/128)][32][min(D,128)/2]
+ *   k_scales  [page_count][kv_heads][page_tokens/32][D/32][32]
+ *   v_payload [page_count][kv_heads][page_tokens/8][D/2][8]
+ *   v_scales  [page_count][kv_heads][page_tokens/8][D/32][8]
+ * A byte holds the values d (low nibble) and d+1, d even.  32 tokens of keys are rows of 64 bytes, the
+ * 4-bit operand of the scaled MFMA as it stands; values are stored eight tokens side by side, because
+ * attention sums over tokens.
+ *   scale byte  s = 127 + max(ceil(log2(amax / 6)), -126) for the block's largest magnitude amax, the
+ *               smallest power of two that brings it to 6 or less; 255 (a block of NaN) when the
+ *               block holds an infinity or a NaN
+ *   nibble      the nearest of {0, .5, 1, 1.5, 2, 3, 4, 6} to |x| / 2^(s-127), a tie to the smaller,
+ *               with x's sign (the rule of ferrule_hip_core_quantize_launch kind 4)
+ *
+ * The three operators share one description of a batch, all int32 on the device:
+ *   query_indptr [batch+1]     rows of sequence b: query_indptr[b] .. query_indptr[b+1], n_b of them
+ *   sequence_lengths [batch]   L_b tokens of sequence b, its n_b rows with them; row i of the
+ *                              sequence stands at position L_b - n_b + i
+ *   page_table [batch][max_pages]  the page of position p is page_table[b][p / page_tokens]
+ * `rows` is how many rows the row tensors hold; rows behind query_indptr[batch] are not touched.
+ * `max_query_length` is an upper bound of the n_b (it sizes the grid).  A page number outside
+ * [0, page_count), a position outside the table, rows beyond `rows` or `max_query_length` are never
+ * followed; whoever meets one stores 1 to `error` (int32 [1], may be 0; the caller clears it). */
+#define FERRULE_HIP_KV_F32 0u
+#define FERRULE_HIP_KV_BF16 1u
+
+typedef struct FerruleHipKvCacheArgs {
+  uint32_t batch;
+  uint32_t rows;
+  uint32_t kv_heads;
+  uint32_t head_dim;
+  uint32_t page_tokens;
+  uint32_t page_count;
+  uint32_t max_pages;
+  uint32_t max_query_length;
+  uint32_t value_type;        /* FERRULE_HIP_KV_*: type of keys and values */
+  uint32_t reserved;          /* 0 */
+  uint64_t key_row_stride;    /* in values; a row's head_dim values are consecutive and every */
+  uint64_t key_head_stride;   /* row of a head starts on 16 bytes */
+  uint64_t value_row_stride;
+  uint64_t value_head_stride;
+  uint64_t keys;              /* [rows, kv_heads, head_dim] */
+  uint64_t values;
+  uint64_t k_payload;         /* 16-byte aligned, as all cache arrays */
+  uint64_t k_scales;
+  uint64_t v_payload;
+  uint64_t v_scales;
+  uint64_t query_indptr;
+  uint64_t sequence_lengths;
+  uint64_t page_table;
+  uint64_t error;             /* int32 [1] or 0 */
+  uint64_t stream;
+} FerruleHipKvCacheArgs;
+
+/* append: quantises the batch's rows and writes them at their positions; a row without a valid
+ * place is dropped.  The pages that one call writes belong to one sequence each.
+ * read: the cache's values at the rows' positions (exact in either type); a row without a valid
+ * place reads as zeros.  To read positions [s, e) of a sequence pass n_b = e - s and L_b = e.
+ * INVALID_ARGUMENT for a bad block, UNSUPPORTED for a head_dim outside the supported set; a block
+ * with rows == 0 or batch == 0 is a successful no-op. */
+int32_t ferrule_hip_kv_cache_append_can_implement(const FerruleHipKvCacheArgs *args);
+int32_t ferrule_hip_kv_cache_append_launch(const FerruleHipKvCacheArgs *args);
+int32_t ferrule_hip_kv_cache_read_can_implement(const FerruleHipKvCacheArgs *args);
+int32_t ferrule_hip_kv_cache_read_launch(const FerruleHipKvCacheArgs *args);
+
+#define FERRULE_HIP_KV_ATTENTION_QUERY_F32 1u  /* flags bit0: q is f32 */
+#define FERRULE_HIP_KV_ATTENTION_OUTPUT_F32 2u /* flags bit1: output is f32, not rounded to BF16 */
+
+/* Attention of the batch's rows over the cache, for one token per sequence as for whole prompts:
+ *   o[r, h, :] = sum_j softmax_j(softmax_scale * q[r, h, :] . k[j, h / group, :]) * v[j, h / group, :]
+ * with group = q_heads / kv_heads, over the positions j that the row at position p sees:
+ *   j <= p and (window == 0 or p - j < window or j < sinks),
+ * i.e. causal, or the last `window` positions and the first `sinks`.  The rows' own keys and values
+ * are in the cache already (append first).  A row that sees nothing (a position before 0, every
+ * visible page invalid) writes zeros; keys and values at positions that a row does not see do not
+ * reach it, whatever they hold.
+ * Arithmetic: q enters rounded to BF16 (exact for BF16, and for the f32 rows of the FP8 projections,
+ * which hold BF16 values); scores, softmax statistics and sums are f32; the softmax weights are
+ * rounded to BF16 before they multiply the values.  Sums are formed in a fixed order.
+ * `max_sequence_length`, a bound of the L_b, sizes the split of long sequences over workgroups and
+ * nothing else.  Workspace: ferrule_hip_kv_attention_workspace_size bytes (may be 0), 256-byte
+ * aligned, used by this call alone until it has completed. */
+typedef struct FerruleHipKvAttentionArgs {
+  uint32_t batch;
+  uint32_t rows;
+  uint32_t q_heads;
+  uint32_t kv_heads;
+  uint32_t head_dim;
+  uint32_t page_tokens;
+  uint32_t page_count;
+  uint32_t max_pages;
+  uint32_t max_query_length;
+  uint32_t max_sequence_length;
+  uint32_t window;            /* 0: every position up to the row's own */
+  uint32_t sinks;             /* ignored when window is 0 */
+  uint32_t flags;
+  float softmax_scale;        /* finite, more than 0 */
+  uint64_t q_row_stride;      /* in values, as in FerruleHipKvCacheArgs */
+  uint64_t q_head_stride;
+  uint64_t output_row_stride;
+  uint64_t output_head_stride;
+  uint64_t q;                 /* [rows, q_heads, head_dim] */
+  uint64_t output;            /* [rows, q_heads, head_dim] */
+  uint64_t k_payload;
+  uint64_t k_scales;
+  uint64_t v_payload;
+  uint64_t v_scales;
+  uint64_t query_indptr;
+  uint64_t sequence_lengths;
+  uint64_t page_table;
+  uint64_t error;             /* int32 [1] or 0 */
+  uint64_t workspace;
+  uint64_t workspace_bytes;
+  uint64_t stream;
+} FerruleHipKvAttentionArgs;
+
+/* Reads scalar fields only (pointers may be zero), like ferrule_hip_moe_decode_workspace_size. */
+uint64_t ferrule_hip_kv_attention_workspace_size(const FerruleHipKvAttentionArgs *args);
+int32_t ferrule_hip_kv_attention_can_implement(const FerruleHipKvAttentionArgs *args);
+int32_t ferrule_hip_kv_attention_launch(const FerruleHipKvAttentionArgs *args);
+
 #ifdef __cplusplus
 } /* extern "C" */
 
@@ -903,6 +1032,8 @@ FERRULE_HIP_ASSERT_LAYOUT(FerruleHipPrepareMxfp4SfbArgs, 40, linear_source, 16, 
 FERRULE_HIP_ASSERT_LAYOUT(FerruleHipPrepareMxfp4BlockMajorArgs, 48, weight_source, 8, 40);
 FERRULE_HIP_ASSERT_LAYOUT(FerruleHipPrepareFp8BlockMajorArgs, 32, weight_source, 8, 24);
 FERRULE_HIP_ASSERT_LAYOUT(FerruleHipSharedFfnArgs, 160, input_fp8, 0, 152);
+FERRULE_HIP_ASSERT_LAYOUT(FerruleHipKvCacheArgs, 160, key_row_stride, 40, 152);
+FERRULE_HIP_ASSERT_LAYOUT(FerruleHipKvAttentionArgs, 192, q_row_stride, 56, 184);
 static_assert(offsetof(FerruleHipExpertGroupRoutePlanArgs, active_expert_slots) == 88, "route plan layout");
 static_assert(offsetof(FerruleHipExpertGroupRoutePlanArgs, expert_route_indptr) == 104, "route plan layout");
 static_assert(offsetof(FerruleHipExpertGroupRoutePlanArgs, host_scalars) == 144, "route plan layout");
