@@ -1,130 +1,585 @@
 // Attention over the MXFP4 key/value cache (no reference symbol; formats, layout and batch
 // description: include/ferrule_hip_provider.h).
+//
+// Rows.  The n_b rows of a sequence times the `group` query heads of one key/value head are one
+// list of packed rows r = row * group + head, cut into tiles of 16: a tile is one column set of
+// the matrix instructions, and one token for eight query heads fills half of it.
+//
+// One step of a wave takes 32 tokens through a tile, everything transposed so that a lane keeps ONE
+// row from the scores to the output (lane = (i, g), i = lane % 16 the row, g = lane / 16):
+//   S^T = K Q^T   v_mfma_scale_f32_16x16x128_f8f6f4: the cache's nibbles and scale bytes are the
+//                 4-bit operand as they stand; a BF16 row of q is split once into two E4M3 terms,
+//                 x = q0 2^s0 + q1 2^s1 (s1 = s0 - 5), exact but for elements below 2^-13 of their
+//                 block's largest, which are held to 2^-22 of it.
+//   softmax       the two 16-token products are fed tokens 8(m/4) + m%4 and 4 more for their rows m,
+//                 so lane (i, g) receives the scores of tokens 8g..8g+7 of row i: weights need no
+//                 exchange between lanes before they are the next product's operand.
+//   O^T += V^T P^T  v_mfma_f32_16x16x32_bf16: values cannot stay in 4 bits here (their scales run
+//                 along the row, the sum runs over tokens), so they are expanded to BF16, exactly, and
+//                 the weights are rounded to BF16 (2^-9 of each weight; the sum of the weights is
+//                 taken in f32 before that rounding).
+// The running maximum m of a row moves only when a score exceeds it by 2^8 (a wave-uniform branch):
+// weights up to 256 cost a 32-bit sum nothing, and most steps rescale nothing.
+//
+// A tile's tokens are shared out over the workgroup's four waves, 32 at a time, and a long range
+// over several workgroups; (m, sum, O) of the parts are joined in a fixed order, in LDS for the
+// waves and by kv_attention_join_kernel for the workgroups.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
 #include "../../include/ferrule_hip_provider.h"
 #include "kv_cache.cuh"
+#include "mx_core.cuh"
 
 namespace ferrule_hip {
 namespace {
 
-constexpr uint32_t kChunk = 256;  // tokens that a workgroup scores at a time, one per thread
+constexpr uint32_t kWaves = 4;
+constexpr uint32_t kTileRows = 16;   // packed rows of a tile
+constexpr uint32_t kTileTokens = 32; // tokens of one step
+constexpr float kLazy = 8.0f;        // how far (in powers of two) scores may exceed the running maximum
 
-__device__ __forceinline__ float load_query(uint64_t q, uint64_t at, bool f32) {
-  return f32 ? bf16_round(global_ptr<const float>(q)[at]) : bf16_bits_to_f32(global_ptr<const uint16_t>(q)[at]);
+struct SplitPlan {
+  uint32_t splits;     // workgroups a token range may be cut into
+  uint32_t min_tiles;  // 32-token tiles that a part has at least
+  uint64_t partials;   // byte offsets in the workspace
+  uint64_t statistics;
+};
+
+// The 32-token tiles that a range of rows sees: tiles [0, head) and [first, first + count - head).
+struct TileRange {
+  uint32_t head;
+  uint32_t first;
+  uint32_t count;
+  __device__ __forceinline__ uint32_t at(uint32_t v) const { return v < head ? v : first + (v - head); }
+};
+
+__device__ __forceinline__ TileRange tile_range(const FerruleHipKvAttentionArgs &a, int32_t low, int32_t high) {
+  // rows at positions low..high; validate() keeps the table below 2^31 tokens
+  TileRange t = {0u, 0u, 0u};
+  const int32_t last = min(high, static_cast<int32_t>(a.max_pages * a.page_tokens) - 1);
+  if (last < 0) return t;
+  const uint32_t end = static_cast<uint32_t>(last) / kTileTokens + 1u;
+  if (a.window != 0u) {
+    const int32_t from = max(0, low - static_cast<int32_t>(a.window - 1u));
+    t.first = min(static_cast<uint32_t>(from) / kTileTokens, end);
+    t.head = min((a.sinks + kTileTokens - 1u) / kTileTokens, t.first);
+  }
+  t.count = t.head + end - t.first;
+  return t;
 }
 
-__device__ __forceinline__ float block_value(uint32_t nibble, uint32_t byte) {
-  return byte == kNanBlock ? __uint_as_float(0x7fc00000u) : fp4_e2m1_decode(nibble) * e8m0_to_f32(byte);
+// Tiles per part: every part but the last has as many.
+__device__ __forceinline__ uint32_t part_tiles(uint32_t count, const SplitPlan &plan) {
+  return max((count + plan.splits - 1u) / plan.splits, plan.min_tiles);
 }
 
-// One workgroup per row and query head: a thread scores one token, then owns values of the row.
 template <uint32_t D>
-__global__ __launch_bounds__(256) void kv_attention_row_kernel(FerruleHipKvAttentionArgs a) {
+struct Core {
   using Layout = KvLayout<D>;
-  __shared__ float query[D];
-  __shared__ float weight[kChunk];
-  __shared__ int32_t page_of[kChunk];
-  __shared__ float reduce[8];
-  const uint32_t b = blockIdx.y, thread = threadIdx.x;
-  const uint32_t head = blockIdx.x % a.q_heads, index = blockIdx.x / a.q_heads;
+  static constexpr uint32_t kChunks = Layout::kKeyChunks;       // 128-value pieces of a row
+  static constexpr uint32_t kTerms = D == 64u ? 1u : 2u;        // products per piece: both terms of 64 values fill one
+  static constexpr uint32_t kUnits = D / 64u;                   // 16-byte value loads of a lane per 32 tokens
+  static constexpr uint32_t kColumns = D / 16u;                 // accumulators of a tile
+
+  struct Query {
+    i32x8_t term[kChunks * kTerms];
+    uint32_t scale[kChunks * kTerms];
+  };
+  struct Keys {
+    u32x4_t payload[kChunks][2];
+    uint2 scale[kChunks];
+  };
+  struct Values {
+    u32x4_t payload[kUnits];
+    uint2 scale[kUnits];
+  };
+
+  // 16 values of a row, as f32 holding BF16
+  static __device__ __forceinline__ void load_row16(uint64_t base, uint64_t at, bool f32, float (&x)[16]) {
+    if (f32) {
+      const f32x4_t *src = reinterpret_cast<const f32x4_t *>(global_ptr<const float>(base) + at);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const f32x4_t w = src[i];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[4 * i + e] = bf16_round(w[e]);
+      }
+    } else {
+      const u32x4_t *src = reinterpret_cast<const u32x4_t *>(global_ptr<const uint16_t>(base) + at);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const u32x4_t w = src[i];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          x[8 * i + 2 * e] = __uint_as_float(w[e] << 16);
+          x[8 * i + 2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
+        }
+      }
+    }
+  }
+
+  // Both terms of 16 values whose block's largest magnitude has the f32 exponent field `field`.
+  static __device__ __forceinline__ uint32_t split16(const float (&x)[16], uint32_t field, u32x4_t &q0, u32x4_t &q1) {
+    // largest magnitude to [128, 256): below E4M3's 448; the remainder is at most 2^3 of this scale, 2^8 of the next
+    const uint32_t byte = min(max(field, 13u), 254u) - 7u;
+    const float inverse0 = __uint_as_float((254u - byte) << 23), scale0 = __uint_as_float(byte << 23);
+    const float inverse1 = __uint_as_float((254u - (byte - 5u)) << 23);
+    const bool finite = field < 255u;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      int a = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * w] * inverse0, x[4 * w + 1] * inverse0, 0, false);
+      a = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * w + 2] * inverse0, x[4 * w + 3] * inverse0, a, true);
+      const f32x2_t lo = __builtin_amdgcn_cvt_pk_f32_fp8(a, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(a, true);
+      int b = __builtin_amdgcn_cvt_pk_fp8_f32((x[4 * w] - lo[0] * scale0) * inverse1,
+                                              (x[4 * w + 1] - lo[1] * scale0) * inverse1, 0, false);
+      b = __builtin_amdgcn_cvt_pk_fp8_f32((x[4 * w + 2] - hi[0] * scale0) * inverse1,
+                                          (x[4 * w + 3] - hi[1] * scale0) * inverse1, b, true);
+      q0[w] = finite ? static_cast<uint32_t>(a) : 0x7f7f7f7fu;  // a row with an infinity or a NaN: NaN scores
+      q1[w] = finite ? static_cast<uint32_t>(b) : 0u;
+    }
+    return byte;
+  }
+
+  static __device__ __forceinline__ uint32_t block_field(const float (&x)[16]) {
+    uint32_t top = 0u;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
+    top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 16, 64)));  // the block's other 16 values
+    return top >> 23;
+  }
+
+  // The lane's part of a tile's query rows; `live` false: zeros.
+  static __device__ __forceinline__ void load_query(uint64_t base, uint64_t row, bool live, bool f32, uint32_t lane, Query &q) {
+    const uint32_t g = lane >> 4;
+    const uint32_t source = (lane & 15u) + ((g & 1u) << 5);  // holds the scales of block g, in its half g / 2
+#pragma unroll
+    for (uint32_t c = 0; c < kChunks; ++c) {
+      float lo[16], hi[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) lo[i] = hi[i] = 0.0f;
+      if (live) {
+        load_row16(base, row + c * 128u + g * 16u, f32, lo);
+        if constexpr (D > 64u) load_row16(base, row + c * 128u + 64u + g * 16u, f32, hi);
+      }
+      u32x4_t lo0, lo1, hi0, hi1;
+      const uint32_t lo_byte = split16(lo, block_field(lo), lo0, lo1);
+      const int32_t lo_scale = __shfl(static_cast<int>(lo_byte), static_cast<int>(source), 64);
+      if constexpr (D == 64u) {
+        // values 0..63 twice along the product: first term against the first copy of a key, second against the second
+        q.term[0] = make_b_fp8(lo0, lo1);
+        q.scale[0] = static_cast<uint32_t>(lo_scale) - (g >= 2u ? 5u : 0u);
+      } else {
+        const uint32_t hi_byte = split16(hi, block_field(hi), hi0, hi1);
+        const int32_t hi_scale = __shfl(static_cast<int>(hi_byte), static_cast<int>(source), 64);
+        const uint32_t scale = static_cast<uint32_t>(g >= 2u ? hi_scale : lo_scale);
+        q.term[2u * c] = make_b_fp8(lo0, hi0);
+        q.term[2u * c + 1u] = make_b_fp8(lo1, hi1);
+        q.scale[2u * c] = scale;
+        q.scale[2u * c + 1u] = scale - 5u;
+      }
+    }
+  }
+
+  // `token`: the step's first token inside its page's head (a multiple of 32)
+  static __device__ __forceinline__ void load_keys(const uint8_t *payload, const uint8_t *scales, uint32_t token, uint32_t lane,
+                                                   Keys &k) {
+    const uint32_t i = lane & 15u, g = lane >> 4;
+    const uint32_t t = 8u * (i >> 2) + (i & 3u);
+#pragma unroll
+    for (uint32_t c = 0; c < kChunks; ++c) {
+      const uint32_t block = D == 64u ? (g & 1u) : g;  // of the piece
+#pragma unroll
+      for (uint32_t half = 0; half < 2u; ++half) {
+        k.payload[c][half] =
+            *reinterpret_cast<const u32x4_t *>(payload + Layout::key_byte(token + t + 4u * half, c) + block * 16u);
+      }
+      k.scale[c] = *reinterpret_cast<const uint2 *>(scales + Layout::key_scale(token + 8u * (i >> 2), 4u * c + block));
+    }
+  }
+
+  static __device__ __forceinline__ void load_values(const uint8_t *payload, const uint8_t *scales, uint32_t token,
+                                                     uint32_t lane, Values &v) {
+    const uint32_t i = lane & 15u, g = lane >> 4;
+#pragma unroll
+    for (uint32_t u = 0; u < kUnits; ++u) {
+      v.payload[u] = *reinterpret_cast<const u32x4_t *>(payload + Layout::value_byte(token + 8u * g, 32u * u + 2u * i));
+      v.scale[u] = *reinterpret_cast<const uint2 *>(scales + Layout::value_scale(token + 8u * g, 2u * u + (i >> 3)));
+    }
+  }
+
+  // Scores of tokens 8g..8g+7 of row i: s[0..3] and s[4..7].
+  static __device__ __forceinline__ void scores(const Keys &k, const Query &q, uint32_t lane, f32x4_t (&s)[2]) {
+    const uint32_t shift = 8u * (lane & 3u);
+    s[0] = s[1] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (uint32_t c = 0; c < kChunks; ++c) {
+      const uint32_t scale[2] = {k.scale[c].x >> shift, k.scale[c].y >> shift};
+#pragma unroll
+      for (uint32_t term = 0; term < kTerms; ++term) {
+#pragma unroll
+        for (uint32_t half = 0; half < 2u; ++half) {
+          s[half] = mfma_fp4_fp8(make_a_fp4(k.payload[c][half]), q.term[c * kTerms + term], s[half], scale[half],
+                                 q.scale[c * kTerms + term]);
+        }
+      }
+    }
+  }
+
+  // Any scale byte 255 (a block of NaN) among the lane's?
+  static __device__ __forceinline__ bool has_nan(const Values &v) {
+    uint32_t found = 0u;
+#pragma unroll
+    for (uint32_t u = 0; u < kUnits; ++u) {
+      found |= ((v.scale[u].x & 0x7f7f7f7fu) + 0x01010101u) & v.scale[u].x;
+      found |= ((v.scale[u].y & 0x7f7f7f7fu) + 0x01010101u) & v.scale[u].y;
+    }
+    return (found & 0x80808080u) != 0u;
+  }
+  static __device__ __forceinline__ uint32_t without_nan(uint32_t x) {  // bytes of 255 become 127
+    return x & ~((((x & 0x7f7f7f7fu) + 0x01010101u) & x) & 0x80808080u);
+  }
+
+  // Four accumulators' operands from one 16-byte piece: values 64u + 4i + e of tokens 8g..8g+7, e = 0..3.
+  static __device__ __forceinline__ void expand(const u32x4_t &w, const uint2 &scale, u32x4_t (&out)[4]) {
+#pragma unroll
+    for (uint32_t quad = 0; quad < 2u; ++quad) {  // four tokens
+      const uint32_t bytes = quad == 0u ? scale.x : scale.y;
+      const float s0 = __uint_as_float((bytes << 23) & 0x7f800000u), s1 = __uint_as_float((bytes << 15) & 0x7f800000u);
+      const float s2 = __uint_as_float((bytes << 7) & 0x7f800000u), s3 = __uint_as_float((bytes >> 1) & 0x7f800000u);
+#pragma unroll
+      for (uint32_t pair = 0; pair < 2u; ++pair) {  // values 2 pair, 2 pair + 1
+        const uint32_t x = w[2u * pair + quad];
+        const uint32_t t0 = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x, s0, 0));
+        const uint32_t t1 = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x, s1, 1));
+        const uint32_t t2 = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x, s2, 2));
+        const uint32_t t3 = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x, s3, 3));
+        out[2u * pair][2u * quad] = __builtin_amdgcn_perm(t1, t0, 0x05040100u);
+        out[2u * pair][2u * quad + 1u] = __builtin_amdgcn_perm(t3, t2, 0x05040100u);
+        out[2u * pair + 1u][2u * quad] = __builtin_amdgcn_perm(t1, t0, 0x07060302u);
+        out[2u * pair + 1u][2u * quad + 1u] = __builtin_amdgcn_perm(t3, t2, 0x07060302u);
+      }
+    }
+  }
+};
+
+// The largest (or the sum) of the four lanes that share a row.
+__device__ __forceinline__ float row_max(float x) {
+  x = fmaxf(x, __shfl_xor(x, 16, 64));
+  return fmaxf(x, __shfl_xor(x, 32, 64));
+}
+__device__ __forceinline__ float row_sum(float x) {
+  x += __shfl_xor(x, 16, 64);
+  return x + __shfl_xor(x, 32, 64);
+}
+
+// What sums relative to the maximum `top` count for relative to `base`; sums that saw nothing (top
+// -inf) are zeros, and an infinite weight would turn them to NaN.
+__device__ __forceinline__ float part_weight(float top, float base) {
+  return top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - base);
+}
+
+// What a packed row is.
+struct PackedRow {
+  uint64_t q;       // offset of its values in q
+  uint64_t output;  // and in the output
+  uint64_t index;   // row * q_heads + head
+  int32_t position;
+  bool live;
+};
+
+__device__ __forceinline__ PackedRow packed_row(const FerruleHipKvAttentionArgs &a, const KvSequence &s, uint32_t kv_head,
+                                                uint32_t group, uint32_t r) {
+  PackedRow p;
+  const uint32_t row = r / group, head = kv_head * group + r % group;
+  p.live = row < s.rows;
+  const uint64_t at = s.row + static_cast<uint64_t>(p.live ? row : 0u);
+  p.q = at * a.q_row_stride + head * a.q_head_stride;
+  p.output = at * a.output_row_stride + head * a.output_head_stride;
+  p.index = at * a.q_heads + head;
+  p.position = s.position + static_cast<int32_t>(row);
+  return p;
+}
+
+__device__ __forceinline__ void store8(uint64_t output, uint64_t at, bool f32, const float (&x)[8]) {
+  if (f32) {
+    f32x4_t *dst = reinterpret_cast<f32x4_t *>(global_ptr<float>(output) + at);
+    dst[0] = f32x4_t{x[0], x[1], x[2], x[3]};
+    dst[1] = f32x4_t{x[4], x[5], x[6], x[7]};
+  } else {
+    u32x4_t w;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[e] = bf16_rne_bits(x[2 * e]) | (static_cast<uint32_t>(bf16_rne_bits(x[2 * e + 1])) << 16);
+    *reinterpret_cast<u32x4_t *>(global_ptr<uint16_t>(output) + at) = w;
+  }
+}
+
+template <uint32_t D>
+__global__ __launch_bounds__(256) void kv_attention_kernel(FerruleHipKvAttentionArgs a, SplitPlan plan, uint32_t row_tiles) {
+  using C = Core<D>;
+  constexpr uint32_t kPitch = 128u + 4u;  // floats of a row in LDS
+  __shared__ __align__(16) float joined[kWaves][kTileRows][kPitch];
+  __shared__ float top_of[kWaves][kTileRows], sum_of[kWaves][kTileRows];
+  const uint32_t lane = threadIdx.x & 63u;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t i = lane & 15u, g = lane >> 4;
+  const uint32_t b = blockIdx.y;
+  const uint32_t split = blockIdx.x % plan.splits;
+  const uint32_t kv_head = blockIdx.x / plan.splits % a.kv_heads;
+  const uint32_t row_tile = blockIdx.x / plan.splits / a.kv_heads;
+  const uint32_t group = a.q_heads / a.kv_heads;
   const KvSequence s = kv_sequence(a.query_indptr, a.sequence_lengths, b, a.rows, a.max_query_length);
-  if (s.bad && blockIdx.x == 0u && thread == 0u) kv_report(a.error);
-  if (index >= s.rows) return;
-  const uint32_t kv_head = head / (a.q_heads / a.kv_heads);
-  const uint64_t row = s.row + static_cast<uint64_t>(index);
-  const bool f32_query = (a.flags & FERRULE_HIP_KV_ATTENTION_QUERY_F32) != 0u;
-  for (uint32_t d = thread; d < D; d += 256u) {
-    query[d] = load_query(a.q, row * a.q_row_stride + head * a.q_head_stride + d, f32_query);
+  if (s.bad && blockIdx.x == 0u && threadIdx.x == 0u) kv_report(a.error);
+  const uint32_t first_row = row_tile * kTileRows;
+  if (first_row >= s.rows * group) return;
+  const uint32_t last_row = min(first_row + kTileRows, s.rows * group) - 1u;
+  const int32_t low = s.position + static_cast<int32_t>(first_row / group);
+  const int32_t high = s.position + static_cast<int32_t>(last_row / group);
+  const TileRange range = tile_range(a, low, high);
+  if (high >= static_cast<int32_t>(a.max_pages * a.page_tokens) && threadIdx.x == 0u) kv_report(a.error);
+  const uint32_t per_part = part_tiles(range.count, plan);
+  const uint32_t begin = split * per_part;
+  if (split != 0u && begin >= range.count) return;
+  const uint32_t end = min(begin + per_part, range.count);
+  const bool whole = per_part >= range.count;  // one part: no join
+
+  const PackedRow mine = packed_row(a, s, kv_head, group, first_row + i);
+  typename C::Query query;
+  C::load_query(a.q, mine.q, mine.live, (a.flags & FERRULE_HIP_KV_ATTENTION_QUERY_F32) != 0u, lane, query);
+  const int32_t from = a.window == 0u ? static_cast<int32_t>(0x80000000u) : mine.position - static_cast<int32_t>(a.window - 1u);
+  const int32_t sinks = a.window == 0u ? 0 : static_cast<int32_t>(a.sinks);
+  const float factor = a.softmax_scale * 1.44269504088896341f;
+
+  f32x4_t out[C::kColumns];
+#pragma unroll
+  for (uint32_t c = 0; c < C::kColumns; ++c) out[c] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+  float top = -INFINITY, base = 0.0f, sum = 0.0f;  // base = top, or 0 while the row has seen nothing
+
+  const int32_t *table = global_ptr<const int32_t>(a.page_table) + static_cast<uint64_t>(b) * a.max_pages;
+  typename C::Keys keys;
+  typename C::Values values;
+  for (uint32_t v = begin + wave; v < end; v += kWaves) {
+    const uint32_t first = range.at(v) * kTileTokens;
+    const uint32_t page = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(table[first / a.page_tokens]));
+    if (page >= a.page_count) {
+      if (lane == 0u) kv_report(a.error);
+      continue;
+    }
+    const uint64_t page_head = static_cast<uint64_t>(page) * a.kv_heads + kv_head;
+    const uint32_t token = first % a.page_tokens;
+    const uint64_t payload_at = C::Layout::payload(page_head, a.page_tokens);
+    const uint64_t scales_at = C::Layout::scales(page_head, a.page_tokens);
+    C::load_keys(global_ptr<const uint8_t>(a.k_payload) + payload_at, global_ptr<const uint8_t>(a.k_scales) + scales_at, token,
+                 lane, keys);
+    C::load_values(global_ptr<const uint8_t>(a.v_payload) + payload_at, global_ptr<const uint8_t>(a.v_scales) + scales_at, token,
+                   lane, values);
+    f32x4_t score[2];
+    C::scores(keys, query, lane, score);
+    float x[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = score[e >> 2][e & 3] * factor;
+    // tokens that every row of the tile sees need no mask
+    const int32_t start = static_cast<int32_t>(first);
+    const bool all = start + 31 <= low && (a.window == 0u || start > high - static_cast<int32_t>(a.window) ||
+                                           start + 31 < static_cast<int32_t>(a.sinks));
+    if (!all) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int32_t j = start + static_cast<int32_t>(8u * g) + e;
+        x[e] = j <= mine.position && (j >= from || j < sinks) ? x[e] : -INFINITY;
+      }
+    }
+    float most = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+    if (__any(most > top + kLazy)) {
+      most = fmaxf(top, row_max(most));
+      const float next = most == -INFINITY ? 0.0f : most;
+      const float keep = part_weight(top, next);  // 0 while nothing was seen: all sums are 0 then
+      top = most;
+      base = next;
+      sum *= keep;
+#pragma unroll
+      for (uint32_t c = 0; c < C::kColumns; ++c) out[c] *= keep;
+    }
+    float w[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w[e] = __builtin_amdgcn_exp2f(x[e] - base);
+    sum += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+    bf16x8_t weight;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) weight[e] = static_cast<__bf16>(w[e]);
+    const bool nan_blocks = __any(C::has_nan(values));
+    if (nan_blocks) {
+#pragma unroll
+      for (uint32_t u = 0; u < C::kUnits; ++u) {
+        values.scale[u].x = C::without_nan(values.scale[u].x);
+        values.scale[u].y = C::without_nan(values.scale[u].y);
+      }
+    }
+#pragma unroll
+    for (uint32_t u = 0; u < C::kUnits; ++u) {
+      u32x4_t operand[4];
+      C::expand(values.payload[u], values.scale[u], operand);
+#pragma unroll
+      for (uint32_t e = 0; e < 4u; ++e) {
+        out[4u * u + e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, operand[e]), weight, out[4u * u + e], 0, 0, 0);
+      }
+    }
+    if (nan_blocks) {  // rare: the rows that see such a token take its NaN, the others must not (0 * NaN)
+      const uint8_t *scales = global_ptr<const uint8_t>(a.v_scales) + scales_at;
+      for (uint32_t t = 0; t < kTileTokens; ++t) {
+        const int32_t j = start + static_cast<int32_t>(t);
+        const bool seen = j <= mine.position && (j >= from || j < sinks);
+#pragma unroll
+        for (uint32_t block = 0; block < D / 32u; ++block) {
+          const bool bad = scales[C::Layout::value_scale(token + t, block)] == kNanBlock;
+          // accumulator 4u + e of lane (i, g) holds values 64u + 16g + 4v + e
+          const bool hit = bad && seen && (g >> 1) == (block & 1u);
+#pragma unroll
+          for (uint32_t e = 0; e < 4u; ++e) {
+            if (hit) out[4u * (block >> 1) + e] = f32x4_t{NAN, NAN, NAN, NAN};
+          }
+        }
+      }
+    }
+  }
+
+  // join the four waves, 128 values at a time
+  sum = row_sum(sum);
+  if (g == 0u) {
+    top_of[wave][i] = top;
+    sum_of[wave][i] = sum;
   }
   __syncthreads();
-  const int32_t position = s.position + static_cast<int32_t>(index);
-  // validate() keeps the table below 2^31 tokens
-  const int32_t last = min(position, static_cast<int32_t>(a.max_pages * a.page_tokens) - 1);
-  if (last < position && thread == 0u) kv_report(a.error);
-  float top = -INFINITY, total = 0.0f;
-  constexpr uint32_t kOwn = D > 256u ? D / 256u : 1u;  // values of the row per thread
-  float sum[kOwn] = {};
-  for (int32_t begin = 0; begin <= last; begin += static_cast<int32_t>(kChunk)) {
-    if (a.window != 0u && position - (begin + static_cast<int32_t>(kChunk) - 1) >= static_cast<int32_t>(a.window) &&
-        begin >= static_cast<int32_t>(a.sinks)) {
-      continue;  // nothing of the chunk is seen
-    }
-    const int32_t j = begin + static_cast<int32_t>(thread);
-    bool seen = j <= last && (a.window == 0u || static_cast<uint32_t>(position - j) < a.window ||
-                                  static_cast<uint32_t>(j) < a.sinks);
-    int32_t page = -1;
-    if (seen) {
-      const uint32_t slot = static_cast<uint32_t>(j) / a.page_tokens;
-      page = global_ptr<const int32_t>(a.page_table)[static_cast<uint64_t>(b) * a.max_pages + slot];
-      if (static_cast<uint32_t>(page) >= a.page_count) {
-        page = -1;
-        seen = false;
-        kv_report(a.error);
-      }
-    }
-    float score = -INFINITY;
-    if (seen) {
-      const uint64_t page_head = static_cast<uint64_t>(page) * a.kv_heads + kv_head;
-      const uint32_t t = static_cast<uint32_t>(j) % a.page_tokens;
-      const uint8_t *payload = global_ptr<const uint8_t>(a.k_payload) + Layout::payload(page_head, a.page_tokens);
-      const uint8_t *scales = global_ptr<const uint8_t>(a.k_scales) + Layout::scales(page_head, a.page_tokens);
-      float dot = 0.0f;
-      for (uint32_t d = 0; d < D; d += 2u) {
-        const uint32_t byte = payload[Layout::key_byte(t, d / 128u) + (d % 128u) / 2u];
-        const uint32_t scale = scales[Layout::key_scale(t, d / 32u)];
-        dot += query[d] * block_value(byte & 15u, scale) + query[d + 1u] * block_value(byte >> 4, scale);
-      }
-      score = dot * a.softmax_scale;
-    }
-    float chunk_top = wave_max(score);  // a NaN score is caught by its weight
-    if ((thread & 63u) == 0u) reduce[thread >> 6] = chunk_top;
-    __syncthreads();
-    chunk_top = fmaxf(fmaxf(reduce[0], reduce[1]), fmaxf(reduce[2], reduce[3]));
-    const float next = fmaxf(top, chunk_top);
-    const float shift = next == -INFINITY ? 0.0f : next;
-    const float w = seen ? expf(score - shift) : 0.0f;
-    weight[thread] = w;
-    page_of[thread] = seen ? page : -1;
-    const float wave_total = wave_sum(w);
-    if ((thread & 63u) == 0u) reduce[4 + (thread >> 6)] = wave_total;
-    __syncthreads();
-    const float keep = top == -INFINITY ? 0.0f : expf(top - shift);
-    total = total * keep + ((reduce[4] + reduce[5]) + (reduce[6] + reduce[7]));
-    top = next;
-    for (uint32_t i = 0; i < kOwn; ++i) {
-      const uint32_t d = thread + i * 256u;
-      if (d >= D) break;
-      float acc = sum[i] * keep;
-      for (uint32_t u = 0; u < kChunk; ++u) {
-        if (page_of[u] < 0) continue;
-        const uint64_t page_head = static_cast<uint64_t>(page_of[u]) * a.kv_heads + kv_head;
-        const uint32_t t = static_cast<uint32_t>(begin + static_cast<int32_t>(u)) % a.page_tokens;
-        const uint32_t byte =
-            (global_ptr<const uint8_t>(a.v_payload) + Layout::payload(page_head, a.page_tokens))[Layout::value_byte(t, d / 2u)];
-        const uint32_t scale =
-            (global_ptr<const uint8_t>(a.v_scales) + Layout::scales(page_head, a.page_tokens))[Layout::value_scale(t, d / 32u)];
-        acc += weight[u] * block_value((d & 1u) ? byte >> 4 : byte & 15u, scale);
-      }
-      sum[i] = acc;
-    }
-    __syncthreads();
+  const uint32_t row_out = threadIdx.x >> 4, d_out = (threadIdx.x & 15u) * 8u;  // 16 rows x 128 values in pieces of 8
+  float row_top = -INFINITY, total = 0.0f;
+#pragma unroll
+  for (uint32_t w = 0; w < kWaves; ++w) row_top = fmaxf(row_top, top_of[w][row_out]);
+  const float row_base = row_top == -INFINITY ? 0.0f : row_top;
+#pragma unroll
+  for (uint32_t w = 0; w < kWaves; ++w) {
+    total += sum_of[w][row_out] * part_weight(top_of[w][row_out], row_base);
   }
-  for (uint32_t i = 0; i < kOwn; ++i) {
-    const uint32_t d = thread + i * 256u;
-    if (d >= D) break;
-    const float o = top == -INFINITY && total == 0.0f ? 0.0f : sum[i] / total;
-    const uint64_t at = row * a.output_row_stride + head * a.output_head_stride + d;
+  float own_top = -INFINITY;
+#pragma unroll
+  for (uint32_t w = 0; w < kWaves; ++w) own_top = fmaxf(own_top, top_of[w][i]);
+  const float keep = part_weight(top, own_top);
+  const PackedRow target = packed_row(a, s, kv_head, group, first_row + row_out);
+  const bool seen_any = total != 0.0f;  // NaN too
+  const float norm = whole ? (seen_any ? 1.0f / total : 0.0f) : 1.0f;
+#pragma unroll
+  for (uint32_t c = 0; c < (D + 127u) / 128u; ++c) {
+    if (c != 0u) __syncthreads();
+#pragma unroll
+    for (uint32_t u = 0; u < (D < 128u ? 1u : 2u); ++u) {
+#pragma unroll
+      for (uint32_t e4 = 0; e4 < 4u; ++e4) {
+        f32x4_t o;
+#pragma unroll
+        for (uint32_t e = 0; e < 4u; ++e) o[e] = out[(2u * c + u) * 4u + e][e4] * keep;
+        *reinterpret_cast<f32x4_t *>(&joined[wave][i][64u * u + 16u * g + 4u * e4]) = o;
+      }
+    }
+    __syncthreads();
+    if (target.live && d_out < D) {
+      float x[8] = {};
+#pragma unroll
+      for (uint32_t w = 0; w < kWaves; ++w) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] += joined[w][row_out][d_out + e];
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] *= norm;
+      const uint32_t d = c * 128u + d_out;
+      if (whole) {
+        store8(a.output, target.output + d, (a.flags & FERRULE_HIP_KV_ATTENTION_OUTPUT_F32) != 0u, x);
+      } else {
+        store8(a.workspace + plan.partials, (target.index * plan.splits + split) * D + d, true, x);
+      }
+    }
+  }
+  if (!whole && target.live && (threadIdx.x & 15u) == 0u) {
+    global_ptr<float2>(a.workspace + plan.statistics)[target.index * plan.splits + split] = make_float2(row_top, total);
+  }
+}
+
+// Joins the parts of every row, in order: a wave per (row, query head).
+template <uint32_t D>
+__global__ __launch_bounds__(256) void kv_attention_join_kernel(FerruleHipKvAttentionArgs a, SplitPlan plan) {
+  const uint32_t b = blockIdx.y;
+  const uint32_t lane = threadIdx.x & 63u;
+  const uint32_t item = __builtin_amdgcn_readfirstlane(blockIdx.x * kWaves + (threadIdx.x >> 6));
+  const uint32_t group = a.q_heads / a.kv_heads;
+  const KvSequence s = kv_sequence(a.query_indptr, a.sequence_lengths, b, a.rows, a.max_query_length);
+  const uint32_t kv_head = item % a.kv_heads, r = item / a.kv_heads;
+  if (r >= s.rows * group) return;
+  const uint32_t first_row = r / kTileRows * kTileRows, last_row = min(first_row + kTileRows, s.rows * group) - 1u;
+  const TileRange range = tile_range(a, s.position + static_cast<int32_t>(first_row / group),
+                                     s.position + static_cast<int32_t>(last_row / group));
+  const uint32_t per_part = part_tiles(range.count, plan);
+  if (per_part >= range.count) return;  // written already
+  const uint32_t parts = (range.count + per_part - 1u) / per_part;
+  const PackedRow row = packed_row(a, s, kv_head, group, r);
+  const float2 *statistics = global_ptr<const float2>(a.workspace + plan.statistics) + row.index * plan.splits;
+  const float *partials = global_ptr<const float>(a.workspace + plan.partials) + row.index * plan.splits * D;
+  float top = -INFINITY;
+  for (uint32_t p = 0; p < parts; ++p) top = fmaxf(top, statistics[p].x);
+  const float base = top == -INFINITY ? 0.0f : top;
+  float total = 0.0f;
+  constexpr uint32_t kPieces = (D + 511u) / 512u, kOwn = D < 512u ? D / 64u : 8u;  // values of a lane, side by side
+  static_assert(kPieces == 1u, "one piece per lane");
+  float x[kOwn] = {};
+  for (uint32_t p = 0; p < parts; ++p) {
+    const float2 part = statistics[p];
+    const float keep = part_weight(part.x, base);
+    total += part.y * keep;
+    const float *src = partials + static_cast<uint64_t>(p) * D + lane * kOwn;
+#pragma unroll
+    for (uint32_t e = 0; e < kOwn; ++e) x[e] += src[e] * keep;
+  }
+  const float norm = total != 0.0f ? 1.0f / total : 0.0f;
+#pragma unroll
+  for (uint32_t e = 0; e < kOwn; ++e) {
+    const uint64_t at = row.output + lane * kOwn + e;
     if (a.flags & FERRULE_HIP_KV_ATTENTION_OUTPUT_F32) {
-      global_ptr<float>(a.output)[at] = o;
+      global_ptr<float>(a.output)[at] = x[e] * norm;
     } else {
-      global_ptr<uint16_t>(a.output)[at] = bf16_rne_bits(o);
+      global_ptr<uint16_t>(a.output)[at] = bf16_rne_bits(x[e] * norm);
     }
   }
 }
 
-// Scalar fields and strides; pointers are looked at by validate().
+uint32_t row_bound(const FerruleHipKvAttentionArgs &a) { return a.max_query_length < a.rows ? a.max_query_length : a.rows; }
+
+uint32_t row_tiles(const FerruleHipKvAttentionArgs &a) {
+  return static_cast<uint32_t>((static_cast<uint64_t>(row_bound(a)) * (a.q_heads / a.kv_heads) + kTileRows - 1u) / kTileRows);
+}
+
+// How far a token range is cut: to four workgroups a CU, while a part keeps two steps of every wave.
+SplitPlan plan_splits(const FerruleHipKvAttentionArgs &a) {
+  SplitPlan plan = {1u, 2u * kWaves, 0u, 0u};
+  const uint64_t base = static_cast<uint64_t>(a.batch) * a.kv_heads * row_tiles(a);
+  uint64_t tokens = a.max_sequence_length;
+  if (a.window != 0u) {
+    const uint64_t seen = static_cast<uint64_t>(a.window) + a.sinks + 16u + 2u * kTileTokens;
+    tokens = tokens < seen ? tokens : seen;
+  }
+  const uint64_t most = (tokens / kTileTokens + 1u) / plan.min_tiles;
+  uint64_t splits = (1024u + base - 1u) / base;
+  if (splits > most) splits = most;
+  if (splits > 256u) splits = 256u;
+  if (splits > 1u) plan.splits = static_cast<uint32_t>(splits);
+  plan.partials = 0u;
+  plan.statistics = static_cast<uint64_t>(a.rows) * a.q_heads * plan.splits * a.head_dim * sizeof(float);
+  return plan;
+}
+
+uint64_t workspace_size(const FerruleHipKvAttentionArgs &a) {
+  const SplitPlan plan = plan_splits(a);
+  if (plan.splits == 1u) return 0u;
+  return plan.statistics + static_cast<uint64_t>(a.rows) * a.q_heads * plan.splits * sizeof(float2);
+}
+
+// Scalar fields; validate() looks at the rest.
 FerruleHipStatus validate_shape(const FerruleHipKvAttentionArgs &a) {
   if (a.q_heads == 0u || a.kv_heads == 0u || a.q_heads % a.kv_heads != 0u || a.head_dim == 0u || a.page_count == 0u ||
       a.max_pages == 0u || a.max_query_length == 0u || !kv_page_tokens_valid(a.page_tokens) ||
@@ -135,7 +590,8 @@ FerruleHipStatus validate_shape(const FerruleHipKvAttentionArgs &a) {
   }
   if (!kv_head_dim_supported(a.head_dim)) return FERRULE_HIP_UNSUPPORTED;
   if (static_cast<uint64_t>(a.max_pages) * a.page_tokens > 0x7fffffffull) return FERRULE_HIP_UNSUPPORTED;
-  if (a.batch > 65535u || static_cast<uint64_t>(a.max_query_length) * a.q_heads > 0x7fffffffull) return FERRULE_HIP_UNSUPPORTED;
+  // packed rows of a sequence and the grid's x count in 32 bits (at most 256 parts)
+  if (a.batch > 65535u || static_cast<uint64_t>(row_bound(a)) * a.q_heads > 0x7fffffull) return FERRULE_HIP_UNSUPPORTED;
   return FERRULE_HIP_SUCCESS;
 }
 
@@ -151,25 +607,32 @@ FerruleHipStatus validate(const FerruleHipKvAttentionArgs &a) {
       a.sequence_lengths == 0u || a.page_table == 0u || ((a.query_indptr | a.sequence_lengths | a.page_table | a.error) & 3u)) {
     return FERRULE_HIP_INVALID_ARGUMENT;
   }
-  const uint64_t needed = ferrule_hip_kv_attention_workspace_size(&a);
+  if (status != FERRULE_HIP_SUCCESS) return status;
+  const uint64_t needed = workspace_size(a);
   if (needed != 0u && (a.workspace == 0u || (a.workspace & 255u) != 0u || a.workspace_bytes < needed)) {
     return FERRULE_HIP_INVALID_ARGUMENT;
   }
-  return status;
+  return FERRULE_HIP_SUCCESS;
 }
 
 template <uint32_t D>
 void launch(const FerruleHipKvAttentionArgs &a, hipStream_t stream) {
-  const uint32_t rows = a.max_query_length < a.rows ? a.max_query_length : a.rows;
-  kv_attention_row_kernel<D><<<dim3(rows * a.q_heads, a.batch), 256, 0, stream>>>(a);
+  const SplitPlan plan = plan_splits(a);
+  const uint32_t tiles = row_tiles(a);
+  kv_attention_kernel<D><<<dim3(tiles * a.kv_heads * plan.splits, a.batch), 256, 0, stream>>>(a, plan, tiles);
+  if (plan.splits > 1u) {
+    const uint32_t items = row_bound(a) * a.q_heads;
+    kv_attention_join_kernel<D><<<dim3((items + kWaves - 1u) / kWaves, a.batch), 256, 0, stream>>>(a, plan);
+  }
 }
 
 }  // namespace
 }  // namespace ferrule_hip
 
 extern "C" uint64_t ferrule_hip_kv_attention_workspace_size(const FerruleHipKvAttentionArgs *args) {
-  (void)args;
-  return 0;
+  using namespace ferrule_hip;
+  if (args == nullptr || args->batch == 0u || args->rows == 0u || validate_shape(*args) != FERRULE_HIP_SUCCESS) return 0u;
+  return workspace_size(*args);
 }
 
 extern "C" int32_t ferrule_hip_kv_attention_can_implement(const FerruleHipKvAttentionArgs *args) {
