@@ -40,8 +40,10 @@ constexpr uint32_t kTileTokens = 32; // tokens of one step
 constexpr float kLazy = 8.0f;        // how far (in powers of two) scores may exceed the running maximum
 
 struct SplitPlan {
+  uint32_t tile_rows;  // packed rows of a workgroup
   uint32_t splits;     // workgroups a token range may be cut into
   uint32_t min_tiles;  // 32-token tiles that a part has at least
+  uint32_t page_shift; // log2 of page_tokens
   uint64_t partials;   // byte offsets in the workspace
   uint64_t statistics;
 };
@@ -198,14 +200,18 @@ struct Core {
     }
   }
 
+  // One 16-byte piece of a lane: values 64u + 4i .. 64u + 4i + 3 of tokens 8g..8g+7, and their scale bytes.
+  static __device__ __forceinline__ void load_piece(const uint8_t *payload, const uint8_t *scales, uint32_t token, uint32_t u,
+                                                    uint32_t lane, u32x4_t &w, uint2 &scale) {
+    const uint32_t i = lane & 15u, g = lane >> 4;
+    w = *reinterpret_cast<const u32x4_t *>(payload + Layout::value_byte(token + 8u * g, 32u * u + 2u * i));
+    scale = *reinterpret_cast<const uint2 *>(scales + Layout::value_scale(token + 8u * g, 2u * u + (i >> 3)));
+  }
+
   static __device__ __forceinline__ void load_values(const uint8_t *payload, const uint8_t *scales, uint32_t token,
                                                      uint32_t lane, Values &v) {
-    const uint32_t i = lane & 15u, g = lane >> 4;
 #pragma unroll
-    for (uint32_t u = 0; u < kUnits; ++u) {
-      v.payload[u] = *reinterpret_cast<const u32x4_t *>(payload + Layout::value_byte(token + 8u * g, 32u * u + 2u * i));
-      v.scale[u] = *reinterpret_cast<const uint2 *>(scales + Layout::value_scale(token + 8u * g, 2u * u + (i >> 3)));
-    }
+    for (uint32_t u = 0; u < kUnits; ++u) load_piece(payload, scales, token, u, lane, v.payload[u], v.scale[u]);
   }
 
   // Scores of tokens 8g..8g+7 of row i: s[0..3] and s[4..7].
@@ -227,14 +233,14 @@ struct Core {
   }
 
   // Any scale byte 255 (a block of NaN) among the lane's?
+  static __device__ __forceinline__ bool has_nan(const uint2 &scale) {
+    return ((((scale.x & 0x7f7f7f7fu) + 0x01010101u) & scale.x) | (((scale.y & 0x7f7f7f7fu) + 0x01010101u) & scale.y)) & 0x80808080u;
+  }
   static __device__ __forceinline__ bool has_nan(const Values &v) {
-    uint32_t found = 0u;
+    bool found = false;
 #pragma unroll
-    for (uint32_t u = 0; u < kUnits; ++u) {
-      found |= ((v.scale[u].x & 0x7f7f7f7fu) + 0x01010101u) & v.scale[u].x;
-      found |= ((v.scale[u].y & 0x7f7f7f7fu) + 0x01010101u) & v.scale[u].y;
-    }
-    return (found & 0x80808080u) != 0u;
+    for (uint32_t u = 0; u < kUnits; ++u) found |= has_nan(v.scale[u]);
+    return found;
   }
   static __device__ __forceinline__ uint32_t without_nan(uint32_t x) {  // bytes of 255 become 127
     return x & ~((((x & 0x7f7f7f7fu) + 0x01010101u) & x) & 0x80808080u);
@@ -279,6 +285,34 @@ __device__ __forceinline__ float part_weight(float top, float base) {
   return top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - base);
 }
 
+// Where a 32-token tile is.  An invalid one stands at page 0, so that what is loaded ahead for it is
+// in bounds; nothing of it is used.
+struct Place {
+  uint32_t first;  // position of its first token
+  uint32_t token;  // inside the page
+  uint64_t payload, scales;  // byte offsets of the page's head
+  bool valid;
+};
+
+template <uint32_t D>
+__device__ __forceinline__ Place place_of(const FerruleHipKvAttentionArgs &a, const SplitPlan &plan, const TileRange &range,
+                                          uint32_t b, uint32_t kv_head, uint32_t v, uint32_t end) {
+  Place p = {0u, 0u, 0u, 0u, false};
+  uint64_t page_head = 0u;
+  if (v < end) {
+    p.first = range.at(v) * kTileTokens;
+    const uint32_t page =
+        static_cast<uint32_t>(kv_uniform(a.page_table, static_cast<uint64_t>(b) * a.max_pages + (p.first >> plan.page_shift)));
+    p.valid = page < a.page_count;
+    if (!p.valid && (threadIdx.x & 63u) == 0u) kv_report(a.error);
+    p.token = p.first & (a.page_tokens - 1u);
+    page_head = p.valid ? static_cast<uint64_t>(page) * a.kv_heads + kv_head : 0u;
+  }
+  p.payload = (page_head << plan.page_shift) * (D / 2u);
+  p.scales = (page_head << plan.page_shift) * (D / 32u);
+  return p;
+}
+
 // What a packed row is.
 struct PackedRow {
   uint64_t q;       // offset of its values in q
@@ -314,8 +348,9 @@ __device__ __forceinline__ void store8(uint64_t output, uint64_t at, bool f32, c
   }
 }
 
+// Few rows: 16 of them, the token tiles shared out over the four waves.
 template <uint32_t D>
-__global__ __launch_bounds__(256) void kv_attention_kernel(FerruleHipKvAttentionArgs a, SplitPlan plan, uint32_t row_tiles) {
+__global__ __launch_bounds__(256, D <= 128u ? 4 : D == 256u ? 2 : 1) void kv_attention_decode_kernel(FerruleHipKvAttentionArgs a, SplitPlan plan) {
   using C = Core<D>;
   constexpr uint32_t kPitch = 128u + 4u;  // floats of a row in LDS
   __shared__ __align__(16) float joined[kWaves][kTileRows][kPitch];
@@ -355,41 +390,35 @@ __global__ __launch_bounds__(256) void kv_attention_kernel(FerruleHipKvAttention
   for (uint32_t c = 0; c < C::kColumns; ++c) out[c] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
   float top = -INFINITY, base = 0.0f, sum = 0.0f;  // base = top, or 0 while the row has seen nothing
 
-  const int32_t *table = global_ptr<const int32_t>(a.page_table) + static_cast<uint64_t>(b) * a.max_pages;
+  const uint8_t *k_payload = global_ptr<const uint8_t>(a.k_payload), *k_scales = global_ptr<const uint8_t>(a.k_scales);
+  const uint8_t *v_payload = global_ptr<const uint8_t>(a.v_payload), *v_scales = global_ptr<const uint8_t>(a.v_scales);
   typename C::Keys keys;
   typename C::Values values;
+  Place next_place = place_of<D>(a, plan, range, b, kv_head, begin + wave, end);
+  C::load_keys(k_payload + next_place.payload, k_scales + next_place.scales, next_place.token, lane, keys);
+  C::load_values(v_payload + next_place.payload, v_scales + next_place.scales, next_place.token, lane, values);
   for (uint32_t v = begin + wave; v < end; v += kWaves) {
-    const uint32_t first = range.at(v) * kTileTokens;
-    const uint32_t page = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(table[first / a.page_tokens]));
-    if (page >= a.page_count) {
-      if (lane == 0u) kv_report(a.error);
-      continue;
-    }
-    const uint64_t page_head = static_cast<uint64_t>(page) * a.kv_heads + kv_head;
-    const uint32_t token = first % a.page_tokens;
-    const uint64_t payload_at = C::Layout::payload(page_head, a.page_tokens);
-    const uint64_t scales_at = C::Layout::scales(page_head, a.page_tokens);
-    C::load_keys(global_ptr<const uint8_t>(a.k_payload) + payload_at, global_ptr<const uint8_t>(a.k_scales) + scales_at, token,
-                 lane, keys);
-    C::load_values(global_ptr<const uint8_t>(a.v_payload) + payload_at, global_ptr<const uint8_t>(a.v_scales) + scales_at, token,
-                   lane, values);
+    // keys and values are loaded one step ahead, as soon as the registers of this step's are free
+    const Place here = next_place;
+    next_place = place_of<D>(a, plan, range, b, kv_head, v + kWaves, end);
     f32x4_t score[2];
     C::scores(keys, query, lane, score);
+    C::load_keys(k_payload + next_place.payload, k_scales + next_place.scales, next_place.token, lane, keys);
     float x[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = score[e >> 2][e & 3] * factor;
+    for (int e = 0; e < 8; ++e) x[e] = score[e >> 2][e & 3];
     // tokens that every row of the tile sees need no mask
-    const int32_t start = static_cast<int32_t>(first);
-    const bool all = start + 31 <= low && (a.window == 0u || start > high - static_cast<int32_t>(a.window) ||
-                                           start + 31 < static_cast<int32_t>(a.sinks));
+    const int32_t start = static_cast<int32_t>(here.first);
+    const bool all = here.valid && start + 31 <= low && (a.window == 0u || start > high - static_cast<int32_t>(a.window) ||
+                                                         start + 31 < static_cast<int32_t>(a.sinks));
     if (!all) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const int32_t j = start + static_cast<int32_t>(8u * g) + e;
-        x[e] = j <= mine.position && (j >= from || j < sinks) ? x[e] : -INFINITY;
+        x[e] = here.valid && j <= mine.position && (j >= from || j < sinks) ? x[e] : -INFINITY;
       }
     }
-    float most = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+    float most = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7]))) * factor;
     if (__any(most > top + kLazy)) {
       most = fmaxf(top, row_max(most));
       const float next = most == -INFINITY ? 0.0f : most;
@@ -402,7 +431,7 @@ __global__ __launch_bounds__(256) void kv_attention_kernel(FerruleHipKvAttention
     }
     float w[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) w[e] = __builtin_amdgcn_exp2f(x[e] - base);
+    for (int e = 0; e < 8; ++e) w[e] = __builtin_amdgcn_exp2f(fmaf(x[e], factor, -base));
     sum += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
     bf16x8_t weight;
 #pragma unroll
@@ -424,14 +453,15 @@ __global__ __launch_bounds__(256) void kv_attention_kernel(FerruleHipKvAttention
         out[4u * u + e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, operand[e]), weight, out[4u * u + e], 0, 0, 0);
       }
     }
-    if (nan_blocks) {  // rare: the rows that see such a token take its NaN, the others must not (0 * NaN)
-      const uint8_t *scales = global_ptr<const uint8_t>(a.v_scales) + scales_at;
+    C::load_values(v_payload + next_place.payload, v_scales + next_place.scales, next_place.token, lane, values);
+    if (nan_blocks && here.valid) {  // rare: the rows that see such a token take its NaN, the others must not (0 * NaN)
+      const uint8_t *scales = v_scales + here.scales;
       for (uint32_t t = 0; t < kTileTokens; ++t) {
         const int32_t j = start + static_cast<int32_t>(t);
         const bool seen = j <= mine.position && (j >= from || j < sinks);
 #pragma unroll
         for (uint32_t block = 0; block < D / 32u; ++block) {
-          const bool bad = scales[C::Layout::value_scale(token + t, block)] == kNanBlock;
+          const bool bad = scales[C::Layout::value_scale(here.token + t, block)] == kNanBlock;
           // accumulator 4u + e of lane (i, g) holds values 64u + 16g + 4v + e
           const bool hit = bad && seen && (g >> 1) == (block & 1u);
 #pragma unroll
@@ -502,6 +532,250 @@ __global__ __launch_bounds__(256) void kv_attention_kernel(FerruleHipKvAttention
   }
 }
 
+// Many rows: a workgroup has 4 * 16 * NQ of them, 16 * NQ to a wave, and its waves go through the same
+// tokens.  Values are expanded to BF16 once per workgroup: of the 16-byte pieces of a step (D/64 per 32
+// tokens) every wave expands one (two at D = 512) into the operands of four accumulators, in LDS, one step ahead
+// of their use; keys are read by every wave, from cache, as they stand.  One barrier per step.
+template <uint32_t D, uint32_t NQ>
+__global__ __launch_bounds__(256, D <= 128u ? (NQ == 1u ? 4 : 2) : D == 256u ? 2 : 1) void kv_attention_rows_kernel(FerruleHipKvAttentionArgs a, SplitPlan plan) {
+  using C = Core<D>;
+  constexpr uint32_t kSub = D == 64u ? 4u : D == 128u ? 2u : 1u;  // 32-token tiles of a step
+  constexpr uint32_t kPieces = kSub * C::kUnits;                  // 16-byte pieces of a step
+  constexpr uint32_t kOwn = kPieces / kWaves;                     // of them, a wave's
+  static_assert(kOwn * kWaves == kPieces, "every wave expands the same number of pieces");
+  __shared__ __align__(16) u32x4_t staged[2][kPieces][4][64];     // operands [piece][accumulator][lane]
+  __shared__ uint32_t nan_of[2][kWaves];
+  const uint32_t lane = threadIdx.x & 63u;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t i = lane & 15u, g = lane >> 4;
+  const uint32_t b = blockIdx.y;
+  const uint32_t split = blockIdx.x % plan.splits;
+  const uint32_t kv_head = blockIdx.x / plan.splits % a.kv_heads;
+  const uint32_t tiles = gridDim.x / plan.splits / a.kv_heads;
+  const uint32_t row_tile = tiles - 1u - blockIdx.x / plan.splits / a.kv_heads;  // the longest causal ranges first
+  const uint32_t group = a.q_heads / a.kv_heads;
+  const KvSequence s = kv_sequence(a.query_indptr, a.sequence_lengths, b, a.rows, a.max_query_length);
+  if (s.bad && blockIdx.x == 0u && threadIdx.x == 0u) kv_report(a.error);
+  const uint32_t first_row = row_tile * plan.tile_rows;
+  const uint32_t all_rows = s.rows * group;
+  if (first_row >= all_rows) return;
+  const uint32_t last_row = min(first_row + plan.tile_rows, all_rows) - 1u;
+  const int32_t high = s.position + static_cast<int32_t>(last_row / group);
+  const TileRange range = tile_range(a, s.position + static_cast<int32_t>(first_row / group), high);
+  if (high >= static_cast<int32_t>(a.max_pages * a.page_tokens) && threadIdx.x == 0u) kv_report(a.error);
+  const uint32_t per_part = part_tiles(range.count, plan);
+  const uint32_t begin = split * per_part;
+  if (split != 0u && begin >= range.count) return;
+  const uint32_t end = min(begin + per_part, range.count);
+  const bool whole = per_part >= range.count;
+
+  // the wave's own rows
+  const uint32_t wave_row = first_row + wave * 16u * NQ;
+  const int32_t wave_low = s.position + static_cast<int32_t>(min(wave_row, last_row) / group);
+  const int32_t wave_high = s.position + static_cast<int32_t>(min(wave_row + 16u * NQ - 1u, last_row) / group);
+  typename C::Query query[NQ];
+  int32_t position[NQ], from[NQ];
+#pragma unroll
+  for (uint32_t n = 0; n < NQ; ++n) {
+    const PackedRow row = packed_row(a, s, kv_head, group, wave_row + 16u * n + i);
+    position[n] = row.position;
+    from[n] = a.window == 0u ? static_cast<int32_t>(0x80000000u) : row.position - static_cast<int32_t>(a.window - 1u);
+    C::load_query(a.q, row.q, row.live, (a.flags & FERRULE_HIP_KV_ATTENTION_QUERY_F32) != 0u, lane, query[n]);
+  }
+  const int32_t sinks = a.window == 0u ? 0 : static_cast<int32_t>(a.sinks);
+  const float factor = a.softmax_scale * 1.44269504088896341f;
+  f32x4_t out[NQ][C::kColumns];
+  float top[NQ], base[NQ], sum[NQ];
+#pragma unroll
+  for (uint32_t n = 0; n < NQ; ++n) {
+    top[n] = -INFINITY;
+    base[n] = sum[n] = 0.0f;
+#pragma unroll
+    for (uint32_t c = 0; c < C::kColumns; ++c) out[n][c] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+
+  auto place = [&](uint32_t v) { return place_of<D>(a, plan, range, b, kv_head, v, end); };
+  const uint8_t *k_payload = global_ptr<const uint8_t>(a.k_payload), *k_scales = global_ptr<const uint8_t>(a.k_scales);
+  const uint8_t *v_payload = global_ptr<const uint8_t>(a.v_payload), *v_scales = global_ptr<const uint8_t>(a.v_scales);
+  u32x4_t raw[kOwn];
+  uint2 raw_scale[kOwn];
+  auto load_pieces = [&](uint32_t v) {
+#pragma unroll
+    for (uint32_t o = 0; o < kOwn; ++o) {
+      const uint32_t piece = wave * kOwn + o;
+      const Place p = place(v + piece / C::kUnits);
+      raw[o] = u32x4_t{0u, 0u, 0u, 0u};
+      raw_scale[o] = make_uint2(0x7f7f7f7fu, 0x7f7f7f7fu);
+      if (p.valid) {
+        C::load_piece(v_payload + p.payload, v_scales + p.scales, p.token, piece % C::kUnits, lane, raw[o], raw_scale[o]);
+      }
+    }
+  };
+  auto stage_pieces = [&](uint32_t buffer) {
+    bool nan = false;
+#pragma unroll
+    for (uint32_t o = 0; o < kOwn; ++o) {
+      nan |= C::has_nan(raw_scale[o]);
+      u32x4_t operand[4];
+      C::expand(raw[o], make_uint2(C::without_nan(raw_scale[o].x), C::without_nan(raw_scale[o].y)), operand);
+#pragma unroll
+      for (uint32_t e = 0; e < 4u; ++e) staged[buffer][wave * kOwn + o][e][lane] = operand[e];
+    }
+    const uint32_t any = __any(nan) ? 1u : 0u;
+    if (lane == 0u) nan_of[buffer][wave] = any;
+  };
+
+  typename C::Keys keys[kSub];
+  uint32_t start_of[kSub], valid_of = 0u;  // of the tiles whose keys are loaded
+  auto load_tiles = [&](uint32_t v) {
+    valid_of = 0u;
+#pragma unroll
+    for (uint32_t t = 0; t < kSub; ++t) {
+      const Place p = place(v + t);
+      start_of[t] = p.first;
+      valid_of |= p.valid ? 1u << t : 0u;
+      C::load_keys(k_payload + p.payload, k_scales + p.scales, p.token, lane, keys[t]);
+    }
+  };
+  load_pieces(begin);
+  load_tiles(begin);
+  stage_pieces(0u);
+  load_pieces(begin + kSub);
+  __syncthreads();
+  uint32_t buffer = 0u;
+  for (uint32_t v = begin; v < end; v += kSub, buffer ^= 1u) {
+    f32x4_t score[NQ][kSub][2];
+    int32_t start[kSub];
+    const uint32_t valid = valid_of;
+#pragma unroll
+    for (uint32_t t = 0; t < kSub; ++t) {
+      start[t] = static_cast<int32_t>(start_of[t]);
+#pragma unroll
+      for (uint32_t n = 0; n < NQ; ++n) C::scores(keys[t], query[n], lane, score[n][t]);
+    }
+    load_tiles(v + kSub);
+    stage_pieces(buffer ^ 1u);
+    load_pieces(v + 2u * kSub);
+    bool grows = false;
+    float most[NQ];
+#pragma unroll
+    for (uint32_t n = 0; n < NQ; ++n) {
+      most[n] = -INFINITY;
+#pragma unroll
+      for (uint32_t t = 0; t < kSub; ++t) {
+        const bool there = (valid >> t) & 1u;
+        // tokens that every row of the wave sees need no mask
+        const bool all = there && start[t] + 31 <= wave_low &&
+                         (a.window == 0u || start[t] > wave_high - static_cast<int32_t>(a.window) ||
+                          start[t] + 31 < static_cast<int32_t>(a.sinks));
+        if (!all) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const int32_t j = start[t] + static_cast<int32_t>(8u * g) + e;
+            const bool seen = there && j <= position[n] && (j >= from[n] || j < sinks);
+            score[n][t][e >> 2][e & 3] = seen ? score[n][t][e >> 2][e & 3] : -INFINITY;
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) most[n] = fmaxf(most[n], score[n][t][e >> 2][e & 3]);
+      }
+      most[n] *= factor;  // more than 0
+      grows |= most[n] > top[n] + kLazy;
+    }
+    if (__any(grows)) {
+#pragma unroll
+      for (uint32_t n = 0; n < NQ; ++n) {
+        const float next_top = fmaxf(top[n], row_max(most[n]));
+        const float next = next_top == -INFINITY ? 0.0f : next_top;
+        const float keep = part_weight(top[n], next);
+        top[n] = next_top;
+        base[n] = next;
+        sum[n] *= keep;
+#pragma unroll
+        for (uint32_t c = 0; c < C::kColumns; ++c) out[n][c] *= keep;
+      }
+    }
+    bf16x8_t weight[NQ][kSub];
+#pragma unroll
+    for (uint32_t n = 0; n < NQ; ++n) {
+#pragma unroll
+      for (uint32_t t = 0; t < kSub; ++t) {
+        float w[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          w[e] = __builtin_amdgcn_exp2f(fmaf(score[n][t][e >> 2][e & 3], factor, -base[n]));
+          weight[n][t][e] = static_cast<__bf16>(w[e]);
+        }
+        sum[n] += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+      }
+    }
+#pragma unroll
+    for (uint32_t t = 0; t < kSub; ++t) {
+#pragma unroll
+      for (uint32_t u = 0; u < C::kUnits; ++u) {
+#pragma unroll
+        for (uint32_t e = 0; e < 4u; ++e) {
+          const bf16x8_t operand = __builtin_bit_cast(bf16x8_t, staged[buffer][t * C::kUnits + u][e][lane]);
+#pragma unroll
+          for (uint32_t n = 0; n < NQ; ++n) {
+            out[n][4u * u + e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(operand, weight[n][t], out[n][4u * u + e], 0, 0, 0);
+          }
+        }
+      }
+    }
+    if ((nan_of[buffer][0] | nan_of[buffer][1] | nan_of[buffer][2] | nan_of[buffer][3]) != 0u) {
+      // rare: the rows that see such a token take its NaN, the others must not (0 * NaN)
+      for (uint32_t t = 0; t < kSub; ++t) {
+        const Place p = place(v + t);
+        if (!p.valid) continue;
+        const uint8_t *scales = v_scales + p.scales;
+        for (uint32_t k = 0; k < kTileTokens; ++k) {
+          const int32_t j = static_cast<int32_t>(p.first + k);
+#pragma unroll
+          for (uint32_t block = 0; block < D / 32u; ++block) {
+            const bool bad = scales[C::Layout::value_scale(p.token + k, block)] == kNanBlock;
+#pragma unroll
+            for (uint32_t n = 0; n < NQ; ++n) {
+              const bool hit = bad && j <= position[n] && (j >= from[n] || j < sinks) && (g >> 1) == (block & 1u);
+#pragma unroll
+              for (uint32_t e = 0; e < 4u; ++e) {
+                if (hit) out[n][4u * (block >> 1) + e] = f32x4_t{NAN, NAN, NAN, NAN};
+              }
+            }
+          }
+        }
+      }
+    }
+    __syncthreads();
+  }
+
+#pragma unroll
+  for (uint32_t n = 0; n < NQ; ++n) {
+    const PackedRow row = packed_row(a, s, kv_head, group, wave_row + 16u * n + i);
+    const float total = row_sum(sum[n]);
+    if (!row.live) continue;
+    const float norm = whole ? (total != 0.0f ? 1.0f / total : 0.0f) : 1.0f;
+#pragma unroll
+    for (uint32_t u = 0; u < C::kUnits; ++u) {
+#pragma unroll
+      for (uint32_t half = 0; half < 2u; ++half) {  // values 64u + 16g + 8 half ..
+        float x[8];
+#pragma unroll
+        for (uint32_t e = 0; e < 8u; ++e) x[e] = out[n][4u * u + (e & 3u)][2u * half + (e >> 2)] * norm;
+        const uint32_t d = 64u * u + 16u * g + 8u * half;
+        if (whole) {
+          store8(a.output, row.output + d, (a.flags & FERRULE_HIP_KV_ATTENTION_OUTPUT_F32) != 0u, x);
+        } else {
+          store8(a.workspace + plan.partials, (row.index * plan.splits + split) * D + d, true, x);
+        }
+      }
+    }
+    if (!whole && g == 0u) {
+      global_ptr<float2>(a.workspace + plan.statistics)[row.index * plan.splits + split] = make_float2(top[n], total);
+    }
+  }
+}
+
 // Joins the parts of every row, in order: a wave per (row, query head).
 template <uint32_t D>
 __global__ __launch_bounds__(256) void kv_attention_join_kernel(FerruleHipKvAttentionArgs a, SplitPlan plan) {
@@ -512,7 +786,8 @@ __global__ __launch_bounds__(256) void kv_attention_join_kernel(FerruleHipKvAtte
   const KvSequence s = kv_sequence(a.query_indptr, a.sequence_lengths, b, a.rows, a.max_query_length);
   const uint32_t kv_head = item % a.kv_heads, r = item / a.kv_heads;
   if (r >= s.rows * group) return;
-  const uint32_t first_row = r / kTileRows * kTileRows, last_row = min(first_row + kTileRows, s.rows * group) - 1u;
+  const uint32_t first_row = r / plan.tile_rows * plan.tile_rows;
+  const uint32_t last_row = min(first_row + plan.tile_rows, s.rows * group) - 1u;
   const TileRange range = tile_range(a, s.position + static_cast<int32_t>(first_row / group),
                                      s.position + static_cast<int32_t>(last_row / group));
   const uint32_t per_part = part_tiles(range.count, plan);
@@ -550,21 +825,31 @@ __global__ __launch_bounds__(256) void kv_attention_join_kernel(FerruleHipKvAtte
 
 uint32_t row_bound(const FerruleHipKvAttentionArgs &a) { return a.max_query_length < a.rows ? a.max_query_length : a.rows; }
 
-uint32_t row_tiles(const FerruleHipKvAttentionArgs &a) {
-  return static_cast<uint32_t>((static_cast<uint64_t>(row_bound(a)) * (a.q_heads / a.kv_heads) + kTileRows - 1u) / kTileRows);
+uint64_t packed_rows(const FerruleHipKvAttentionArgs &a) { return static_cast<uint64_t>(row_bound(a)) * (a.q_heads / a.kv_heads); }
+
+uint32_t row_tiles(const FerruleHipKvAttentionArgs &a, uint32_t tile_rows) {
+  return static_cast<uint32_t>((packed_rows(a) + tile_rows - 1u) / tile_rows);
+}
+
+// Rows of a wave of kv_attention_rows_kernel, in sixteens; 0: kv_attention_decode_kernel.
+uint32_t wave_tiles(const FerruleHipKvAttentionArgs &a) {
+  if (packed_rows(a) <= 32u) return 0u;
+  return a.head_dim > 128u || packed_rows(a) <= 64u ? 1u : 2u;
 }
 
 // How far a token range is cut: to four workgroups a CU, while a part keeps two steps of every wave.
 SplitPlan plan_splits(const FerruleHipKvAttentionArgs &a) {
-  SplitPlan plan = {1u, 2u * kWaves, 0u, 0u};
-  const uint64_t base = static_cast<uint64_t>(a.batch) * a.kv_heads * row_tiles(a);
+  const uint32_t tiles = wave_tiles(a);
+  SplitPlan plan = {tiles == 0u ? kTileRows : 64u * tiles, 1u, tiles == 0u ? 2u * kWaves : 4u,
+                    static_cast<uint32_t>(__builtin_ctz(a.page_tokens)), 0u, 0u};
+  const uint64_t base = static_cast<uint64_t>(a.batch) * a.kv_heads * row_tiles(a, plan.tile_rows);
   uint64_t tokens = a.max_sequence_length;
   if (a.window != 0u) {
-    const uint64_t seen = static_cast<uint64_t>(a.window) + a.sinks + 16u + 2u * kTileTokens;
+    const uint64_t seen = static_cast<uint64_t>(a.window) + a.sinks + plan.tile_rows + 2u * kTileTokens;
     tokens = tokens < seen ? tokens : seen;
   }
   const uint64_t most = (tokens / kTileTokens + 1u) / plan.min_tiles;
-  uint64_t splits = (1024u + base - 1u) / base;
+  uint64_t splits = ((tiles == 0u ? 1024u : 512u) + base - 1u) / base;
   if (splits > most) splits = most;
   if (splits > 256u) splits = 256u;
   if (splits > 1u) plan.splits = static_cast<uint32_t>(splits);
@@ -618,8 +903,14 @@ FerruleHipStatus validate(const FerruleHipKvAttentionArgs &a) {
 template <uint32_t D>
 void launch(const FerruleHipKvAttentionArgs &a, hipStream_t stream) {
   const SplitPlan plan = plan_splits(a);
-  const uint32_t tiles = row_tiles(a);
-  kv_attention_kernel<D><<<dim3(tiles * a.kv_heads * plan.splits, a.batch), 256, 0, stream>>>(a, plan, tiles);
+  const dim3 grid(row_tiles(a, plan.tile_rows) * a.kv_heads * plan.splits, a.batch);
+  switch (wave_tiles(a)) {
+    case 0: kv_attention_decode_kernel<D><<<grid, 256, 0, stream>>>(a, plan); break;
+    case 1: kv_attention_rows_kernel<D, 1><<<grid, 256, 0, stream>>>(a, plan); break;
+    default:
+      if constexpr (D <= 128u) kv_attention_rows_kernel<D, 2><<<grid, 256, 0, stream>>>(a, plan);
+      break;
+  }
   if (plan.splits > 1u) {
     const uint32_t items = row_bound(a) * a.q_heads;
     kv_attention_join_kernel<D><<<dim3((items + kWaves - 1u) / kWaves, a.batch), 256, 0, stream>>>(a, plan);

@@ -20,11 +20,19 @@ struct KvSequence {
   bool bad;          // something was clamped
 };
 
+// Metadata that nothing writes while the kernel runs, at a wave-uniform index: through the constant
+// address space it is a scalar load, which is counted apart from the vector loads in flight - as a
+// vector load its wait would drain them.
+__device__ __forceinline__ int32_t kv_uniform(uint64_t address, uint64_t index) {
+  typedef __attribute__((address_space(4))) const int32_t constant_t;
+  return reinterpret_cast<constant_t *>(static_cast<uintptr_t>(address))[index];
+}
+
 __device__ __forceinline__ KvSequence kv_sequence(uint64_t query_indptr, uint64_t sequence_lengths, uint32_t b,
                                                   uint32_t rows, uint32_t max_query_length) {
-  const int32_t first = global_ptr<const int32_t>(query_indptr)[b];
-  const int32_t last = global_ptr<const int32_t>(query_indptr)[b + 1u];
-  const int32_t length = global_ptr<const int32_t>(sequence_lengths)[b];
+  const int32_t first = kv_uniform(query_indptr, b);
+  const int32_t last = kv_uniform(query_indptr, b + 1u);
+  const int32_t length = kv_uniform(sequence_lengths, b);
   KvSequence s;
   const int32_t row = min(max(first, 0), static_cast<int32_t>(rows));
   const int32_t end = min(max(last, row), static_cast<int32_t>(rows));

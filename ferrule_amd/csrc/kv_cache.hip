@@ -42,7 +42,7 @@ __device__ __forceinline__ bool kv_tile(const FerruleHipKvCacheArgs &a, KvTile &
   tile.page_token = 0;
   const uint32_t slot = static_cast<uint32_t>(tile.first) / a.page_tokens;
   if (tile.first >= 0 && slot < a.max_pages) {
-    const int32_t page = global_ptr<const int32_t>(a.page_table)[static_cast<uint64_t>(b) * a.max_pages + slot];
+    const int32_t page = kv_uniform(a.page_table, static_cast<uint64_t>(b) * a.max_pages + slot);
     tile.page_token = static_cast<uint32_t>(tile.first) % a.page_tokens;
     tile.page_valid = static_cast<uint32_t>(page) < a.page_count;
     if (tile.page_valid) tile.page_head = static_cast<uint64_t>(page) * a.kv_heads + tile.head;

@@ -128,6 +128,8 @@ class HipKvCache:
                 raise ValueError(f"HIP KV cache array must be contiguous uint8 {shape}, got {t.dtype} {tuple(t.shape)}")
         if self.page_count < 1:
             raise ValueError("HIP KV cache needs at least one page")
+        self.device = k_payload.device
+        self.pointers = tuple(_ptr(t) for t in arrays)     # the arrays stay: this object holds them
 
 
 class HipKvBatch:
@@ -154,6 +156,8 @@ class HipKvBatch:
         if self.rows < 0 or self.max_query_length < min(self.rows, 1) or \
                 (self.max_sequence_length is not None and self.max_sequence_length < 0):
             raise ValueError("HIP KV batch needs rows >= 0 and bounds of at least one row")
+        self.device = query_indptr.device
+        self.pointers = (_ptr(query_indptr), _ptr(sequence_lengths), _ptr(page_table))
 
 
 def validate_dsv4_router_token_ids(token_ids, hash_rows: int) -> list[int]:
@@ -1092,48 +1096,56 @@ class HipArtifactOperatorContext:
                   for shape in kv_cache_shapes(page_count, page_tokens, kv_heads, head_dim))
         return HipKvCache(page_tokens, kv_heads, head_dim, *arrays)
 
-    def _check_kv(self, cache: HipKvCache, batch: HipKvBatch, error: torch.Tensor | None, *tensors) -> None:
-        device = cache.k_payload.device
+    # A decode step's operators take a few microseconds on the GPU, so their host side is kept short: argument
+    # blocks are filled by position, and the raw stream handle is asked for without a stream object.
+    def _check_kv(self, cache: HipKvCache, batch: HipKvBatch, error: torch.Tensor | None) -> torch.device:
+        device = cache.device
         if device.type != "cuda" or device.index != (torch.cuda.current_device() if self.device.index is None
                                                      else self.device.index):
             raise ValueError(f"HIP KV operators run on {self.device}, the cache is on {device}")
-        if batch.page_table.device != device or any(t.device != device for t in tensors):
+        if batch.device != device:
             raise ValueError(f"HIP KV operators need every tensor on the cache's device {device}")
         if error is not None and (error.dtype != torch.int32 or error.numel() != 1 or error.device != device):
             raise ValueError("HIP KV error flag must be one int32 on the device")
-
-    def _kv_launch(self, what: str, can_implement, launch, args) -> None:
-        """``_two_phase`` with this context's device current, which a launch on its stream needs."""
-        if self.device.index is None or torch.cuda.current_device() == self.device.index:
-            self._two_phase(what, can_implement, launch, args)
-        else:
-            with torch.cuda.device(self.device):
-                self._two_phase(what, can_implement, launch, args)
+        return device
 
     @staticmethod
-    def _check_kv_rows(what: str, t: torch.Tensor, rows: int, heads: int, head_dim: int) -> None:
-        if t.dtype not in (torch.bfloat16, torch.float32) or tuple(t.shape) != (rows, heads, head_dim) or \
-                (t.stride(2) != 1 and t.numel() > 0):
-            raise ValueError(f"HIP KV {what} must be bf16 or f32 {(rows, heads, head_dim)} with consecutive values, "
-                             f"got {t.dtype} {tuple(t.shape)} strides {t.stride()}")
+    def _check_kv_rows(what: str, t: torch.Tensor, shape: tuple[int, int, int], device: torch.device) -> tuple[int, ...]:
+        """The row tensor's strides, once it is what the operators take."""
+        strides = t.stride()
+        if t.dtype not in (torch.bfloat16, torch.float32) or t.shape != shape or strides[2] != 1:
+            raise ValueError(f"HIP KV {what} must be bf16 or f32 {shape} with consecutive values, "
+                             f"got {t.dtype} {tuple(t.shape)} strides {strides}")
+        if t.device != device:
+            raise ValueError(f"HIP KV {what} must be on the cache's device {device}, not on {t.device}")
+        return strides
+
+    def _kv_launch(self, what: str, can_implement, launch, args, device: torch.device) -> None:
+        """``_two_phase`` with the cache's device current, which a launch on its stream needs."""
+        index = device.index
+        if torch.cuda.current_device() != index:
+            with torch.cuda.device(index):
+                return self._kv_launch(what, can_implement, launch, args, device)
+        args.stream = torch._C._cuda_getCurrentRawStream(index) if self._stream is None else self._stream.cuda_stream
+        status = can_implement(C.byref(args))
+        if status != abi.SUCCESS:
+            raise ProviderError(f"validate {what}", status)
+        status = launch(C.byref(args))
+        if status != abi.SUCCESS:
+            raise ProviderError(f"launch {what}", status)
+        self.kernel_launches += 1
 
     def _kv_cache_args(self, cache: HipKvCache, batch: HipKvBatch, k: torch.Tensor, v: torch.Tensor,
-                       error: torch.Tensor | None) -> abi.KvCacheArgs:
-        self._check_kv(cache, batch, error, k, v)
-        self._check_kv_rows("keys", k, batch.rows, cache.kv_heads, cache.head_dim)
-        self._check_kv_rows("values", v, batch.rows, cache.kv_heads, cache.head_dim)
+                       error: torch.Tensor | None, device: torch.device) -> abi.KvCacheArgs:
+        shape = (batch.rows, cache.kv_heads, cache.head_dim)
+        ks = self._check_kv_rows("keys", k, shape, device)
+        vs = self._check_kv_rows("values", v, shape, device)
         if k.dtype != v.dtype:
             raise ValueError("HIP KV keys and values share one type")
         return abi.KvCacheArgs(
-            batch=batch.batch, rows=batch.rows, kv_heads=cache.kv_heads, head_dim=cache.head_dim,
-            page_tokens=cache.page_tokens, page_count=cache.page_count, max_pages=batch.max_pages,
-            max_query_length=batch.max_query_length,
-            value_type=abi.KV_BF16 if k.dtype == torch.bfloat16 else abi.KV_F32,
-            key_row_stride=k.stride(0), key_head_stride=k.stride(1), value_row_stride=v.stride(0),
-            value_head_stride=v.stride(1), keys=_ptr(k), values=_ptr(v), k_payload=_ptr(cache.k_payload),
-            k_scales=_ptr(cache.k_scales), v_payload=_ptr(cache.v_payload), v_scales=_ptr(cache.v_scales),
-            query_indptr=_ptr(batch.query_indptr), sequence_lengths=_ptr(batch.sequence_lengths),
-            page_table=_ptr(batch.page_table), error=_ptr(error))
+            batch.batch, batch.rows, cache.kv_heads, cache.head_dim, cache.page_tokens, cache.page_count, batch.max_pages,
+            batch.max_query_length, abi.KV_BF16 if k.dtype == torch.bfloat16 else abi.KV_F32, 0, ks[0], ks[1], vs[0], vs[1],
+            _ptr(k), _ptr(v), *cache.pointers, *batch.pointers, _ptr(error))
 
     def kv_cache_append(self, cache: HipKvCache, batch: HipKvBatch, k: torch.Tensor, v: torch.Tensor,
                         error: torch.Tensor | None = None) -> None:
@@ -1142,43 +1154,47 @@ class HipArtifactOperatorContext:
         ``pack_fp4_rows_from_f32`` (its default rounding), except that a block holding an infinity or
         a NaN is written as a block of NaN.  ``error`` (int32 [1], cleared by the caller) becomes 1 when
         a row has no valid place; such rows are dropped.  The pages written belong to one sequence each."""
+        device = self._check_kv(cache, batch, error)
         if batch.rows == 0 or batch.batch == 0:
             return
         self._kv_launch("KV cache append", self.lib.ferrule_hip_kv_cache_append_can_implement,
-                        self.lib.ferrule_hip_kv_cache_append_launch, self._kv_cache_args(cache, batch, k, v, error))
+                        self.lib.ferrule_hip_kv_cache_append_launch,
+                        self._kv_cache_args(cache, batch, k, v, error, device), device)
 
     def kv_cache_read_into(self, cache: HipKvCache, batch: HipKvBatch, k: torch.Tensor, v: torch.Tensor,
                            error: torch.Tensor | None = None) -> None:
         """The cache's values at the batch's positions into BF16 or f32 [rows, kv_heads, head_dim], exact
         in either type.  To read positions s..e of a sequence give it e - s rows and length e.  A row
         without a valid place reads as zeros and sets ``error``."""
+        device = self._check_kv(cache, batch, error)
         if batch.rows == 0 or batch.batch == 0:
             return
         self._kv_launch("KV cache read", self.lib.ferrule_hip_kv_cache_read_can_implement,
-                        self.lib.ferrule_hip_kv_cache_read_launch, self._kv_cache_args(cache, batch, k, v, error))
+                        self.lib.ferrule_hip_kv_cache_read_launch,
+                        self._kv_cache_args(cache, batch, k, v, error, device), device)
 
-    def _kv_attention_args(self, cache: HipKvCache, batch: HipKvBatch, q_heads: int, window: int,
-                           sinks: int) -> abi.KvAttentionArgs:
+    def _kv_attention_args(self, cache: HipKvCache, batch: HipKvBatch, q_heads: int, window: int, sinks: int,
+                           flags: int = 0, softmax_scale: float = 1.0, *tensors) -> abi.KvAttentionArgs:
         if q_heads < 1 or q_heads % cache.kv_heads:
             raise ValueError(f"HIP KV attention needs a multiple of {cache.kv_heads} query heads, got {q_heads}")
         if window < 0 or sinks < 0:
             raise ValueError("HIP KV attention window and sinks must not be negative")
-        limit = batch.max_pages * cache.page_tokens
+        longest = batch.max_sequence_length
+        if longest is None:
+            longest = min(batch.max_pages * cache.page_tokens, 0x7fffffff)
         return abi.KvAttentionArgs(
-            batch=batch.batch, rows=batch.rows, q_heads=q_heads, kv_heads=cache.kv_heads, head_dim=cache.head_dim,
-            page_tokens=cache.page_tokens, page_count=cache.page_count, max_pages=batch.max_pages,
-            max_query_length=batch.max_query_length,
-            max_sequence_length=min(limit, 0x7fffffff) if batch.max_sequence_length is None else batch.max_sequence_length,
-            window=window, sinks=sinks, softmax_scale=1.0)
+            batch.batch, batch.rows, q_heads, cache.kv_heads, cache.head_dim, cache.page_tokens, cache.page_count,
+            batch.max_pages, batch.max_query_length, longest, window, sinks, flags, softmax_scale, *tensors)
 
     def kv_cache_attention_workspace(self, cache: HipKvCache, batch: HipKvBatch, q_heads: int, window: int = 0,
                                      sinks: int = 0) -> torch.Tensor:
         """The scratch that ``kv_cache_attention_into`` needs for batches of this shape (uint8, possibly
         empty).  It belongs to one call at a time: keep one per stream, and one per captured graph that
         may replay while another runs."""
+        device = self._check_kv(cache, batch, None)
         args = self._kv_attention_args(cache, batch, q_heads, window, sinks)
         size = self.lib.ferrule_hip_kv_attention_workspace_size(C.byref(args))
-        return torch.empty(size, dtype=torch.uint8, device=self.device)
+        return torch.empty(size, dtype=torch.uint8, device=device)
 
     def kv_cache_attention_into(self, cache: HipKvCache, batch: HipKvBatch, q: torch.Tensor, out: torch.Tensor,
                                 softmax_scale: float, window: int = 0, sinks: int = 0,
@@ -1189,31 +1205,26 @@ class HipArtifactOperatorContext:
         reads key/value head h // (q_heads // kv_heads), and the row at position p sees position j when
         ``j <= p and (window == 0 or p - j < window or j < sinks)``.  A row that sees nothing writes
         zeros.  Without ``workspace`` one is taken from torch's allocator for the call."""
-        self._check_kv(cache, batch, error, q, out)
+        device = self._check_kv(cache, batch, error)
         q_heads = q.shape[1] if q.dim() == 3 else 0
-        self._check_kv_rows("queries", q, batch.rows, q_heads, cache.head_dim)
-        self._check_kv_rows("output", out, batch.rows, q_heads, cache.head_dim)
+        shape = (batch.rows, q_heads, cache.head_dim)
+        qs = self._check_kv_rows("queries", q, shape, device)
+        os = self._check_kv_rows("output", out, shape, device)
+        flags = (abi.KV_ATTENTION_QUERY_F32 if q.dtype == torch.float32 else 0) | \
+            (abi.KV_ATTENTION_OUTPUT_F32 if out.dtype == torch.float32 else 0)
+        a = self._kv_attention_args(cache, batch, q_heads, window, sinks, flags, softmax_scale, qs[0], qs[1], os[0], os[1],
+                                    _ptr(q), _ptr(out), *cache.pointers, *batch.pointers, _ptr(error))
         if batch.rows == 0 or batch.batch == 0:
             return out
-        a = self._kv_attention_args(cache, batch, q_heads, window, sinks)
-        a.flags = (abi.KV_ATTENTION_QUERY_F32 if q.dtype == torch.float32 else 0) | \
-            (abi.KV_ATTENTION_OUTPUT_F32 if out.dtype == torch.float32 else 0)
-        a.softmax_scale = softmax_scale
-        a.q_row_stride, a.q_head_stride, a.output_row_stride, a.output_head_stride = *q.stride()[:2], *out.stride()[:2]
-        a.q, a.output = _ptr(q), _ptr(out)
-        a.k_payload, a.k_scales = _ptr(cache.k_payload), _ptr(cache.k_scales)
-        a.v_payload, a.v_scales = _ptr(cache.v_payload), _ptr(cache.v_scales)
-        a.query_indptr, a.sequence_lengths = _ptr(batch.query_indptr), _ptr(batch.sequence_lengths)
-        a.page_table, a.error = _ptr(batch.page_table), _ptr(error)
         if workspace is None:
             size = self.lib.ferrule_hip_kv_attention_workspace_size(C.byref(a))
             with torch.cuda.stream(self.stream):       # the block is reused in this stream's order
-                workspace = torch.empty(size, dtype=torch.uint8, device=self.device)
-        elif workspace.dtype != torch.uint8 or workspace.device != self.device or not workspace.is_contiguous():
+                workspace = torch.empty(size, dtype=torch.uint8, device=device)
+        elif workspace.dtype != torch.uint8 or workspace.device != device or not workspace.is_contiguous():
             raise ValueError("HIP KV attention workspace must be contiguous uint8 on the device")
         a.workspace, a.workspace_bytes = _ptr(workspace), workspace.numel()
         self._kv_launch("KV attention", self.lib.ferrule_hip_kv_attention_can_implement,
-                        self.lib.ferrule_hip_kv_attention_launch, a)
+                        self.lib.ferrule_hip_kv_attention_launch, a, device)
         return out
 
     # -- routed MoE ---------------------------------------------------------------
