@@ -40,11 +40,11 @@ constexpr uint32_t kTileTokens = 32; // tokens of one step
 constexpr float kLazy = 8.0f;        // how far (in powers of two) scores may exceed the running maximum
 
 struct SplitPlan {
-  uint32_t tile_rows;  // packed rows of a workgroup
-  uint32_t splits;     // workgroups a token range may be cut into
-  uint32_t min_tiles;  // 32-token tiles that a part has at least
-  uint32_t page_shift; // log2 of page_tokens
-  uint64_t partials;   // byte offsets in the workspace
+  uint32_t tile_rows;   // packed rows of a workgroup
+  uint32_t page_shift;  // log2 of page_tokens
+  uint32_t part_tiles;  // 32-token tiles of a part, a multiple of what a workgroup takes at a time
+  uint32_t splits;      // parts at most; the last takes what is left
+  uint64_t partials;    // byte offsets in the workspace
   uint64_t statistics;
 };
 
@@ -71,9 +71,9 @@ __device__ __forceinline__ TileRange tile_range(const FerruleHipKvAttentionArgs 
   return t;
 }
 
-// Tiles per part: every part but the last has as many.
-__device__ __forceinline__ uint32_t part_tiles(uint32_t count, const SplitPlan &plan) {
-  return max((count + plan.splits - 1u) / plan.splits, plan.min_tiles);
+// How many parts a range has.
+__device__ __forceinline__ uint32_t parts_of(uint32_t count, const SplitPlan &plan) {
+  return max(1u, min((count + plan.part_tiles - 1u) / plan.part_tiles, plan.splits));
 }
 
 template <uint32_t D>
@@ -194,7 +194,7 @@ struct Core {
 #pragma unroll
       for (uint32_t half = 0; half < 2u; ++half) {
         k.payload[c][half] =
-            *reinterpret_cast<const u32x4_t *>(payload + Layout::key_byte(token + t + 4u * half, c) + block * 16u);
+            __builtin_nontemporal_load(reinterpret_cast<const u32x4_t *>(payload + Layout::key_byte(token + t + 4u * half, c) + block * 16u));
       }
       k.scale[c] = *reinterpret_cast<const uint2 *>(scales + Layout::key_scale(token + 8u * (i >> 2), 4u * c + block));
     }
@@ -204,7 +204,7 @@ struct Core {
   static __device__ __forceinline__ void load_piece(const uint8_t *payload, const uint8_t *scales, uint32_t token, uint32_t u,
                                                     uint32_t lane, u32x4_t &w, uint2 &scale) {
     const uint32_t i = lane & 15u, g = lane >> 4;
-    w = *reinterpret_cast<const u32x4_t *>(payload + Layout::value_byte(token + 8u * g, 32u * u + 2u * i));
+    w = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t *>(payload + Layout::value_byte(token + 8u * g, 32u * u + 2u * i)));
     scale = *reinterpret_cast<const uint2 *>(scales + Layout::value_scale(token + 8u * g, 2u * u + (i >> 3)));
   }
 
@@ -372,11 +372,11 @@ __global__ __launch_bounds__(256, D <= 128u ? 4 : D == 256u ? 2 : 1) void kv_att
   const int32_t high = s.position + static_cast<int32_t>(last_row / group);
   const TileRange range = tile_range(a, low, high);
   if (high >= static_cast<int32_t>(a.max_pages * a.page_tokens) && threadIdx.x == 0u) kv_report(a.error);
-  const uint32_t per_part = part_tiles(range.count, plan);
-  const uint32_t begin = split * per_part;
-  if (split != 0u && begin >= range.count) return;
-  const uint32_t end = min(begin + per_part, range.count);
-  const bool whole = per_part >= range.count;  // one part: no join
+  const uint32_t parts = parts_of(range.count, plan);
+  if (split >= parts) return;
+  const uint32_t begin = split * plan.part_tiles;
+  const uint32_t end = split + 1u == parts ? range.count : begin + plan.part_tiles;
+  const bool whole = parts == 1u;  // no join
 
   const PackedRow mine = packed_row(a, s, kv_head, group, first_row + i);
   typename C::Query query;
@@ -398,7 +398,8 @@ __global__ __launch_bounds__(256, D <= 128u ? 4 : D == 256u ? 2 : 1) void kv_att
   C::load_keys(k_payload + next_place.payload, k_scales + next_place.scales, next_place.token, lane, keys);
   C::load_values(v_payload + next_place.payload, v_scales + next_place.scales, next_place.token, lane, values);
   for (uint32_t v = begin + wave; v < end; v += kWaves) {
-    // keys and values are loaded one step ahead, as soon as the registers of this step's are free
+    // keys and values are loaded one step ahead, as soon as the registers of this step's are free; two or
+    // three steps ahead at 3 or 2 waves per SIMD took as long (64 x 8192 tokens, 8 heads: 112, 110, 122 us)
     const Place here = next_place;
     next_place = place_of<D>(a, plan, range, b, kv_head, v + kWaves, end);
     f32x4_t score[2];
@@ -563,11 +564,11 @@ __global__ __launch_bounds__(256, D <= 128u ? (NQ == 1u ? 4 : 2) : D == 256u ? 2
   const int32_t high = s.position + static_cast<int32_t>(last_row / group);
   const TileRange range = tile_range(a, s.position + static_cast<int32_t>(first_row / group), high);
   if (high >= static_cast<int32_t>(a.max_pages * a.page_tokens) && threadIdx.x == 0u) kv_report(a.error);
-  const uint32_t per_part = part_tiles(range.count, plan);
-  const uint32_t begin = split * per_part;
-  if (split != 0u && begin >= range.count) return;
-  const uint32_t end = min(begin + per_part, range.count);
-  const bool whole = per_part >= range.count;
+  const uint32_t parts = parts_of(range.count, plan);
+  if (split >= parts) return;
+  const uint32_t begin = split * plan.part_tiles;
+  const uint32_t end = split + 1u == parts ? range.count : begin + plan.part_tiles;
+  const bool whole = parts == 1u;
 
   // the wave's own rows
   const uint32_t wave_row = first_row + wave * 16u * NQ;
@@ -776,51 +777,118 @@ __global__ __launch_bounds__(256, D <= 128u ? (NQ == 1u ? 4 : 2) : D == 256u ? 2
   }
 }
 
-// Joins the parts of every row, in order: a wave per (row, query head).
+// The row and the number of parts of the threads that join one (row, query head); 0: written already.
+struct Joined {
+  PackedRow row;
+  uint32_t parts;
+};
+__device__ __forceinline__ Joined joined_row(const FerruleHipKvAttentionArgs &a, const SplitPlan &plan, const KvSequence &s,
+                                             uint32_t item) {
+  const uint32_t group = a.q_heads / a.kv_heads;
+  const uint32_t kv_head = item % a.kv_heads, r = item / a.kv_heads;
+  Joined j;
+  j.parts = 0u;
+  if (r < s.rows * group) {
+    const uint32_t first_row = r / plan.tile_rows * plan.tile_rows;
+    const uint32_t last_row = min(first_row + plan.tile_rows, s.rows * group) - 1u;
+    j.parts = parts_of(tile_range(a, s.position + static_cast<int32_t>(first_row / group),
+                                  s.position + static_cast<int32_t>(last_row / group)).count, plan);
+    if (j.parts == 1u) j.parts = 0u;
+  }
+  j.row = packed_row(a, s, kv_head, group, j.parts != 0u ? r : 0u);
+  return j;
+}
+
+__device__ __forceinline__ void store4(uint64_t output, uint64_t at, bool f32, const f32x4_t &x) {
+  if (f32) {
+    *reinterpret_cast<f32x4_t *>(global_ptr<float>(output) + at) = x;
+  } else {
+    *reinterpret_cast<uint2 *>(global_ptr<uint16_t>(output) + at) =
+        make_uint2(bf16_rne_bits(x[0]) | (static_cast<uint32_t>(bf16_rne_bits(x[1])) << 16),
+                   bf16_rne_bits(x[2]) | (static_cast<uint32_t>(bf16_rne_bits(x[3])) << 16));
+  }
+}
+
+// Joins the parts of every row, in their order.  Up to kFewParts parts: a thread has four values of a
+// row and everything it reads is asked for at once, so the launch is two memory latencies long.
+constexpr uint32_t kFewParts = 8;
+template <uint32_t D>
+__global__ __launch_bounds__(256) void kv_attention_join_few_kernel(FerruleHipKvAttentionArgs a, SplitPlan plan) {
+  constexpr uint32_t kQuads = D / 4u;
+  const KvSequence s = kv_sequence(a.query_indptr, a.sequence_lengths, blockIdx.y, a.rows, a.max_query_length);
+  const uint32_t quad = threadIdx.x % kQuads;
+  const Joined j = joined_row(a, plan, s, (blockIdx.x * 256u + threadIdx.x) / kQuads);
+  if (j.parts == 0u) return;
+  const float2 *statistics = global_ptr<const float2>(a.workspace + plan.statistics) + j.row.index * plan.splits;
+  const f32x4_t *partials = reinterpret_cast<const f32x4_t *>(global_ptr<const float>(a.workspace + plan.partials)) +
+                            j.row.index * plan.splits * kQuads + quad;
+  float2 part[kFewParts];
+  f32x4_t value[kFewParts];
+#pragma unroll
+  for (uint32_t p = 0; p < kFewParts; ++p) {
+    const uint32_t at = min(p, j.parts - 1u);
+    part[p] = statistics[at];
+    value[p] = partials[at * kQuads];
+  }
+  float top = -INFINITY, total = 0.0f;
+#pragma unroll
+  for (uint32_t p = 0; p < kFewParts; ++p) top = fmaxf(top, part[p].x);  // the last part again does not change it
+  const float base = top == -INFINITY ? 0.0f : top;
+  f32x4_t x = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (uint32_t p = 0; p < kFewParts; ++p) {
+    if (p >= j.parts) break;
+    const float weight = part_weight(part[p].x, base);
+    total += part[p].y * weight;
+    x += value[p] * weight;
+  }
+  store4(a.output, j.row.output + 4u * quad, (a.flags & FERRULE_HIP_KV_ATTENTION_OUTPUT_F32) != 0u,
+         x * (total != 0.0f ? 1.0f / total : 0.0f));
+}
+
+// More parts: a workgroup per (row, query head).  The maximum and the sum go over all parts at once; the
+// values are added by 256 / (D / 4) threads per four values, each over a fixed set of parts, and those
+// sums in turn.
 template <uint32_t D>
 __global__ __launch_bounds__(256) void kv_attention_join_kernel(FerruleHipKvAttentionArgs a, SplitPlan plan) {
-  const uint32_t b = blockIdx.y;
-  const uint32_t lane = threadIdx.x & 63u;
-  const uint32_t item = __builtin_amdgcn_readfirstlane(blockIdx.x * kWaves + (threadIdx.x >> 6));
-  const uint32_t group = a.q_heads / a.kv_heads;
-  const KvSequence s = kv_sequence(a.query_indptr, a.sequence_lengths, b, a.rows, a.max_query_length);
-  const uint32_t kv_head = item % a.kv_heads, r = item / a.kv_heads;
-  if (r >= s.rows * group) return;
-  const uint32_t first_row = r / plan.tile_rows * plan.tile_rows;
-  const uint32_t last_row = min(first_row + plan.tile_rows, s.rows * group) - 1u;
-  const TileRange range = tile_range(a, s.position + static_cast<int32_t>(first_row / group),
-                                     s.position + static_cast<int32_t>(last_row / group));
-  const uint32_t per_part = part_tiles(range.count, plan);
-  if (per_part >= range.count) return;  // written already
-  const uint32_t parts = (range.count + per_part - 1u) / per_part;
-  const PackedRow row = packed_row(a, s, kv_head, group, r);
-  const float2 *statistics = global_ptr<const float2>(a.workspace + plan.statistics) + row.index * plan.splits;
-  const float *partials = global_ptr<const float>(a.workspace + plan.partials) + row.index * plan.splits * D;
+  constexpr uint32_t kQuads = D / 4u, kLanes = 256u / kQuads;
+  __shared__ float wave_top[kWaves], wave_sums[kWaves];
+  __shared__ __align__(16) f32x4_t added[256];
+  const KvSequence s = kv_sequence(a.query_indptr, a.sequence_lengths, blockIdx.y, a.rows, a.max_query_length);
+  const Joined j = joined_row(a, plan, s, blockIdx.x);
+  if (j.parts == 0u) return;
+  const float2 *statistics = global_ptr<const float2>(a.workspace + plan.statistics) + j.row.index * plan.splits;
+  const f32x4_t *partials = reinterpret_cast<const f32x4_t *>(global_ptr<const float>(a.workspace + plan.partials)) +
+                            j.row.index * plan.splits * kQuads;
+  const uint32_t wave = threadIdx.x >> 6;
   float top = -INFINITY;
-  for (uint32_t p = 0; p < parts; ++p) top = fmaxf(top, statistics[p].x);
+  for (uint32_t p = threadIdx.x; p < j.parts; p += 256u) top = fmaxf(top, statistics[p].x);
+  top = wave_max(top);
+  if ((threadIdx.x & 63u) == 0u) wave_top[wave] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(wave_top[0], wave_top[1]), fmaxf(wave_top[2], wave_top[3]));
   const float base = top == -INFINITY ? 0.0f : top;
   float total = 0.0f;
-  constexpr uint32_t kPieces = (D + 511u) / 512u, kOwn = D < 512u ? D / 64u : 8u;  // values of a lane, side by side
-  static_assert(kPieces == 1u, "one piece per lane");
-  float x[kOwn] = {};
-  for (uint32_t p = 0; p < parts; ++p) {
+  for (uint32_t p = threadIdx.x; p < j.parts; p += 256u) {
     const float2 part = statistics[p];
-    const float keep = part_weight(part.x, base);
-    total += part.y * keep;
-    const float *src = partials + static_cast<uint64_t>(p) * D + lane * kOwn;
-#pragma unroll
-    for (uint32_t e = 0; e < kOwn; ++e) x[e] += src[e] * keep;
+    total += part.y * part_weight(part.x, base);
   }
-  const float norm = total != 0.0f ? 1.0f / total : 0.0f;
-#pragma unroll
-  for (uint32_t e = 0; e < kOwn; ++e) {
-    const uint64_t at = row.output + lane * kOwn + e;
-    if (a.flags & FERRULE_HIP_KV_ATTENTION_OUTPUT_F32) {
-      global_ptr<float>(a.output)[at] = x[e] * norm;
-    } else {
-      global_ptr<uint16_t>(a.output)[at] = bf16_rne_bits(x[e] * norm);
-    }
+  total = wave_sum(total);
+  if ((threadIdx.x & 63u) == 0u) wave_sums[wave] = total;
+  const uint32_t quad = threadIdx.x % kQuads;
+  f32x4_t x = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 8
+  for (uint32_t p = threadIdx.x / kQuads; p < j.parts; p += kLanes) {
+    x += partials[p * kQuads + quad] * part_weight(statistics[p].x, base);
   }
+  added[threadIdx.x] = x;
+  __syncthreads();
+  if (threadIdx.x >= kQuads) return;
+#pragma unroll
+  for (uint32_t l = 1; l < kLanes; ++l) x += added[l * kQuads + threadIdx.x];
+  total = (wave_sums[0] + wave_sums[1]) + (wave_sums[2] + wave_sums[3]);
+  store4(a.output, j.row.output + 4u * threadIdx.x, (a.flags & FERRULE_HIP_KV_ATTENTION_OUTPUT_F32) != 0u,
+         x * (total != 0.0f ? 1.0f / total : 0.0f));
 }
 
 uint32_t row_bound(const FerruleHipKvAttentionArgs &a) { return a.max_query_length < a.rows ? a.max_query_length : a.rows; }
@@ -837,31 +905,35 @@ uint32_t wave_tiles(const FerruleHipKvAttentionArgs &a) {
   return a.head_dim > 128u || packed_rows(a) <= 64u ? 1u : 2u;
 }
 
-// How far a token range is cut: to four workgroups a CU, while a part keeps two steps of every wave.
+// How the token ranges are cut: into parts of equal length, so that sequences of different lengths give
+// workgroups of the same work.
 SplitPlan plan_splits(const FerruleHipKvAttentionArgs &a) {
   const uint32_t tiles = wave_tiles(a);
-  SplitPlan plan = {tiles == 0u ? kTileRows : 64u * tiles, 1u, tiles == 0u ? 2u * kWaves : 4u,
-                    static_cast<uint32_t>(__builtin_ctz(a.page_tokens)), 0u, 0u};
-  const uint64_t base = static_cast<uint64_t>(a.batch) * a.kv_heads * row_tiles(a, plan.tile_rows);
+  SplitPlan plan = {};
+  plan.tile_rows = tiles == 0u ? kTileRows : 64u * tiles;
+  plan.page_shift = static_cast<uint32_t>(__builtin_ctz(a.page_tokens));
   uint64_t tokens = a.max_sequence_length;
   if (a.window != 0u) {
     const uint64_t seen = static_cast<uint64_t>(a.window) + a.sinks + plan.tile_rows + 2u * kTileTokens;
     tokens = tokens < seen ? tokens : seen;
   }
-  const uint64_t most = (tokens / kTileTokens + 1u) / plan.min_tiles;
-  uint64_t splits = ((tiles == 0u ? 1024u : 512u) + base - 1u) / base;
-  if (splits > most) splits = most;
-  if (splits > 256u) splits = 256u;
-  if (splits > 1u) plan.splits = static_cast<uint32_t>(splits);
-  plan.partials = 0u;
+  const uint64_t token_tiles = tokens / kTileTokens + 1u;
+  const uint64_t segments = static_cast<uint64_t>(a.batch) * a.kv_heads * row_tiles(a, plan.tile_rows);
+  const uint64_t target = tiles == 0u ? 1024u : 512u;
+  const uint64_t least = tiles == 0u ? 2u * kWaves : 4u;
+  uint64_t part = (segments * token_tiles + target - 1u) / target;
+  part = (part < least ? least : part) + 3u & ~3ull;
+  uint64_t splits = (token_tiles + part - 1u) / part;
+  plan.part_tiles = static_cast<uint32_t>(part < 0x40000000u ? part : 0x40000000u);
+  plan.splits = static_cast<uint32_t>(splits);
+  if (plan.splits == 1u) return plan;
   plan.statistics = static_cast<uint64_t>(a.rows) * a.q_heads * plan.splits * a.head_dim * sizeof(float);
   return plan;
 }
 
 uint64_t workspace_size(const FerruleHipKvAttentionArgs &a) {
-  const SplitPlan plan = plan_splits(a);
-  if (plan.splits == 1u) return 0u;
-  return plan.statistics + static_cast<uint64_t>(a.rows) * a.q_heads * plan.splits * sizeof(float2);
+  const SplitPlan plan = plan_splits(a);  // statistics are two floats for head_dim values
+  return plan.statistics + plan.statistics / a.head_dim * 2u;
 }
 
 // Scalar fields; validate() looks at the rest.
@@ -913,7 +985,12 @@ void launch(const FerruleHipKvAttentionArgs &a, hipStream_t stream) {
   }
   if (plan.splits > 1u) {
     const uint32_t items = row_bound(a) * a.q_heads;
-    kv_attention_join_kernel<D><<<dim3((items + kWaves - 1u) / kWaves, a.batch), 256, 0, stream>>>(a, plan);
+    if (plan.splits <= kFewParts) {
+      constexpr uint32_t kRows = 256u / (D / 4u);
+      kv_attention_join_few_kernel<D><<<dim3((items + kRows - 1u) / kRows, a.batch), 256, 0, stream>>>(a, plan);
+    } else {
+      kv_attention_join_kernel<D><<<dim3(items, a.batch), 256, 0, stream>>>(a, plan);
+    }
   }
 }
 
