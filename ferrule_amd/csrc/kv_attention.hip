@@ -37,6 +37,7 @@ namespace {
 constexpr uint32_t kWaves = 4;
 constexpr uint32_t kTileRows = 16;   // packed rows of a tile
 constexpr uint32_t kTileTokens = 32; // tokens of one step
+constexpr float kLargest = 65536.0f; // rows kernel: sum of a lane's weights of one step that moves the maximum
 constexpr float kLazy = 8.0f;        // how far (in powers of two) scores may exceed the running maximum
 
 struct SplitPlan {
@@ -183,35 +184,51 @@ struct Core {
     }
   }
 
-  // `token`: the step's first token inside its page's head (a multiple of 32)
-  static __device__ __forceinline__ void load_keys(const uint8_t *payload, const uint8_t *scales, uint32_t token, uint32_t lane,
-                                                   Keys &k) {
-    const uint32_t i = lane & 15u, g = lane >> 4;
-    const uint32_t t = 8u * (i >> 2) + (i & 3u);
+  // Byte offsets of a lane's loads from the first byte of a 32-token tile (Place).
+  struct Offsets {
+    uint32_t key, key_scale, value, value_scale;
+  };
+  static __device__ __forceinline__ Offsets offsets(uint32_t lane) {
+    const uint32_t i = lane & 15u, g = lane >> 4, block = D == 64u ? (g & 1u) : g;
+    Offsets o;
+    o.key = Layout::key_byte(8u * (i >> 2) + (i & 3u), 0u) + block * 16u;
+    o.key_scale = Layout::key_scale(8u * (i >> 2), block);
+    o.value = Layout::value_byte(8u * g, 2u * i);
+    o.value_scale = Layout::value_scale(8u * g, i >> 3);
+    return o;
+  }
+
+  // STREAM: read once, past the caches' other lines
+  template <bool STREAM, typename T>
+  static __device__ __forceinline__ T load(const uint8_t *p) {
+    if constexpr (STREAM) return __builtin_nontemporal_load(reinterpret_cast<const T *>(p));
+    return *reinterpret_cast<const T *>(p);
+  }
+
+  template <bool STREAM>
+  static __device__ __forceinline__ void load_keys(const uint8_t *payload, const uint8_t *scales, const Offsets &o, Keys &k) {
 #pragma unroll
     for (uint32_t c = 0; c < kChunks; ++c) {
-      const uint32_t block = D == 64u ? (g & 1u) : g;  // of the piece
 #pragma unroll
       for (uint32_t half = 0; half < 2u; ++half) {
-        k.payload[c][half] =
-            __builtin_nontemporal_load(reinterpret_cast<const u32x4_t *>(payload + Layout::key_byte(token + t + 4u * half, c) + block * 16u));
+        k.payload[c][half] = load<STREAM, u32x4_t>(payload + o.key + (c * 32u + 4u * half) * Layout::kKeyBytes);
       }
-      k.scale[c] = *reinterpret_cast<const uint2 *>(scales + Layout::key_scale(token + 8u * (i >> 2), 4u * c + block));
+      k.scale[c] = *reinterpret_cast<const uint2 *>(scales + o.key_scale + c * 128u);
     }
   }
 
   // One 16-byte piece of a lane: values 64u + 4i .. 64u + 4i + 3 of tokens 8g..8g+7, and their scale bytes.
-  static __device__ __forceinline__ void load_piece(const uint8_t *payload, const uint8_t *scales, uint32_t token, uint32_t u,
-                                                    uint32_t lane, u32x4_t &w, uint2 &scale) {
-    const uint32_t i = lane & 15u, g = lane >> 4;
-    w = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t *>(payload + Layout::value_byte(token + 8u * g, 32u * u + 2u * i)));
-    scale = *reinterpret_cast<const uint2 *>(scales + Layout::value_scale(token + 8u * g, 2u * u + (i >> 3)));
+  template <bool STREAM>
+  static __device__ __forceinline__ void load_piece(const uint8_t *payload, const uint8_t *scales, uint32_t u, const Offsets &o,
+                                                    u32x4_t &w, uint2 &scale) {
+    w = load<STREAM, u32x4_t>(payload + o.value + u * 256u);
+    scale = *reinterpret_cast<const uint2 *>(scales + o.value_scale + u * 16u);
   }
 
-  static __device__ __forceinline__ void load_values(const uint8_t *payload, const uint8_t *scales, uint32_t token,
-                                                     uint32_t lane, Values &v) {
+  template <bool STREAM>
+  static __device__ __forceinline__ void load_values(const uint8_t *payload, const uint8_t *scales, const Offsets &o, Values &v) {
 #pragma unroll
-    for (uint32_t u = 0; u < kUnits; ++u) load_piece(payload, scales, token, u, lane, v.payload[u], v.scale[u]);
+    for (uint32_t u = 0; u < kUnits; ++u) load_piece<STREAM>(payload, scales, u, o, v.payload[u], v.scale[u]);
   }
 
   // Scores of tokens 8g..8g+7 of row i: s[0..3] and s[4..7].
@@ -289,27 +306,30 @@ __device__ __forceinline__ float part_weight(float top, float base) {
 // in bounds; nothing of it is used.
 struct Place {
   uint32_t first;  // position of its first token
-  uint32_t token;  // inside the page
-  uint64_t payload, scales;  // byte offsets of the page's head
+  uint64_t payload, scales;  // byte offsets
   bool valid;
 };
 
+// A tile's page comes from the table by a scalar load: page_of asks for it, place_at uses it, and a
+// loop keeps a step or more between the two.  `count`: the range's tiles, at least 1.
+__device__ __forceinline__ int32_t page_of(const FerruleHipKvAttentionArgs &a, const SplitPlan &plan, const TileRange &range,
+                                           uint32_t b, uint32_t v, uint32_t count) {
+  return kv_uniform(a.page_table,
+                    static_cast<uint64_t>(b) * a.max_pages + ((range.at(min(v, count - 1u)) * kTileTokens) >> plan.page_shift));
+}
+
 template <uint32_t D>
-__device__ __forceinline__ Place place_of(const FerruleHipKvAttentionArgs &a, const SplitPlan &plan, const TileRange &range,
-                                          uint32_t b, uint32_t kv_head, uint32_t v, uint32_t end) {
-  Place p = {0u, 0u, 0u, 0u, false};
-  uint64_t page_head = 0u;
-  if (v < end) {
-    p.first = range.at(v) * kTileTokens;
-    const uint32_t page =
-        static_cast<uint32_t>(kv_uniform(a.page_table, static_cast<uint64_t>(b) * a.max_pages + (p.first >> plan.page_shift)));
-    p.valid = page < a.page_count;
-    if (!p.valid && (threadIdx.x & 63u) == 0u) kv_report(a.error);
-    p.token = p.first & (a.page_tokens - 1u);
-    page_head = p.valid ? static_cast<uint64_t>(page) * a.kv_heads + kv_head : 0u;
-  }
-  p.payload = (page_head << plan.page_shift) * (D / 2u);
-  p.scales = (page_head << plan.page_shift) * (D / 32u);
+__device__ __forceinline__ Place place_at(const FerruleHipKvAttentionArgs &a, const SplitPlan &plan, const TileRange &range,
+                                          uint32_t kv_head, uint32_t v, uint32_t end, int32_t page, bool &bad) {
+  Place p;
+  p.first = range.at(v) * kTileTokens;
+  p.valid = v < end && static_cast<uint32_t>(page) < a.page_count;
+  bad |= v < end && !p.valid;
+  // tokens in front of the tile, of every page and head
+  const uint64_t head = static_cast<uint64_t>(p.valid ? static_cast<uint32_t>(page) : 0u) * a.kv_heads + kv_head;
+  const uint64_t tokens = (head << plan.page_shift) + (p.valid ? p.first & (a.page_tokens - 1u) : 0u);
+  p.payload = tokens * (D / 2u);
+  p.scales = tokens * (D / 32u);
   return p;
 }
 
@@ -392,19 +412,27 @@ __global__ __launch_bounds__(256, D <= 128u ? 4 : D == 256u ? 2 : 1) void kv_att
 
   const uint8_t *k_payload = global_ptr<const uint8_t>(a.k_payload), *k_scales = global_ptr<const uint8_t>(a.k_scales);
   const uint8_t *v_payload = global_ptr<const uint8_t>(a.v_payload), *v_scales = global_ptr<const uint8_t>(a.v_scales);
+  const typename C::Offsets offset = C::offsets(lane);
   typename C::Keys keys;
   typename C::Values values;
-  Place next_place = place_of<D>(a, plan, range, b, kv_head, begin + wave, end);
-  C::load_keys(k_payload + next_place.payload, k_scales + next_place.scales, next_place.token, lane, keys);
-  C::load_values(v_payload + next_place.payload, v_scales + next_place.scales, next_place.token, lane, values);
+  bool bad = false;  // a page number outside the cache
+  int32_t next_page = 0;
+  Place next_place = {0u, 0u, 0u, false};
+  if (begin < end) {
+    next_place = place_at<D>(a, plan, range, kv_head, begin + wave, end, page_of(a, plan, range, b, begin + wave, end), bad);
+    next_page = page_of(a, plan, range, b, begin + wave + kWaves, end);
+  }
+  C::template load_keys<true>(k_payload + next_place.payload, k_scales + next_place.scales, offset, keys);
+  C::template load_values<true>(v_payload + next_place.payload, v_scales + next_place.scales, offset, values);
   for (uint32_t v = begin + wave; v < end; v += kWaves) {
     // keys and values are loaded one step ahead, as soon as the registers of this step's are free; two or
     // three steps ahead at 3 or 2 waves per SIMD took as long (64 x 8192 tokens, 8 heads: 112, 110, 122 us)
     const Place here = next_place;
-    next_place = place_of<D>(a, plan, range, b, kv_head, v + kWaves, end);
+    next_place = place_at<D>(a, plan, range, kv_head, v + kWaves, end, next_page, bad);
+    next_page = page_of(a, plan, range, b, v + 2u * kWaves, end);
     f32x4_t score[2];
     C::scores(keys, query, lane, score);
-    C::load_keys(k_payload + next_place.payload, k_scales + next_place.scales, next_place.token, lane, keys);
+    C::template load_keys<true>(k_payload + next_place.payload, k_scales + next_place.scales, offset, keys);
     float x[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] = score[e >> 2][e & 3];
@@ -454,7 +482,7 @@ __global__ __launch_bounds__(256, D <= 128u ? 4 : D == 256u ? 2 : 1) void kv_att
         out[4u * u + e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, operand[e]), weight, out[4u * u + e], 0, 0, 0);
       }
     }
-    C::load_values(v_payload + next_place.payload, v_scales + next_place.scales, next_place.token, lane, values);
+    C::template load_values<true>(v_payload + next_place.payload, v_scales + next_place.scales, offset, values);
     if (nan_blocks && here.valid) {  // rare: the rows that see such a token take its NaN, the others must not (0 * NaN)
       const uint8_t *scales = v_scales + here.scales;
       for (uint32_t t = 0; t < kTileTokens; ++t) {
@@ -462,7 +490,7 @@ __global__ __launch_bounds__(256, D <= 128u ? 4 : D == 256u ? 2 : 1) void kv_att
         const bool seen = j <= mine.position && (j >= from || j < sinks);
 #pragma unroll
         for (uint32_t block = 0; block < D / 32u; ++block) {
-          const bool bad = scales[C::Layout::value_scale(here.token + t, block)] == kNanBlock;
+          const bool bad = scales[C::Layout::value_scale(t, block)] == kNanBlock;
           // accumulator 4u + e of lane (i, g) holds values 64u + 16g + 4v + e
           const bool hit = bad && seen && (g >> 1) == (block & 1u);
 #pragma unroll
@@ -474,6 +502,7 @@ __global__ __launch_bounds__(256, D <= 128u ? 4 : D == 256u ? 2 : 1) void kv_att
     }
   }
 
+  if (bad && lane == 0u) kv_report(a.error);
   // join the four waves, 128 values at a time
   sum = row_sum(sum);
   if (g == 0u) {
@@ -533,19 +562,28 @@ __global__ __launch_bounds__(256, D <= 128u ? 4 : D == 256u ? 2 : 1) void kv_att
   }
 }
 
-// Many rows: a workgroup has 4 * 16 * NQ of them, 16 * NQ to a wave, and its waves go through the same
-// tokens.  Values are expanded to BF16 once per workgroup: of the 16-byte pieces of a step (D/64 per 32
-// tokens) every wave expands one (two at D = 512) into the operands of four accumulators, in LDS, one step ahead
-// of their use; keys are read by every wave, from cache, as they stand.  One barrier per step.
-template <uint32_t D, uint32_t NQ>
-__global__ __launch_bounds__(256, D <= 128u ? (NQ == 1u ? 4 : 2) : D == 256u ? 2 : 1) void kv_attention_rows_kernel(FerruleHipKvAttentionArgs a, SplitPlan plan) {
+// Many rows: 16 * NQ of them to a wave, and the WAVES waves of a workgroup go through the same tokens.
+// Values are expanded to BF16 once per workgroup: a step has as many 16-byte pieces (D/64 per 32 tokens)
+// as waves, or twice that, and every wave expands its own into the operands of four accumulators, in LDS,
+// one step ahead of their use; keys are read by every wave, from cache, as they stand.  One barrier per step.
+template <uint32_t D, uint32_t NQ, uint32_t WAVES>
+struct Rows {
+  static constexpr uint32_t kUnits = D / 64u;
+  static constexpr uint32_t kPieces = kUnits > WAVES ? kUnits : WAVES;  // of a step
+  static constexpr uint32_t kOwn = kPieces / WAVES;                     // of them, a wave's
+  static constexpr uint32_t kSub = kPieces / kUnits;                    // 32-token tiles of a step
+  static constexpr uint32_t kInner = D >= 512u || NQ >= 4u ? 1u : kSub < 2u ? 1u : 2u;  // tiles between two looks at the maximum
+  static constexpr uint32_t kRows = 16u * NQ * WAVES;
+  static constexpr uint32_t kOccupancy = WAVES * 64u == 512u ? 2u : D >= 512u ? 1u : 2u;  // waves per SIMD
+};
+
+template <uint32_t D, uint32_t NQ, uint32_t WAVES>
+__global__ __launch_bounds__(WAVES * 64u, (Rows<D, NQ, WAVES>::kOccupancy)) void kv_attention_rows_kernel(FerruleHipKvAttentionArgs a, SplitPlan plan) {
   using C = Core<D>;
-  constexpr uint32_t kSub = D == 64u ? 4u : D == 128u ? 2u : 1u;  // 32-token tiles of a step
-  constexpr uint32_t kPieces = kSub * C::kUnits;                  // 16-byte pieces of a step
-  constexpr uint32_t kOwn = kPieces / kWaves;                     // of them, a wave's
-  static_assert(kOwn * kWaves == kPieces, "every wave expands the same number of pieces");
-  __shared__ __align__(16) u32x4_t staged[2][kPieces][4][64];     // operands [piece][accumulator][lane]
-  __shared__ uint32_t nan_of[2][kWaves];
+  using R = Rows<D, NQ, WAVES>;
+  constexpr uint32_t kSub = R::kSub, kInner = R::kInner, kOwn = R::kOwn;
+  __shared__ __align__(16) u32x4_t staged[2][R::kPieces][4][64];  // operands [piece][accumulator][lane]
+  __shared__ uint32_t nan_of[2][WAVES];
   const uint32_t lane = threadIdx.x & 63u;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t i = lane & 15u, g = lane >> 4;
@@ -557,10 +595,10 @@ __global__ __launch_bounds__(256, D <= 128u ? (NQ == 1u ? 4 : 2) : D == 256u ? 2
   const uint32_t group = a.q_heads / a.kv_heads;
   const KvSequence s = kv_sequence(a.query_indptr, a.sequence_lengths, b, a.rows, a.max_query_length);
   if (s.bad && blockIdx.x == 0u && threadIdx.x == 0u) kv_report(a.error);
-  const uint32_t first_row = row_tile * plan.tile_rows;
+  const uint32_t first_row = row_tile * R::kRows;
   const uint32_t all_rows = s.rows * group;
   if (first_row >= all_rows) return;
-  const uint32_t last_row = min(first_row + plan.tile_rows, all_rows) - 1u;
+  const uint32_t last_row = min(first_row + R::kRows, all_rows) - 1u;
   const int32_t high = s.position + static_cast<int32_t>(last_row / group);
   const TileRange range = tile_range(a, s.position + static_cast<int32_t>(first_row / group), high);
   if (high >= static_cast<int32_t>(a.max_pages * a.page_tokens) && threadIdx.x == 0u) kv_report(a.error);
@@ -587,6 +625,7 @@ __global__ __launch_bounds__(256, D <= 128u ? (NQ == 1u ? 4 : 2) : D == 256u ? 2
   const float factor = a.softmax_scale * 1.44269504088896341f;
   f32x4_t out[NQ][C::kColumns];
   float top[NQ], base[NQ], sum[NQ];
+  bool unset = true;  // some row has seen no token yet
 #pragma unroll
   for (uint32_t n = 0; n < NQ; ++n) {
     top[n] = -INFINITY;
@@ -595,27 +634,31 @@ __global__ __launch_bounds__(256, D <= 128u ? (NQ == 1u ? 4 : 2) : D == 256u ? 2
     for (uint32_t c = 0; c < C::kColumns; ++c) out[n][c] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
   }
 
-  auto place = [&](uint32_t v) { return place_of<D>(a, plan, range, b, kv_head, v, end); };
   const uint8_t *k_payload = global_ptr<const uint8_t>(a.k_payload), *k_scales = global_ptr<const uint8_t>(a.k_scales);
   const uint8_t *v_payload = global_ptr<const uint8_t>(a.v_payload), *v_scales = global_ptr<const uint8_t>(a.v_scales);
+  const typename C::Offsets offset = C::offsets(lane);
+  bool bad = false;  // a page number outside the cache
   u32x4_t raw[kOwn];
   uint2 raw_scale[kOwn];
-  auto load_pieces = [&](uint32_t v) {
+  bool raw_valid[kOwn];
+  const uint32_t own_tile = wave * kOwn / C::kUnits;  // of a step: the tile that holds the wave's pieces
+  auto load_pieces = [&](uint32_t v, int32_t page) {
+    const Place p = place_at<D>(a, plan, range, kv_head, v + own_tile, end, page, bad);
 #pragma unroll
     for (uint32_t o = 0; o < kOwn; ++o) {
-      const uint32_t piece = wave * kOwn + o;
-      const Place p = place(v + piece / C::kUnits);
-      raw[o] = u32x4_t{0u, 0u, 0u, 0u};
-      raw_scale[o] = make_uint2(0x7f7f7f7fu, 0x7f7f7f7fu);
-      if (p.valid) {
-        C::load_piece(v_payload + p.payload, v_scales + p.scales, p.token, piece % C::kUnits, lane, raw[o], raw_scale[o]);
-      }
+      raw_valid[o] = p.valid;
+      C::template load_piece<false>(v_payload + p.payload, v_scales + p.scales, (wave * kOwn + o) % C::kUnits, offset, raw[o],
+                                    raw_scale[o]);
     }
   };
   auto stage_pieces = [&](uint32_t buffer) {
     bool nan = false;
 #pragma unroll
     for (uint32_t o = 0; o < kOwn; ++o) {
+      if (!raw_valid[o]) {  // of no use, but 0 * it has to be 0
+        raw[o] = u32x4_t{0u, 0u, 0u, 0u};
+        raw_scale[o] = make_uint2(0x7f7f7f7fu, 0x7f7f7f7fu);
+      }
       nan |= C::has_nan(raw_scale[o]);
       u32x4_t operand[4];
       C::expand(raw[o], make_uint2(C::without_nan(raw_scale[o].x), C::without_nan(raw_scale[o].y)), operand);
@@ -625,119 +668,161 @@ __global__ __launch_bounds__(256, D <= 128u ? (NQ == 1u ? 4 : 2) : D == 256u ? 2
     const uint32_t any = __any(nan) ? 1u : 0u;
     if (lane == 0u) nan_of[buffer][wave] = any;
   };
-
-  typename C::Keys keys[kSub];
-  uint32_t start_of[kSub], valid_of = 0u;  // of the tiles whose keys are loaded
-  auto load_tiles = [&](uint32_t v) {
-    valid_of = 0u;
+  typename C::Keys keys[kInner];
+  int32_t start[kInner];
+  bool there[kInner];
+  auto load_tiles = [&](uint32_t v, const int32_t *page) {
 #pragma unroll
-    for (uint32_t t = 0; t < kSub; ++t) {
-      const Place p = place(v + t);
-      start_of[t] = p.first;
-      valid_of |= p.valid ? 1u << t : 0u;
-      C::load_keys(k_payload + p.payload, k_scales + p.scales, p.token, lane, keys[t]);
+    for (uint32_t t = 0; t < kInner; ++t) {
+      const Place p = place_at<D>(a, plan, range, kv_head, v + t, end, page[t], bad);
+      start[t] = static_cast<int32_t>(p.first);
+      there[t] = p.valid;
+      C::template load_keys<false>(k_payload + p.payload, k_scales + p.scales, offset, keys[t]);
     }
   };
-  load_pieces(begin);
-  load_tiles(begin);
-  stage_pieces(0u);
-  load_pieces(begin + kSub);
-  __syncthreads();
+  auto page = [&](uint32_t v) { return page_of(a, plan, range, b, v, end); };
+
+  int32_t now[kSub], next[kSub], piece_page = 0;  // pages of this step's tiles, of the next one's, of the next piece
   uint32_t buffer = 0u;
+  if (begin < end) {
+#pragma unroll
+    for (uint32_t t = 0; t < kSub; ++t) now[t] = page(begin + t);
+    load_pieces(begin, page(begin + own_tile));
+    load_tiles(begin, now);
+    stage_pieces(0u);
+    load_pieces(begin + kSub, page(begin + kSub + own_tile));
+    piece_page = page(begin + 2u * kSub + own_tile);
+    lds_barrier();  // not a full one: it would wait for the loads in flight
+  }
   for (uint32_t v = begin; v < end; v += kSub, buffer ^= 1u) {
-    f32x4_t score[NQ][kSub][2];
-    int32_t start[kSub];
-    const uint32_t valid = valid_of;
 #pragma unroll
-    for (uint32_t t = 0; t < kSub; ++t) {
-      start[t] = static_cast<int32_t>(start_of[t]);
+    for (uint32_t t = 0; t < kSub; ++t) next[t] = page(v + kSub + t);
+    const int32_t later_piece = page(v + 3u * kSub + own_tile);
 #pragma unroll
-      for (uint32_t n = 0; n < NQ; ++n) C::scores(keys[t], query[n], lane, score[n][t]);
-    }
-    load_tiles(v + kSub);
-    stage_pieces(buffer ^ 1u);
-    load_pieces(v + 2u * kSub);
-    bool grows = false;
-    float most[NQ];
+    for (uint32_t inner = 0; inner < kSub; inner += kInner) {
+      f32x4_t score[NQ][kInner][2];
+      int32_t first[kInner];
+      bool valid[kInner];
 #pragma unroll
-    for (uint32_t n = 0; n < NQ; ++n) {
-      most[n] = -INFINITY;
+      for (uint32_t t = 0; t < kInner; ++t) {
+        first[t] = start[t];
+        valid[t] = there[t];
 #pragma unroll
-      for (uint32_t t = 0; t < kSub; ++t) {
-        const bool there = (valid >> t) & 1u;
+        for (uint32_t n = 0; n < NQ; ++n) C::scores(keys[t], query[n], lane, score[n][t]);
+      }
+      load_tiles(v + inner + kInner, inner + kInner < kSub ? now + (inner + kInner) % kSub : next);
+      if (inner == 0u) {
+        stage_pieces(buffer ^ 1u);
+        load_pieces(v + 2u * kSub, piece_page);
+      }
+#pragma unroll
+      for (uint32_t t = 0; t < kInner; ++t) {
         // tokens that every row of the wave sees need no mask
-        const bool all = there && start[t] + 31 <= wave_low &&
-                         (a.window == 0u || start[t] > wave_high - static_cast<int32_t>(a.window) ||
-                          start[t] + 31 < static_cast<int32_t>(a.sinks));
+        const bool all = valid[t] && first[t] + 31 <= wave_low &&
+                         (a.window == 0u || first[t] > wave_high - static_cast<int32_t>(a.window) ||
+                          first[t] + 31 < static_cast<int32_t>(a.sinks));
         if (!all) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const int32_t j = start[t] + static_cast<int32_t>(8u * g) + e;
-            const bool seen = there && j <= position[n] && (j >= from[n] || j < sinks);
-            score[n][t][e >> 2][e & 3] = seen ? score[n][t][e >> 2][e & 3] : -INFINITY;
+          for (uint32_t n = 0; n < NQ; ++n) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const int32_t j = first[t] + static_cast<int32_t>(8u * g) + e;
+              const bool seen = valid[t] && j <= position[n] && (j >= from[n] || j < sinks);
+              score[n][t][e >> 2][e & 3] = seen ? score[n][t][e >> 2][e & 3] : -INFINITY;
+            }
           }
         }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) most[n] = fmaxf(most[n], score[n][t][e >> 2][e & 3]);
       }
-      most[n] *= factor;  // more than 0
-      grows |= most[n] > top[n] + kLazy;
-    }
-    if (__any(grows)) {
-#pragma unroll
-      for (uint32_t n = 0; n < NQ; ++n) {
-        const float next_top = fmaxf(top[n], row_max(most[n]));
-        const float next = next_top == -INFINITY ? 0.0f : next_top;
-        const float keep = part_weight(top[n], next);
-        top[n] = next_top;
-        base[n] = next;
-        sum[n] *= keep;
-#pragma unroll
-        for (uint32_t c = 0; c < C::kColumns; ++c) out[n][c] *= keep;
-      }
-    }
-    bf16x8_t weight[NQ][kSub];
-#pragma unroll
-    for (uint32_t n = 0; n < NQ; ++n) {
-#pragma unroll
-      for (uint32_t t = 0; t < kSub; ++t) {
-        float w[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          w[e] = __builtin_amdgcn_exp2f(fmaf(score[n][t][e >> 2][e & 3], factor, -base[n]));
-          weight[n][t][e] = static_cast<__bf16>(w[e]);
-        }
-        sum[n] += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
-      }
-    }
-#pragma unroll
-    for (uint32_t t = 0; t < kSub; ++t) {
-#pragma unroll
-      for (uint32_t u = 0; u < C::kUnits; ++u) {
-#pragma unroll
-        for (uint32_t e = 0; e < 4u; ++e) {
-          const bf16x8_t operand = __builtin_bit_cast(bf16x8_t, staged[buffer][t * C::kUnits + u][e][lane]);
+      // Weights relative to the maximum as it stands.  Whether that is too low shows in their sum, which is
+      // needed anyway; only then (and until every row has seen a token) is the maximum looked for.
+      bf16x8_t weight[NQ][kInner];
+      float added[NQ];
+      for (bool again = unset;; again = true) {
+        if (again) {
+          bool none = false;
 #pragma unroll
           for (uint32_t n = 0; n < NQ; ++n) {
-            out[n][4u * u + e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(operand, weight[n][t], out[n][4u * u + e], 0, 0, 0);
+            float most = -INFINITY;
+#pragma unroll
+            for (uint32_t t = 0; t < kInner; ++t) {
+#pragma unroll
+              for (int e = 0; e < 8; ++e) most = fmaxf(most, score[n][t][e >> 2][e & 3]);
+            }
+            const float next_top = fmaxf(top[n], row_max(most) * factor);
+            const float next_base = next_top == -INFINITY ? 0.0f : next_top;
+            const float keep = part_weight(top[n], next_base);
+            top[n] = next_top;
+            base[n] = next_base;
+            sum[n] *= keep;
+#pragma unroll
+            for (uint32_t c = 0; c < C::kColumns; ++c) out[n][c] *= keep;
+            none |= next_top == -INFINITY;
           }
+          unset = __any(none);
         }
+        bool grows = false;
+#pragma unroll
+        for (uint32_t n = 0; n < NQ; ++n) {
+          added[n] = 0.0f;
+#pragma unroll
+          for (uint32_t t = 0; t < kInner; ++t) {
+            float w[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              w[e] = __builtin_amdgcn_exp2f(fmaf(score[n][t][e >> 2][e & 3], factor, -base[n]));
+              weight[n][t][e] = static_cast<__bf16>(w[e]);
+            }
+            added[n] += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+          }
+          grows |= added[n] > kLargest;
+        }
+        if (again || !__any(grows)) break;
+      }
+#pragma unroll
+      for (uint32_t n = 0; n < NQ; ++n) sum[n] += added[n];
+      // the value operands come from LDS kRing products ahead
+      constexpr uint32_t kOperands = kInner * C::kUnits * 4u, kRing = kOperands < 8u ? kOperands : 8u;
+      u32x4_t ring[kRing];
+      const u32x4_t(*operands)[64] = staged[buffer][inner * C::kUnits];
+#pragma unroll
+      for (uint32_t f = 0; f < kRing; ++f) ring[f] = operands[f][lane];
+#pragma unroll
+      for (uint32_t f = 0; f < kOperands; ++f) {
+        const uint32_t t = f / (4u * C::kUnits), c = f % (4u * C::kUnits);
+        const bf16x8_t operand = __builtin_bit_cast(bf16x8_t, ring[f % kRing]);
+#pragma unroll
+        for (uint32_t n = 0; n < NQ; ++n) {
+          out[n][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(operand, weight[n][t], out[n][c], 0, 0, 0);
+        }
+        if (f + kRing < kOperands) ring[f % kRing] = operands[f + kRing][lane];
+      }
+      __builtin_amdgcn_sched_group_barrier(0x100, kRing, 0);
+#pragma unroll
+      for (uint32_t f = 0; f < kOperands; ++f) {
+        __builtin_amdgcn_sched_group_barrier(0x008, NQ, 0);
+        if (f + kRing < kOperands) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
       }
     }
-    if ((nan_of[buffer][0] | nan_of[buffer][1] | nan_of[buffer][2] | nan_of[buffer][3]) != 0u) {
+#pragma unroll
+    for (uint32_t t = 0; t < kSub; ++t) now[t] = next[t];
+    piece_page = later_piece;
+    uint32_t nan_blocks = 0u;
+#pragma unroll
+    for (uint32_t w = 0; w < WAVES; ++w) nan_blocks |= nan_of[buffer][w];
+    if (nan_blocks != 0u) {
       // rare: the rows that see such a token take its NaN, the others must not (0 * NaN)
       for (uint32_t t = 0; t < kSub; ++t) {
-        const Place p = place(v + t);
+        const Place p = place_at<D>(a, plan, range, kv_head, v + t, end, page(v + t), bad);
         if (!p.valid) continue;
         const uint8_t *scales = v_scales + p.scales;
         for (uint32_t k = 0; k < kTileTokens; ++k) {
           const int32_t j = static_cast<int32_t>(p.first + k);
 #pragma unroll
           for (uint32_t block = 0; block < D / 32u; ++block) {
-            const bool bad = scales[C::Layout::value_scale(p.token + k, block)] == kNanBlock;
+            const bool nan = scales[C::Layout::value_scale(k, block)] == kNanBlock;
 #pragma unroll
             for (uint32_t n = 0; n < NQ; ++n) {
-              const bool hit = bad && j <= position[n] && (j >= from[n] || j < sinks) && (g >> 1) == (block & 1u);
+              const bool hit = nan && j <= position[n] && (j >= from[n] || j < sinks) && (g >> 1) == (block & 1u);
 #pragma unroll
               for (uint32_t e = 0; e < 4u; ++e) {
                 if (hit) out[n][4u * (block >> 1) + e] = f32x4_t{NAN, NAN, NAN, NAN};
@@ -747,8 +832,9 @@ __global__ __launch_bounds__(256, D <= 128u ? (NQ == 1u ? 4 : 2) : D == 256u ? 2
         }
       }
     }
-    __syncthreads();
+    lds_barrier();
   }
+  if (bad && lane == 0u) kv_report(a.error);
 
 #pragma unroll
   for (uint32_t n = 0; n < NQ; ++n) {
@@ -899,18 +985,21 @@ uint32_t row_tiles(const FerruleHipKvAttentionArgs &a, uint32_t tile_rows) {
   return static_cast<uint32_t>((packed_rows(a) + tile_rows - 1u) / tile_rows);
 }
 
-// Rows of a wave of kv_attention_rows_kernel, in sixteens; 0: kv_attention_decode_kernel.
-uint32_t wave_tiles(const FerruleHipKvAttentionArgs &a) {
-  if (packed_rows(a) <= 32u) return 0u;
-  return a.head_dim > 128u || packed_rows(a) <= 64u ? 1u : 2u;
+// Which kernel: packed rows of a workgroup of kv_attention_rows_kernel, 0 for kv_attention_decode_kernel.
+uint32_t rows_of_workgroup(const FerruleHipKvAttentionArgs &a) {
+  const uint64_t rows = packed_rows(a);
+  if (rows <= 32u) return 0u;
+  if (rows <= 64u || a.head_dim == 512u) return 64u;
+  if (rows <= 128u) return 128u;
+  return a.head_dim == 256u ? 128u : 256u;
 }
 
 // How the token ranges are cut: into parts of equal length, so that sequences of different lengths give
 // workgroups of the same work.
 SplitPlan plan_splits(const FerruleHipKvAttentionArgs &a) {
-  const uint32_t tiles = wave_tiles(a);
+  const uint32_t tiles = rows_of_workgroup(a);
   SplitPlan plan = {};
-  plan.tile_rows = tiles == 0u ? kTileRows : 64u * tiles;
+  plan.tile_rows = tiles == 0u ? kTileRows : tiles;
   plan.page_shift = static_cast<uint32_t>(__builtin_ctz(a.page_tokens));
   uint64_t tokens = a.max_sequence_length;
   if (a.window != 0u) {
@@ -976,11 +1065,15 @@ template <uint32_t D>
 void launch(const FerruleHipKvAttentionArgs &a, hipStream_t stream) {
   const SplitPlan plan = plan_splits(a);
   const dim3 grid(row_tiles(a, plan.tile_rows) * a.kv_heads * plan.splits, a.batch);
-  switch (wave_tiles(a)) {
+  switch (rows_of_workgroup(a)) {
     case 0: kv_attention_decode_kernel<D><<<grid, 256, 0, stream>>>(a, plan); break;
-    case 1: kv_attention_rows_kernel<D, 1><<<grid, 256, 0, stream>>>(a, plan); break;
+    case 64: kv_attention_rows_kernel<D, 1, 4><<<grid, 256, 0, stream>>>(a, plan); break;
+    case 128:
+      if constexpr (D == 256u) kv_attention_rows_kernel<D, 1, 8><<<grid, 512, 0, stream>>>(a, plan);
+      if constexpr (D <= 128u) kv_attention_rows_kernel<D, 2, 4><<<grid, 256, 0, stream>>>(a, plan);
+      break;
     default:
-      if constexpr (D <= 128u) kv_attention_rows_kernel<D, 2><<<grid, 256, 0, stream>>>(a, plan);
+      if constexpr (D <= 128u) kv_attention_rows_kernel<D, 2, 8><<<grid, 512, 0, stream>>>(a, plan);
       break;
   }
   if (plan.splits > 1u) {
