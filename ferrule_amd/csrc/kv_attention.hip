@@ -98,26 +98,29 @@ struct Core {
     uint2 scale[kUnits];
   };
 
-  // 16 values of a row, as f32 holding BF16
-  static __device__ __forceinline__ void load_row16(uint64_t base, uint64_t at, bool f32, float (&x)[16]) {
-    if (f32) {
-      const f32x4_t *src = reinterpret_cast<const f32x4_t *>(global_ptr<const float>(base) + at);
+  // 16 values of a row as they are in memory, and as f32 holding BF16
+  template <bool F32>
+  struct Raw16 {
+    u32x4_t w[F32 ? 4 : 2];
+  };
+  template <bool F32>
+  static __device__ __forceinline__ Raw16<F32> load16(uint64_t base, uint64_t at) {
+    const u32x4_t *src = F32 ? reinterpret_cast<const u32x4_t *>(global_ptr<const float>(base) + at)
+                             : reinterpret_cast<const u32x4_t *>(global_ptr<const uint16_t>(base) + at);
+    Raw16<F32> r;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const f32x4_t w = src[i];
+    for (int i = 0; i < (F32 ? 4 : 2); ++i) r.w[i] = src[i];
+    return r;
+  }
+  template <bool F32>
+  static __device__ __forceinline__ void widen16(const Raw16<F32> &r, float (&x)[16]) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[4 * i + e] = bf16_round(w[e]);
-      }
-    } else {
-      const u32x4_t *src = reinterpret_cast<const u32x4_t *>(global_ptr<const uint16_t>(base) + at);
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const u32x4_t w = src[i];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          x[8 * i + 2 * e] = __uint_as_float(w[e] << 16);
-          x[8 * i + 2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
-        }
+    for (int e = 0; e < 16; ++e) {
+      if constexpr (F32) {
+        x[e] = bf16_round(__uint_as_float(r.w[e >> 2][e & 3]));
+      } else {
+        const uint32_t w = r.w[e >> 3][(e >> 1) & 3];
+        x[e] = __uint_as_float((e & 1) ? w & 0xffff0000u : w << 16);
       }
     }
   }
@@ -152,28 +155,31 @@ struct Core {
     return top >> 23;
   }
 
-  // The lane's part of a tile's query rows; `live` false: zeros.
-  static __device__ __forceinline__ void load_query(uint64_t base, uint64_t row, bool live, bool f32, uint32_t lane, Query &q) {
+  // The lane's part of a tile's query rows.
+  template <bool F32>
+  static __device__ __forceinline__ void load_query(uint64_t base, uint64_t row, uint32_t lane, Query &q) {
     const uint32_t g = lane >> 4;
     const uint32_t source = (lane & 15u) + ((g & 1u) << 5);  // holds the scales of block g, in its half g / 2
+    Raw16<F32> lo_raw[kChunks], hi_raw[kChunks];
 #pragma unroll
     for (uint32_t c = 0; c < kChunks; ++c) {
-      float lo[16], hi[16];
+      lo_raw[c] = load16<F32>(base, row + c * 128u + g * 16u);
+      if constexpr (D > 64u) hi_raw[c] = load16<F32>(base, row + c * 128u + 64u + g * 16u);
+    }
 #pragma unroll
-      for (int i = 0; i < 16; ++i) lo[i] = hi[i] = 0.0f;
-      if (live) {
-        load_row16(base, row + c * 128u + g * 16u, f32, lo);
-        if constexpr (D > 64u) load_row16(base, row + c * 128u + 64u + g * 16u, f32, hi);
-      }
+    for (uint32_t c = 0; c < kChunks; ++c) {
+      float x[16];
       u32x4_t lo0, lo1, hi0, hi1;
-      const uint32_t lo_byte = split16(lo, block_field(lo), lo0, lo1);
+      widen16<F32>(lo_raw[c], x);
+      const uint32_t lo_byte = split16(x, block_field(x), lo0, lo1);
       const int32_t lo_scale = __shfl(static_cast<int>(lo_byte), static_cast<int>(source), 64);
       if constexpr (D == 64u) {
         // values 0..63 twice along the product: first term against the first copy of a key, second against the second
         q.term[0] = make_b_fp8(lo0, lo1);
         q.scale[0] = static_cast<uint32_t>(lo_scale) - (g >= 2u ? 5u : 0u);
       } else {
-        const uint32_t hi_byte = split16(hi, block_field(hi), hi0, hi1);
+        widen16<F32>(hi_raw[c], x);
+        const uint32_t hi_byte = split16(x, block_field(x), hi0, hi1);
         const int32_t hi_scale = __shfl(static_cast<int>(hi_byte), static_cast<int>(source), 64);
         const uint32_t scale = static_cast<uint32_t>(g >= 2u ? hi_scale : lo_scale);
         q.term[2u * c] = make_b_fp8(lo0, hi0);
@@ -181,6 +187,13 @@ struct Core {
         q.scale[2u * c] = scale;
         q.scale[2u * c + 1u] = scale - 5u;
       }
+    }
+  }
+  static __device__ __forceinline__ void load_query(uint64_t base, uint64_t row, bool f32, uint32_t lane, Query &q) {
+    if (f32) {
+      load_query<true>(base, row, lane, q);
+    } else {
+      load_query<false>(base, row, lane, q);
     }
   }
 
@@ -333,7 +346,7 @@ __device__ __forceinline__ Place place_at(const FerruleHipKvAttentionArgs &a, co
   return p;
 }
 
-// What a packed row is.
+// What a packed row is.  One behind the sequence's last stands at its first: what it computes is not written.
 struct PackedRow {
   uint64_t q;       // offset of its values in q
   uint64_t output;  // and in the output
@@ -400,7 +413,7 @@ __global__ __launch_bounds__(256, D <= 128u ? 4 : D == 256u ? 2 : 1) void kv_att
 
   const PackedRow mine = packed_row(a, s, kv_head, group, first_row + i);
   typename C::Query query;
-  C::load_query(a.q, mine.q, mine.live, (a.flags & FERRULE_HIP_KV_ATTENTION_QUERY_F32) != 0u, lane, query);
+  C::load_query(a.q, mine.q, (a.flags & FERRULE_HIP_KV_ATTENTION_QUERY_F32) != 0u, lane, query);
   const int32_t from = a.window == 0u ? static_cast<int32_t>(0x80000000u) : mine.position - static_cast<int32_t>(a.window - 1u);
   const int32_t sinks = a.window == 0u ? 0 : static_cast<int32_t>(a.sinks);
   const float factor = a.softmax_scale * 1.44269504088896341f;
@@ -619,7 +632,7 @@ __global__ __launch_bounds__(WAVES * 64u, (Rows<D, NQ, WAVES>::kOccupancy)) void
     const PackedRow row = packed_row(a, s, kv_head, group, wave_row + 16u * n + i);
     position[n] = row.position;
     from[n] = a.window == 0u ? static_cast<int32_t>(0x80000000u) : row.position - static_cast<int32_t>(a.window - 1u);
-    C::load_query(a.q, row.q, row.live, (a.flags & FERRULE_HIP_KV_ATTENTION_QUERY_F32) != 0u, lane, query[n]);
+    C::load_query(a.q, row.q, (a.flags & FERRULE_HIP_KV_ATTENTION_QUERY_F32) != 0u, lane, query[n]);
   }
   const int32_t sinks = a.window == 0u ? 0 : static_cast<int32_t>(a.sinks);
   const float factor = a.softmax_scale * 1.44269504088896341f;
@@ -1011,7 +1024,7 @@ SplitPlan plan_splits(const FerruleHipKvAttentionArgs &a) {
   const uint64_t target = tiles == 0u ? 1024u : 512u;
   const uint64_t least = tiles == 0u ? 2u * kWaves : 4u;
   uint64_t part = (segments * token_tiles + target - 1u) / target;
-  part = (part < least ? least : part) + 3u & ~3ull;
+  part = part < least ? least : part;
   uint64_t splits = (token_tiles + part - 1u) / part;
   plan.part_tiles = static_cast<uint32_t>(part < 0x40000000u ? part : 0x40000000u);
   plan.splits = static_cast<uint32_t>(splits);
@@ -1073,7 +1086,8 @@ void launch(const FerruleHipKvAttentionArgs &a, hipStream_t stream) {
       if constexpr (D <= 128u) kv_attention_rows_kernel<D, 2, 4><<<grid, 256, 0, stream>>>(a, plan);
       break;
     default:
-      if constexpr (D <= 128u) kv_attention_rows_kernel<D, 2, 8><<<grid, 512, 0, stream>>>(a, plan);
+      if constexpr (D == 64u) kv_attention_rows_kernel<D, 4, 4><<<grid, 256, 0, stream>>>(a, plan);
+      if constexpr (D == 128u) kv_attention_rows_kernel<D, 2, 8><<<grid, 512, 0, stream>>>(a, plan);
       break;
   }
   if (plan.splits > 1u) {
