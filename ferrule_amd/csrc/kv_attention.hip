@@ -98,102 +98,103 @@ struct Core {
     uint2 scale[kUnits];
   };
 
-  // 16 values of a row as they are in memory, and as f32 holding BF16
-  template <bool F32>
-  struct Raw16 {
-    u32x4_t w[F32 ? 4 : 2];
+  // 16 values of a row, as BF16 pairs
+  struct Pairs {
+    uint32_t w[8];
   };
   template <bool F32>
-  static __device__ __forceinline__ Raw16<F32> load16(uint64_t base, uint64_t at) {
-    const u32x4_t *src = F32 ? reinterpret_cast<const u32x4_t *>(global_ptr<const float>(base) + at)
-                             : reinterpret_cast<const u32x4_t *>(global_ptr<const uint16_t>(base) + at);
-    Raw16<F32> r;
+  static __device__ __forceinline__ Pairs load16(uint64_t base, uint64_t at) {
+    Pairs r;
+    if constexpr (F32) {
+      const f32x4_t *src = reinterpret_cast<const f32x4_t *>(global_ptr<const float>(base) + at);
 #pragma unroll
-    for (int i = 0; i < (F32 ? 4 : 2); ++i) r.w[i] = src[i];
-    return r;
-  }
-  template <bool F32>
-  static __device__ __forceinline__ void widen16(const Raw16<F32> &r, float (&x)[16]) {
+      for (int i = 0; i < 4; ++i) {
+        const f32x4_t x = src[i];
+        r.w[2 * i] = __builtin_bit_cast(uint32_t, bf16x2_t{static_cast<__bf16>(x[0]), static_cast<__bf16>(x[1])});
+        r.w[2 * i + 1] = __builtin_bit_cast(uint32_t, bf16x2_t{static_cast<__bf16>(x[2]), static_cast<__bf16>(x[3])});
+      }
+    } else {
+      const u32x4_t *src = reinterpret_cast<const u32x4_t *>(global_ptr<const uint16_t>(base) + at);
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      if constexpr (F32) {
-        x[e] = bf16_round(__uint_as_float(r.w[e >> 2][e & 3]));
-      } else {
-        const uint32_t w = r.w[e >> 3][(e >> 1) & 3];
-        x[e] = __uint_as_float((e & 1) ? w & 0xffff0000u : w << 16);
+      for (int i = 0; i < 2; ++i) {
+        const u32x4_t x = src[i];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) r.w[4 * i + e] = x[e];
       }
     }
+    return r;
   }
 
-  // Both terms of 16 values whose block's largest magnitude has the f32 exponent field `field`.
-  static __device__ __forceinline__ uint32_t split16(const float (&x)[16], uint32_t field, u32x4_t &q0, u32x4_t &q1) {
+  // Exponent field of the largest magnitude of a block of 32: the lane's 16 values and lane ^ 16's.
+  static __device__ __forceinline__ uint32_t block_field(const Pairs &x) {
+    typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
+    u16x2_t top = {0, 0};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2_t, x.w[i] & 0x7fff7fffu));
+    const uint32_t most = max(static_cast<uint32_t>(top[0]), static_cast<uint32_t>(top[1]));
+    return max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), 16, 64))) >> 7;
+  }
+
+  // Both terms of 16 values whose block's largest magnitude has the exponent field `field`; the converters take
+  // the scale with them.
+  static __device__ __forceinline__ uint32_t split16(const Pairs &x, uint32_t field, u32x4_t &q0, u32x4_t &q1) {
+    typedef short i16x2_t __attribute__((ext_vector_type(2)));
     // largest magnitude to [128, 256): below E4M3's 448; the remainder is at most 2^3 of this scale, 2^8 of the next
     const uint32_t byte = min(max(field, 13u), 254u) - 7u;
-    const float inverse0 = __uint_as_float((254u - byte) << 23), scale0 = __uint_as_float(byte << 23);
-    const float inverse1 = __uint_as_float((254u - (byte - 5u)) << 23);
+    const float scale0 = __uint_as_float(byte << 23), scale1 = __uint_as_float((byte - 5u) << 23);
     const bool finite = field < 255u;
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-      int a = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * w] * inverse0, x[4 * w + 1] * inverse0, 0, false);
-      a = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * w + 2] * inverse0, x[4 * w + 3] * inverse0, a, true);
-      const f32x2_t lo = __builtin_amdgcn_cvt_pk_f32_fp8(a, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(a, true);
-      int b = __builtin_amdgcn_cvt_pk_fp8_f32((x[4 * w] - lo[0] * scale0) * inverse1,
-                                              (x[4 * w + 1] - lo[1] * scale0) * inverse1, 0, false);
-      b = __builtin_amdgcn_cvt_pk_fp8_f32((x[4 * w + 2] - hi[0] * scale0) * inverse1,
-                                          (x[4 * w + 3] - hi[1] * scale0) * inverse1, b, true);
-      q0[w] = finite ? static_cast<uint32_t>(a) : 0x7f7f7f7fu;  // a row with an infinity or a NaN: NaN scores
-      q1[w] = finite ? static_cast<uint32_t>(b) : 0u;
+      const uint32_t lo = x.w[2 * w], hi = x.w[2 * w + 1];
+      i16x2_t a = {0, 0}, b = {0, 0};
+      a = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(a, __builtin_bit_cast(bf16x2_t, lo), scale0, false);
+      a = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(a, __builtin_bit_cast(bf16x2_t, hi), scale0, true);
+      const uint32_t first = __builtin_bit_cast(uint32_t, a);
+      const f32x2_t back0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(first, scale0, false);
+      const f32x2_t back1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(first, scale0, true);
+      b = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(b, __uint_as_float(lo << 16) - back0[0],
+                                                   __uint_as_float(lo & 0xffff0000u) - back0[1], scale1, false);
+      b = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(b, __uint_as_float(hi << 16) - back1[0],
+                                                   __uint_as_float(hi & 0xffff0000u) - back1[1], scale1, true);
+      q0[w] = finite ? first : 0x7f7f7f7fu;  // a row with an infinity or a NaN: NaN scores
+      q1[w] = finite ? __builtin_bit_cast(uint32_t, b) : 0u;
     }
     return byte;
   }
 
-  static __device__ __forceinline__ uint32_t block_field(const float (&x)[16]) {
-    uint32_t top = 0u;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
-    top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 16, 64)));  // the block's other 16 values
-    return top >> 23;
-  }
-
   // The lane's part of a tile's query rows.
-  template <bool F32>
-  static __device__ __forceinline__ void load_query(uint64_t base, uint64_t row, uint32_t lane, Query &q) {
+  static __device__ __forceinline__ void load_query(uint64_t base, uint64_t row, bool f32, uint32_t lane, Query &q) {
     const uint32_t g = lane >> 4;
     const uint32_t source = (lane & 15u) + ((g & 1u) << 5);  // holds the scales of block g, in its half g / 2
-    Raw16<F32> lo_raw[kChunks], hi_raw[kChunks];
+    constexpr uint32_t kHalves = D == 64u ? 1u : 2u;         // of a 128-value piece
+    Pairs pairs[kChunks][kHalves];
 #pragma unroll
     for (uint32_t c = 0; c < kChunks; ++c) {
-      lo_raw[c] = load16<F32>(base, row + c * 128u + g * 16u);
-      if constexpr (D > 64u) hi_raw[c] = load16<F32>(base, row + c * 128u + 64u + g * 16u);
-    }
 #pragma unroll
-    for (uint32_t c = 0; c < kChunks; ++c) {
-      float x[16];
-      u32x4_t lo0, lo1, hi0, hi1;
-      widen16<F32>(lo_raw[c], x);
-      const uint32_t lo_byte = split16(x, block_field(x), lo0, lo1);
-      const int32_t lo_scale = __shfl(static_cast<int>(lo_byte), static_cast<int>(source), 64);
-      if constexpr (D == 64u) {
-        // values 0..63 twice along the product: first term against the first copy of a key, second against the second
-        q.term[0] = make_b_fp8(lo0, lo1);
-        q.scale[0] = static_cast<uint32_t>(lo_scale) - (g >= 2u ? 5u : 0u);
-      } else {
-        widen16<F32>(hi_raw[c], x);
-        const uint32_t hi_byte = split16(x, block_field(x), hi0, hi1);
-        const int32_t hi_scale = __shfl(static_cast<int>(hi_byte), static_cast<int>(source), 64);
-        const uint32_t scale = static_cast<uint32_t>(g >= 2u ? hi_scale : lo_scale);
-        q.term[2u * c] = make_b_fp8(lo0, hi0);
-        q.term[2u * c + 1u] = make_b_fp8(lo1, hi1);
-        q.scale[2u * c] = scale;
-        q.scale[2u * c + 1u] = scale - 5u;
+      for (uint32_t h = 0; h < kHalves; ++h) {
+        const uint64_t at = row + c * 128u + h * 64u + g * 16u;
+        pairs[c][h] = f32 ? load16<true>(base, at) : load16<false>(base, at);
       }
     }
-  }
-  static __device__ __forceinline__ void load_query(uint64_t base, uint64_t row, bool f32, uint32_t lane, Query &q) {
-    if (f32) {
-      load_query<true>(base, row, lane, q);
-    } else {
-      load_query<false>(base, row, lane, q);
+#pragma unroll
+    for (uint32_t c = 0; c < kChunks; ++c) {
+      u32x4_t first[kHalves], second[kHalves];
+      int32_t scale[kHalves];
+#pragma unroll
+      for (uint32_t h = 0; h < kHalves; ++h) {
+        const uint32_t byte = split16(pairs[c][h], block_field(pairs[c][h]), first[h], second[h]);
+        scale[h] = __shfl(static_cast<int>(byte), static_cast<int>(source), 64);
+      }
+      if constexpr (D == 64u) {
+        // values 0..63 twice along the product: first term against the first copy of a key, second against the second
+        q.term[0] = make_b_fp8(first[0], second[0]);
+        q.scale[0] = static_cast<uint32_t>(scale[0]) - (g >= 2u ? 5u : 0u);
+      } else {
+        q.term[2u * c] = make_b_fp8(first[0], first[kHalves - 1u]);
+        q.term[2u * c + 1u] = make_b_fp8(second[0], second[kHalves - 1u]);
+        q.scale[2u * c] = static_cast<uint32_t>(g >= 2u ? scale[kHalves - 1u] : scale[0]);
+        q.scale[2u * c + 1u] = q.scale[2u * c] - 5u;
+      }
     }
   }
 
