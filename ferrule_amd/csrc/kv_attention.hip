@@ -31,6 +31,9 @@
 #include "kv_cache.cuh"
 #include "mx_core.cuh"
 
+#ifndef VWT
+#define VWT 64u
+#endif
 namespace ferrule_hip {
 namespace {
 
@@ -45,6 +48,7 @@ struct SplitPlan {
   uint32_t page_shift;  // log2 of page_tokens
   uint32_t part_tiles;  // 32-token tiles of a part, a multiple of what a workgroup takes at a time
   uint32_t splits;      // parts at most; the last takes what is left
+  uint32_t wide;        // decode kernel: one workgroup of as many waves as a CU holds instead of parts
   uint64_t partials;    // byte offsets in the workspace
   uint64_t statistics;
 };
@@ -369,26 +373,44 @@ __device__ __forceinline__ PackedRow packed_row(const FerruleHipKvAttentionArgs 
   return p;
 }
 
-__device__ __forceinline__ void store8(uint64_t output, uint64_t at, bool f32, const float (&x)[8]) {
+__device__ __forceinline__ uint32_t bf16_pair(float x, float y) {  // to nearest, ties to even
+  return __builtin_bit_cast(uint32_t, bf16x2_t{static_cast<__bf16>(x), static_cast<__bf16>(y)});
+}
+
+// N consecutive values of a row
+template <uint32_t N>
+__device__ __forceinline__ void store(uint64_t output, uint64_t at, bool f32, const float (&x)[N]) {
+  static_assert(N == 2u || N == 4u || N == 8u, "whole stores");
   if (f32) {
-    f32x4_t *dst = reinterpret_cast<f32x4_t *>(global_ptr<float>(output) + at);
-    dst[0] = f32x4_t{x[0], x[1], x[2], x[3]};
-    dst[1] = f32x4_t{x[4], x[5], x[6], x[7]};
-  } else {
-    u32x4_t w;
+    float *dst = global_ptr<float>(output) + at;
+    if constexpr (N == 2u) {
+      *reinterpret_cast<float2 *>(dst) = make_float2(x[0], x[1]);
+    } else {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) w[e] = bf16_rne_bits(x[2 * e]) | (static_cast<uint32_t>(bf16_rne_bits(x[2 * e + 1])) << 16);
-    *reinterpret_cast<u32x4_t *>(global_ptr<uint16_t>(output) + at) = w;
+      for (uint32_t q = 0; q < N / 4u; ++q) {
+        reinterpret_cast<f32x4_t *>(dst)[q] = f32x4_t{x[4u * q], x[4u * q + 1u], x[4u * q + 2u], x[4u * q + 3u]};
+      }
+    }
+  } else {
+    uint16_t *dst = global_ptr<uint16_t>(output) + at;
+    uint32_t w[N / 2u];
+#pragma unroll
+    for (uint32_t e = 0; e < N / 2u; ++e) w[e] = bf16_pair(x[2u * e], x[2u * e + 1u]);
+    if constexpr (N == 2u) *reinterpret_cast<uint32_t *>(dst) = w[0];
+    if constexpr (N == 4u) *reinterpret_cast<uint2 *>(dst) = make_uint2(w[0], w[1]);
+    if constexpr (N == 8u) *reinterpret_cast<u32x4_t *>(dst) = u32x4_t{w[0], w[1], w[2], w[3]};
   }
 }
 
-// Few rows: 16 of them, the token tiles shared out over the four waves.
+// Few rows: 16 of them, the token tiles shared out over the WAVES waves.
 template <uint32_t D>
-__global__ __launch_bounds__(256, D <= 128u ? 4 : D == 256u ? 2 : 1) void kv_attention_decode_kernel(FerruleHipKvAttentionArgs a, SplitPlan plan) {
+constexpr uint32_t kDecodeOccupancy = D <= 128u ? 4u : D == 256u ? 2u : 1u;  // waves per SIMD that the registers allow
+template <uint32_t D, uint32_t WAVES>
+__global__ __launch_bounds__(WAVES * 64u, kDecodeOccupancy<D>) void kv_attention_decode_kernel(FerruleHipKvAttentionArgs a, SplitPlan plan) {
   using C = Core<D>;
   constexpr uint32_t kPitch = 128u + 4u;  // floats of a row in LDS
-  __shared__ __align__(16) float joined[kWaves][kTileRows][kPitch];
-  __shared__ float top_of[kWaves][kTileRows], sum_of[kWaves][kTileRows];
+  __shared__ __align__(16) float joined[WAVES][kTileRows][kPitch];
+  __shared__ float top_of[WAVES][kTileRows], sum_of[WAVES][kTileRows];
   const uint32_t lane = threadIdx.x & 63u;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t i = lane & 15u, g = lane >> 4;
@@ -434,16 +456,16 @@ __global__ __launch_bounds__(256, D <= 128u ? 4 : D == 256u ? 2 : 1) void kv_att
   Place next_place = {0u, 0u, 0u, false};
   if (begin < end) {
     next_place = place_at<D>(a, plan, range, kv_head, begin + wave, end, page_of(a, plan, range, b, begin + wave, end), bad);
-    next_page = page_of(a, plan, range, b, begin + wave + kWaves, end);
+    next_page = page_of(a, plan, range, b, begin + wave + WAVES, end);
   }
   C::template load_keys<true>(k_payload + next_place.payload, k_scales + next_place.scales, offset, keys);
   C::template load_values<true>(v_payload + next_place.payload, v_scales + next_place.scales, offset, values);
-  for (uint32_t v = begin + wave; v < end; v += kWaves) {
+  for (uint32_t v = begin + wave; v < end; v += WAVES) {
     // keys and values are loaded one step ahead, as soon as the registers of this step's are free; two or
     // three steps ahead at 3 or 2 waves per SIMD took as long (64 x 8192 tokens, 8 heads: 112, 110, 122 us)
     const Place here = next_place;
-    next_place = place_at<D>(a, plan, range, kv_head, v + kWaves, end, next_page, bad);
-    next_page = page_of(a, plan, range, b, v + 2u * kWaves, end);
+    next_place = place_at<D>(a, plan, range, kv_head, v + WAVES, end, next_page, bad);
+    next_page = page_of(a, plan, range, b, v + 2u * WAVES, end);
     f32x4_t score[2];
     C::scores(keys, query, lane, score);
     C::template load_keys<true>(k_payload + next_place.payload, k_scales + next_place.scales, offset, keys);
@@ -517,25 +539,26 @@ __global__ __launch_bounds__(256, D <= 128u ? 4 : D == 256u ? 2 : 1) void kv_att
   }
 
   if (bad && lane == 0u) kv_report(a.error);
-  // join the four waves, 128 values at a time
+  // join the waves, 128 values at a time: 16 rows in pieces of kPiece
+  constexpr uint32_t kPiece = 32u / WAVES, kPieces = 128u / kPiece;
   sum = row_sum(sum);
   if (g == 0u) {
     top_of[wave][i] = top;
     sum_of[wave][i] = sum;
   }
   __syncthreads();
-  const uint32_t row_out = threadIdx.x >> 4, d_out = (threadIdx.x & 15u) * 8u;  // 16 rows x 128 values in pieces of 8
+  const uint32_t row_out = threadIdx.x / kPieces, d_out = threadIdx.x % kPieces * kPiece;
   float row_top = -INFINITY, total = 0.0f;
 #pragma unroll
-  for (uint32_t w = 0; w < kWaves; ++w) row_top = fmaxf(row_top, top_of[w][row_out]);
+  for (uint32_t w = 0; w < WAVES; ++w) row_top = fmaxf(row_top, top_of[w][row_out]);
   const float row_base = row_top == -INFINITY ? 0.0f : row_top;
 #pragma unroll
-  for (uint32_t w = 0; w < kWaves; ++w) {
+  for (uint32_t w = 0; w < WAVES; ++w) {
     total += sum_of[w][row_out] * part_weight(top_of[w][row_out], row_base);
   }
   float own_top = -INFINITY;
 #pragma unroll
-  for (uint32_t w = 0; w < kWaves; ++w) own_top = fmaxf(own_top, top_of[w][i]);
+  for (uint32_t w = 0; w < WAVES; ++w) own_top = fmaxf(own_top, top_of[w][i]);
   const float keep = part_weight(top, own_top);
   const PackedRow target = packed_row(a, s, kv_head, group, first_row + row_out);
   const bool seen_any = total != 0.0f;  // NaN too
@@ -555,23 +578,23 @@ __global__ __launch_bounds__(256, D <= 128u ? 4 : D == 256u ? 2 : 1) void kv_att
     }
     __syncthreads();
     if (target.live && d_out < D) {
-      float x[8] = {};
+      float x[kPiece] = {};
 #pragma unroll
-      for (uint32_t w = 0; w < kWaves; ++w) {
+      for (uint32_t w = 0; w < WAVES; ++w) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] += joined[w][row_out][d_out + e];
+        for (uint32_t e = 0; e < kPiece; ++e) x[e] += joined[w][row_out][d_out + e];
       }
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] *= norm;
+      for (uint32_t e = 0; e < kPiece; ++e) x[e] *= norm;
       const uint32_t d = c * 128u + d_out;
       if (whole) {
-        store8(a.output, target.output + d, (a.flags & FERRULE_HIP_KV_ATTENTION_OUTPUT_F32) != 0u, x);
+        store<kPiece>(a.output, target.output + d, (a.flags & FERRULE_HIP_KV_ATTENTION_OUTPUT_F32) != 0u, x);
       } else {
-        store8(a.workspace + plan.partials, (target.index * plan.splits + split) * D + d, true, x);
+        store<kPiece>(a.workspace + plan.partials, (target.index * plan.splits + split) * D + d, true, x);
       }
     }
   }
-  if (!whole && target.live && (threadIdx.x & 15u) == 0u) {
+  if (!whole && target.live && threadIdx.x % kPieces == 0u) {
     global_ptr<float2>(a.workspace + plan.statistics)[target.index * plan.splits + split] = make_float2(row_top, total);
   }
 }
@@ -865,9 +888,9 @@ __global__ __launch_bounds__(WAVES * 64u, (Rows<D, NQ, WAVES>::kOccupancy)) void
         for (uint32_t e = 0; e < 8u; ++e) x[e] = out[n][4u * u + (e & 3u)][2u * half + (e >> 2)] * norm;
         const uint32_t d = 64u * u + 16u * g + 8u * half;
         if (whole) {
-          store8(a.output, row.output + d, (a.flags & FERRULE_HIP_KV_ATTENTION_OUTPUT_F32) != 0u, x);
+          store(a.output, row.output + d, (a.flags & FERRULE_HIP_KV_ATTENTION_OUTPUT_F32) != 0u, x);
         } else {
-          store8(a.workspace + plan.partials, (row.index * plan.splits + split) * D + d, true, x);
+          store(a.workspace + plan.partials, (row.index * plan.splits + split) * D + d, true, x);
         }
       }
     }
@@ -897,16 +920,6 @@ __device__ __forceinline__ Joined joined_row(const FerruleHipKvAttentionArgs &a,
   }
   j.row = packed_row(a, s, kv_head, group, j.parts != 0u ? r : 0u);
   return j;
-}
-
-__device__ __forceinline__ void store4(uint64_t output, uint64_t at, bool f32, const f32x4_t &x) {
-  if (f32) {
-    *reinterpret_cast<f32x4_t *>(global_ptr<float>(output) + at) = x;
-  } else {
-    *reinterpret_cast<uint2 *>(global_ptr<uint16_t>(output) + at) =
-        make_uint2(bf16_rne_bits(x[0]) | (static_cast<uint32_t>(bf16_rne_bits(x[1])) << 16),
-                   bf16_rne_bits(x[2]) | (static_cast<uint32_t>(bf16_rne_bits(x[3])) << 16));
-  }
 }
 
 // Joins the parts of every row, in their order.  Up to kFewParts parts: a thread has four values of a
@@ -942,8 +955,9 @@ __global__ __launch_bounds__(256) void kv_attention_join_few_kernel(FerruleHipKv
     total += part[p].y * weight;
     x += value[p] * weight;
   }
-  store4(a.output, j.row.output + 4u * quad, (a.flags & FERRULE_HIP_KV_ATTENTION_OUTPUT_F32) != 0u,
-         x * (total != 0.0f ? 1.0f / total : 0.0f));
+  const float norm = total != 0.0f ? 1.0f / total : 0.0f;
+  const float y[4] = {x[0] * norm, x[1] * norm, x[2] * norm, x[3] * norm};
+  store(a.output, j.row.output + 4u * quad, (a.flags & FERRULE_HIP_KV_ATTENTION_OUTPUT_F32) != 0u, y);
 }
 
 // More parts: a workgroup per (row, query head).  The maximum and the sum go over all parts at once; the
@@ -987,8 +1001,9 @@ __global__ __launch_bounds__(256) void kv_attention_join_kernel(FerruleHipKvAtte
 #pragma unroll
   for (uint32_t l = 1; l < kLanes; ++l) x += added[l * kQuads + threadIdx.x];
   total = (wave_sums[0] + wave_sums[1]) + (wave_sums[2] + wave_sums[3]);
-  store4(a.output, j.row.output + 4u * threadIdx.x, (a.flags & FERRULE_HIP_KV_ATTENTION_OUTPUT_F32) != 0u,
-         x * (total != 0.0f ? 1.0f / total : 0.0f));
+  const float norm = total != 0.0f ? 1.0f / total : 0.0f;
+  const float y[4] = {x[0] * norm, x[1] * norm, x[2] * norm, x[3] * norm};
+  store(a.output, j.row.output + 4u * threadIdx.x, (a.flags & FERRULE_HIP_KV_ATTENTION_OUTPUT_F32) != 0u, y);
 }
 
 uint32_t row_bound(const FerruleHipKvAttentionArgs &a) { return a.max_query_length < a.rows ? a.max_query_length : a.rows; }
@@ -1022,10 +1037,18 @@ SplitPlan plan_splits(const FerruleHipKvAttentionArgs &a) {
   }
   const uint64_t token_tiles = tokens / kTileTokens + 1u;
   const uint64_t segments = static_cast<uint64_t>(a.batch) * a.kv_heads * row_tiles(a, plan.tile_rows);
-  const uint64_t target = tiles == 0u ? 1024u : 512u;
-  const uint64_t least = tiles == 0u ? 2u * kWaves : 4u;
+  // Decode: about a thousand parts, which the card holds at once (64 sequences of 8192 tokens, 8 heads: 99 us, with
+  // 2048 parts 112).  Rows: no more than fill it once, and parts long enough to pay for their f32 partials
+  // (4 x 512 rows over 8192 tokens: 244 us, with 512 parts 285).
+  const uint64_t target = tiles == 0u ? 1024u : 256u;
+  const uint64_t least = tiles == 0u ? 2u * kWaves : 16u;
   uint64_t part = (segments * token_tiles + target - 1u) / target;
   part = part < least ? least : part;
+  // A range of a few steps of a CU's sixteen waves is not worth a second launch while there are CUs for all segments.
+  if (tiles == 0u && a.head_dim <= 128u && part < token_tiles && token_tiles <= VWT && segments <= 256u) {
+    plan.wide = 1u;
+    part = token_tiles;
+  }
   uint64_t splits = (token_tiles + part - 1u) / part;
   plan.part_tiles = static_cast<uint32_t>(part < 0x40000000u ? part : 0x40000000u);
   plan.splits = static_cast<uint32_t>(splits);
@@ -1080,7 +1103,15 @@ void launch(const FerruleHipKvAttentionArgs &a, hipStream_t stream) {
   const SplitPlan plan = plan_splits(a);
   const dim3 grid(row_tiles(a, plan.tile_rows) * a.kv_heads * plan.splits, a.batch);
   switch (rows_of_workgroup(a)) {
-    case 0: kv_attention_decode_kernel<D><<<grid, 256, 0, stream>>>(a, plan); break;
+    case 0:
+      if constexpr (D <= 128u) {
+        if (plan.wide != 0u) {
+          kv_attention_decode_kernel<D, 16><<<grid, 1024, 0, stream>>>(a, plan);
+          break;
+        }
+      }
+      kv_attention_decode_kernel<D, kWaves><<<grid, 256, 0, stream>>>(a, plan);
+      break;
     case 64: kv_attention_rows_kernel<D, 1, 4><<<grid, 256, 0, stream>>>(a, plan); break;
     case 128:
       if constexpr (D == 256u) kv_attention_rows_kernel<D, 1, 8><<<grid, 512, 0, stream>>>(a, plan);
