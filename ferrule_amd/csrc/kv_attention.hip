@@ -31,9 +31,6 @@
 #include "kv_cache.cuh"
 #include "mx_core.cuh"
 
-#ifndef VWT
-#define VWT 64u
-#endif
 namespace ferrule_hip {
 namespace {
 
@@ -166,27 +163,32 @@ struct Core {
     return byte;
   }
 
-  // The lane's part of a tile's query rows.
-  static __device__ __forceinline__ void load_query(uint64_t base, uint64_t row, bool f32, uint32_t lane, Query &q) {
-    const uint32_t g = lane >> 4;
-    const uint32_t source = (lane & 15u) + ((g & 1u) << 5);  // holds the scales of block g, in its half g / 2
-    constexpr uint32_t kHalves = D == 64u ? 1u : 2u;         // of a 128-value piece
+  // The lane's part of a tile's query rows, in two steps: what is asked for between them need not wait for q.
+  static constexpr uint32_t kHalves = D == 64u ? 1u : 2u;  // of a 128-value piece
+  struct RawQuery {
     Pairs pairs[kChunks][kHalves];
+  };
+  static __device__ __forceinline__ void load_query(uint64_t base, uint64_t row, bool f32, uint32_t lane, RawQuery &raw) {
+    const uint32_t g = lane >> 4;
 #pragma unroll
     for (uint32_t c = 0; c < kChunks; ++c) {
 #pragma unroll
       for (uint32_t h = 0; h < kHalves; ++h) {
         const uint64_t at = row + c * 128u + h * 64u + g * 16u;
-        pairs[c][h] = f32 ? load16<true>(base, at) : load16<false>(base, at);
+        raw.pairs[c][h] = f32 ? load16<true>(base, at) : load16<false>(base, at);
       }
     }
+  }
+  static __device__ __forceinline__ void split_query(const RawQuery &raw, uint32_t lane, Query &q) {
+    const uint32_t g = lane >> 4;
+    const uint32_t source = (lane & 15u) + ((g & 1u) << 5);  // holds the scales of block g, in its half g / 2
 #pragma unroll
     for (uint32_t c = 0; c < kChunks; ++c) {
       u32x4_t first[kHalves], second[kHalves];
       int32_t scale[kHalves];
 #pragma unroll
       for (uint32_t h = 0; h < kHalves; ++h) {
-        const uint32_t byte = split16(pairs[c][h], block_field(pairs[c][h]), first[h], second[h]);
+        const uint32_t byte = split16(raw.pairs[c][h], block_field(raw.pairs[c][h]), first[h], second[h]);
         scale[h] = __shfl(static_cast<int>(byte), static_cast<int>(source), 64);
       }
       if constexpr (D == 64u) {
@@ -435,8 +437,24 @@ __global__ __launch_bounds__(WAVES * 64u, kDecodeOccupancy<D>) void kv_attention
   const bool whole = parts == 1u;  // no join
 
   const PackedRow mine = packed_row(a, s, kv_head, group, first_row + i);
+  // a short range is a chain of memory latencies: the page number, then everything else at once
+  bool bad = false;  // a page number outside the cache
+  int32_t next_page = 0;
+  Place next_place = {0u, 0u, 0u, false};
+  const int32_t first_page = begin < end ? page_of(a, plan, range, b, begin + wave, end) : 0;
+  if (begin < end) next_page = page_of(a, plan, range, b, begin + wave + WAVES, end);
+  typename C::RawQuery raw_query;
+  C::load_query(a.q, mine.q, (a.flags & FERRULE_HIP_KV_ATTENTION_QUERY_F32) != 0u, lane, raw_query);
+  if (begin < end) next_place = place_at<D>(a, plan, range, kv_head, begin + wave, end, first_page, bad);
+  const uint8_t *k_payload = global_ptr<const uint8_t>(a.k_payload), *k_scales = global_ptr<const uint8_t>(a.k_scales);
+  const uint8_t *v_payload = global_ptr<const uint8_t>(a.v_payload), *v_scales = global_ptr<const uint8_t>(a.v_scales);
+  const typename C::Offsets offset = C::offsets(lane);
+  typename C::Keys keys;
+  typename C::Values values;
+  C::template load_keys<true>(k_payload + next_place.payload, k_scales + next_place.scales, offset, keys);
+  C::template load_values<true>(v_payload + next_place.payload, v_scales + next_place.scales, offset, values);
   typename C::Query query;
-  C::load_query(a.q, mine.q, (a.flags & FERRULE_HIP_KV_ATTENTION_QUERY_F32) != 0u, lane, query);
+  C::split_query(raw_query, lane, query);
   const int32_t from = a.window == 0u ? static_cast<int32_t>(0x80000000u) : mine.position - static_cast<int32_t>(a.window - 1u);
   const int32_t sinks = a.window == 0u ? 0 : static_cast<int32_t>(a.sinks);
   const float factor = a.softmax_scale * 1.44269504088896341f;
@@ -446,20 +464,6 @@ __global__ __launch_bounds__(WAVES * 64u, kDecodeOccupancy<D>) void kv_attention
   for (uint32_t c = 0; c < C::kColumns; ++c) out[c] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
   float top = -INFINITY, base = 0.0f, sum = 0.0f;  // base = top, or 0 while the row has seen nothing
 
-  const uint8_t *k_payload = global_ptr<const uint8_t>(a.k_payload), *k_scales = global_ptr<const uint8_t>(a.k_scales);
-  const uint8_t *v_payload = global_ptr<const uint8_t>(a.v_payload), *v_scales = global_ptr<const uint8_t>(a.v_scales);
-  const typename C::Offsets offset = C::offsets(lane);
-  typename C::Keys keys;
-  typename C::Values values;
-  bool bad = false;  // a page number outside the cache
-  int32_t next_page = 0;
-  Place next_place = {0u, 0u, 0u, false};
-  if (begin < end) {
-    next_place = place_at<D>(a, plan, range, kv_head, begin + wave, end, page_of(a, plan, range, b, begin + wave, end), bad);
-    next_page = page_of(a, plan, range, b, begin + wave + WAVES, end);
-  }
-  C::template load_keys<true>(k_payload + next_place.payload, k_scales + next_place.scales, offset, keys);
-  C::template load_values<true>(v_payload + next_place.payload, v_scales + next_place.scales, offset, values);
   for (uint32_t v = begin + wave; v < end; v += WAVES) {
     // keys and values are loaded one step ahead, as soon as the registers of this step's are free; two or
     // three steps ahead at 3 or 2 waves per SIMD took as long (64 x 8192 tokens, 8 heads: 112, 110, 122 us)
@@ -649,14 +653,14 @@ __global__ __launch_bounds__(WAVES * 64u, (Rows<D, NQ, WAVES>::kOccupancy)) void
   const uint32_t wave_row = first_row + wave * 16u * NQ;
   const int32_t wave_low = s.position + static_cast<int32_t>(min(wave_row, last_row) / group);
   const int32_t wave_high = s.position + static_cast<int32_t>(min(wave_row + 16u * NQ - 1u, last_row) / group);
-  typename C::Query query[NQ];
   int32_t position[NQ], from[NQ];
+  uint64_t row_q[NQ];
 #pragma unroll
   for (uint32_t n = 0; n < NQ; ++n) {
     const PackedRow row = packed_row(a, s, kv_head, group, wave_row + 16u * n + i);
     position[n] = row.position;
     from[n] = a.window == 0u ? static_cast<int32_t>(0x80000000u) : row.position - static_cast<int32_t>(a.window - 1u);
-    C::load_query(a.q, row.q, (a.flags & FERRULE_HIP_KV_ATTENTION_QUERY_F32) != 0u, lane, query[n]);
+    row_q[n] = row.q;
   }
   const int32_t sinks = a.window == 0u ? 0 : static_cast<int32_t>(a.sinks);
   const float factor = a.softmax_scale * 1.44269504088896341f;
@@ -726,6 +730,15 @@ __global__ __launch_bounds__(WAVES * 64u, (Rows<D, NQ, WAVES>::kOccupancy)) void
     for (uint32_t t = 0; t < kSub; ++t) now[t] = page(begin + t);
     load_pieces(begin, page(begin + own_tile));
     load_tiles(begin, now);
+  }
+  typename C::Query query[NQ];
+#pragma unroll
+  for (uint32_t n = 0; n < NQ; ++n) {
+    typename C::RawQuery raw_query;
+    C::load_query(a.q, row_q[n], (a.flags & FERRULE_HIP_KV_ATTENTION_QUERY_F32) != 0u, lane, raw_query);
+    C::split_query(raw_query, lane, query[n]);
+  }
+  if (begin < end) {
     stage_pieces(0u);
     load_pieces(begin + kSub, page(begin + kSub + own_tile));
     piece_page = page(begin + 2u * kSub + own_tile);
@@ -1045,7 +1058,7 @@ SplitPlan plan_splits(const FerruleHipKvAttentionArgs &a) {
   uint64_t part = (segments * token_tiles + target - 1u) / target;
   part = part < least ? least : part;
   // A range of a few steps of a CU's sixteen waves is not worth a second launch while there are CUs for all segments.
-  if (tiles == 0u && a.head_dim <= 128u && part < token_tiles && token_tiles <= VWT && segments <= 256u) {
+  if (tiles == 0u && a.head_dim <= 128u && part < token_tiles && token_tiles <= 64u && segments <= 256u) {
     plan.wide = 1u;
     part = token_tiles;
   }
@@ -1106,7 +1119,7 @@ void launch(const FerruleHipKvAttentionArgs &a, hipStream_t stream) {
     case 0:
       if constexpr (D <= 128u) {
         if (plan.wide != 0u) {
-          kv_attention_decode_kernel<D, 16><<<grid, 1024, 0, stream>>>(a, plan);
+          kv_attention_decode_kernel<D, 8><<<grid, 512, 0, stream>>>(a, plan);
           break;
         }
       }
