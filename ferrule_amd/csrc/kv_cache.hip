@@ -1,10 +1,8 @@
 // Writing the MXFP4 key/value cache and reading it back (no reference symbol; formats, layout and
 // batch description: include/ferrule_hip_provider.h).
 //
-// A wave owns one head of eight neighbouring tokens, the unit of the value layout: lane = (token
-// lane / 8, piece lane % 8), a piece being 16 values, so a scale block is two adjacent lanes and
-// its maximum one exchange.  Both kernels move a row's bytes once and are bound by memory for
-// whole prompts, by launch and latency for a decode step's rows.
+// Both kernels move a row's bytes once and are bound by memory for whole prompts, by launch and latency
+// for a decode step's rows.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -16,26 +14,27 @@ namespace {
 
 constexpr uint32_t kWaves = 4;
 
-// Where a wave works: eight tokens of one head.
+// Where a wave works: some neighbouring tokens of one head.
 struct KvTile {
   KvSequence sequence;
   uint32_t head;
   uint32_t page_token;  // of the tile's first token
   uint64_t page_head;   // page * kv_heads + head
   bool page_valid;      // false: no token of the tile has a place
-  int32_t first;        // position of the tile's first token, a multiple of 8
+  int32_t first;        // position of the tile's first token, a multiple of TOKENS
 };
 
-__device__ __forceinline__ bool kv_tile(const FerruleHipKvCacheArgs &a, KvTile &tile) {
+// Tile `index` of sequence blockIdx.y, by head first; false when the sequence has no such tile.
+template <uint32_t TOKENS>
+__device__ __forceinline__ bool kv_tile(const FerruleHipKvCacheArgs &a, uint32_t index, KvTile &tile) {
   const uint32_t b = blockIdx.y;
-  const uint32_t wave = __builtin_amdgcn_readfirstlane(blockIdx.x * kWaves + (threadIdx.x >> 6));
-  tile.head = wave % a.kv_heads;
-  const uint32_t group = wave / a.kv_heads;
+  tile.head = index % a.kv_heads;
+  const uint32_t group = index / a.kv_heads;
   tile.sequence = kv_sequence(a.query_indptr, a.sequence_lengths, b, a.rows, a.max_query_length);
-  if (tile.sequence.bad && wave == 0u && (threadIdx.x & 63u) == 0u) kv_report(a.error);
-  // groups of eight are counted from the one that holds the first row; position may be negative
-  const int32_t base = tile.sequence.position & ~7;
-  tile.first = base + static_cast<int32_t>(group * 8u);
+  if (tile.sequence.bad && index == 0u && (threadIdx.x & 63u) == 0u) kv_report(a.error);
+  // tiles are counted from the one that holds the first row; position may be negative
+  const int32_t base = tile.sequence.position & ~static_cast<int32_t>(TOKENS - 1u);
+  tile.first = base + static_cast<int32_t>(group * TOKENS);
   if (tile.first >= tile.sequence.position + static_cast<int32_t>(tile.sequence.rows)) return false;
   tile.page_valid = false;
   tile.page_head = 0;
@@ -102,6 +101,9 @@ __device__ __forceinline__ uint32_t quantise16(const float (&x)[16], uint32_t (&
   return static_cast<uint32_t>(n + 127);
 }
 
+// A wave owns one head of eight neighbouring tokens, the unit of the value layout: lane = (token
+// lane / 8, piece lane % 8), a piece being 16 values, so a scale block is two adjacent lanes and
+// its maximum one exchange.
 template <typename T, uint32_t D>
 __global__ __launch_bounds__(256) void kv_append_kernel(FerruleHipKvCacheArgs a) {
   using Layout = KvLayout<D>;
@@ -109,7 +111,8 @@ __global__ __launch_bounds__(256) void kv_append_kernel(FerruleHipKvCacheArgs a)
   __shared__ __align__(16) uint8_t turned[kWaves][64][8];
   const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
   KvTile tile;
-  if (!kv_tile(a, tile) || !tile.page_valid) return;
+  const uint32_t index8 = __builtin_amdgcn_readfirstlane(blockIdx.x * kWaves + wave);
+  if (!kv_tile<8>(a, index8, tile) || !tile.page_valid) return;
   const uint32_t t = lane >> 3, piece = lane & 7u;
   const int32_t index = tile.first + static_cast<int32_t>(t) - tile.sequence.position;  // row of the sequence
   const bool live = index >= 0 && index < static_cast<int32_t>(tile.sequence.rows);
@@ -161,75 +164,95 @@ __global__ __launch_bounds__(256) void kv_append_kernel(FerruleHipKvCacheArgs a)
   }
 }
 
-// A pair of values as stored in the output row.
-__device__ __forceinline__ void store_pair(float *dst, float x, float y) {
-  *reinterpret_cast<float2 *>(dst) = make_float2(x, y);
-}
-__device__ __forceinline__ void store_pair(uint16_t *dst, float x, float y) {  // exact in BF16
-  *reinterpret_cast<uint32_t *>(dst) = (__float_as_uint(x) >> 16) | (__float_as_uint(y) & 0xffff0000u);
+// Eight values of a row from four payload bytes (values 0, 1 in the low byte) and their scale byte.
+__device__ __forceinline__ void expand8(uint32_t bytes, uint32_t scale_byte, float (&x)[8]) {
+  // 2^(byte - 127); 255 is a block of NaN.  The converter's scale is an f32 exponent field, which has no 2^-127:
+  // a byte of 0 (which the writer never writes) goes through the product below instead.
+  const float scale = scale_byte == kNanBlock ? __uint_as_float(0x7fc00000u) : e8m0_to_f32(scale_byte);
+#pragma unroll
+  for (int p = 0; p < 4; ++p) {
+    f32x2_t v;
+    // the byte is an immediate of the instruction
+    if (p == 0) v = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(bytes, 1.0f, 0);
+    if (p == 1) v = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(bytes, 1.0f, 1);
+    if (p == 2) v = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(bytes, 1.0f, 2);
+    if (p == 3) v = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(bytes, 1.0f, 3);
+    x[2 * p] = v[0] * scale;
+    x[2 * p + 1] = v[1] * scale;
+  }
 }
 
-__device__ __forceinline__ float block_scale(uint32_t byte) {
-  return byte == kNanBlock ? __uint_as_float(0x7fc00000u) : e8m0_to_f32(byte);
+__device__ __forceinline__ void store8(float *dst, const float (&x)[8]) {
+  reinterpret_cast<f32x4_t *>(dst)[0] = f32x4_t{x[0], x[1], x[2], x[3]};
+  reinterpret_cast<f32x4_t *>(dst)[1] = f32x4_t{x[4], x[5], x[6], x[7]};
+}
+__device__ __forceinline__ void store8(uint16_t *dst, const float (&x)[8]) {  // exact in BF16
+  i32x4_t w;
+#pragma unroll
+  for (int p = 0; p < 4; ++p) {
+    w[p] = static_cast<int>((__float_as_uint(x[2 * p]) >> 16) | (__float_as_uint(x[2 * p + 1]) & 0xffff0000u));
+  }
+  *reinterpret_cast<i32x4_t *>(dst) = w;
 }
 
+// A wave has the keys, or the values, of one head of 32 neighbouring tokens: a lane takes eight values
+// at a time, so that it stores 16 (BF16) or 32 bytes and a row is D / 8 lanes side by side.  With two values a lane
+// and store this took 45 us for 4 sequences of up to 8192 tokens, 8 heads of 128.
 template <typename T, uint32_t D>
 __global__ __launch_bounds__(256) void kv_read_kernel(FerruleHipKvCacheArgs a) {
   using Layout = KvLayout<D>;
+  constexpr uint32_t kLanes = D / 8u;       // of a row
+  constexpr uint32_t kTogether = 64u / kLanes;  // rows (keys) or groups of eight tokens (values) side by side
   const uint32_t lane = threadIdx.x & 63u;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(blockIdx.x * kWaves + (threadIdx.x >> 6));
+  const bool values = (wave & 1u) != 0u;
   KvTile tile;
-  if (!kv_tile(a, tile)) return;
-  const uint8_t *k_payload = global_ptr<const uint8_t>(a.k_payload) + Layout::payload(tile.page_head, a.page_tokens);
-  const uint8_t *k_scales = global_ptr<const uint8_t>(a.k_scales) + Layout::scales(tile.page_head, a.page_tokens);
-  const uint8_t *v_payload = global_ptr<const uint8_t>(a.v_payload) + Layout::payload(tile.page_head, a.page_tokens);
-  const uint8_t *v_scales = global_ptr<const uint8_t>(a.v_scales) + Layout::scales(tile.page_head, a.page_tokens);
+  if (!kv_tile<32>(a, wave >> 1, tile)) return;
+  const uint32_t column = lane % kLanes, part = lane / kLanes;
   const int32_t offset = tile.first - tile.sequence.position;  // row of the sequence of the tile's first token
   const int32_t rows = static_cast<int32_t>(tile.sequence.rows);
-  // keys: lane = (token, piece) as in the writer
-  {
-    const uint32_t t = lane >> 3, piece = lane & 7u;
-    const int32_t index = offset + static_cast<int32_t>(t);
-    if (index >= 0 && index < rows) {
-      T *out = global_ptr<T>(a.keys) + (tile.sequence.row + static_cast<uint64_t>(index)) * a.key_row_stride +
-               tile.head * a.key_head_stride;
+  const uint32_t block = column / 4u;
+  if (!values) {
+    const uint8_t *payload = global_ptr<const uint8_t>(a.k_payload) + Layout::payload(tile.page_head, a.page_tokens);
+    const uint8_t *scales = global_ptr<const uint8_t>(a.k_scales) + Layout::scales(tile.page_head, a.page_tokens);
+    T *out = global_ptr<T>(a.keys) + tile.head * a.key_head_stride + column * 8u;
+#pragma unroll 8
+    for (uint32_t t = part; t < 32u; t += kTogether) {
+      const int32_t index = offset + static_cast<int32_t>(t);
       const uint32_t token = tile.page_token + t;
-#pragma unroll
-      for (uint32_t c = 0; c < Layout::kKeyChunks; ++c) {
-        const uint32_t d = c * 128u + piece * 16u;
-        if (d >= D) break;
-        uint2 bytes = make_uint2(0u, 0u);
-        float scale = 0.0f;
-        if (tile.page_valid) {
-          bytes = *reinterpret_cast<const uint2 *>(k_payload + Layout::key_byte(token, c) + piece * 8u);
-          scale = block_scale(k_scales[Layout::key_scale(token, d / 32u)]);
-        }
-#pragma unroll
-        for (uint32_t i = 0; i < 8u; ++i) {
-          const uint32_t byte = (i < 4u ? bytes.x : bytes.y) >> (8u * (i & 3u));
-          store_pair(out + d + 2u * i, fp4_e2m1_decode(byte & 15u) * scale, fp4_e2m1_decode((byte >> 4) & 15u) * scale);
-        }
-      }
+      const uint32_t bytes = *reinterpret_cast<const uint32_t *>(payload + Layout::key_byte(token, column / 16u) +
+                                                                 (column % 16u) * 4u);
+      const uint32_t scale = scales[Layout::key_scale(token, block)];
+      if (index < 0 || index >= rows) continue;
+      float x[8];
+      expand8(tile.page_valid ? bytes : 0u, tile.page_valid ? scale : 127u, x);
+      store8(out + (tile.sequence.row + static_cast<uint64_t>(index)) * a.key_row_stride, x);
     }
+    return;
   }
-  // values: a lane has one pair of values of all eight tokens, a token's row is 64 lanes side by side
+  const uint8_t *payload = global_ptr<const uint8_t>(a.v_payload) + Layout::payload(tile.page_head, a.page_tokens);
+  const uint8_t *scales = global_ptr<const uint8_t>(a.v_scales) + Layout::scales(tile.page_head, a.page_tokens);
+  T *out = global_ptr<T>(a.values) + tile.head * a.value_head_stride + column * 8u;
 #pragma unroll
-  for (uint32_t c = 0; c < Layout::kKeyChunks; ++c) {
-    const uint32_t pair = c * 64u + lane;
-    if (pair >= D / 2u) break;
-    uint2 bytes = make_uint2(0u, 0u), scales = make_uint2(0u, 0u);
-    if (tile.page_valid) {
-      bytes = *reinterpret_cast<const uint2 *>(v_payload + Layout::value_byte(tile.page_token, pair));
-      scales = *reinterpret_cast<const uint2 *>(v_scales + Layout::value_scale(tile.page_token, pair / 16u));
-    }
+  for (uint32_t eight = 0; eight < 32u; eight += 8u * kTogether) {
+    const uint32_t first = eight + 8u * part;
+    if (first >= 32u) break;
+    // four pairs of values of eight tokens: [pair][token]
+    const uint2 *src = reinterpret_cast<const uint2 *>(payload + Layout::value_byte(tile.page_token + first, column * 4u));
+    const uint2 pair[4] = {src[0], src[1], src[2], src[3]};
+    const uint2 scale = *reinterpret_cast<const uint2 *>(scales + Layout::value_scale(tile.page_token + first, block));
 #pragma unroll
     for (uint32_t t = 0; t < 8u; ++t) {
-      const int32_t index = offset + static_cast<int32_t>(t);
+      const int32_t index = offset + static_cast<int32_t>(first + t);
       if (index < 0 || index >= rows) continue;
-      const uint32_t byte = (t < 4u ? bytes.x : bytes.y) >> (8u * (t & 3u));
-      const float scale = tile.page_valid ? block_scale(((t < 4u ? scales.x : scales.y) >> (8u * (t & 3u))) & 255u) : 0.0f;
-      T *out = global_ptr<T>(a.values) + (tile.sequence.row + static_cast<uint64_t>(index)) * a.value_row_stride +
-               tile.head * a.value_head_stride;
-      store_pair(out + 2u * pair, fp4_e2m1_decode(byte & 15u) * scale, fp4_e2m1_decode((byte >> 4) & 15u) * scale);
+      // byte t of every pair
+      const uint32_t sel = 0x0c0c0000u | (4u + (t & 3u)) << 8 | (t & 3u);
+      const uint32_t lo = __builtin_amdgcn_perm(t < 4u ? pair[1].x : pair[1].y, t < 4u ? pair[0].x : pair[0].y, sel);
+      const uint32_t hi = __builtin_amdgcn_perm(t < 4u ? pair[3].x : pair[3].y, t < 4u ? pair[2].x : pair[2].y, sel);
+      const uint32_t scale_byte = ((t < 4u ? scale.x : scale.y) >> (8u * (t & 3u))) & 255u;
+      float x[8];
+      expand8(tile.page_valid ? lo | (hi << 16) : 0u, tile.page_valid ? scale_byte : 127u, x);
+      store8(out + (tile.sequence.row + static_cast<uint64_t>(index)) * a.value_row_stride, x);
     }
   }
 }
@@ -262,10 +285,11 @@ FerruleHipStatus dispatch(const FerruleHipKvCacheArgs *args) {
   if (status != FERRULE_HIP_SUCCESS || args->batch == 0u || args->rows == 0u) return status;
   const FerruleHipKvCacheArgs &a = *args;
   hipStream_t stream = reinterpret_cast<hipStream_t>(static_cast<uintptr_t>(a.stream));
-  // rows that start inside a group of eight touch one group more
+  // rows that start inside a tile touch one tile more
+  constexpr uint32_t kTokens = Launch<float, 64>::kTokens;
   const uint32_t rows = a.max_query_length < a.rows ? a.max_query_length : a.rows;
-  const uint32_t groups = rows == 1u ? 1u : (rows + 7u) / 8u + 1u;
-  const dim3 grid((groups * a.kv_heads + kWaves - 1u) / kWaves, a.batch);
+  const uint32_t tiles = rows == 1u ? 1u : (rows + kTokens - 1u) / kTokens + 1u;
+  const dim3 grid((tiles * a.kv_heads * Launch<float, 64>::kWavesPerTile + kWaves - 1u) / kWaves, a.batch);
   clear_launch_error();
   if (a.value_type == FERRULE_HIP_KV_BF16) {
     switch (a.head_dim) {
@@ -287,12 +311,14 @@ FerruleHipStatus dispatch(const FerruleHipKvCacheArgs *args) {
 
 template <typename T, uint32_t D>
 struct Append {
+  static constexpr uint32_t kTokens = 8u, kWavesPerTile = 1u;
   static void run(const FerruleHipKvCacheArgs &a, dim3 grid, hipStream_t stream) {
     kv_append_kernel<T, D><<<grid, 256, 0, stream>>>(a);
   }
 };
 template <typename T, uint32_t D>
 struct Read {
+  static constexpr uint32_t kTokens = 32u, kWavesPerTile = 2u;  // keys and values
   static void run(const FerruleHipKvCacheArgs &a, dim3 grid, hipStream_t stream) {
     kv_read_kernel<T, D><<<grid, 256, 0, stream>>>(a);
   }
