@@ -50,116 +50,123 @@ __device__ __forceinline__ bool kv_tile(const FerruleHipKvCacheArgs &a, uint32_t
   return true;
 }
 
-// Sixteen consecutive values of a row as f32.
-template <typename T>
-__device__ __forceinline__ void load16(const T *src, float (&x)[16]) {
-  if constexpr (sizeof(T) == 2) {
+// Eight consecutive values of a row as f32.
+__device__ __forceinline__ void load8(const uint16_t *src, float (&x)[8]) {
+  const i32x4_t w = *reinterpret_cast<const i32x4_t *>(src);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const i32x4_t w = reinterpret_cast<const i32x4_t *>(src)[i];
+  for (int e = 0; e < 4; ++e) {
+    x[2 * e] = __uint_as_float(static_cast<uint32_t>(w[e]) << 16);
+    x[2 * e + 1] = __uint_as_float(static_cast<uint32_t>(w[e]) & 0xffff0000u);
+  }
+}
+__device__ __forceinline__ void load8(const float *src, float (&x)[8]) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        x[8 * i + 2 * e] = __uint_as_float(static_cast<uint32_t>(w[e]) << 16);
-        x[8 * i + 2 * e + 1] = __uint_as_float(static_cast<uint32_t>(w[e]) & 0xffff0000u);
-      }
-    }
-  } else {
+  for (int i = 0; i < 2; ++i) {
+    const f32x4_t w = reinterpret_cast<const f32x4_t *>(src)[i];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const f32x4_t w = reinterpret_cast<const f32x4_t *>(src)[i];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) x[4 * i + e] = w[e];
-    }
+    for (int e = 0; e < 4; ++e) x[4 * i + e] = w[e];
   }
 }
 
-// Half a scale block (16 values; the other half is in lane ^ 1) -> its eight payload bytes and the
-// block's scale byte.  All in bits: with amax = 1.f * 2^e the smallest n with 6 * 2^n >= amax is
+// A quarter of a scale block (8 values; lanes ^ 1, 2, 3 have the others) -> its four payload bytes and
+// the block's scale byte.  All in bits: with amax = 1.f * 2^e the smallest n with 6 * 2^n >= amax is
 // e - 2 while 1.f <= 1.5, else e - 1; and |x| / 2^n rounds to the one-mantissa-bit grid by adding
 // just under half a step, which sends a tie down.
-__device__ __forceinline__ uint32_t quantise16(const float (&x)[16], uint32_t (&packed)[2]) {
+__device__ __forceinline__ uint32_t quantise8(const float (&x)[8], uint32_t &packed) {
   uint32_t top = 0u;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
+  for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
   top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 1, 64)));
-  packed[0] = packed[1] = 0u;
+  top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 2, 64)));
+  packed = 0u;
   if (top >= 0x7f800000u) return kNanBlock;
   const int32_t exponent = static_cast<int32_t>(top >> 23) - 127;
   int32_t n = exponent - 2 + ((top & 0x7fffffu) > 0x400000u ? 1 : 0);
   n = max(n, -126);
   const float inverse = __uint_as_float(static_cast<uint32_t>(127 - n) << 23);  // n <= 126: normal
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
+  for (int i = 0; i < 8; ++i) {
     const float q = x[i] * inverse;  // exact, |q| <= 6, or below every threshold
     const uint32_t bits = __float_as_uint(q) & 0x7fffffffu;
     const float m = __uint_as_float(bits);
     const uint32_t large = ((bits + 0x1fffffu) >> 22) - 252u;            // m >= 1: 2..7
     const uint32_t small = (m > 0.25f ? 1u : 0u) + (m > 0.75f ? 1u : 0u);  // m < 1: 0..2
     const uint32_t code = (m >= 1.0f ? large : small) | ((__float_as_uint(q) >> 28) & 8u);
-    packed[i >> 3] |= code << (4 * (i & 7));
+    packed |= code << (4 * i);
   }
   return static_cast<uint32_t>(n + 127);
 }
 
-// A wave owns one head of eight neighbouring tokens, the unit of the value layout: lane = (token
-// lane / 8, piece lane % 8), a piece being 16 values, so a scale block is two adjacent lanes and
-// its maximum one exchange.
+// A wave has one head of eight neighbouring tokens, the unit of the value layout: a lane takes eight
+// values, so that a row of 128 is sixteen lanes side by side, and keys and values are asked for together.
 template <typename T, uint32_t D>
 __global__ __launch_bounds__(256) void kv_append_kernel(FerruleHipKvCacheArgs a) {
   using Layout = KvLayout<D>;
-  // the value bytes of 128 values of eight tokens, turned in LDS: [value pair][token]
+  constexpr uint32_t kLanes = (D < 128u ? D : 128u) / 8u;  // of a row
+  constexpr uint32_t kTogether = 64u / kLanes;             // rows side by side: 4, or 8 at D = 64
+  constexpr uint32_t kPasses = 8u / kTogether;
+  // the bytes of 128 values of eight tokens, turned in LDS: [value pair][token]
   __shared__ __align__(16) uint8_t turned[kWaves][64][8];
   const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
   KvTile tile;
-  const uint32_t index8 = __builtin_amdgcn_readfirstlane(blockIdx.x * kWaves + wave);
-  if (!kv_tile<8>(a, index8, tile) || !tile.page_valid) return;
-  const uint32_t t = lane >> 3, piece = lane & 7u;
-  const int32_t index = tile.first + static_cast<int32_t>(t) - tile.sequence.position;  // row of the sequence
-  const bool live = index >= 0 && index < static_cast<int32_t>(tile.sequence.rows);
-  const bool whole = __ballot(live) == ~0ull;
-  const uint64_t row = tile.sequence.row + static_cast<uint64_t>(live ? index : 0);
-  const T *keys = global_ptr<const T>(a.keys) + row * a.key_row_stride + tile.head * a.key_head_stride;
-  const T *values = global_ptr<const T>(a.values) + row * a.value_row_stride + tile.head * a.value_head_stride;
+  // a workgroup has 32 tokens: the scale bytes of a cache line come from one place
+  if (!kv_tile<32>(a, blockIdx.x, tile) || !tile.page_valid) return;
+  tile.first += static_cast<int32_t>(8u * wave);
+  tile.page_token += 8u * wave;
+  const uint32_t column = lane % kLanes, part = lane / kLanes;
+  const int32_t offset = tile.first - tile.sequence.position;  // row of the sequence of the tile's first token
+  const int32_t rows = static_cast<int32_t>(tile.sequence.rows);
+  if (offset >= rows || offset <= -8) return;
+  const bool whole = offset >= 0 && offset + 8 <= rows;
+  const T *keys = global_ptr<const T>(a.keys) + tile.head * a.key_head_stride + column * 8u;
+  const T *values = global_ptr<const T>(a.values) + tile.head * a.value_head_stride + column * 8u;
   uint8_t *k_payload = global_ptr<uint8_t>(a.k_payload) + Layout::payload(tile.page_head, a.page_tokens);
   uint8_t *k_scales = global_ptr<uint8_t>(a.k_scales) + Layout::scales(tile.page_head, a.page_tokens);
   uint8_t *v_payload = global_ptr<uint8_t>(a.v_payload) + Layout::payload(tile.page_head, a.page_tokens);
   uint8_t *v_scales = global_ptr<uint8_t>(a.v_scales) + Layout::scales(tile.page_head, a.page_tokens);
-  const uint32_t token = tile.page_token + t;
 #pragma unroll
   for (uint32_t c = 0; c < Layout::kKeyChunks; ++c) {
-    const uint32_t d = c * 128u + piece * 16u;
-    const bool inside = live && d < D;
-    float k[16], v[16];
+    float k[kPasses][8], v[kPasses][8];
+    bool live[kPasses];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) k[i] = v[i] = 0.0f;
-    if (inside) {
-      load16(keys + d, k);
-      load16(values + d, v);
+    for (uint32_t p = 0; p < kPasses; ++p) {
+      const int32_t row = offset + static_cast<int32_t>(p * kTogether + part);
+      live[p] = row >= 0 && row < rows;
+      // a row that is not there is read as one that is: its bytes are not written
+      const uint64_t at = tile.sequence.row + static_cast<uint64_t>(live[p] ? row : max(offset, 0));
+      load8(keys + at * a.key_row_stride + c * 128u, k[p]);
+      load8(values + at * a.value_row_stride + c * 128u, v[p]);
     }
-    uint32_t kq[2], vq[2];
-    const uint32_t ks = quantise16(k, kq);
-    const uint32_t vs = quantise16(v, vq);
-    if (inside) {
-      *reinterpret_cast<uint2 *>(k_payload + Layout::key_byte(token, c) + piece * 8u) = make_uint2(kq[0], kq[1]);
-      if ((piece & 1u) == 0u) {
-        k_scales[Layout::key_scale(token, d / 32u)] = static_cast<uint8_t>(ks);
-        v_scales[Layout::value_scale(token, d / 32u)] = static_cast<uint8_t>(vs);
+#pragma unroll
+    for (uint32_t p = 0; p < kPasses; ++p) {
+      const uint32_t t = p * kTogether + part, token = tile.page_token + t, block = c * 4u + column / 4u;
+      uint32_t kq, vq;
+      const uint32_t ks = quantise8(k[p], kq);
+      const uint32_t vs = quantise8(v[p], vq);
+      if (live[p]) {
+        *reinterpret_cast<uint32_t *>(k_payload + Layout::key_byte(token, c) + column * 4u) = kq;
+        if ((column & 3u) == 0u) {
+          k_scales[Layout::key_scale(token, block)] = static_cast<uint8_t>(ks);
+          v_scales[Layout::value_scale(token, block)] = static_cast<uint8_t>(vs);
+        }
+      }
+#pragma unroll
+      for (uint32_t i = 0; i < 4u; ++i) {
+        const uint8_t byte = static_cast<uint8_t>(vq >> (8u * i));
+        if (whole) {  // wave-uniform
+          turned[wave][column * 4u + i][t] = byte;
+        } else if (live[p]) {
+          v_payload[Layout::value_byte(token, c * 64u + column * 4u + i)] = byte;
+        }
       }
     }
-    if (whole) {  // wave-uniform
-#pragma unroll
-      for (uint32_t i = 0; i < 8u; ++i) turned[wave][piece * 8u + i][t] = static_cast<uint8_t>(vq[i >> 2] >> (8u * (i & 3u)));
+    if (whole) {
       wave_lds_fence();
       const uint2 pair = *reinterpret_cast<const uint2 *>(&turned[wave][lane][0]);
       if (c * 64u + lane < D / 2u) {
         *reinterpret_cast<uint2 *>(v_payload + Layout::value_byte(tile.page_token, c * 64u + lane)) = pair;
       }
       wave_lds_fence();
-    } else if (inside) {
-#pragma unroll
-      for (uint32_t i = 0; i < 8u; ++i) {
-        v_payload[Layout::value_byte(token, d / 2u + i)] = static_cast<uint8_t>(vq[i >> 2] >> (8u * (i & 3u)));
-      }
     }
   }
 }
@@ -183,8 +190,9 @@ __device__ __forceinline__ void expand8(uint32_t bytes, uint32_t scale_byte, flo
 }
 
 __device__ __forceinline__ void store8(float *dst, const float (&x)[8]) {
-  reinterpret_cast<f32x4_t *>(dst)[0] = f32x4_t{x[0], x[1], x[2], x[3]};
-  reinterpret_cast<f32x4_t *>(dst)[1] = f32x4_t{x[4], x[5], x[6], x[7]};
+  const f32x4_t lo = {x[0], x[1], x[2], x[3]}, hi = {x[4], x[5], x[6], x[7]};
+  __builtin_nontemporal_store(lo, reinterpret_cast<f32x4_t *>(dst));
+  __builtin_nontemporal_store(hi, reinterpret_cast<f32x4_t *>(dst) + 1);
 }
 __device__ __forceinline__ void store8(uint16_t *dst, const float (&x)[8]) {  // exact in BF16
   i32x4_t w;
@@ -192,12 +200,13 @@ __device__ __forceinline__ void store8(uint16_t *dst, const float (&x)[8]) {  //
   for (int p = 0; p < 4; ++p) {
     w[p] = static_cast<int>((__float_as_uint(x[2 * p]) >> 16) | (__float_as_uint(x[2 * p + 1]) & 0xffff0000u));
   }
-  *reinterpret_cast<i32x4_t *>(dst) = w;
+  __builtin_nontemporal_store(w, reinterpret_cast<i32x4_t *>(dst));
 }
 
 // A wave has the keys, or the values, of one head of 32 neighbouring tokens: a lane takes eight values
-// at a time, so that it stores 16 (BF16) or 32 bytes and a row is D / 8 lanes side by side.  With two values a lane
-// and store this took 45 us for 4 sequences of up to 8192 tokens, 8 heads of 128.
+// at a time, so that it stores 16 (BF16) or 32 bytes and a row is D / 8 lanes side by side, past the caches:
+// the rows are more than they hold.  4 sequences of up to 8192 tokens, 8 heads of 128: 17.6 us, 6.0 TB/s
+// (24.3 us with ordinary stores, 45 us with two values a lane and store).
 template <typename T, uint32_t D>
 __global__ __launch_bounds__(256) void kv_read_kernel(FerruleHipKvCacheArgs a) {
   using Layout = KvLayout<D>;
@@ -216,17 +225,25 @@ __global__ __launch_bounds__(256) void kv_read_kernel(FerruleHipKvCacheArgs a) {
     const uint8_t *payload = global_ptr<const uint8_t>(a.k_payload) + Layout::payload(tile.page_head, a.page_tokens);
     const uint8_t *scales = global_ptr<const uint8_t>(a.k_scales) + Layout::scales(tile.page_head, a.page_tokens);
     T *out = global_ptr<T>(a.keys) + tile.head * a.key_head_stride + column * 8u;
-#pragma unroll 8
-    for (uint32_t t = part; t < 32u; t += kTogether) {
-      const int32_t index = offset + static_cast<int32_t>(t);
-      const uint32_t token = tile.page_token + t;
-      const uint32_t bytes = *reinterpret_cast<const uint32_t *>(payload + Layout::key_byte(token, column / 16u) +
-                                                                 (column % 16u) * 4u);
-      const uint32_t scale = scales[Layout::key_scale(token, block)];
-      if (index < 0 || index >= rows) continue;
-      float x[8];
-      expand8(tile.page_valid ? bytes : 0u, tile.page_valid ? scale : 127u, x);
-      store8(out + (tile.sequence.row + static_cast<uint64_t>(index)) * a.key_row_stride, x);
+    constexpr uint32_t kAtOnce = 8u;  // loads in flight
+#pragma unroll 1
+    for (uint32_t first = part; first < 32u; first += kAtOnce * kTogether) {
+      uint32_t bytes[kAtOnce], scale[kAtOnce];
+#pragma unroll
+      for (uint32_t k = 0; k < kAtOnce; ++k) {
+        const uint32_t token = tile.page_token + min(first + k * kTogether, 31u);
+        bytes[k] = *reinterpret_cast<const uint32_t *>(payload + Layout::key_byte(token, column / 16u) + (column % 16u) * 4u);
+        scale[k] = scales[Layout::key_scale(token, block)];
+      }
+#pragma unroll
+      for (uint32_t k = 0; k < kAtOnce; ++k) {
+        const uint32_t t = first + k * kTogether;
+        const int32_t index = offset + static_cast<int32_t>(t);
+        if (t >= 32u || index < 0 || index >= rows) continue;
+        float x[8];
+        expand8(tile.page_valid ? bytes[k] : 0u, tile.page_valid ? scale[k] : 127u, x);
+        store8(out + (tile.sequence.row + static_cast<uint64_t>(index)) * a.key_row_stride, x);
+      }
     }
     return;
   }
@@ -274,7 +291,7 @@ FerruleHipStatus validate(const FerruleHipKvCacheArgs &a) {
   if (!kv_head_dim_supported(a.head_dim)) return FERRULE_HIP_UNSUPPORTED;
   // the grid: batch in y, eight-token groups times heads in x
   const uint64_t groups = (static_cast<uint64_t>(a.max_query_length) + 7u) / 8u + 1u;
-  if (a.batch > 65535u || groups * a.kv_heads > 0x7fffffffull) return FERRULE_HIP_UNSUPPORTED;
+  if (a.batch > 65535u || groups * a.kv_heads > 0x3fffffffull) return FERRULE_HIP_UNSUPPORTED;
   return FERRULE_HIP_SUCCESS;
 }
 
@@ -286,7 +303,7 @@ FerruleHipStatus dispatch(const FerruleHipKvCacheArgs *args) {
   const FerruleHipKvCacheArgs &a = *args;
   hipStream_t stream = reinterpret_cast<hipStream_t>(static_cast<uintptr_t>(a.stream));
   // rows that start inside a tile touch one tile more
-  constexpr uint32_t kTokens = Launch<float, 64>::kTokens;
+  constexpr uint32_t kTokens = 32u;
   const uint32_t rows = a.max_query_length < a.rows ? a.max_query_length : a.rows;
   const uint32_t tiles = rows == 1u ? 1u : (rows + kTokens - 1u) / kTokens + 1u;
   const dim3 grid((tiles * a.kv_heads * Launch<float, 64>::kWavesPerTile + kWaves - 1u) / kWaves, a.batch);
@@ -311,14 +328,14 @@ FerruleHipStatus dispatch(const FerruleHipKvCacheArgs *args) {
 
 template <typename T, uint32_t D>
 struct Append {
-  static constexpr uint32_t kTokens = 8u, kWavesPerTile = 1u;
+  static constexpr uint32_t kWavesPerTile = 4u;  // eight tokens each
   static void run(const FerruleHipKvCacheArgs &a, dim3 grid, hipStream_t stream) {
     kv_append_kernel<T, D><<<grid, 256, 0, stream>>>(a);
   }
 };
 template <typename T, uint32_t D>
 struct Read {
-  static constexpr uint32_t kTokens = 32u, kWavesPerTile = 2u;  // keys and values
+  static constexpr uint32_t kWavesPerTile = 2u;  // keys and values
   static void run(const FerruleHipKvCacheArgs &a, dim3 grid, hipStream_t stream) {
     kv_read_kernel<T, D><<<grid, 256, 0, stream>>>(a);
   }
