@@ -27,6 +27,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "../../include/ferrule_hip_provider.h"
 #include "kv_cache.cuh"
 #include "mx_core.cuh"
@@ -89,14 +91,27 @@ struct Core {
   struct Query {
     i32x8_t term[kChunks * kTerms];
     uint32_t scale[kChunks * kTerms];
+    __device__ __forceinline__ i32x8_t get(uint32_t t, uint32_t &s) const {
+      s = scale[t];
+      return term[t];
+    }
+  };
+  // The same in LDS, for waves that share their rows: at D = 512 the terms would take 72 registers.
+  struct SharedQuery {
+    u32x4_t term[kChunks * kTerms][2][64];
+    uint32_t scale[kChunks * kTerms][64];
+  };
+  struct SharedReader {
+    const SharedQuery &q;
+    uint32_t lane;
+    __device__ __forceinline__ i32x8_t get(uint32_t t, uint32_t &s) const {
+      s = q.scale[t][lane];
+      return make_b_fp8(q.term[t][0][lane], q.term[t][1][lane]);
+    }
   };
   struct Keys {
     u32x4_t payload[kChunks][2];
     uint2 scale[kChunks];
-  };
-  struct Values {
-    u32x4_t payload[kUnits];
-    uint2 scale[kUnits];
   };
 
   // 16 values of a row, as BF16 pairs
@@ -163,44 +178,39 @@ struct Core {
     return byte;
   }
 
-  // The lane's part of a tile's query rows, in two steps: what is asked for between them need not wait for q.
-  static constexpr uint32_t kHalves = D == 64u ? 1u : 2u;  // of a 128-value piece
-  struct RawQuery {
-    Pairs pairs[kChunks][kHalves];
+  // The lane's part of a 128-value piece of a tile's query rows, in two steps: what is asked for between
+  // them need not wait for q.
+  static constexpr uint32_t kHalves = D == 64u ? 1u : 2u;
+  struct RawPiece {
+    Pairs pairs[kHalves];
   };
-  static __device__ __forceinline__ void load_query(uint64_t base, uint64_t row, bool f32, uint32_t lane, RawQuery &raw) {
-    const uint32_t g = lane >> 4;
+  static __device__ __forceinline__ void load_query(uint64_t base, uint64_t row, uint32_t c, bool f32, uint32_t lane, RawPiece &raw) {
 #pragma unroll
-    for (uint32_t c = 0; c < kChunks; ++c) {
-#pragma unroll
-      for (uint32_t h = 0; h < kHalves; ++h) {
-        const uint64_t at = row + c * 128u + h * 64u + g * 16u;
-        raw.pairs[c][h] = f32 ? load16<true>(base, at) : load16<false>(base, at);
-      }
+    for (uint32_t h = 0; h < kHalves; ++h) {
+      const uint64_t at = row + c * 128u + h * 64u + (lane >> 4) * 16u;
+      raw.pairs[h] = f32 ? load16<true>(base, at) : load16<false>(base, at);
     }
   }
-  static __device__ __forceinline__ void split_query(const RawQuery &raw, uint32_t lane, Query &q) {
+  static __device__ __forceinline__ void split_query(const RawPiece &raw, uint32_t lane, i32x8_t (&term)[kTerms],
+                                                     uint32_t (&scale)[kTerms]) {
     const uint32_t g = lane >> 4;
     const uint32_t source = (lane & 15u) + ((g & 1u) << 5);  // holds the scales of block g, in its half g / 2
+    u32x4_t first[kHalves], second[kHalves];
+    uint32_t byte[kHalves];
 #pragma unroll
-    for (uint32_t c = 0; c < kChunks; ++c) {
-      u32x4_t first[kHalves], second[kHalves];
-      int32_t scale[kHalves];
-#pragma unroll
-      for (uint32_t h = 0; h < kHalves; ++h) {
-        const uint32_t byte = split16(raw.pairs[c][h], block_field(raw.pairs[c][h]), first[h], second[h]);
-        scale[h] = __shfl(static_cast<int>(byte), static_cast<int>(source), 64);
-      }
-      if constexpr (D == 64u) {
-        // values 0..63 twice along the product: first term against the first copy of a key, second against the second
-        q.term[0] = make_b_fp8(first[0], second[0]);
-        q.scale[0] = static_cast<uint32_t>(scale[0]) - (g >= 2u ? 5u : 0u);
-      } else {
-        q.term[2u * c] = make_b_fp8(first[0], first[kHalves - 1u]);
-        q.term[2u * c + 1u] = make_b_fp8(second[0], second[kHalves - 1u]);
-        q.scale[2u * c] = static_cast<uint32_t>(g >= 2u ? scale[kHalves - 1u] : scale[0]);
-        q.scale[2u * c + 1u] = q.scale[2u * c] - 5u;
-      }
+    for (uint32_t h = 0; h < kHalves; ++h) {
+      const uint32_t own = split16(raw.pairs[h], block_field(raw.pairs[h]), first[h], second[h]);
+      byte[h] = static_cast<uint32_t>(__shfl(static_cast<int>(own), static_cast<int>(source), 64));
+    }
+    if constexpr (D == 64u) {
+      // values 0..63 twice along the product: first term against the first copy of a key, second against the second
+      term[0] = make_b_fp8(first[0], second[0]);
+      scale[0] = byte[0] - (g >= 2u ? 5u : 0u);
+    } else {
+      term[0] = make_b_fp8(first[0], first[kHalves - 1u]);
+      term[kTerms - 1u] = make_b_fp8(second[0], second[kHalves - 1u]);
+      scale[0] = g >= 2u ? byte[kHalves - 1u] : byte[0];
+      scale[kTerms - 1u] = scale[0] - 5u;
     }
   }
 
@@ -245,14 +255,9 @@ struct Core {
     scale = *reinterpret_cast<const uint2 *>(scales + o.value_scale + u * 16u);
   }
 
-  template <bool STREAM>
-  static __device__ __forceinline__ void load_values(const uint8_t *payload, const uint8_t *scales, const Offsets &o, Values &v) {
-#pragma unroll
-    for (uint32_t u = 0; u < kUnits; ++u) load_piece<STREAM>(payload, scales, u, o, v.payload[u], v.scale[u]);
-  }
-
   // Scores of tokens 8g..8g+7 of row i: s[0..3] and s[4..7].
-  static __device__ __forceinline__ void scores(const Keys &k, const Query &q, uint32_t lane, f32x4_t (&s)[2]) {
+  template <typename Q>
+  static __device__ __forceinline__ void scores(const Keys &k, const Q &q, uint32_t lane, f32x4_t (&s)[2]) {
     const uint32_t shift = 8u * (lane & 3u);
     s[0] = s[1] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -260,12 +265,15 @@ struct Core {
       const uint32_t scale[2] = {k.scale[c].x >> shift, k.scale[c].y >> shift};
 #pragma unroll
       for (uint32_t term = 0; term < kTerms; ++term) {
+        uint32_t q_scale;
+        const i32x8_t q_term = q.get(c * kTerms + term, q_scale);
 #pragma unroll
         for (uint32_t half = 0; half < 2u; ++half) {
-          s[half] = mfma_fp4_fp8(make_a_fp4(k.payload[c][half]), q.term[c * kTerms + term], s[half], scale[half],
-                                 q.scale[c * kTerms + term]);
+          s[half] = mfma_fp4_fp8(make_a_fp4(k.payload[c][half]), q_term, s[half], scale[half], q_scale);
         }
       }
+      // terms from LDS: not all of them at once, they would take the registers that the reader saves
+      if constexpr (!std::is_same<Q, Query>::value) __builtin_amdgcn_sched_barrier(0);
     }
   }
 
@@ -273,14 +281,30 @@ struct Core {
   static __device__ __forceinline__ bool has_nan(const uint2 &scale) {
     return ((((scale.x & 0x7f7f7f7fu) + 0x01010101u) & scale.x) | (((scale.y & 0x7f7f7f7fu) + 0x01010101u) & scale.y)) & 0x80808080u;
   }
-  static __device__ __forceinline__ bool has_nan(const Values &v) {
-    bool found = false;
-#pragma unroll
-    for (uint32_t u = 0; u < kUnits; ++u) found |= has_nan(v.scale[u]);
-    return found;
+  static __device__ __forceinline__ uint2 without_nan(const uint2 &scale) {
+    return make_uint2(without_nan(scale.x), without_nan(scale.y));
   }
   static __device__ __forceinline__ uint32_t without_nan(uint32_t x) {  // bytes of 255 become 127
     return x & ~((((x & 0x7f7f7f7fu) + 0x01010101u) & x) & 0x80808080u);
+  }
+
+  // A block of NaN is expanded as if its scale were 1, since 0 * NaN would reach rows that do not see it; the
+  // rows that do take the NaN in the end.  Bit u: the lane's row sees a token whose values 64u + 16g .. 64u + 16g + 15
+  // are NaN.  Rare, so it is kept small, and `scales` (of a 32-token tile) are read again.
+  static __device__ __forceinline__ uint32_t nan_units(const uint8_t *scales, int32_t start, int32_t position, int32_t from,
+                                                       int32_t sinks, uint32_t g) {
+    uint32_t units = 0u;
+#pragma unroll 1
+    for (uint32_t t = 0; t < kTileTokens; ++t) {
+      const int32_t j = start + static_cast<int32_t>(t);
+      const bool seen = j <= position && (j >= from || j < sinks);
+#pragma unroll 1
+      for (uint32_t u = 0; u < kUnits; ++u) {
+        const bool bad = scales[Layout::value_scale(t, 2u * u + (g >> 1))] == kNanBlock;
+        units |= bad && seen ? 1u << u : 0u;
+      }
+    }
+    return units;
   }
 
   // Four accumulators' operands from one 16-byte piece: values 64u + 4i + e of tokens 8g..8g+7, e = 0..3.
@@ -411,6 +435,9 @@ template <uint32_t D, uint32_t WAVES>
 __global__ __launch_bounds__(WAVES * 64u, kDecodeOccupancy<D>) void kv_attention_decode_kernel(FerruleHipKvAttentionArgs a, SplitPlan plan) {
   using C = Core<D>;
   constexpr uint32_t kPitch = 128u + 4u;  // floats of a row in LDS
+  constexpr bool kShared = D >= 256u;     // query terms in LDS
+  constexpr uint32_t kRing = C::kUnits < 4u ? C::kUnits : 4u;
+  __shared__ __align__(16) typename std::conditional<kShared, typename C::SharedQuery, uint32_t>::type shared;
   __shared__ __align__(16) float joined[WAVES][kTileRows][kPitch];
   __shared__ float top_of[WAVES][kTileRows], sum_of[WAVES][kTileRows];
   const uint32_t lane = threadIdx.x & 63u;
@@ -443,18 +470,53 @@ __global__ __launch_bounds__(WAVES * 64u, kDecodeOccupancy<D>) void kv_attention
   Place next_place = {0u, 0u, 0u, false};
   const int32_t first_page = begin < end ? page_of(a, plan, range, b, begin + wave, end) : 0;
   if (begin < end) next_page = page_of(a, plan, range, b, begin + wave + WAVES, end);
-  typename C::RawQuery raw_query;
-  C::load_query(a.q, mine.q, (a.flags & FERRULE_HIP_KV_ATTENTION_QUERY_F32) != 0u, lane, raw_query);
+  const bool f32_query = (a.flags & FERRULE_HIP_KV_ATTENTION_QUERY_F32) != 0u;
+  typename C::RawPiece raw_query;  // the wave's piece: of few, every wave makes all, of several each makes one
+  const uint32_t own_piece = kShared ? wave % C::kChunks : 0u;
+  C::load_query(a.q, mine.q, own_piece, f32_query, lane, raw_query);
   if (begin < end) next_place = place_at<D>(a, plan, range, kv_head, begin + wave, end, first_page, bad);
   const uint8_t *k_payload = global_ptr<const uint8_t>(a.k_payload), *k_scales = global_ptr<const uint8_t>(a.k_scales);
   const uint8_t *v_payload = global_ptr<const uint8_t>(a.v_payload), *v_scales = global_ptr<const uint8_t>(a.v_scales);
   const typename C::Offsets offset = C::offsets(lane);
   typename C::Keys keys;
-  typename C::Values values;
+  // values: kRing 16-byte pieces, each taking the one kRing pieces on as soon as it is expanded
+  u32x4_t ring[kRing];
+  uint2 ring_scale[kRing];
+  auto load_ring = [&](const Place &p) {
+#pragma unroll
+    for (uint32_t u = 0; u < kRing; ++u) {
+      C::template load_piece<true>(v_payload + p.payload, v_scales + p.scales, u, offset, ring[u], ring_scale[u]);
+    }
+  };
   C::template load_keys<true>(k_payload + next_place.payload, k_scales + next_place.scales, offset, keys);
-  C::template load_values<true>(v_payload + next_place.payload, v_scales + next_place.scales, offset, values);
-  typename C::Query query;
-  C::split_query(raw_query, lane, query);
+  load_ring(next_place);
+  i32x8_t term[C::kTerms];
+  uint32_t term_scale[C::kTerms];
+  C::split_query(raw_query, lane, term, term_scale);
+  if constexpr (kShared) {
+    if (wave < C::kChunks) {
+#pragma unroll
+      for (uint32_t t = 0; t < C::kTerms; ++t) {
+        const uint32_t at = own_piece * C::kTerms + t;
+        const u32x4_t lo = {static_cast<uint32_t>(term[t][0]), static_cast<uint32_t>(term[t][1]),
+                            static_cast<uint32_t>(term[t][2]), static_cast<uint32_t>(term[t][3])};
+        const u32x4_t hi = {static_cast<uint32_t>(term[t][4]), static_cast<uint32_t>(term[t][5]),
+                            static_cast<uint32_t>(term[t][6]), static_cast<uint32_t>(term[t][7])};
+        shared.term[at][0][lane] = lo;
+        shared.term[at][1][lane] = hi;
+        shared.scale[at][lane] = term_scale[t];
+      }
+    }
+    lds_barrier();
+  }
+  typename C::Query own_query;
+  if constexpr (!kShared) {
+#pragma unroll
+    for (uint32_t t = 0; t < C::kTerms; ++t) {
+      own_query.term[t] = term[t];
+      own_query.scale[t] = term_scale[t];
+    }
+  }
   const int32_t from = a.window == 0u ? static_cast<int32_t>(0x80000000u) : mine.position - static_cast<int32_t>(a.window - 1u);
   const int32_t sinks = a.window == 0u ? 0 : static_cast<int32_t>(a.sinks);
   const float factor = a.softmax_scale * 1.44269504088896341f;
@@ -463,6 +525,7 @@ __global__ __launch_bounds__(WAVES * 64u, kDecodeOccupancy<D>) void kv_attention
 #pragma unroll
   for (uint32_t c = 0; c < C::kColumns; ++c) out[c] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
   float top = -INFINITY, base = 0.0f, sum = 0.0f;  // base = top, or 0 while the row has seen nothing
+  uint32_t nan_units = 0u;
 
   for (uint32_t v = begin + wave; v < end; v += WAVES) {
     // keys and values are loaded one step ahead, as soon as the registers of this step's are free; two or
@@ -471,7 +534,11 @@ __global__ __launch_bounds__(WAVES * 64u, kDecodeOccupancy<D>) void kv_attention
     next_place = place_at<D>(a, plan, range, kv_head, v + WAVES, end, next_page, bad);
     next_page = page_of(a, plan, range, b, v + 2u * WAVES, end);
     f32x4_t score[2];
-    C::scores(keys, query, lane, score);
+    if constexpr (kShared) {
+      C::scores(keys, typename C::SharedReader{shared, lane}, lane, score);
+    } else {
+      C::scores(keys, own_query, lane, score);
+    }
     C::template load_keys<true>(k_payload + next_place.payload, k_scales + next_place.scales, offset, keys);
     float x[8];
 #pragma unroll
@@ -505,41 +572,38 @@ __global__ __launch_bounds__(WAVES * 64u, kDecodeOccupancy<D>) void kv_attention
     bf16x8_t weight;
 #pragma unroll
     for (int e = 0; e < 8; ++e) weight[e] = static_cast<__bf16>(w[e]);
-    const bool nan_blocks = __any(C::has_nan(values));
-    if (nan_blocks) {
+    bool nan = false;
+    if constexpr (C::kUnits <= 2u) {
 #pragma unroll
-      for (uint32_t u = 0; u < C::kUnits; ++u) {
-        values.scale[u].x = C::without_nan(values.scale[u].x);
-        values.scale[u].y = C::without_nan(values.scale[u].y);
+      for (uint32_t u = 0; u < C::kUnits; ++u) nan |= C::has_nan(ring_scale[u]);
+      if (__any(nan)) {
+#pragma unroll
+        for (uint32_t u = 0; u < C::kUnits; ++u) ring_scale[u] = C::without_nan(ring_scale[u]);
       }
     }
 #pragma unroll
     for (uint32_t u = 0; u < C::kUnits; ++u) {
       u32x4_t operand[4];
-      C::expand(values.payload[u], values.scale[u], operand);
+      if constexpr (C::kUnits <= 2u) {
+        C::expand(ring[u], ring_scale[u], operand);
+      } else {
+        nan |= C::has_nan(ring_scale[u % kRing]);
+        C::expand(ring[u % kRing], C::without_nan(ring_scale[u % kRing]), operand);
+      }
 #pragma unroll
       for (uint32_t e = 0; e < 4u; ++e) {
         out[4u * u + e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, operand[e]), weight, out[4u * u + e], 0, 0, 0);
       }
-    }
-    C::template load_values<true>(v_payload + next_place.payload, v_scales + next_place.scales, offset, values);
-    if (nan_blocks && here.valid) {  // rare: the rows that see such a token take its NaN, the others must not (0 * NaN)
-      const uint8_t *scales = v_scales + here.scales;
-      for (uint32_t t = 0; t < kTileTokens; ++t) {
-        const int32_t j = start + static_cast<int32_t>(t);
-        const bool seen = j <= mine.position && (j >= from || j < sinks);
-#pragma unroll
-        for (uint32_t block = 0; block < D / 32u; ++block) {
-          const bool bad = scales[C::Layout::value_scale(t, block)] == kNanBlock;
-          // accumulator 4u + e of lane (i, g) holds values 64u + 16g + 4v + e
-          const bool hit = bad && seen && (g >> 1) == (block & 1u);
-#pragma unroll
-          for (uint32_t e = 0; e < 4u; ++e) {
-            if (hit) out[4u * (block >> 1) + e] = f32x4_t{NAN, NAN, NAN, NAN};
-          }
-        }
+      if constexpr (C::kUnits > 2u) {
+        __builtin_amdgcn_sched_barrier(0);  // one piece's operands at a time
+        const Place &source = u + kRing < C::kUnits ? here : next_place;
+        C::template load_piece<true>(v_payload + source.payload, v_scales + source.scales, (u + kRing) % C::kUnits, offset,
+                                     ring[u % kRing], ring_scale[u % kRing]);
       }
     }
+    if constexpr (C::kUnits <= 2u) load_ring(next_place);
+    const bool nan_blocks = __any(nan);
+    if (nan_blocks && here.valid) nan_units |= C::nan_units(v_scales + here.scales, start, mine.position, from, sinks, g);
   }
 
   if (bad && lane == 0u) kv_report(a.error);
@@ -576,7 +640,9 @@ __global__ __launch_bounds__(WAVES * 64u, kDecodeOccupancy<D>) void kv_attention
       for (uint32_t e4 = 0; e4 < 4u; ++e4) {
         f32x4_t o;
 #pragma unroll
-        for (uint32_t e = 0; e < 4u; ++e) o[e] = out[(2u * c + u) * 4u + e][e4] * keep;
+        for (uint32_t e = 0; e < 4u; ++e) {
+          o[e] = (nan_units >> (2u * c + u)) & 1u ? NAN : out[(2u * c + u) * 4u + e][e4] * keep;
+        }
         *reinterpret_cast<f32x4_t *>(&joined[wave][i][64u * u + 16u * g + 4u * e4]) = o;
       }
     }
@@ -666,11 +732,13 @@ __global__ __launch_bounds__(WAVES * 64u, (Rows<D, NQ, WAVES>::kOccupancy)) void
   const float factor = a.softmax_scale * 1.44269504088896341f;
   f32x4_t out[NQ][C::kColumns];
   float top[NQ], base[NQ], sum[NQ];
+  uint32_t nan_units[NQ];
   bool unset = true;  // some row has seen no token yet
 #pragma unroll
   for (uint32_t n = 0; n < NQ; ++n) {
     top[n] = -INFINITY;
     base[n] = sum[n] = 0.0f;
+    nan_units[n] = 0u;
 #pragma unroll
     for (uint32_t c = 0; c < C::kColumns; ++c) out[n][c] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
   }
@@ -702,7 +770,7 @@ __global__ __launch_bounds__(WAVES * 64u, (Rows<D, NQ, WAVES>::kOccupancy)) void
       }
       nan |= C::has_nan(raw_scale[o]);
       u32x4_t operand[4];
-      C::expand(raw[o], make_uint2(C::without_nan(raw_scale[o].x), C::without_nan(raw_scale[o].y)), operand);
+      C::expand(raw[o], C::without_nan(raw_scale[o]), operand);
 #pragma unroll
       for (uint32_t e = 0; e < 4u; ++e) staged[buffer][wave * kOwn + o][e][lane] = operand[e];
     }
@@ -734,9 +802,22 @@ __global__ __launch_bounds__(WAVES * 64u, (Rows<D, NQ, WAVES>::kOccupancy)) void
   typename C::Query query[NQ];
 #pragma unroll
   for (uint32_t n = 0; n < NQ; ++n) {
-    typename C::RawQuery raw_query;
-    C::load_query(a.q, row_q[n], (a.flags & FERRULE_HIP_KV_ATTENTION_QUERY_F32) != 0u, lane, raw_query);
-    C::split_query(raw_query, lane, query[n]);
+    typename C::RawPiece piece[C::kChunks];
+#pragma unroll
+    for (uint32_t c = 0; c < C::kChunks; ++c) {
+      C::load_query(a.q, row_q[n], c, (a.flags & FERRULE_HIP_KV_ATTENTION_QUERY_F32) != 0u, lane, piece[c]);
+    }
+#pragma unroll
+    for (uint32_t c = 0; c < C::kChunks; ++c) {
+      i32x8_t term[C::kTerms];
+      uint32_t scale[C::kTerms];
+      C::split_query(piece[c], lane, term, scale);
+#pragma unroll
+      for (uint32_t t = 0; t < C::kTerms; ++t) {
+        query[n].term[c * C::kTerms + t] = term[t];
+        query[n].scale[c * C::kTerms + t] = scale[t];
+      }
+    }
   }
   if (begin < end) {
     stage_pieces(0u);
@@ -860,25 +941,13 @@ __global__ __launch_bounds__(WAVES * 64u, (Rows<D, NQ, WAVES>::kOccupancy)) void
 #pragma unroll
     for (uint32_t w = 0; w < WAVES; ++w) nan_blocks |= nan_of[buffer][w];
     if (nan_blocks != 0u) {
-      // rare: the rows that see such a token take its NaN, the others must not (0 * NaN)
+#pragma unroll 1
       for (uint32_t t = 0; t < kSub; ++t) {
         const Place p = place_at<D>(a, plan, range, kv_head, v + t, end, page(v + t), bad);
         if (!p.valid) continue;
-        const uint8_t *scales = v_scales + p.scales;
-        for (uint32_t k = 0; k < kTileTokens; ++k) {
-          const int32_t j = static_cast<int32_t>(p.first + k);
 #pragma unroll
-          for (uint32_t block = 0; block < D / 32u; ++block) {
-            const bool nan = scales[C::Layout::value_scale(k, block)] == kNanBlock;
-#pragma unroll
-            for (uint32_t n = 0; n < NQ; ++n) {
-              const bool hit = nan && j <= position[n] && (j >= from[n] || j < sinks) && (g >> 1) == (block & 1u);
-#pragma unroll
-              for (uint32_t e = 0; e < 4u; ++e) {
-                if (hit) out[n][4u * (block >> 1) + e] = f32x4_t{NAN, NAN, NAN, NAN};
-              }
-            }
-          }
+        for (uint32_t n = 0; n < NQ; ++n) {
+          nan_units[n] |= C::nan_units(v_scales + p.scales, static_cast<int32_t>(p.first), position[n], from[n], sinks, g);
         }
       }
     }
@@ -898,7 +967,9 @@ __global__ __launch_bounds__(WAVES * 64u, (Rows<D, NQ, WAVES>::kOccupancy)) void
       for (uint32_t half = 0; half < 2u; ++half) {  // values 64u + 16g + 8 half ..
         float x[8];
 #pragma unroll
-        for (uint32_t e = 0; e < 8u; ++e) x[e] = out[n][4u * u + (e & 3u)][2u * half + (e >> 2)] * norm;
+        for (uint32_t e = 0; e < 8u; ++e) {
+          x[e] = (nan_units[n] >> u) & 1u ? NAN : out[n][4u * u + (e & 3u)][2u * half + (e >> 2)] * norm;
+        }
         const uint32_t d = 64u * u + 16u * g + 8u * half;
         if (whole) {
           store(a.output, row.output + d, (a.flags & FERRULE_HIP_KV_ATTENTION_OUTPUT_F32) != 0u, x);
