@@ -1098,10 +1098,30 @@ uint32_t row_tiles(const FerruleHipKvAttentionArgs &a, uint32_t tile_rows) {
   return static_cast<uint32_t>((packed_rows(a) + tile_rows - 1u) / tile_rows);
 }
 
+// 32-token tiles that a workgroup of tile_rows packed rows can see, at most.
+uint64_t token_tiles(const FerruleHipKvAttentionArgs &a, uint32_t tile_rows) {
+  uint64_t tokens = a.max_sequence_length;
+  if (a.window != 0u) {
+    const uint64_t seen = static_cast<uint64_t>(a.window) + a.sinks + tile_rows + 2u * kTileTokens;
+    tokens = tokens < seen ? tokens : seen;
+  }
+  return tokens / kTileTokens + 1u;
+}
+
+uint64_t segments_of(const FerruleHipKvAttentionArgs &a, uint32_t tile_rows) {
+  return static_cast<uint64_t>(a.batch) * a.kv_heads * row_tiles(a, tile_rows);
+}
+
 // Which kernel: packed rows of a workgroup of kv_attention_rows_kernel, 0 for kv_attention_decode_kernel.
+// The latter reads and expands the range once for every 16 rows, but needs no second part of it: for 33 to 64 rows
+// of 512 values it is the faster one where every tile has a CU and a wave no more than two steps (64 sequences of
+// 64 heads over 128 tokens: 19.0 us, rows kernel 23.9; over 256 tokens 39.8 and 28.6; 128 sequences 31.6 and 24.1).
 uint32_t rows_of_workgroup(const FerruleHipKvAttentionArgs &a) {
   const uint64_t rows = packed_rows(a);
   if (rows <= 32u) return 0u;
+  if (rows <= 64u && a.head_dim == 512u && segments_of(a, kTileRows) <= 256u && token_tiles(a, kTileRows) <= 2u * kWaves) {
+    return 0u;
+  }
   if (rows <= 64u || a.head_dim == 512u) return 64u;
   if (rows <= 128u) return 128u;
   return a.head_dim == 256u ? 128u : 256u;
@@ -1114,26 +1134,21 @@ SplitPlan plan_splits(const FerruleHipKvAttentionArgs &a) {
   SplitPlan plan = {};
   plan.tile_rows = tiles == 0u ? kTileRows : tiles;
   plan.page_shift = static_cast<uint32_t>(__builtin_ctz(a.page_tokens));
-  uint64_t tokens = a.max_sequence_length;
-  if (a.window != 0u) {
-    const uint64_t seen = static_cast<uint64_t>(a.window) + a.sinks + plan.tile_rows + 2u * kTileTokens;
-    tokens = tokens < seen ? tokens : seen;
-  }
-  const uint64_t token_tiles = tokens / kTileTokens + 1u;
-  const uint64_t segments = static_cast<uint64_t>(a.batch) * a.kv_heads * row_tiles(a, plan.tile_rows);
+  const uint64_t range = token_tiles(a, plan.tile_rows);
+  const uint64_t segments = segments_of(a, plan.tile_rows);
   // Decode: about a thousand parts, which the card holds at once (64 sequences of 8192 tokens, 8 heads: 99 us, with
   // 2048 parts 112).  Rows: no more than fill it once, and parts long enough to pay for their f32 partials
   // (4 x 512 rows over 8192 tokens: 244 us, with 512 parts 285).
   const uint64_t target = tiles == 0u ? 1024u : 256u;
   const uint64_t least = tiles == 0u ? 2u * kWaves : 16u;
-  uint64_t part = (segments * token_tiles + target - 1u) / target;
+  uint64_t part = (segments * range + target - 1u) / target;
   part = part < least ? least : part;
   // A range of a few steps of a CU's sixteen waves is not worth a second launch while there are CUs for all segments.
-  if (tiles == 0u && a.head_dim <= 128u && part < token_tiles && token_tiles <= 64u && segments <= 256u) {
+  if (tiles == 0u && a.head_dim <= 128u && part < range && range <= 64u && segments <= 256u) {
     plan.wide = 1u;
-    part = token_tiles;
+    part = range;
   }
-  uint64_t splits = (token_tiles + part - 1u) / part;
+  uint64_t splits = (range + part - 1u) / part;
   plan.part_tiles = static_cast<uint32_t>(part < 0x40000000u ? part : 0x40000000u);
   plan.splits = static_cast<uint32_t>(splits);
   if (plan.splits == 1u) return plan;
