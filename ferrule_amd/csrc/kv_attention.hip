@@ -67,7 +67,7 @@ __device__ __forceinline__ TileRange tile_range(const FerruleHipKvAttentionArgs 
   if (last < 0) return t;
   const uint32_t end = static_cast<uint32_t>(last) / kTileTokens + 1u;
   if (a.window != 0u) {
-    const int32_t from = max(0, low - static_cast<int32_t>(a.window - 1u));
+    const int32_t from = max(0, max(0, low) - static_cast<int32_t>(a.window - 1u));  // no row below 0 sees anything
     t.first = min(static_cast<uint32_t>(from) / kTileTokens, end);
     t.head = min((a.sinks + kTileTokens - 1u) / kTileTokens, t.first);
   }
@@ -277,18 +277,18 @@ struct Core {
     }
   }
 
-  // Any scale byte 255 (a block of NaN) among the lane's?
-  static __device__ __forceinline__ bool has_nan(const uint2 &scale) {
-    return ((((scale.x & 0x7f7f7f7fu) + 0x01010101u) & scale.x) | (((scale.y & 0x7f7f7f7fu) + 0x01010101u) & scale.y)) & 0x80808080u;
+  // Blocks that cannot be multiplied: NaN (scale byte 255), and those whose largest values BF16 and f32 cannot hold
+  // (4 * 2^126); both count as NaN.  The bytes' top bits, set for bytes of kLargestScale + 1 = 253 and more:
+  static constexpr uint32_t kLargestScale = 252u;
+  static __device__ __forceinline__ uint32_t not_finite(uint32_t scales) {
+    return ((scales & 0x7f7f7f7fu) + 0x03030303u) & scales & 0x80808080u;
   }
-  static __device__ __forceinline__ uint2 without_nan(const uint2 &scale) {
-    return make_uint2(without_nan(scale.x), without_nan(scale.y));
-  }
-  static __device__ __forceinline__ uint32_t without_nan(uint32_t x) {  // bytes of 255 become 127
-    return x & ~((((x & 0x7f7f7f7fu) + 0x01010101u) & x) & 0x80808080u);
+  static __device__ __forceinline__ bool has_nan(const uint2 &scale) { return (not_finite(scale.x) | not_finite(scale.y)) != 0u; }
+  static __device__ __forceinline__ uint2 without_nan(const uint2 &scale) {  // such bytes lose their top bit: 2^-2 .. 2^0
+    return make_uint2(scale.x & ~not_finite(scale.x), scale.y & ~not_finite(scale.y));
   }
 
-  // A block of NaN is expanded as if its scale were 1, since 0 * NaN would reach rows that do not see it; the
+  // A block of NaN is expanded as if its scale were 1 or less, since 0 * NaN would reach rows that do not see it; the
   // rows that do take the NaN in the end.  Bit u: the lane's row sees a token whose values 64u + 16g .. 64u + 16g + 15
   // are NaN.  Rare, so it is kept small, and `scales` (of a 32-token tile) are read again.
   static __device__ __forceinline__ uint32_t nan_units(const uint8_t *scales, int32_t start, int32_t position, int32_t from,
@@ -300,7 +300,7 @@ struct Core {
       const bool seen = j <= position && (j >= from || j < sinks);
 #pragma unroll 1
       for (uint32_t u = 0; u < kUnits; ++u) {
-        const bool bad = scales[Layout::value_scale(t, 2u * u + (g >> 1))] == kNanBlock;
+        const bool bad = scales[Layout::value_scale(t, 2u * u + (g >> 1))] > kLargestScale;
         units |= bad && seen ? 1u << u : 0u;
       }
     }
@@ -1169,7 +1169,7 @@ FerruleHipStatus validate_shape(const FerruleHipKvAttentionArgs &a) {
       a.max_pages == 0u || a.max_query_length == 0u || !kv_page_tokens_valid(a.page_tokens) ||
       a.page_count > 0x7fffffffu || a.rows > 0x7fffffffu || a.window > 0x7fffffffu || a.sinks > 0x7fffffffu ||
       (a.flags & ~(FERRULE_HIP_KV_ATTENTION_QUERY_F32 | FERRULE_HIP_KV_ATTENTION_OUTPUT_F32)) != 0u ||
-      !(a.softmax_scale > 0.0f && a.softmax_scale <= 3.4028234e38f)) {
+      !(a.softmax_scale > 0.0f && a.softmax_scale <= 0x1p127f)) {
     return FERRULE_HIP_INVALID_ARGUMENT;
   }
   if (!kv_head_dim_supported(a.head_dim)) return FERRULE_HIP_UNSUPPORTED;

@@ -953,7 +953,10 @@ int32_t ferrule_hip_kv_cache_read_launch(const FerruleHipKvCacheArgs *args);
  * reach it, whatever they hold.
  * Arithmetic: q enters rounded to BF16 (exact for BF16, and for the f32 rows of the FP8 projections,
  * which hold BF16 values); scores, softmax statistics and sums are f32; the softmax weights are
- * rounded to BF16 before they multiply the values.  Sums are formed in a fixed order.
+ * rounded to BF16 before they multiply the values.  Sums are formed in a fixed order, over weights that
+ * are divided by their sum at the end and may be 2^16 large until then: values of 2^90 and more can
+ * overflow, and a block of values with a scale byte of 253 or more, whose largest values f32 cannot
+ * hold, counts as a block of NaN.
  * `max_sequence_length`, a bound of the L_b, sizes the split of long sequences over workgroups and
  * nothing else.  Workspace: ferrule_hip_kv_attention_workspace_size bytes (may be 0), 256-byte
  * aligned, used by this call alone until it has completed. */
@@ -971,7 +974,7 @@ typedef struct FerruleHipKvAttentionArgs {
   uint32_t window;            /* 0: every position up to the row's own */
   uint32_t sinks;             /* ignored when window is 0 */
   uint32_t flags;
-  float softmax_scale;        /* finite, more than 0 */
+  float softmax_scale;        /* more than 0, at most 2^127 */
   uint64_t q_row_stride;      /* in values, as in FerruleHipKvCacheArgs */
   uint64_t q_head_stride;
   uint64_t output_row_stride;

@@ -1,0 +1,191 @@
+"""Attention over the MXFP4 cache in each of its kernels: token ranges in several parts and their joins, short ranges,
+blocks that are not finite, graphs.  Same float64 reference and derived bound as tests/test_kv_cache_gpu.py."""
+import numpy as np
+import pytest
+
+from tests import kv_helpers as K
+from tests.test_kv_cache_gpu import _attend, _case, _place, ctx  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+
+MANY = [1] * 135  # two key/value heads: more segments than the card has CUs
+
+
+def _many_lengths():
+    rng = np.random.default_rng(3)
+    lengths = rng.integers(1, 60, len(MANY))
+    lengths[[0, 7, 77, 134]] = 600, 513, 512, 255
+    return lengths.tolist()
+
+
+PARTS = [  # new rows, lengths, page, kv heads, group, head size, window, sinks
+    # few rows: parts of eight 32-token tiles, joined eight or fewer at a time or in chunks
+    ([1], [5000], 64, 1, 2, 64, 0, 0), ([1, 1], [5000, 330], 32, 1, 8, 128, 0, 0), ([2], [4700], 128, 1, 8, 256, 0, 0),
+    ([1, 2], [4700, 257], 64, 1, 16, 512, 0, 0), ([1], [500], 32, 1, 16, 512, 0, 0), ([3], [6000], 64, 1, 8, 128, 4500, 40),
+    (MANY, _many_lengths(), 32, 2, 2, 64, 0, 0), (MANY, _many_lengths(), 64, 2, 3, 128, 300, 5),
+    # many rows: parts of sixteen tiles and more
+    ([100], [5000], 64, 1, 1, 64, 0, 0), ([20, 9], [3100, 1700], 64, 1, 2, 128, 0, 0), ([60], [2500], 32, 1, 2, 128, 0, 0),
+    ([300], [2000], 64, 1, 1, 64, 0, 0), ([300, 1], [2000, 700], 128, 1, 1, 128, 1500, 40), ([150], [2000], 256, 1, 1, 256, 0, 0),
+    ([50], [1800], 32, 1, 1, 256, 0, 0), ([70], [1500], 64, 1, 1, 512, 0, 0), ([2], [1200], 64, 1, 64, 512, 900, 3),
+]
+
+
+@pytest.mark.parametrize("types", ["bf16", "f32"])
+@pytest.mark.parametrize("new,lengths,page,heads,group,d,window,sinks", PARTS)
+def test_ranges_in_parts_equal_float64(ctx, new, lengths, page, heads, group, d, window, sinks, types):  # noqa: F811
+    rng = np.random.default_rng(len(new) + d + lengths[0])
+    batch, host, q = _case(rng, new, lengths, page, heads, group, d)
+    scale = float(d) ** -0.5
+    want, bound = K.attention_reference(host, batch, q, scale, window, sinks, f32_output=types == "f32")
+    t = torch.float32 if types == "f32" else torch.bfloat16
+    K.check_attention(_attend(ctx, host, batch, q, scale, window, sinks, t, t), want, bound)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("length", [255, 256, 257, 289, 513, 2015, 2016, 2047, 2049])
+def test_short_ranges_around_the_shares_of_the_waves(ctx, d, length):  # noqa: F811
+    rng = np.random.default_rng(length)
+    batch, host, q = _case(rng, [1, 2], [length, 1 + length // 3], 64, 1, 3, d)
+    for window, sinks in ((0, 0), (length - 20, 1)):
+        want, bound = K.attention_reference(host, batch, q, 0.1, window, sinks)
+        K.check_attention(_attend(ctx, host, batch, q, 0.1, window, sinks), want, bound)
+
+
+@pytest.mark.parametrize("new,lengths,group,window,sinks", [
+    ([1, 1, 1], [16, 700, 129], 64, 128, 4), ([2, 1], [90, 5], 32, 0, 0), ([1, 3], [300, 64], 16, 100, 0), ([1], [1], 33, 0, 0),
+    ([1, 1], [2000, 250], 64, 160, 4)])
+def test_heads_of_512_over_short_ranges(ctx, new, lengths, group, window, sinks):  # noqa: F811
+    rng = np.random.default_rng(61)
+    batch, host, q = _case(rng, new, lengths, 64, 1, group, 512)
+    want, bound = K.attention_reference(host, batch, q, 0.05, window, sinks)
+    K.check_attention(_attend(ctx, host, batch, q, 0.05, window, sinks), want, bound)
+
+
+def test_more_sequences_than_a_small_table(ctx):  # noqa: F811
+    rng = np.random.default_rng(67)
+    lengths = rng.integers(0, 5, 700).tolist()
+    batch, host, q = _case(rng, [min(n, 1) for n in lengths], lengths, 32, 1, 2, 64)
+    want, bound = K.attention_reference(host, batch, q, 0.1)
+    K.check_attention(_attend(ctx, host, batch, q, 0.1), want, bound)
+
+
+EVERY_KERNEL = [  # new rows, lengths, group, head size, window, sinks
+    ([1], [300], 4, 64, 0, 0), ([1], [300], 4, 128, 100, 5), ([1, 2], [2300, 40], 4, 128, 0, 0), ([1], [300], 4, 256, 0, 0),
+    ([1], [2300], 2, 256, 2100, 1), ([1], [400], 16, 512, 0, 0), ([1], [130], 64, 512, 100, 3), ([50], [130], 1, 64, 20, 2),
+    ([100], [130], 1, 64, 0, 0), ([270], [300], 1, 64, 50, 0), ([50], [700], 1, 128, 0, 0), ([100], [130], 1, 128, 33, 1),
+    ([270], [300], 1, 128, 0, 0), ([50], [130], 1, 256, 0, 0), ([100], [700], 1, 256, 40, 0), ([50], [130], 2, 512, 30, 3),
+]
+
+
+@pytest.mark.parametrize("scale_byte,nibbles", [(255, 0x00), (254, 0xf7), (253, 0x6e)])
+@pytest.mark.parametrize("new,lengths,group,d,window,sinks", EVERY_KERNEL)
+def test_unseen_blocks_of_nan_and_beyond_the_range_of_f32_reach_nobody(ctx, new, lengths, group, d, window, sinks,  # noqa: F811
+                                                                       scale_byte, nibbles):
+    rng = np.random.default_rng(71)
+    batch, host, q = _case(rng, new, lengths, 64, 1, group, d)
+    want, bound = K.attention_reference(host, batch, q, 0.1, window, sinks)
+    keep = K.HostCache(batch.pages, 64, 1, d, fill=nibbles)
+    keep.arrays[1][:] = keep.arrays[3][:] = scale_byte
+    for b in range(len(new)):
+        seen = np.zeros(lengths[b], bool)
+        for p in batch.positions(b):
+            j = np.arange(lengths[b])
+            seen |= (j <= p) & ((window == 0) | (p - j < window) | (j < sinks))
+        for j in np.flatnonzero(seen):
+            for which in (0, 1):
+                keep.put(*_place(batch, b, j, 0), which, *host.get(*_place(batch, b, j, 0), which))
+    K.check_attention(_attend(ctx, keep, batch, q, 0.1, window, sinks), want, bound)
+
+
+@pytest.mark.parametrize("new,lengths,group,d,window,sinks", EVERY_KERNEL)
+def test_a_row_takes_its_own_nan_and_not_its_neighbours(ctx, new, lengths, group, d, window, sinks):  # noqa: F811
+    """One block of NaN at the first rows' position: the rows from there on see it, within the window."""
+    rng = np.random.default_rng(73)
+    batch, host, q = _case(rng, new, lengths, 32, 1, group, d)
+    places = [(0, lengths[0] - (new[0] + 1) // 2, d // 32 - 1), (0, max(0, lengths[0] - 40), 0)]
+    for b, j, block in places:
+        code, scale = host.get(*_place(batch, b, j, 0), 1)
+        scale = scale.copy()
+        scale[block] = 255
+        host.put(*_place(batch, b, j, 0), 1, code, scale)
+    want, bound = K.attention_reference(host, batch, q, 0.1, window, sinks)
+    assert np.isnan(want).any()
+    K.check_attention(_attend(ctx, host, batch, q, 0.1, window, sinks), want, bound)
+
+
+def test_the_widest_window_is_no_window(ctx):  # noqa: F811
+    """Also with rows in front of position 0, which see nothing."""
+    rng = np.random.default_rng(79)
+    for new, lengths in (([1, 4], [300, 2]), ([90, 40], [60, 300])):
+        batch, host, q = _case(rng, new, lengths, 32, 1, 2, 64)
+        want = _attend(ctx, host, batch, q, 0.1)
+        for sinks in (0, 0x7fffffff):
+            got = _attend(ctx, host, batch, q, 0.1, 0x7fffffff, sinks)
+            assert np.array_equal(got, want)
+        reference, bound = K.attention_reference(host, batch, q, 0.1)
+        K.check_attention(want, reference, bound)
+
+
+def test_an_infinity_or_a_nan_of_a_query_stays_in_its_row(ctx):  # noqa: F811
+    rng = np.random.default_rng(83)
+    for new, lengths, d in (([2], [300], 128), ([1, 1], [300, 40], 512), ([60], [90], 64)):
+        batch, host, q = _case(rng, new, lengths, 32, 1, 2, d)
+        want, bound = K.attention_reference(host, batch, q, 0.1)
+        q[0, 1, 5], q[1, 0, d - 1] = np.inf, np.nan
+        got = _attend(ctx, host, batch, q, 0.1)
+        lost = np.zeros(got.shape, bool)
+        lost[0, 1], lost[1, 0] = True, True
+        K.check_attention(got, np.where(lost, np.nan, want), bound)
+
+
+def test_two_graphs_share_a_workspace_when_they_follow_each_other(ctx):  # noqa: F811
+    """A split decode step and a split prompt chunk, captured with one workspace and replayed in turn on one stream."""
+    from ferrule_amd.provider import HipArtifactOperatorContext
+    rng = np.random.default_rng(89)
+    steps = []
+    for new, lengths, group, d in (([1, 1], [3500, 2600], 4, 128), ([70], [2400], 1, 128)):
+        batch, host, q = _case(rng, new, lengths, 64, 2, group, d)
+        steps.append((host.device(), batch.device(), torch.from_numpy(q).bfloat16().cuda(), 2 * group))
+    stream = torch.cuda.Stream()
+    side = HipArtifactOperatorContext(0, stream)
+    ws = max((side.kv_cache_attention_workspace(c, b, heads) for c, b, _, heads in steps), key=lambda t: t.numel())
+    outs = [torch.empty_like(q) for _, _, q, _ in steps]
+    run = lambda who, i, out, **kw: who.kv_cache_attention_into(*steps[i][:2], steps[i][2], out, 0.09, **kw)  # noqa: E731
+    torch.cuda.synchronize()
+    for i in range(2):
+        run(side, i, outs[i], workspace=ws)
+    torch.cuda.synchronize()
+    graphs = []
+    for i in range(2):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[i], stream=stream):
+            run(side, i, outs[i], workspace=ws)
+    for turn in range(4):
+        for _, _, q, _ in steps:
+            q.copy_(torch.from_numpy(rng.standard_normal(q.shape).astype(np.float32)))
+        torch.cuda.synchronize()
+        for i in range(2):
+            graphs[i].replay()
+        torch.cuda.synchronize()
+        for i in range(2):
+            want = run(ctx, i, torch.empty_like(outs[i]))
+            same = torch.equal(outs[i], want)
+            assert same, (turn, i)
+
+
+@pytest.mark.parametrize("new,d", [(1, 64), (1, 128), (1, 256), (1, 512), (90, 64), (90, 128)])
+def test_value_blocks_beyond_the_range_of_f32_count_as_nan(ctx, new, d):  # noqa: F811
+    rng = np.random.default_rng(97)
+    batch, host, q = _case(rng, [new], [200], 32, 1, 1, d)
+    for j, byte in ((100, 253), (90, 254), (80, 252)):                  # 2^125 * 6 is finite: a value like any other
+        code, scale = host.get(*_place(batch, 0, j, 0), 1)
+        scale = scale.copy()
+        scale[(byte - 252) % (d // 32)] = byte
+        host.put(*_place(batch, 0, j, 0), 1, code, scale)
+    got = _attend(ctx, host, batch, q, 0.1)
+    blocks = np.isnan(got).reshape(*got.shape[:2], -1, 32)
+    lost = np.zeros(d // 32, bool)
+    lost[[1 % (d // 32), 2 % (d // 32)]] = True
+    assert (blocks == lost[None, None, :, None]).all()
