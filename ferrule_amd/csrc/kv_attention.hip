@@ -1174,9 +1174,12 @@ FerruleHipStatus validate_shape(const FerruleHipKvAttentionArgs &a) {
   }
   if (!kv_head_dim_supported(a.head_dim)) return FERRULE_HIP_UNSUPPORTED;
   if (static_cast<uint64_t>(a.max_pages) * a.page_tokens > 0x7fffffffull) return FERRULE_HIP_UNSUPPORTED;
-  // packed rows of a sequence and the grid's x count in 32 bits (at most 256 parts)
-  if (a.batch > 65535u || static_cast<uint64_t>(row_bound(a)) * a.q_heads > 0x7fffffull) return FERRULE_HIP_UNSUPPORTED;
-  return FERRULE_HIP_SUCCESS;
+  // packed rows of a sequence count in 32 bits, and so do the threads of a grid's x (at most 512 to a workgroup)
+  const uint64_t items = static_cast<uint64_t>(row_bound(a)) * a.q_heads;
+  if (a.batch > 65535u || items > 0x0fffffffull) return FERRULE_HIP_UNSUPPORTED;
+  const SplitPlan plan = plan_splits(a);
+  const uint64_t workgroups = static_cast<uint64_t>(row_tiles(a, plan.tile_rows)) * a.kv_heads * plan.splits;
+  return workgroups > 0x7fffffull || (plan.splits > 1u && items > 0x7fffffull) ? FERRULE_HIP_UNSUPPORTED : FERRULE_HIP_SUCCESS;
 }
 
 FerruleHipStatus validate(const FerruleHipKvAttentionArgs &a) {

@@ -13,6 +13,7 @@ namespace ferrule_hip {
 namespace {
 
 constexpr uint32_t kWaves = 4;
+constexpr uint32_t kTokens = 32;  // of a tile
 
 // Where a wave works: some neighbouring tokens of one head.
 struct KvTile {
@@ -33,9 +34,9 @@ __device__ __forceinline__ bool kv_tile(const FerruleHipKvCacheArgs &a, uint32_t
   tile.sequence = kv_sequence(a.query_indptr, a.sequence_lengths, b, a.rows, a.max_query_length);
   if (tile.sequence.bad && index == 0u && (threadIdx.x & 63u) == 0u) kv_report(a.error);
   // tiles are counted from the one that holds the first row; position may be negative
-  const int32_t base = tile.sequence.position & ~static_cast<int32_t>(TOKENS - 1u);
-  tile.first = base + static_cast<int32_t>(group * TOKENS);
-  if (tile.first >= tile.sequence.position + static_cast<int32_t>(tile.sequence.rows)) return false;
+  const uint32_t before = static_cast<uint32_t>(tile.sequence.position) & (TOKENS - 1u);
+  if (group * TOKENS >= before + tile.sequence.rows) return false;
+  tile.first = tile.sequence.position + static_cast<int32_t>(group * TOKENS - before);
   tile.page_valid = false;
   tile.page_head = 0;
   tile.page_token = 0;
@@ -110,7 +111,7 @@ __global__ __launch_bounds__(256) void kv_append_kernel(FerruleHipKvCacheArgs a)
   const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
   KvTile tile;
   // a workgroup has 32 tokens: the scale bytes of a cache line come from one place
-  if (!kv_tile<32>(a, blockIdx.x, tile) || !tile.page_valid) return;
+  if (!kv_tile<kTokens>(a, blockIdx.x, tile) || !tile.page_valid) return;
   tile.first += static_cast<int32_t>(8u * wave);
   tile.page_token += 8u * wave;
   const uint32_t column = lane % kLanes, part = lane / kLanes;
@@ -216,7 +217,7 @@ __global__ __launch_bounds__(256) void kv_read_kernel(FerruleHipKvCacheArgs a) {
   const uint32_t wave = __builtin_amdgcn_readfirstlane(blockIdx.x * kWaves + (threadIdx.x >> 6));
   const bool values = (wave & 1u) != 0u;
   KvTile tile;
-  if (!kv_tile<32>(a, wave >> 1, tile)) return;
+  if (!kv_tile<kTokens>(a, wave >> 1, tile)) return;
   const uint32_t column = lane % kLanes, part = lane / kLanes;
   const int32_t offset = tile.first - tile.sequence.position;  // row of the sequence of the tile's first token
   const int32_t rows = static_cast<int32_t>(tile.sequence.rows);
@@ -274,6 +275,9 @@ __global__ __launch_bounds__(256) void kv_read_kernel(FerruleHipKvCacheArgs a) {
   }
 }
 
+// Tiles that some rows of a sequence can touch, starting at the last token of one.
+uint32_t tiles_of(uint32_t rows) { return rows / kTokens + (rows % kTokens + kTokens - 2u) / kTokens + 1u; }
+
 FerruleHipStatus validate(const FerruleHipKvCacheArgs &a) {
   if (a.batch == 0u || a.rows == 0u) return FERRULE_HIP_SUCCESS;  // nothing to do
   if (a.reserved != 0u || a.value_type > FERRULE_HIP_KV_BF16) return FERRULE_HIP_INVALID_ARGUMENT;
@@ -289,9 +293,10 @@ FerruleHipStatus validate(const FerruleHipKvCacheArgs &a) {
     return FERRULE_HIP_INVALID_ARGUMENT;
   }
   if (!kv_head_dim_supported(a.head_dim)) return FERRULE_HIP_UNSUPPORTED;
-  // the grid: batch in y, eight-token groups times heads in x
-  const uint64_t groups = (static_cast<uint64_t>(a.max_query_length) + 7u) / 8u + 1u;
-  if (a.batch > 65535u || groups * a.kv_heads > 0x3fffffffull) return FERRULE_HIP_UNSUPPORTED;
+  // batch in the grid's y; the threads of x, 256 for each head of a tile at most, count in 32 bits
+  if (a.batch > 65535u || static_cast<uint64_t>(tiles_of(a.max_query_length)) * a.kv_heads > 0xffffffull) {
+    return FERRULE_HIP_UNSUPPORTED;
+  }
   return FERRULE_HIP_SUCCESS;
 }
 
@@ -302,10 +307,7 @@ FerruleHipStatus dispatch(const FerruleHipKvCacheArgs *args) {
   if (status != FERRULE_HIP_SUCCESS || args->batch == 0u || args->rows == 0u) return status;
   const FerruleHipKvCacheArgs &a = *args;
   hipStream_t stream = reinterpret_cast<hipStream_t>(static_cast<uintptr_t>(a.stream));
-  // rows that start inside a tile touch one tile more
-  constexpr uint32_t kTokens = 32u;
-  const uint32_t rows = a.max_query_length < a.rows ? a.max_query_length : a.rows;
-  const uint32_t tiles = rows == 1u ? 1u : (rows + kTokens - 1u) / kTokens + 1u;
+  const uint32_t tiles = tiles_of(a.max_query_length < a.rows ? a.max_query_length : a.rows);
   const dim3 grid((tiles * a.kv_heads * Launch<float, 64>::kWavesPerTile + kWaves - 1u) / kWaves, a.batch);
   clear_launch_error();
   if (a.value_type == FERRULE_HIP_KV_BF16) {

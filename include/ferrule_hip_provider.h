@@ -930,7 +930,7 @@ typedef struct FerruleHipKvCacheArgs {
 } FerruleHipKvCacheArgs;
 
 /* append: quantises the batch's rows and writes them at their positions; a row without a valid
- * place is dropped.  The pages that one call writes belong to one sequence each.
+ * place is dropped.  A page that one call writes belongs to one sequence and stands once in its table.
  * read: the cache's values at the rows' positions (exact in either type); a row without a valid
  * place reads as zeros.  To read positions [s, e) of a sequence pass n_b = e - s and L_b = e.
  * INVALID_ARGUMENT for a bad block, UNSUPPORTED for a head_dim outside the supported set; a block

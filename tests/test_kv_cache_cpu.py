@@ -146,3 +146,22 @@ def test_the_helpers_quantiser_is_the_oracles_on_bf16_values():
     assert (np.asarray(scales).reshape(scale.shape) == scale).all()
     packed = np.asarray(packed).reshape(64, 64)
     assert (packed == (code[:, 0::2] | code[:, 1::2] << 4)).all()
+
+
+def test_grids_that_a_launch_cannot_count_are_refused_and_the_largest_that_it_can_are_not():
+    lib = abi.load()
+    can = lib.ferrule_hip_kv_cache_append_can_implement
+    # 2^24 - 1 tiles of 32 rows: the first row is the last one of its tile, then full tiles
+    most = 1 + (0xffffff - 1) * 32
+    assert can(C.byref(_cache_args(rows=most, max_query_length=most, kv_heads=1))) == abi.SUCCESS
+    assert can(C.byref(_cache_args(rows=most, max_query_length=most + 1, kv_heads=1))) == abi.UNSUPPORTED
+    assert can(C.byref(_cache_args(kv_heads=0x1000000))) == abi.UNSUPPORTED
+    can = lib.ferrule_hip_kv_attention_can_implement
+    # a prompt of 131072 tokens with 64 heads: 2^23 rows and heads
+    long = dict(rows=131072, max_query_length=131072, q_heads=64, kv_heads=8)
+    assert can(C.byref(_attention_args(**long))) == abi.SUCCESS
+    assert can(C.byref(_attention_args(**dict(long, rows=0x400000, max_query_length=0x400000)))) == abi.UNSUPPORTED
+    # one row with as many heads as the cache: a workgroup for each
+    assert can(C.byref(_attention_args(rows=1, max_query_length=1, q_heads=0x800000, kv_heads=0x800000))) == abi.UNSUPPORTED
+    assert can(C.byref(_attention_args(softmax_scale=2.0 ** 127))) == abi.SUCCESS
+    assert can(C.byref(_attention_args(softmax_scale=2.5e38))) == abi.INVALID_ARGUMENT
