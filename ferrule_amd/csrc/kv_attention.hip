@@ -1123,8 +1123,16 @@ uint32_t rows_of_workgroup(const FerruleHipKvAttentionArgs &a) {
     return 0u;
   }
   if (rows <= 64u || a.head_dim == 512u) return 64u;
-  if (rows <= 128u) return 128u;
-  return a.head_dim == 256u ? 128u : 256u;
+  // A workgroup of more rows reads and expands the tokens less often (a prompt of 8192 tokens, 32 heads of 128: 506 us
+  // with 256 rows, 543 with 128, 645 with 64).  But the ranges of a prompt's rows differ, and cutting them costs more
+  // than it gives: two workgroups for a CU even them out (2048 tokens: 66, 60 and 61 us; 512 tokens: 28, 24 and 16.6).
+  // Nor are there enough steps in a short range to pay for the larger start (16 prompts of 256 tokens: 37, 32, 29).
+  const uint64_t range = token_tiles(a, 64u);
+  const uint64_t total = static_cast<uint64_t>(a.rows) * a.q_heads;
+  const bool prompts = 2ull * a.max_query_length > kTileTokens * range;
+  uint32_t tile = a.head_dim == 256u || rows <= 128u ? 128u : 256u;
+  while (tile > 64u && (range < 16u || (prompts && total < 512u * tile))) tile /= 2u;
+  return tile;
 }
 
 // How the token ranges are cut: into parts of equal length, so that sequences of different lengths give
