@@ -76,6 +76,8 @@ EVERY_KERNEL = [  # new rows, lengths, group, head size, window, sinks
     ([1], [2300], 2, 256, 2100, 1), ([1], [400], 16, 512, 0, 0), ([1], [130], 64, 512, 100, 3), ([50], [130], 1, 64, 20, 2),
     ([100], [130], 1, 64, 0, 0), ([270], [300], 1, 64, 50, 0), ([50], [700], 1, 128, 0, 0), ([100], [130], 1, 128, 33, 1),
     ([270], [300], 1, 128, 0, 0), ([50], [130], 1, 256, 0, 0), ([100], [700], 1, 256, 40, 0), ([50], [130], 2, 512, 30, 3),
+    ([270], [700], 1, 64, 0, 0), ([100], [700], 1, 64, 0, 0), ([270], [800], 1, 128, 600, 3), ([100], [700], 1, 128, 0, 0),
+    ([100], [800], 1, 256, 620, 2),
 ]
 
 
@@ -189,3 +191,33 @@ def test_value_blocks_beyond_the_range_of_f32_count_as_nan(ctx, new, d):  # noqa
     lost = np.zeros(d // 32, bool)
     lost[[1 % (d // 32), 2 % (d // 32)]] = True
     assert (blocks == lost[None, None, :, None]).all()
+
+
+@pytest.mark.parametrize("n,length,heads,group,d,window,sinks", [
+    (2100, 2100, 1, 64, 64, 0, 0), (2100, 2300, 2, 32, 128, 0, 0), (1100, 1100, 2, 32, 256, 0, 0), (2200, 2200, 1, 64, 128, 900, 7),
+    (1030, 1030, 4, 16, 128, 0, 0), (600, 600, 1, 64, 512, 0, 0)])
+def test_prompts_of_many_rows_equal_float64(ctx, n, length, heads, group, d, window, sinks):  # noqa: F811
+    """Enough rows for the largest workgroups.  The reference is float64 on the GPU over the values that the read operator
+    gives back (exact), the bound that of tests/kv_helpers.py."""
+    rng = np.random.default_rng(n + d)
+    batch, host, q = _case(rng, [n], [length], 64, heads, group, d)
+    cache, dev = host.device(), batch.device()
+    qd = torch.from_numpy(q).bfloat16().cuda()
+    out = ctx.kv_cache_attention_into(cache, dev, qd, torch.empty_like(qd), d ** -0.5, window=window, sinks=sinks)
+    every = K.HostBatch.__new__(K.HostBatch)                            # all tokens as rows
+    every.__dict__ = dict(batch.__dict__, new=[length], indptr=np.array([0, length], np.int32))
+    k, v = (torch.empty((length, heads, d), device="cuda") for _ in range(2))
+    ctx.kv_cache_read_into(cache, every.device(), k, v)
+    p = torch.arange(length - n, length, device="cuda")[:, None]
+    j = torch.arange(length, device="cuda")[None, :]
+    seen = (j <= p) & ((p - j < window) | (j < sinks)) if window else j <= p
+    count = seen.sum(1, keepdim=True).double()
+    for h in range(heads * group):
+        qs, ks, vs = qd[:, h].double(), k[:, h // group].double(), v[:, h // group].double()
+        w = torch.softmax((qs @ ks.T * d ** -0.5).masked_fill(~seen, -np.inf), -1)
+        want, size = w @ vs, w @ vs.abs()
+        most = (qs.abs() @ ks.abs().T * d ** -0.5).masked_fill(~seen, 0).amax(-1, keepdim=True)
+        e = most * (32 * 2.0 ** -20 + d * 2.0 ** -23 + 2.0 ** -20) + 2.0 ** -20
+        bound = size * (2.0 ** -8 + 2.2 * e + 2 * count * 2.0 ** -23) + want.abs() * 2.0 ** -8 + 1e-37
+        worst = ((out[:, h].double() - want).abs() / bound).max().item()
+        assert worst <= 1, (h, worst)
