@@ -128,7 +128,7 @@ class HipKvCache:
                 raise ValueError(f"HIP KV cache array must be contiguous uint8 {shape}, got {t.dtype} {tuple(t.shape)}")
         if self.page_count < 1:
             raise ValueError("HIP KV cache needs at least one page")
-        self.device = k_payload.device
+        self.device, self.device_index = k_payload.device, k_payload.get_device()
         self.pointers = tuple(_ptr(t) for t in arrays)     # the arrays stay: this object holds them
 
 
@@ -156,7 +156,9 @@ class HipKvBatch:
         if self.rows < 0 or self.max_query_length < min(self.rows, 1) or \
                 (self.max_sequence_length is not None and self.max_sequence_length < 0):
             raise ValueError("HIP KV batch needs rows >= 0 and bounds of at least one row")
-        self.device = query_indptr.device
+        if max(self.rows, self.max_query_length, self.max_sequence_length or 0) > 0x7fffffff:
+            raise ValueError("HIP KV batch counts rows and tokens in 31 bits")
+        self.device, self.device_index = query_indptr.device, query_indptr.get_device()
         self.pointers = (_ptr(query_indptr), _ptr(sequence_lengths), _ptr(page_table))
 
 
@@ -1098,54 +1100,55 @@ class HipArtifactOperatorContext:
 
     # A decode step's operators take a few microseconds on the GPU, so their host side is kept short: argument
     # blocks are filled by position, and the raw stream handle is asked for without a stream object.
-    def _check_kv(self, cache: HipKvCache, batch: HipKvBatch, error: torch.Tensor | None) -> torch.device:
-        device = cache.device
-        if device.type != "cuda" or device.index != (torch.cuda.current_device() if self.device.index is None
-                                                     else self.device.index):
-            raise ValueError(f"HIP KV operators run on {self.device}, the cache is on {device}")
-        if batch.device != device:
-            raise ValueError(f"HIP KV operators need every tensor on the cache's device {device}")
-        if error is not None and (error.dtype != torch.int32 or error.numel() != 1 or error.device != device):
+    # The three operators are called for a few microseconds of work: a decode step's rows take the GPU less time
+    # than these checks take the host.
+    def _check_kv(self, cache: HipKvCache, batch: HipKvBatch, error: torch.Tensor | None) -> int:
+        """The index of the device that everything is on."""
+        index, own = cache.device_index, self.device.index
+        if index < 0 or index != (torch.cuda.current_device() if own is None else own):
+            raise ValueError(f"HIP KV operators run on {self.device}, the cache is on {cache.device}")
+        if batch.device_index != index:
+            raise ValueError(f"HIP KV operators need every tensor on the cache's device {cache.device}")
+        if error is not None and (error.dtype != torch.int32 or error.numel() != 1 or error.get_device() != index):
             raise ValueError("HIP KV error flag must be one int32 on the device")
-        return device
+        return index
 
     @staticmethod
-    def _check_kv_rows(what: str, t: torch.Tensor, shape: tuple[int, int, int], device: torch.device) -> tuple[int, ...]:
+    def _check_kv_rows(what: str, t: torch.Tensor, shape: tuple[int, int, int], index: int) -> tuple[int, ...]:
         """The row tensor's strides, once it is what the operators take."""
-        strides = t.stride()
-        if t.dtype not in (torch.bfloat16, torch.float32) or t.shape != shape or strides[2] != 1:
+        strides, dtype = t.stride(), t.dtype
+        if (dtype is not torch.bfloat16 and dtype is not torch.float32) or t.shape != shape or strides[2] != 1:
             raise ValueError(f"HIP KV {what} must be bf16 or f32 {shape} with consecutive values, "
                              f"got {t.dtype} {tuple(t.shape)} strides {strides}")
-        if t.device != device:
-            raise ValueError(f"HIP KV {what} must be on the cache's device {device}, not on {t.device}")
+        if t.get_device() != index:
+            raise ValueError(f"HIP KV {what} must be on the cache's device, not on {t.device}")
         return strides
 
-    def _kv_launch(self, what: str, can_implement, launch, args, device: torch.device) -> None:
-        """``_two_phase`` with the cache's device current, which a launch on its stream needs."""
-        index = device.index
-        if torch.cuda.current_device() != index:
+    def _kv_launch(self, what: str, can_implement, launch, args, index: int) -> None:
+        """One call, which validates and launches (``can_implement`` only tells the two errors apart), with the
+        cache's device current, which a launch on its stream needs."""
+        if torch._C._cuda_getDevice() != index:
             with torch.cuda.device(index):
-                return self._kv_launch(what, can_implement, launch, args, device)
+                return self._kv_launch(what, can_implement, launch, args, index)
         args.stream = torch._C._cuda_getCurrentRawStream(index) if self._stream is None else self._stream.cuda_stream
-        status = can_implement(C.byref(args))
-        if status != abi.SUCCESS:
-            raise ProviderError(f"validate {what}", status)
         status = launch(C.byref(args))
         if status != abi.SUCCESS:
-            raise ProviderError(f"launch {what}", status)
+            refused = can_implement(C.byref(args)) != abi.SUCCESS
+            raise ProviderError(f"{'validate' if refused else 'launch'} {what}", status)
         self.kernel_launches += 1
 
     def _kv_cache_args(self, cache: HipKvCache, batch: HipKvBatch, k: torch.Tensor, v: torch.Tensor,
-                       error: torch.Tensor | None, device: torch.device) -> abi.KvCacheArgs:
+                       error: torch.Tensor | None, index: int) -> abi.KvCacheArgs:
         shape = (batch.rows, cache.kv_heads, cache.head_dim)
-        ks = self._check_kv_rows("keys", k, shape, device)
-        vs = self._check_kv_rows("values", v, shape, device)
-        if k.dtype != v.dtype:
+        ks = self._check_kv_rows("keys", k, shape, index)
+        vs = self._check_kv_rows("values", v, shape, index)
+        dtype = k.dtype
+        if dtype is not v.dtype:
             raise ValueError("HIP KV keys and values share one type")
         return abi.KvCacheArgs(
             batch.batch, batch.rows, cache.kv_heads, cache.head_dim, cache.page_tokens, cache.page_count, batch.max_pages,
-            batch.max_query_length, abi.KV_BF16 if k.dtype == torch.bfloat16 else abi.KV_F32, 0, ks[0], ks[1], vs[0], vs[1],
-            _ptr(k), _ptr(v), *cache.pointers, *batch.pointers, _ptr(error))
+            batch.max_query_length, abi.KV_BF16 if dtype is torch.bfloat16 else abi.KV_F32, 0, ks[0], ks[1], vs[0], vs[1],
+            k.data_ptr(), v.data_ptr(), *cache.pointers, *batch.pointers, _ptr(error))
 
     def kv_cache_append(self, cache: HipKvCache, batch: HipKvBatch, k: torch.Tensor, v: torch.Tensor,
                         error: torch.Tensor | None = None) -> None:
@@ -1153,32 +1156,33 @@ class HipArtifactOperatorContext:
         heads strided as they like) and write them at their positions.  The bytes are those of
         ``pack_fp4_rows_from_f32`` (its default rounding), except that a block holding an infinity or
         a NaN is written as a block of NaN.  ``error`` (int32 [1], cleared by the caller) becomes 1 when
-        a row has no valid place; such rows are dropped.  The pages written belong to one sequence each."""
-        device = self._check_kv(cache, batch, error)
+        a row has no valid place; such rows are dropped.  A page that is
+        written belongs to one sequence and stands once in its table."""
+        index = self._check_kv(cache, batch, error)
         if batch.rows == 0 or batch.batch == 0:
             return
         self._kv_launch("KV cache append", self.lib.ferrule_hip_kv_cache_append_can_implement,
                         self.lib.ferrule_hip_kv_cache_append_launch,
-                        self._kv_cache_args(cache, batch, k, v, error, device), device)
+                        self._kv_cache_args(cache, batch, k, v, error, index), index)
 
     def kv_cache_read_into(self, cache: HipKvCache, batch: HipKvBatch, k: torch.Tensor, v: torch.Tensor,
                            error: torch.Tensor | None = None) -> None:
         """The cache's values at the batch's positions into BF16 or f32 [rows, kv_heads, head_dim], exact
         in either type.  To read positions s..e of a sequence give it e - s rows and length e.  A row
         without a valid place reads as zeros and sets ``error``."""
-        device = self._check_kv(cache, batch, error)
+        index = self._check_kv(cache, batch, error)
         if batch.rows == 0 or batch.batch == 0:
             return
         self._kv_launch("KV cache read", self.lib.ferrule_hip_kv_cache_read_can_implement,
                         self.lib.ferrule_hip_kv_cache_read_launch,
-                        self._kv_cache_args(cache, batch, k, v, error, device), device)
+                        self._kv_cache_args(cache, batch, k, v, error, index), index)
 
     def _kv_attention_args(self, cache: HipKvCache, batch: HipKvBatch, q_heads: int, window: int, sinks: int,
                            flags: int = 0, softmax_scale: float = 1.0, *tensors) -> abi.KvAttentionArgs:
         if q_heads < 1 or q_heads % cache.kv_heads:
             raise ValueError(f"HIP KV attention needs a multiple of {cache.kv_heads} query heads, got {q_heads}")
-        if window < 0 or sinks < 0:
-            raise ValueError("HIP KV attention window and sinks must not be negative")
+        if not (0 <= window <= 0x7fffffff and 0 <= sinks <= 0x7fffffff):
+            raise ValueError("HIP KV attention window and sinks must be in 0..2^31 - 1")
         longest = batch.max_sequence_length
         if longest is None:
             longest = min(batch.max_pages * cache.page_tokens, 0x7fffffff)
@@ -1191,10 +1195,10 @@ class HipArtifactOperatorContext:
         """The scratch that ``kv_cache_attention_into`` needs for batches of this shape (uint8, possibly
         empty).  It belongs to one call at a time: keep one per stream, and one per captured graph that
         may replay while another runs."""
-        device = self._check_kv(cache, batch, None)
+        index = self._check_kv(cache, batch, None)
         args = self._kv_attention_args(cache, batch, q_heads, window, sinks)
         size = self.lib.ferrule_hip_kv_attention_workspace_size(C.byref(args))
-        return torch.empty(size, dtype=torch.uint8, device=device)
+        return torch.empty(size, dtype=torch.uint8, device=cache.device)
 
     def kv_cache_attention_into(self, cache: HipKvCache, batch: HipKvBatch, q: torch.Tensor, out: torch.Tensor,
                                 softmax_scale: float, window: int = 0, sinks: int = 0,
@@ -1205,26 +1209,26 @@ class HipArtifactOperatorContext:
         reads key/value head h // (q_heads // kv_heads), and the row at position p sees position j when
         ``j <= p and (window == 0 or p - j < window or j < sinks)``.  A row that sees nothing writes
         zeros.  Without ``workspace`` one is taken from torch's allocator for the call."""
-        device = self._check_kv(cache, batch, error)
+        index = self._check_kv(cache, batch, error)
         q_heads = q.shape[1] if q.dim() == 3 else 0
         shape = (batch.rows, q_heads, cache.head_dim)
-        qs = self._check_kv_rows("queries", q, shape, device)
-        os = self._check_kv_rows("output", out, shape, device)
-        flags = (abi.KV_ATTENTION_QUERY_F32 if q.dtype == torch.float32 else 0) | \
-            (abi.KV_ATTENTION_OUTPUT_F32 if out.dtype == torch.float32 else 0)
+        qs = self._check_kv_rows("queries", q, shape, index)
+        os = self._check_kv_rows("output", out, shape, index)
+        flags = (abi.KV_ATTENTION_QUERY_F32 if q.dtype is torch.float32 else 0) | \
+            (abi.KV_ATTENTION_OUTPUT_F32 if out.dtype is torch.float32 else 0)
         a = self._kv_attention_args(cache, batch, q_heads, window, sinks, flags, softmax_scale, qs[0], qs[1], os[0], os[1],
-                                    _ptr(q), _ptr(out), *cache.pointers, *batch.pointers, _ptr(error))
+                                    q.data_ptr(), out.data_ptr(), *cache.pointers, *batch.pointers, _ptr(error))
         if batch.rows == 0 or batch.batch == 0:
             return out
         if workspace is None:
             size = self.lib.ferrule_hip_kv_attention_workspace_size(C.byref(a))
             with torch.cuda.stream(self.stream):       # the block is reused in this stream's order
-                workspace = torch.empty(size, dtype=torch.uint8, device=device)
-        elif workspace.dtype != torch.uint8 or workspace.device != device or not workspace.is_contiguous():
+                workspace = torch.empty(size, dtype=torch.uint8, device=cache.device)
+        elif workspace.dtype != torch.uint8 or workspace.get_device() != index or not workspace.is_contiguous():
             raise ValueError("HIP KV attention workspace must be contiguous uint8 on the device")
         a.workspace, a.workspace_bytes = _ptr(workspace), workspace.numel()
         self._kv_launch("KV attention", self.lib.ferrule_hip_kv_attention_can_implement,
-                        self.lib.ferrule_hip_kv_attention_launch, a, device)
+                        self.lib.ferrule_hip_kv_attention_launch, a, index)
         return out
 
     # -- routed MoE ---------------------------------------------------------------

@@ -221,3 +221,11 @@ def test_prompts_of_many_rows_equal_float64(ctx, n, length, heads, group, d, win
         bound = size * (2.0 ** -8 + 2.2 * e + 2 * count * 2.0 ** -23) + want.abs() * 2.0 ** -8 + 1e-37
         worst = ((out[:, h].double() - want).abs() / bound).max().item()
         assert worst <= 1, (h, worst)
+
+
+def test_windows_beyond_31_bits_are_refused(ctx):  # noqa: F811
+    rng = np.random.default_rng(1)
+    batch, host, q = _case(rng, [1], [40], 32, 1, 1, 64)
+    for kw in (dict(window=2 ** 31), dict(window=2 ** 32 + 5), dict(window=5, sinks=2 ** 32)):
+        with pytest.raises(ValueError):
+            _attend(ctx, host, batch, q, 0.1, **kw)

@@ -165,3 +165,13 @@ def test_grids_that_a_launch_cannot_count_are_refused_and_the_largest_that_it_ca
     assert can(C.byref(_attention_args(rows=1, max_query_length=1, q_heads=0x800000, kv_heads=0x800000))) == abi.UNSUPPORTED
     assert can(C.byref(_attention_args(softmax_scale=2.0 ** 127))) == abi.SUCCESS
     assert can(C.byref(_attention_args(softmax_scale=2.5e38))) == abi.INVALID_ARGUMENT
+
+
+def test_batches_beyond_31_bits_are_refused():
+    import torch
+    from ferrule_amd.provider import HipKvBatch
+    i32 = lambda *shape: torch.zeros(shape, dtype=torch.int32)  # noqa: E731
+    HipKvBatch(i32(2), i32(1), i32(1, 4), 0x7fffffff, 0x7fffffff, 0x7fffffff)
+    for more in ((2 ** 31, 1, 1), (1, 2 ** 32 + 1, 1), (1, 1, 2 ** 32)):
+        with pytest.raises(ValueError):
+            HipKvBatch(i32(2), i32(1), i32(1, 4), *more)
