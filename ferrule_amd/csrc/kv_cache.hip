@@ -15,41 +15,43 @@ namespace {
 constexpr uint32_t kWaves = 4;
 constexpr uint32_t kTokens = 32;  // of a tile
 
-// Where a wave works: some neighbouring tokens of one head.
+// Where a wave works: 32 neighbouring tokens of one head.  In two steps, since rows can be asked for before the page
+// is known.
 struct KvTile {
   KvSequence sequence;
   uint32_t head;
-  uint32_t page_token;  // of the tile's first token
+  int32_t offset;       // row of the sequence of the tile's first token, may be negative
+  uint32_t page_token;  // of that token
   uint64_t page_head;   // page * kv_heads + head
   bool page_valid;      // false: no token of the tile has a place
-  int32_t first;        // position of the tile's first token, a multiple of TOKENS
-};
 
-// Tile `index` of sequence blockIdx.y, by head first; false when the sequence has no such tile.
-template <uint32_t TOKENS>
-__device__ __forceinline__ bool kv_tile(const FerruleHipKvCacheArgs &a, uint32_t index, KvTile &tile) {
-  const uint32_t b = blockIdx.y;
-  tile.head = index % a.kv_heads;
-  const uint32_t group = index / a.kv_heads;
-  tile.sequence = kv_sequence(a.query_indptr, a.sequence_lengths, b, a.rows, a.max_query_length);
-  if (tile.sequence.bad && index == 0u && (threadIdx.x & 63u) == 0u) kv_report(a.error);
-  // tiles are counted from the one that holds the first row; position may be negative
-  const uint32_t before = static_cast<uint32_t>(tile.sequence.position) & (TOKENS - 1u);
-  if (group * TOKENS >= before + tile.sequence.rows) return false;
-  tile.first = tile.sequence.position + static_cast<int32_t>(group * TOKENS - before);
-  tile.page_valid = false;
-  tile.page_head = 0;
-  tile.page_token = 0;
-  const uint32_t slot = static_cast<uint32_t>(tile.first) / a.page_tokens;
-  if (tile.first >= 0 && slot < a.max_pages) {
-    const int32_t page = kv_uniform(a.page_table, static_cast<uint64_t>(b) * a.max_pages + slot);
-    tile.page_token = static_cast<uint32_t>(tile.first) % a.page_tokens;
-    tile.page_valid = static_cast<uint32_t>(page) < a.page_count;
-    if (tile.page_valid) tile.page_head = static_cast<uint64_t>(page) * a.kv_heads + tile.head;
+  // Tile `index` of sequence blockIdx.y, by head first; false when the sequence has no such tile.
+  __device__ __forceinline__ bool rows_of(const FerruleHipKvCacheArgs &a, uint32_t index) {
+    head = index % a.kv_heads;
+    const uint32_t group = index / a.kv_heads;
+    sequence = kv_sequence(a.query_indptr, a.sequence_lengths, blockIdx.y, a.rows, a.max_query_length);
+    if (sequence.bad && index == 0u && (threadIdx.x & 63u) == 0u) kv_report(a.error);
+    // tiles are counted from the one that holds the first row; its position may be negative
+    const uint32_t before = static_cast<uint32_t>(sequence.position) & (kTokens - 1u);
+    if (group * kTokens >= before + sequence.rows) return false;
+    offset = static_cast<int32_t>(group * kTokens - before);
+    return true;
   }
-  if (!tile.page_valid && (threadIdx.x & 63u) == 0u) kv_report(a.error);
-  return true;
-}
+  __device__ __forceinline__ void page_of(const FerruleHipKvCacheArgs &a) {
+    const int32_t first = sequence.position + offset;
+    page_valid = false;
+    page_head = 0;
+    page_token = 0;
+    const uint32_t slot = static_cast<uint32_t>(first) / a.page_tokens;
+    if (first >= 0 && slot < a.max_pages) {
+      const int32_t page = kv_uniform(a.page_table, static_cast<uint64_t>(blockIdx.y) * a.max_pages + slot);
+      page_token = static_cast<uint32_t>(first) % a.page_tokens;
+      page_valid = static_cast<uint32_t>(page) < a.page_count;
+      if (page_valid) page_head = static_cast<uint64_t>(page) * a.kv_heads + head;
+    }
+    if (!page_valid && (threadIdx.x & 63u) == 0u) kv_report(a.error);
+  }
+};
 
 // Eight consecutive values of a row as f32.
 __device__ __forceinline__ void load8(const uint16_t *src, float (&x)[8]) {
@@ -98,8 +100,10 @@ __device__ __forceinline__ uint32_t quantise8(const float (&x)[8], uint32_t &pac
   return static_cast<uint32_t>(n + 127);
 }
 
-// A wave has one head of eight neighbouring tokens, the unit of the value layout: a lane takes eight
-// values, so that a row of 128 is sixteen lanes side by side, and keys and values are asked for together.
+// A wave has up to 128 values of one head of eight neighbouring tokens, the unit of the value layout, and a workgroup
+// those of 32 tokens: the scale bytes of a cache line come from one place.  A lane takes eight values, so that 128 of
+// a row are sixteen lanes side by side, and keys and values are asked for together, before the page is known: a decode
+// step's rows are a chain of memory latencies.
 template <typename T, uint32_t D>
 __global__ __launch_bounds__(256) void kv_append_kernel(FerruleHipKvCacheArgs a) {
   using Layout = KvLayout<D>;
@@ -109,65 +113,64 @@ __global__ __launch_bounds__(256) void kv_append_kernel(FerruleHipKvCacheArgs a)
   // the bytes of 128 values of eight tokens, turned in LDS: [value pair][token]
   __shared__ __align__(16) uint8_t turned[kWaves][64][8];
   const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+  const uint32_t c = blockIdx.x % Layout::kKeyChunks;  // 128-value piece of the rows
   KvTile tile;
-  // a workgroup has 32 tokens: the scale bytes of a cache line come from one place
-  if (!kv_tile<kTokens>(a, blockIdx.x, tile) || !tile.page_valid) return;
-  tile.first += static_cast<int32_t>(8u * wave);
-  tile.page_token += 8u * wave;
+  if (!tile.rows_of(a, blockIdx.x / Layout::kKeyChunks)) return;
   const uint32_t column = lane % kLanes, part = lane / kLanes;
-  const int32_t offset = tile.first - tile.sequence.position;  // row of the sequence of the tile's first token
+  const int32_t offset = tile.offset + static_cast<int32_t>(8u * wave);
   const int32_t rows = static_cast<int32_t>(tile.sequence.rows);
-  if (offset >= rows || offset <= -8) return;
+  const bool any = offset < rows && offset > -8;
   const bool whole = offset >= 0 && offset + 8 <= rows;
-  const T *keys = global_ptr<const T>(a.keys) + tile.head * a.key_head_stride + column * 8u;
-  const T *values = global_ptr<const T>(a.values) + tile.head * a.value_head_stride + column * 8u;
-  uint8_t *k_payload = global_ptr<uint8_t>(a.k_payload) + Layout::payload(tile.page_head, a.page_tokens);
-  uint8_t *k_scales = global_ptr<uint8_t>(a.k_scales) + Layout::scales(tile.page_head, a.page_tokens);
-  uint8_t *v_payload = global_ptr<uint8_t>(a.v_payload) + Layout::payload(tile.page_head, a.page_tokens);
-  uint8_t *v_scales = global_ptr<uint8_t>(a.v_scales) + Layout::scales(tile.page_head, a.page_tokens);
-#pragma unroll
-  for (uint32_t c = 0; c < Layout::kKeyChunks; ++c) {
-    float k[kPasses][8], v[kPasses][8];
-    bool live[kPasses];
+  float k[kPasses][8], v[kPasses][8];
+  bool live[kPasses];
+  if (any) {
+    const T *keys = global_ptr<const T>(a.keys) + tile.head * a.key_head_stride + c * 128u + column * 8u;
+    const T *values = global_ptr<const T>(a.values) + tile.head * a.value_head_stride + c * 128u + column * 8u;
 #pragma unroll
     for (uint32_t p = 0; p < kPasses; ++p) {
       const int32_t row = offset + static_cast<int32_t>(p * kTogether + part);
       live[p] = row >= 0 && row < rows;
       // a row that is not there is read as one that is: its bytes are not written
       const uint64_t at = tile.sequence.row + static_cast<uint64_t>(live[p] ? row : max(offset, 0));
-      load8(keys + at * a.key_row_stride + c * 128u, k[p]);
-      load8(values + at * a.value_row_stride + c * 128u, v[p]);
+      load8(keys + at * a.key_row_stride, k[p]);
+      load8(values + at * a.value_row_stride, v[p]);
+    }
+  }
+  tile.page_of(a);
+  if (!any || !tile.page_valid) return;
+  const uint32_t first = tile.page_token + 8u * wave;
+  uint8_t *k_payload = global_ptr<uint8_t>(a.k_payload) + Layout::payload(tile.page_head, a.page_tokens);
+  uint8_t *k_scales = global_ptr<uint8_t>(a.k_scales) + Layout::scales(tile.page_head, a.page_tokens);
+  uint8_t *v_payload = global_ptr<uint8_t>(a.v_payload) + Layout::payload(tile.page_head, a.page_tokens);
+  uint8_t *v_scales = global_ptr<uint8_t>(a.v_scales) + Layout::scales(tile.page_head, a.page_tokens);
+#pragma unroll
+  for (uint32_t p = 0; p < kPasses; ++p) {
+    const uint32_t t = p * kTogether + part, token = first + t, block = c * 4u + column / 4u;
+    uint32_t kq, vq;
+    const uint32_t ks = quantise8(k[p], kq);
+    const uint32_t vs = quantise8(v[p], vq);
+    if (live[p]) {
+      *reinterpret_cast<uint32_t *>(k_payload + Layout::key_byte(token, c) + column * 4u) = kq;
+      if ((column & 3u) == 0u) {
+        k_scales[Layout::key_scale(token, block)] = static_cast<uint8_t>(ks);
+        v_scales[Layout::value_scale(token, block)] = static_cast<uint8_t>(vs);
+      }
     }
 #pragma unroll
-    for (uint32_t p = 0; p < kPasses; ++p) {
-      const uint32_t t = p * kTogether + part, token = tile.page_token + t, block = c * 4u + column / 4u;
-      uint32_t kq, vq;
-      const uint32_t ks = quantise8(k[p], kq);
-      const uint32_t vs = quantise8(v[p], vq);
-      if (live[p]) {
-        *reinterpret_cast<uint32_t *>(k_payload + Layout::key_byte(token, c) + column * 4u) = kq;
-        if ((column & 3u) == 0u) {
-          k_scales[Layout::key_scale(token, block)] = static_cast<uint8_t>(ks);
-          v_scales[Layout::value_scale(token, block)] = static_cast<uint8_t>(vs);
-        }
-      }
-#pragma unroll
-      for (uint32_t i = 0; i < 4u; ++i) {
-        const uint8_t byte = static_cast<uint8_t>(vq >> (8u * i));
-        if (whole) {  // wave-uniform
-          turned[wave][column * 4u + i][t] = byte;
-        } else if (live[p]) {
-          v_payload[Layout::value_byte(token, c * 64u + column * 4u + i)] = byte;
-        }
+    for (uint32_t i = 0; i < 4u; ++i) {
+      const uint8_t byte = static_cast<uint8_t>(vq >> (8u * i));
+      if (whole) {  // wave-uniform
+        turned[wave][column * 4u + i][t] = byte;
+      } else if (live[p]) {
+        v_payload[Layout::value_byte(token, c * 64u + column * 4u + i)] = byte;
       }
     }
-    if (whole) {
-      wave_lds_fence();
-      const uint2 pair = *reinterpret_cast<const uint2 *>(&turned[wave][lane][0]);
-      if (c * 64u + lane < D / 2u) {
-        *reinterpret_cast<uint2 *>(v_payload + Layout::value_byte(tile.page_token, c * 64u + lane)) = pair;
-      }
-      wave_lds_fence();
+  }
+  if (whole) {
+    wave_lds_fence();
+    const uint2 pair = *reinterpret_cast<const uint2 *>(&turned[wave][lane][0]);
+    if (c * 64u + lane < D / 2u) {
+      *reinterpret_cast<uint2 *>(v_payload + Layout::value_byte(first, c * 64u + lane)) = pair;
     }
   }
 }
@@ -217,9 +220,10 @@ __global__ __launch_bounds__(256) void kv_read_kernel(FerruleHipKvCacheArgs a) {
   const uint32_t wave = __builtin_amdgcn_readfirstlane(blockIdx.x * kWaves + (threadIdx.x >> 6));
   const bool values = (wave & 1u) != 0u;
   KvTile tile;
-  if (!kv_tile<kTokens>(a, wave >> 1, tile)) return;
+  if (!tile.rows_of(a, wave >> 1)) return;
+  tile.page_of(a);
   const uint32_t column = lane % kLanes, part = lane / kLanes;
-  const int32_t offset = tile.first - tile.sequence.position;  // row of the sequence of the tile's first token
+  const int32_t offset = tile.offset;
   const int32_t rows = static_cast<int32_t>(tile.sequence.rows);
   const uint32_t block = column / 4u;
   if (!values) {
@@ -293,8 +297,9 @@ FerruleHipStatus validate(const FerruleHipKvCacheArgs &a) {
     return FERRULE_HIP_INVALID_ARGUMENT;
   }
   if (!kv_head_dim_supported(a.head_dim)) return FERRULE_HIP_UNSUPPORTED;
-  // batch in the grid's y; the threads of x, 256 for each head of a tile at most, count in 32 bits
-  if (a.batch > 65535u || static_cast<uint64_t>(tiles_of(a.max_query_length)) * a.kv_heads > 0xffffffull) {
+  // batch in the grid's y; the threads of x, 256 for each head of a tile and 128 values of it at most, count in 32 bits
+  const uint64_t workgroups = static_cast<uint64_t>(tiles_of(a.max_query_length)) * a.kv_heads * ((a.head_dim + 127u) / 128u);
+  if (a.batch > 65535u || workgroups > 0xffffffull) {
     return FERRULE_HIP_UNSUPPORTED;
   }
   return FERRULE_HIP_SUCCESS;
@@ -308,7 +313,7 @@ FerruleHipStatus dispatch(const FerruleHipKvCacheArgs *args) {
   const FerruleHipKvCacheArgs &a = *args;
   hipStream_t stream = reinterpret_cast<hipStream_t>(static_cast<uintptr_t>(a.stream));
   const uint32_t tiles = tiles_of(a.max_query_length < a.rows ? a.max_query_length : a.rows);
-  const dim3 grid((tiles * a.kv_heads * Launch<float, 64>::kWavesPerTile + kWaves - 1u) / kWaves, a.batch);
+  const dim3 grid((tiles * a.kv_heads * Launch<float, 64>::waves_per_tile(a.head_dim) + kWaves - 1u) / kWaves, a.batch);
   clear_launch_error();
   if (a.value_type == FERRULE_HIP_KV_BF16) {
     switch (a.head_dim) {
@@ -330,14 +335,15 @@ FerruleHipStatus dispatch(const FerruleHipKvCacheArgs *args) {
 
 template <typename T, uint32_t D>
 struct Append {
-  static constexpr uint32_t kWavesPerTile = 4u;  // eight tokens each
+  // eight tokens and up to 128 values each
+  static uint32_t waves_per_tile(uint32_t head_dim) { return 4u * ((head_dim + 127u) / 128u); }
   static void run(const FerruleHipKvCacheArgs &a, dim3 grid, hipStream_t stream) {
     kv_append_kernel<T, D><<<grid, 256, 0, stream>>>(a);
   }
 };
 template <typename T, uint32_t D>
 struct Read {
-  static constexpr uint32_t kWavesPerTile = 2u;  // keys and values
+  static uint32_t waves_per_tile(uint32_t) { return 2u; }  // keys and values
   static void run(const FerruleHipKvCacheArgs &a, dim3 grid, hipStream_t stream) {
     kv_read_kernel<T, D><<<grid, 256, 0, stream>>>(a);
   }
