@@ -1,29 +1,38 @@
 // Attention over the MXFP4 key/value cache (no reference symbol; formats, layout and batch
 // description: include/ferrule_hip_provider.h).
 //
-// Rows.  The n_b rows of a sequence times the `group` query heads of one key/value head are one
-// list of packed rows r = row * group + head, cut into tiles of 16: a tile is one column set of
-// the matrix instructions, and one token for eight query heads fills half of it.
+// Rows.  The n_b rows of a sequence times the `group` query heads of one key/value head are one list of packed
+// rows r = row * group + head, cut into tiles: 16 rows are one column set of the matrix instructions, and one
+// token for eight query heads fills half of it.
 //
-// One step of a wave takes 32 tokens through a tile, everything transposed so that a lane keeps ONE
-// row from the scores to the output (lane = (i, g), i = lane % 16 the row, g = lane / 16):
-//   S^T = K Q^T   v_mfma_scale_f32_16x16x128_f8f6f4: the cache's nibbles and scale bytes are the
-//                 4-bit operand as they stand; a BF16 row of q is split once into two E4M3 terms,
-//                 x = q0 2^s0 + q1 2^s1 (s1 = s0 - 5), exact but for elements below 2^-13 of their
-//                 block's largest, which are held to 2^-22 of it.
-//   softmax       the two 16-token products are fed tokens 8(m/4) + m%4 and 4 more for their rows m,
-//                 so lane (i, g) receives the scores of tokens 8g..8g+7 of row i: weights need no
-//                 exchange between lanes before they are the next product's operand.
-//   O^T += V^T P^T  v_mfma_f32_16x16x32_bf16: values cannot stay in 4 bits here (their scales run
-//                 along the row, the sum runs over tokens), so they are expanded to BF16, exactly, and
-//                 the weights are rounded to BF16 (2^-9 of each weight; the sum of the weights is
-//                 taken in f32 before that rounding).
-// The running maximum m of a row moves only when a score exceeds it by 2^8 (a wave-uniform branch):
-// weights up to 256 cost a 32-bit sum nothing, and most steps rescale nothing.
+// One step takes 32 tokens through 16 rows, everything transposed so that a lane keeps ONE row from the scores to
+// the output (lane = (i, g), i = lane % 16 the row, g = lane / 16):
+//   S^T = K Q^T   v_mfma_scale_f32_16x16x128_f8f6f4: the cache's nibbles and scale bytes are the 4-bit operand as
+//                 they stand; a BF16 row of q is split once into two E4M3 terms, x = q0 2^s0 + q1 2^s1
+//                 (s1 = s0 - 5), exact but for elements below 2^-13 of their block's largest, which are held to
+//                 2^-22 of it.
+//   softmax       the two 16-token products are fed tokens 8(m/4) + m%4 and 4 more for their rows m, so lane
+//                 (i, g) receives the scores of tokens 8g..8g+7 of row i: weights need no exchange between lanes
+//                 before they are the next product's operand.
+//   O^T += V^T P^T  v_mfma_f32_16x16x32_bf16: values cannot stay in 4 bits here (their scales run along the row,
+//                 the sum runs over tokens), so they are expanded to BF16, exactly, and the weights are rounded
+//                 to BF16: off by 2^-8 of a weight at most, as much as the output's own rounding, where 8-bit
+//                 weights would be off by 2^-4; their sum is taken in f32 before that rounding.
+// The running maximum of a row moves only when a score exceeds it by far (2^8 here, a lane's step of weights beyond
+// 2^16 in the rows kernel; a wave-uniform branch): weights of that size cost a 32-bit sum nothing, and most steps
+// rescale nothing.
 //
-// A tile's tokens are shared out over the workgroup's four waves, 32 at a time, and a long range
-// over several workgroups; (m, sum, O) of the parts are joined in a fixed order, in LDS for the
-// waves and by kv_attention_join_kernel for the workgroups.
+// Three kernels.  kv_attention_decode_kernel has 16 rows of which each wave takes its own tokens, four waves or
+// eight, so that the cache is read once and in as many places as possible; its bound is memory.
+// kv_attention_rows_kernel has 64 to 256 rows, its waves share the tokens and the expanded values; its bounds are
+// the matrix pipe and, for heads of 64, the exponentials beside it.  Where rows leave CUs idle, the tokens of a
+// tile are cut into parts of equal length for several workgroups, and (maximum, sum, O) of the parts are joined in
+// a fixed order by the join kernels.
+//   64 sequences of 8192 tokens, 8 heads of 128 for 8 query heads each: 99 us, 5.8 TB/s
+//   the same with heads of 64: 55 us, 5.3 TB/s; 4096 tokens, heads of 256: 100 us, 5.7 TB/s
+//   64 x 8192 tokens of one 512-wide row for 16 heads: 97 us, for 64 heads 157 us (the cache is 0.29 GB)
+//   a prompt of 8192 tokens, 32 heads of 128: 490-505 us, 1.1 PFLOP/s (a large bf16 matrix product: 1.2)
+//   heads of 64: 315-350 us, 0.82; 4096 tokens, 16 heads of 256: 153 us, 0.9; 1024 tokens, 64 of 512: 131 us, 0.53
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -88,20 +97,24 @@ struct Core {
   static constexpr uint32_t kUnits = D / 64u;                   // 16-byte value loads of a lane per 32 tokens
   static constexpr uint32_t kColumns = D / 16u;                 // accumulators of a tile
 
-  struct Query {
-    i32x8_t term[kChunks * kTerms];
-    uint32_t scale[kChunks * kTerms];
+  template <uint32_t N>  // of a row's 128-value pieces
+  struct QueryOf {
+    static constexpr bool kRegisters = true;
+    i32x8_t term[N * kTerms];
+    uint32_t scale[N * kTerms];
     __device__ __forceinline__ i32x8_t get(uint32_t t, uint32_t &s) const {
       s = scale[t];
       return term[t];
     }
   };
+  using Query = QueryOf<kChunks>;
   // The same in LDS, for waves that share their rows: at D = 512 the terms would take 72 registers.
   struct SharedQuery {
     u32x4_t term[kChunks * kTerms][2][64];
     uint32_t scale[kChunks * kTerms][64];
   };
   struct SharedReader {
+    static constexpr bool kRegisters = false;
     const SharedQuery &q;
     uint32_t lane;
     __device__ __forceinline__ i32x8_t get(uint32_t t, uint32_t &s) const {
@@ -109,10 +122,12 @@ struct Core {
       return make_b_fp8(q.term[t][0][lane], q.term[t][1][lane]);
     }
   };
-  struct Keys {
-    u32x4_t payload[kChunks][2];
-    uint2 scale[kChunks];
+  template <uint32_t N>
+  struct KeysOf {
+    u32x4_t payload[N][2];
+    uint2 scale[N];
   };
+  using Keys = KeysOf<kChunks>;
 
   // 16 values of a row, as BF16 pairs
   struct Pairs {
@@ -235,15 +250,16 @@ struct Core {
     return *reinterpret_cast<const T *>(p);
   }
 
-  template <bool STREAM>
-  static __device__ __forceinline__ void load_keys(const uint8_t *payload, const uint8_t *scales, const Offsets &o, Keys &k) {
+  template <bool STREAM, uint32_t N>  // pieces first .. first + N - 1
+  static __device__ __forceinline__ void load_keys(const uint8_t *payload, const uint8_t *scales, const Offsets &o, KeysOf<N> &k,
+                                                   uint32_t first = 0u) {
 #pragma unroll
-    for (uint32_t c = 0; c < kChunks; ++c) {
+    for (uint32_t c = 0; c < N; ++c) {
 #pragma unroll
       for (uint32_t half = 0; half < 2u; ++half) {
-        k.payload[c][half] = load<STREAM, u32x4_t>(payload + o.key + (c * 32u + 4u * half) * Layout::kKeyBytes);
+        k.payload[c][half] = load<STREAM, u32x4_t>(payload + o.key + ((first + c) * 32u + 4u * half) * Layout::kKeyBytes);
       }
-      k.scale[c] = *reinterpret_cast<const uint2 *>(scales + o.key_scale + c * 128u);
+      k.scale[c] = *reinterpret_cast<const uint2 *>(scales + o.key_scale + (first + c) * 128u);
     }
   }
 
@@ -256,12 +272,12 @@ struct Core {
   }
 
   // Scores of tokens 8g..8g+7 of row i: s[0..3] and s[4..7].
-  template <typename Q>
-  static __device__ __forceinline__ void scores(const Keys &k, const Q &q, uint32_t lane, f32x4_t (&s)[2]) {
+  template <uint32_t N, typename Q>
+  static __device__ __forceinline__ void scores(const KeysOf<N> &k, const Q &q, uint32_t lane, f32x4_t (&s)[2]) {
     const uint32_t shift = 8u * (lane & 3u);
     s[0] = s[1] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (uint32_t c = 0; c < kChunks; ++c) {
+    for (uint32_t c = 0; c < N; ++c) {
       const uint32_t scale[2] = {k.scale[c].x >> shift, k.scale[c].y >> shift};
 #pragma unroll
       for (uint32_t term = 0; term < kTerms; ++term) {
@@ -273,7 +289,7 @@ struct Core {
         }
       }
       // terms from LDS: not all of them at once, they would take the registers that the reader saves
-      if constexpr (!std::is_same<Q, Query>::value) __builtin_amdgcn_sched_barrier(0);
+      if constexpr (!Q::kRegisters) __builtin_amdgcn_sched_barrier(0);
     }
   }
 
@@ -289,18 +305,18 @@ struct Core {
   }
 
   // A block of NaN is expanded as if its scale were 1 or less, since 0 * NaN would reach rows that do not see it; the
-  // rows that do take the NaN in the end.  Bit u: the lane's row sees a token whose values 64u + 16g .. 64u + 16g + 15
-  // are NaN.  Rare, so it is kept small, and `scales` (of a 32-token tile) are read again.
+  // rows that do take the NaN in the end.  Bit u: the lane's row sees a token whose values 16g .. 16g + 15 of the
+  // 64 of unit first + u are NaN.  Rare, so it is kept small, and `scales` (of a 32-token tile) are read again.
   static __device__ __forceinline__ uint32_t nan_units(const uint8_t *scales, int32_t start, int32_t position, int32_t from,
-                                                       int32_t sinks, uint32_t g) {
+                                                       int32_t sinks, uint32_t g, uint32_t first = 0u, uint32_t units_of = kUnits) {
     uint32_t units = 0u;
 #pragma unroll 1
     for (uint32_t t = 0; t < kTileTokens; ++t) {
       const int32_t j = start + static_cast<int32_t>(t);
       const bool seen = j <= position && (j >= from || j < sinks);
 #pragma unroll 1
-      for (uint32_t u = 0; u < kUnits; ++u) {
-        const bool bad = scales[Layout::value_scale(t, 2u * u + (g >> 1))] > kLargestScale;
+      for (uint32_t u = 0; u < units_of; ++u) {
+        const bool bad = scales[Layout::value_scale(t, 2u * (first + u) + (g >> 1))] > kLargestScale;
         units |= bad && seen ? 1u << u : 0u;
       }
     }
@@ -428,7 +444,14 @@ __device__ __forceinline__ void store(uint64_t output, uint64_t at, bool f32, co
   }
 }
 
-// Few rows: 16 of them, the token tiles shared out over the WAVES waves.
+// Few rows: 16 of them, the token tiles shared out over the WAVES waves.  Keys and values go from memory to registers
+// with loads that leave no line behind (decode of 64 x 8192 tokens, 8 heads of 128: 117 -> 99 us with those and parts
+// of equal length), a step ahead; what a wave has in flight, 4.25 KB at heads of 128, times 16 waves is 68 KB a CU.
+// Heads of 256 and 512 have too many query terms for registers: one copy in LDS serves the four waves, and of a step's
+// values four 16-byte pieces are in flight at a time (16 heads on a row of 512: 157 -> 100 us).
+// One sequence of 1000 tokens, 8 heads of 128 for 8 query heads each: 9.3 us, of which 5 are a single step's chain of
+// launch, table, cache and join; the others are a step's arithmetic, about 0.9 us for two waves of a SIMD (loads two,
+// three or four steps ahead change nothing).
 template <uint32_t D>
 constexpr uint32_t kDecodeOccupancy = D <= 128u ? 4u : D == 256u ? 2u : 1u;  // waves per SIMD that the registers allow
 template <uint32_t D, uint32_t WAVES>
@@ -673,27 +696,44 @@ __global__ __launch_bounds__(WAVES * 64u, kDecodeOccupancy<D>) void kv_attention
 // Values are expanded to BF16 once per workgroup: a step has as many 16-byte pieces (D/64 per 32 tokens)
 // as waves, or twice that, and every wave expands its own into the operands of four accumulators, in LDS,
 // one step ahead of their use; keys are read by every wave, from cache, as they stand.  One barrier per step.
-template <uint32_t D, uint32_t NQ, uint32_t WAVES>
+// Heads of 128 take 256 rows in eight waves: per 32 tokens and 16 rows the matrix pipe is busy for 256 cycles, the
+// vector pipe for about 230 (8 exponentials of 16 cycles each, and their sums, conversions and address steps): 41 %
+// and 52 % busy by the counters, at 2.1 GHz.  Heads of 64 halve the first and not the second, and are bound by it.
+// Eight waves have the next tile's scores made before this one's weights, so that neither waits for the other (heads of
+// 256, 128 rows, 4 x 512 rows over 8192 tokens, 32 heads: 534 -> 438 us; a prompt of 4096 tokens, heads of 128: 146 ->
+// 142 us; four waves gain nothing).  At heads of 512 a wave's accumulators alone are half of the registers, so that only four waves of 16 rows
+// would stand on a CU, one for a SIMD: instead SHARES = 2 waves have the same 16 rows, each half of the values, and
+// add up their halves of the scores in LDS (4 x 512 rows over 4096 tokens, 64 heads: 1160 -> 890 us; four shares of
+// 32 rows 996).
+template <uint32_t D, uint32_t NQ, uint32_t WAVES, uint32_t SHARES>
 struct Rows {
   static constexpr uint32_t kUnits = D / 64u;
+  static constexpr uint32_t kShareUnits = kUnits / SHARES;  // of values and of the output, a wave's
+  static constexpr uint32_t kShareChunks = Core<D>::kChunks / SHARES;  // of queries and keys
   static constexpr uint32_t kPieces = kUnits > WAVES ? kUnits : WAVES;  // of a step
   static constexpr uint32_t kOwn = kPieces / WAVES;                     // of them, a wave's
   static constexpr uint32_t kSub = kPieces / kUnits;                    // 32-token tiles of a step
-  static constexpr uint32_t kInner = D >= 512u || NQ >= 4u ? 1u : kSub < 2u ? 1u : 2u;  // tiles between two looks at the maximum
-  static constexpr uint32_t kRows = 16u * NQ * WAVES;
+  static constexpr bool kAhead = WAVES == 8u;  // the next tile's scores are made before this one's weights
+  static constexpr uint32_t kInner = kAhead || D >= 512u || NQ >= 4u ? 1u : kSub < 2u ? 1u : 2u;  // tiles between two looks at the maximum
+  static constexpr uint32_t kRows = 16u * NQ * WAVES / SHARES;
   static constexpr uint32_t kOccupancy = WAVES * 64u == 512u ? 2u : D >= 512u ? 1u : 2u;  // waves per SIMD
 };
 
-template <uint32_t D, uint32_t NQ, uint32_t WAVES>
-__global__ __launch_bounds__(WAVES * 64u, (Rows<D, NQ, WAVES>::kOccupancy)) void kv_attention_rows_kernel(FerruleHipKvAttentionArgs a, SplitPlan plan) {
+template <uint32_t D, uint32_t NQ, uint32_t WAVES, uint32_t SHARES>
+__global__ __launch_bounds__(WAVES * 64u, (Rows<D, NQ, WAVES, SHARES>::kOccupancy)) void kv_attention_rows_kernel(
+    FerruleHipKvAttentionArgs a, SplitPlan plan) {
   using C = Core<D>;
-  using R = Rows<D, NQ, WAVES>;
+  using R = Rows<D, NQ, WAVES, SHARES>;
   constexpr uint32_t kSub = R::kSub, kInner = R::kInner, kOwn = R::kOwn;
+  constexpr bool kAhead = R::kAhead;
+  static_assert(SHARES == 1u || (kAhead && kSub == 1u), "shares of scores are exchanged once a step");
   __shared__ __align__(16) u32x4_t staged[2][R::kPieces][4][64];  // operands [piece][accumulator][lane]
   __shared__ uint32_t nan_of[2][WAVES];
+  __shared__ __align__(16) f32x4_t shared_scores[2][SHARES > 1u ? WAVES : 1u][SHARES > 1u ? NQ * 2u : 1u][64];
   const uint32_t lane = threadIdx.x & 63u;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t i = lane & 15u, g = lane >> 4;
+  const uint32_t share = wave % SHARES, first_unit = share * R::kShareUnits, first_chunk = share * R::kShareChunks;
   const uint32_t b = blockIdx.y;
   const uint32_t split = blockIdx.x % plan.splits;
   const uint32_t kv_head = blockIdx.x / plan.splits % a.kv_heads;
@@ -716,7 +756,7 @@ __global__ __launch_bounds__(WAVES * 64u, (Rows<D, NQ, WAVES>::kOccupancy)) void
   const bool whole = parts == 1u;
 
   // the wave's own rows
-  const uint32_t wave_row = first_row + wave * 16u * NQ;
+  const uint32_t wave_row = first_row + wave / SHARES * 16u * NQ;
   const int32_t wave_low = s.position + static_cast<int32_t>(min(wave_row, last_row) / group);
   const int32_t wave_high = s.position + static_cast<int32_t>(min(wave_row + 16u * NQ - 1u, last_row) / group);
   int32_t position[NQ], from[NQ];
@@ -730,7 +770,8 @@ __global__ __launch_bounds__(WAVES * 64u, (Rows<D, NQ, WAVES>::kOccupancy)) void
   }
   const int32_t sinks = a.window == 0u ? 0 : static_cast<int32_t>(a.sinks);
   const float factor = a.softmax_scale * 1.44269504088896341f;
-  f32x4_t out[NQ][C::kColumns];
+  constexpr uint32_t kColumns = C::kColumns / SHARES;
+  f32x4_t out[NQ][kColumns];
   float top[NQ], base[NQ], sum[NQ];
   uint32_t nan_units[NQ];
   bool unset = true;  // some row has seen no token yet
@@ -740,7 +781,7 @@ __global__ __launch_bounds__(WAVES * 64u, (Rows<D, NQ, WAVES>::kOccupancy)) void
     base[n] = sum[n] = 0.0f;
     nan_units[n] = 0u;
 #pragma unroll
-    for (uint32_t c = 0; c < C::kColumns; ++c) out[n][c] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    for (uint32_t c = 0; c < kColumns; ++c) out[n][c] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
   }
 
   const uint8_t *k_payload = global_ptr<const uint8_t>(a.k_payload), *k_scales = global_ptr<const uint8_t>(a.k_scales);
@@ -777,7 +818,7 @@ __global__ __launch_bounds__(WAVES * 64u, (Rows<D, NQ, WAVES>::kOccupancy)) void
     const uint32_t any = __any(nan) ? 1u : 0u;
     if (lane == 0u) nan_of[buffer][wave] = any;
   };
-  typename C::Keys keys[kInner];
+  typename C::template KeysOf<R::kShareChunks> keys[kInner];
   int32_t start[kInner];
   bool there[kInner];
   auto load_tiles = [&](uint32_t v, const int32_t *page) {
@@ -786,7 +827,7 @@ __global__ __launch_bounds__(WAVES * 64u, (Rows<D, NQ, WAVES>::kOccupancy)) void
       const Place p = place_at<D>(a, plan, range, kv_head, v + t, end, page[t], bad);
       start[t] = static_cast<int32_t>(p.first);
       there[t] = p.valid;
-      C::template load_keys<false>(k_payload + p.payload, k_scales + p.scales, offset, keys[t]);
+      C::template load_keys<false>(k_payload + p.payload, k_scales + p.scales, offset, keys[t], first_chunk);
     }
   };
   auto page = [&](uint32_t v) { return page_of(a, plan, range, b, v, end); };
@@ -795,20 +836,23 @@ __global__ __launch_bounds__(WAVES * 64u, (Rows<D, NQ, WAVES>::kOccupancy)) void
   uint32_t buffer = 0u;
   if (begin < end) {
 #pragma unroll
-    for (uint32_t t = 0; t < kSub; ++t) now[t] = page(begin + t);
+    for (uint32_t t = 0; t < kSub; ++t) now[t] = page(begin + t + (kAhead ? 2u : 0u));
     load_pieces(begin, page(begin + own_tile));
-    load_tiles(begin, now);
+    int32_t first_pages[kInner];
+#pragma unroll
+    for (uint32_t t = 0; t < kInner; ++t) first_pages[t] = page(begin + t);
+    load_tiles(begin, first_pages);
   }
-  typename C::Query query[NQ];
+  typename C::template QueryOf<R::kShareChunks> query[NQ];
 #pragma unroll
   for (uint32_t n = 0; n < NQ; ++n) {
-    typename C::RawPiece piece[C::kChunks];
+    typename C::RawPiece piece[R::kShareChunks];
 #pragma unroll
-    for (uint32_t c = 0; c < C::kChunks; ++c) {
-      C::load_query(a.q, row_q[n], c, (a.flags & FERRULE_HIP_KV_ATTENTION_QUERY_F32) != 0u, lane, piece[c]);
+    for (uint32_t c = 0; c < R::kShareChunks; ++c) {
+      C::load_query(a.q, row_q[n], first_chunk + c, (a.flags & FERRULE_HIP_KV_ATTENTION_QUERY_F32) != 0u, lane, piece[c]);
     }
 #pragma unroll
-    for (uint32_t c = 0; c < C::kChunks; ++c) {
+    for (uint32_t c = 0; c < R::kShareChunks; ++c) {
       i32x8_t term[C::kTerms];
       uint32_t scale[C::kTerms];
       C::split_query(piece[c], lane, term, scale);
@@ -819,7 +863,28 @@ __global__ __launch_bounds__(WAVES * 64u, (Rows<D, NQ, WAVES>::kOccupancy)) void
       }
     }
   }
+  f32x4_t later[NQ][2];  // scores of the tile behind this one, or a share of them
+  int32_t later_first = 0;
+  bool later_valid = false;
+  auto look_ahead = [&](uint32_t v, const int32_t *page, uint32_t buffer) {
+    later_first = start[0];
+    later_valid = there[0];
+#pragma unroll
+    for (uint32_t n = 0; n < NQ; ++n) C::scores(keys[0], query[n], lane, later[n]);
+    load_tiles(v, page);
+    if constexpr (SHARES > 1u) {
+#pragma unroll
+      for (uint32_t n = 0; n < NQ; ++n) {
+#pragma unroll
+        for (uint32_t half = 0; half < 2u; ++half) shared_scores[buffer][wave][n * 2u + half][lane] = later[n][half];
+      }
+    }
+  };
   if (begin < end) {
+    if constexpr (kAhead) {
+      const int32_t second = page(begin + 1u);
+      look_ahead(begin + 1u, &second, 0u);
+    }
     stage_pieces(0u);
     load_pieces(begin + kSub, page(begin + kSub + own_tile));
     piece_page = page(begin + 2u * kSub + own_tile);
@@ -827,21 +892,41 @@ __global__ __launch_bounds__(WAVES * 64u, (Rows<D, NQ, WAVES>::kOccupancy)) void
   }
   for (uint32_t v = begin; v < end; v += kSub, buffer ^= 1u) {
 #pragma unroll
-    for (uint32_t t = 0; t < kSub; ++t) next[t] = page(v + kSub + t);
+    for (uint32_t t = 0; t < kSub; ++t) next[t] = page(v + kSub + t + (kAhead ? 2u : 0u));
     const int32_t later_piece = page(v + 3u * kSub + own_tile);
 #pragma unroll
     for (uint32_t inner = 0; inner < kSub; inner += kInner) {
       f32x4_t score[NQ][kInner][2];
       int32_t first[kInner];
       bool valid[kInner];
+      if constexpr (kAhead) {
+        first[0] = later_first;
+        valid[0] = later_valid;
 #pragma unroll
-      for (uint32_t t = 0; t < kInner; ++t) {
-        first[t] = start[t];
-        valid[t] = there[t];
+        for (uint32_t n = 0; n < NQ; ++n) {
 #pragma unroll
-        for (uint32_t n = 0; n < NQ; ++n) C::scores(keys[t], query[n], lane, score[n][t]);
+          for (uint32_t half = 0; half < 2u; ++half) {
+            if constexpr (SHARES > 1u) {  // every wave adds the shares in the same order: the same bits in all of them
+              f32x4_t x = shared_scores[buffer][wave - share][n * 2u + half][lane];
+#pragma unroll
+              for (uint32_t other = 1; other < SHARES; ++other) x += shared_scores[buffer][wave - share + other][n * 2u + half][lane];
+              score[n][0][half] = x;
+            } else {
+              score[n][0][half] = later[n][half];
+            }
+          }
+        }
+        look_ahead(v + inner + 2u, now + inner, buffer ^ 1u);
+      } else {
+#pragma unroll
+        for (uint32_t t = 0; t < kInner; ++t) {
+          first[t] = start[t];
+          valid[t] = there[t];
+#pragma unroll
+          for (uint32_t n = 0; n < NQ; ++n) C::scores(keys[t], query[n], lane, score[n][t]);
+        }
+        load_tiles(v + inner + kInner, inner + kInner < kSub ? now + (inner + kInner) % kSub : next);
       }
-      load_tiles(v + inner + kInner, inner + kInner < kSub ? now + (inner + kInner) % kSub : next);
       if (inner == 0u) {
         stage_pieces(buffer ^ 1u);
         load_pieces(v + 2u * kSub, piece_page);
@@ -886,7 +971,7 @@ __global__ __launch_bounds__(WAVES * 64u, (Rows<D, NQ, WAVES>::kOccupancy)) void
             base[n] = next_base;
             sum[n] *= keep;
 #pragma unroll
-            for (uint32_t c = 0; c < C::kColumns; ++c) out[n][c] *= keep;
+            for (uint32_t c = 0; c < kColumns; ++c) out[n][c] *= keep;
             none |= next_top == -INFINITY;
           }
           unset = __any(none);
@@ -912,20 +997,21 @@ __global__ __launch_bounds__(WAVES * 64u, (Rows<D, NQ, WAVES>::kOccupancy)) void
 #pragma unroll
       for (uint32_t n = 0; n < NQ; ++n) sum[n] += added[n];
       // the value operands come from LDS kRing products ahead
-      constexpr uint32_t kOperands = kInner * C::kUnits * 4u, kRing = kOperands < 8u ? kOperands : 8u;
+      constexpr uint32_t kOperands = kInner * kColumns, kRing = kOperands < 8u ? kOperands : SHARES > 1u ? 4u : 8u;
       u32x4_t ring[kRing];
-      const u32x4_t(*operands)[64] = staged[buffer][inner * C::kUnits];
+      const u32x4_t(*operands)[64] = staged[buffer][inner * C::kUnits + first_unit];  // the share's of a tile; the next tile's
+      constexpr uint32_t kTileOperands = C::kUnits * 4u;                              // are this far on
 #pragma unroll
-      for (uint32_t f = 0; f < kRing; ++f) ring[f] = operands[f][lane];
+      for (uint32_t f = 0; f < kRing; ++f) ring[f] = operands[f / kColumns * kTileOperands + f % kColumns][lane];
 #pragma unroll
       for (uint32_t f = 0; f < kOperands; ++f) {
-        const uint32_t t = f / (4u * C::kUnits), c = f % (4u * C::kUnits);
+        const uint32_t t = f / kColumns, c = f % kColumns, ahead = f + kRing;
         const bf16x8_t operand = __builtin_bit_cast(bf16x8_t, ring[f % kRing]);
 #pragma unroll
         for (uint32_t n = 0; n < NQ; ++n) {
           out[n][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(operand, weight[n][t], out[n][c], 0, 0, 0);
         }
-        if (f + kRing < kOperands) ring[f % kRing] = operands[f + kRing][lane];
+        if (ahead < kOperands) ring[f % kRing] = operands[ahead / kColumns * kTileOperands + ahead % kColumns][lane];
       }
       __builtin_amdgcn_sched_group_barrier(0x100, kRing, 0);
 #pragma unroll
@@ -947,7 +1033,7 @@ __global__ __launch_bounds__(WAVES * 64u, (Rows<D, NQ, WAVES>::kOccupancy)) void
         if (!p.valid) continue;
 #pragma unroll
         for (uint32_t n = 0; n < NQ; ++n) {
-          nan_units[n] |= C::nan_units(v_scales + p.scales, static_cast<int32_t>(p.first), position[n], from[n], sinks, g);
+          nan_units[n] |= C::nan_units(v_scales + p.scales, static_cast<int32_t>(p.first), position[n], from[n], sinks, g, first_unit, R::kShareUnits);
         }
       }
     }
@@ -962,15 +1048,15 @@ __global__ __launch_bounds__(WAVES * 64u, (Rows<D, NQ, WAVES>::kOccupancy)) void
     if (!row.live) continue;
     const float norm = whole ? (total != 0.0f ? 1.0f / total : 0.0f) : 1.0f;
 #pragma unroll
-    for (uint32_t u = 0; u < C::kUnits; ++u) {
+    for (uint32_t u = 0; u < R::kShareUnits; ++u) {
 #pragma unroll
-      for (uint32_t half = 0; half < 2u; ++half) {  // values 64u + 16g + 8 half ..
+      for (uint32_t half = 0; half < 2u; ++half) {  // values 64u + 16g + 8 half .. of the share's
         float x[8];
 #pragma unroll
         for (uint32_t e = 0; e < 8u; ++e) {
           x[e] = (nan_units[n] >> u) & 1u ? NAN : out[n][4u * u + (e & 3u)][2u * half + (e >> 2)] * norm;
         }
-        const uint32_t d = 64u * u + 16u * g + 8u * half;
+        const uint32_t d = 64u * (first_unit + u) + 16u * g + 8u * half;
         if (whole) {
           store(a.output, row.output + d, (a.flags & FERRULE_HIP_KV_ATTENTION_OUTPUT_F32) != 0u, x);
         } else {
@@ -978,7 +1064,7 @@ __global__ __launch_bounds__(WAVES * 64u, (Rows<D, NQ, WAVES>::kOccupancy)) void
         }
       }
     }
-    if (!whole && g == 0u) {
+    if (!whole && g == 0u && share == 0u) {
       global_ptr<float2>(a.workspace + plan.statistics)[row.index * plan.splits + split] = make_float2(top[n], total);
     }
   }
@@ -1224,14 +1310,17 @@ void launch(const FerruleHipKvAttentionArgs &a, hipStream_t stream) {
       }
       kv_attention_decode_kernel<D, kWaves><<<grid, 256, 0, stream>>>(a, plan);
       break;
-    case 64: kv_attention_rows_kernel<D, 1, 4><<<grid, 256, 0, stream>>>(a, plan); break;
+    case 64:
+      if constexpr (D == 512u) kv_attention_rows_kernel<D, 1, 8, 2><<<grid, 512, 0, stream>>>(a, plan);
+      if constexpr (D < 512u) kv_attention_rows_kernel<D, 1, 4, 1><<<grid, 256, 0, stream>>>(a, plan);
+      break;
     case 128:
-      if constexpr (D == 256u) kv_attention_rows_kernel<D, 1, 8><<<grid, 512, 0, stream>>>(a, plan);
-      if constexpr (D <= 128u) kv_attention_rows_kernel<D, 2, 4><<<grid, 256, 0, stream>>>(a, plan);
+      if constexpr (D == 256u) kv_attention_rows_kernel<D, 1, 8, 1><<<grid, 512, 0, stream>>>(a, plan);
+      if constexpr (D <= 128u) kv_attention_rows_kernel<D, 2, 4, 1><<<grid, 256, 0, stream>>>(a, plan);
       break;
     default:
-      if constexpr (D == 64u) kv_attention_rows_kernel<D, 4, 4><<<grid, 256, 0, stream>>>(a, plan);
-      if constexpr (D == 128u) kv_attention_rows_kernel<D, 2, 8><<<grid, 512, 0, stream>>>(a, plan);
+      if constexpr (D == 64u) kv_attention_rows_kernel<D, 4, 4, 1><<<grid, 256, 0, stream>>>(a, plan);
+      if constexpr (D == 128u) kv_attention_rows_kernel<D, 2, 8, 1><<<grid, 512, 0, stream>>>(a, plan);
       break;
   }
   if (plan.splits > 1u) {
