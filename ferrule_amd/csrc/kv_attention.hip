@@ -1199,12 +1199,13 @@ uint64_t segments_of(const FerruleHipKvAttentionArgs &a, uint32_t tile_rows) {
 }
 
 // Which kernel: packed rows of a workgroup of kv_attention_rows_kernel, 0 for kv_attention_decode_kernel.
-// The latter reads and expands the range once for every 16 rows, but needs no second part of it: for 33 to 64 rows
-// of 512 values it is the faster one where every tile has a CU and a wave no more than two steps (64 sequences of
-// 64 heads over 128 tokens: 19.0 us, rows kernel 23.9; over 256 tokens 39.8 and 28.6; 128 sequences 31.6 and 24.1).
+// The latter reads and expands the range once for every 16 rows, but needs no second part of it.  At heads of 512 that
+// pays for more than 16 rows where every tile has a CU and a wave no more than two steps (64 sequences of 64 heads over
+// 128 tokens: 15-18 us, rows kernel 17-21; over 256 tokens 39 and 26; 128 sequences 29 and 21; 32 heads over 4096 tokens
+// 89 and 73).
 uint32_t rows_of_workgroup(const FerruleHipKvAttentionArgs &a) {
   const uint64_t rows = packed_rows(a);
-  if (rows <= 32u) return 0u;
+  if (rows <= (a.head_dim == 512u ? 16u : 32u)) return 0u;
   if (rows <= 64u && a.head_dim == 512u && segments_of(a, kTileRows) <= 256u && token_tiles(a, kTileRows) <= 2u * kWaves) {
     return 0u;
   }
