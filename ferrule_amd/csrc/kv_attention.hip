@@ -1194,21 +1194,24 @@ uint64_t token_tiles(const FerruleHipKvAttentionArgs &a, uint32_t tile_rows) {
   return tokens / kTileTokens + 1u;
 }
 
+constexpr uint32_t kSegments = 256;   // CUs
+constexpr uint32_t kShortRange = 64;  // tiles that eight waves take without parts
+
 uint64_t segments_of(const FerruleHipKvAttentionArgs &a, uint32_t tile_rows) {
   return static_cast<uint64_t>(a.batch) * a.kv_heads * row_tiles(a, tile_rows);
 }
 
 // Which kernel: packed rows of a workgroup of kv_attention_rows_kernel, 0 for kv_attention_decode_kernel.
-// The latter reads and expands the range once for every 16 rows, but needs no second part of it.  At heads of 512 that
-// pays for more than 16 rows where every tile has a CU and a wave no more than two steps (64 sequences of 64 heads over
-// 128 tokens: 15-18 us, rows kernel 17-21; over 256 tokens 39 and 26; 128 sequences 29 and 21; 32 heads over 4096 tokens
-// 89 and 73).
+// The latter reads and expands the range once for every 16 rows.  Two tiles of 16 are worth that everywhere but at heads
+// of 512 (64 sequences of 4096 tokens, 32 rows: heads of 128 48 us, rows kernel 81; heads of 512 89 and 73), four where
+// every tile has a CU and a range is so short that it needs no parts (16 sequences, 4 heads, 64 rows over a window of
+// 1024: heads of 64 12 us, rows kernel 19, of 256 16 and 32; at 512 over 128 tokens 15-18 and 17-21, but over 256 tokens
+// 39 and 26).
 uint32_t rows_of_workgroup(const FerruleHipKvAttentionArgs &a) {
   const uint64_t rows = packed_rows(a);
-  if (rows <= (a.head_dim == 512u ? 16u : 32u)) return 0u;
-  if (rows <= 64u && a.head_dim == 512u && segments_of(a, kTileRows) <= 256u && token_tiles(a, kTileRows) <= 2u * kWaves) {
-    return 0u;
-  }
+  const bool wide = a.head_dim == 512u;
+  if (rows <= (wide ? 16u : 32u)) return 0u;
+  if (rows <= 64u && segments_of(a, kTileRows) <= kSegments && token_tiles(a, kTileRows) <= (wide ? 2u * kWaves : kShortRange)) return 0u;
   if (rows <= 64u || a.head_dim == 512u) return 64u;
   // A workgroup of more rows reads and expands the tokens less often (a prompt of 8192 tokens, 32 heads of 128: 506 us
   // with 256 rows, 543 with 128, 645 with 64).  But the ranges of a prompt's rows differ, and cutting them costs more
@@ -1241,7 +1244,7 @@ SplitPlan plan_splits(const FerruleHipKvAttentionArgs &a) {
   // A range of a few steps of eight waves is not worth a second launch while there are CUs for all segments (32
   // sequences of 8 heads of 256: 1000 tokens 25.3 -> 17.3 us, 2000 tokens 34.6 -> 26.8).  At 512 values eight waves
   // would have half of the registers that the kernel needs (1 sequence of 500 tokens: 17.9 -> 30.8 us).
-  if (tiles == 0u && a.head_dim <= 256u && part < range && range <= 64u && segments <= 256u) {
+  if (tiles == 0u && a.head_dim <= 256u && part < range && range <= kShortRange && segments <= kSegments) {
     plan.wide = 1u;
     part = range;
   }

@@ -77,7 +77,8 @@ EVERY_KERNEL = [  # new rows, lengths, group, head size, window, sinks
     ([100], [130], 1, 64, 0, 0), ([270], [300], 1, 64, 50, 0), ([50], [700], 1, 128, 0, 0), ([100], [130], 1, 128, 33, 1),
     ([270], [300], 1, 128, 0, 0), ([50], [130], 1, 256, 0, 0), ([100], [700], 1, 256, 40, 0), ([50], [130], 2, 512, 30, 3),
     ([270], [700], 1, 64, 0, 0), ([100], [700], 1, 64, 0, 0), ([270], [800], 1, 128, 600, 3), ([100], [700], 1, 128, 0, 0),
-    ([100], [800], 1, 256, 620, 2),
+    ([100], [800], 1, 256, 620, 2), ([40, 3], [2500, 600], 1, 128, 0, 0), ([60], [2400], 1, 64, 0, 0), ([45], [2500], 1, 256, 2200, 3),
+    ([30], [700], 2, 512, 0, 0),
 ]
 
 
