@@ -1197,8 +1197,11 @@ uint64_t token_tiles(const FerruleHipKvAttentionArgs &a, uint32_t tile_rows) {
 constexpr uint32_t kSegments = 256;   // CUs
 constexpr uint32_t kShortRange = 64;  // tiles that eight waves take without parts
 
+// Tiles of rows of all heads, at most: the longest sequence's for every sequence, or what all rows make.
 uint64_t segments_of(const FerruleHipKvAttentionArgs &a, uint32_t tile_rows) {
-  return static_cast<uint64_t>(a.batch) * a.kv_heads * row_tiles(a, tile_rows);
+  const uint64_t each = static_cast<uint64_t>(a.batch) * row_tiles(a, tile_rows);
+  const uint64_t all = static_cast<uint64_t>(a.rows) * (a.q_heads / a.kv_heads) / tile_rows + a.batch;
+  return (each < all ? each : all) * a.kv_heads;
 }
 
 // Which kernel: packed rows of a workgroup of kv_attention_rows_kernel, 0 for kv_attention_decode_kernel.

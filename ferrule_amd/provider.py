@@ -1098,10 +1098,8 @@ class HipArtifactOperatorContext:
                   for shape in kv_cache_shapes(page_count, page_tokens, kv_heads, head_dim))
         return HipKvCache(page_tokens, kv_heads, head_dim, *arrays)
 
-    # A decode step's operators take a few microseconds on the GPU, so their host side is kept short: argument
-    # blocks are filled by position, and the raw stream handle is asked for without a stream object.
-    # The three operators are called for a few microseconds of work: a decode step's rows take the GPU less time
-    # than these checks take the host.
+    # A decode step's operators take the GPU a few microseconds, so their host side is kept short: argument blocks are
+    # filled by position, devices compared by index, and the raw stream handle is asked for without a stream object.
     def _check_kv(self, cache: HipKvCache, batch: HipKvBatch, error: torch.Tensor | None) -> int:
         """The index of the device that everything is on."""
         index, own = cache.device_index, self.device.index
@@ -1153,11 +1151,11 @@ class HipArtifactOperatorContext:
     def kv_cache_append(self, cache: HipKvCache, batch: HipKvBatch, k: torch.Tensor, v: torch.Tensor,
                         error: torch.Tensor | None = None) -> None:
         """Quantise the batch's key and value rows (BF16 or f32 [rows, kv_heads, head_dim], rows and
-        heads strided as they like) and write them at their positions.  The bytes are those of
-        ``pack_fp4_rows_from_f32`` (its default rounding), except that a block holding an infinity or
-        a NaN is written as a block of NaN.  ``error`` (int32 [1], cleared by the caller) becomes 1 when
-        a row has no valid place; such rows are dropped.  A page that is
-        written belongs to one sequence and stands once in its table."""
+        heads strided as they like, every row on 16 bytes) and write them at their positions.  The bytes
+        are those of ``pack_fp4_rows_from_f32`` (its default rounding), except that a block holding an
+        infinity or a NaN is written as a block of NaN.  ``error`` (int32 [1], cleared by the caller)
+        becomes 1 when a row has no valid place; such rows are dropped.  A page that is written belongs
+        to one sequence and stands once in its table."""
         index = self._check_kv(cache, batch, error)
         if batch.rows == 0 or batch.batch == 0:
             return
@@ -1208,7 +1206,8 @@ class HipArtifactOperatorContext:
         ``q`` and ``out`` are BF16 or f32 [rows, q_heads, head_dim] (f32 queries are rounded to BF16), head h
         reads key/value head h // (q_heads // kv_heads), and the row at position p sees position j when
         ``j <= p and (window == 0 or p - j < window or j < sinks)``.  A row that sees nothing writes
-        zeros.  Without ``workspace`` one is taken from torch's allocator for the call."""
+        zeros.  Without ``workspace`` one is taken from torch's allocator for the call.  One call has one
+        kernel, chosen for its longest rows: give decode rows and prompt chunks calls of their own."""
         index = self._check_kv(cache, batch, error)
         q_heads = q.shape[1] if q.dim() == 3 else 0
         shape = (batch.rows, q_heads, cache.head_dim)
