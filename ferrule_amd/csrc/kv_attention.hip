@@ -54,9 +54,11 @@ constexpr float kLazy = 8.0f;        // how far (in powers of two) scores may ex
 struct SplitPlan {
   uint32_t tile_rows;   // packed rows of a workgroup
   uint32_t page_shift;  // log2 of page_tokens
-  uint32_t part_tiles;  // 32-token tiles of a part, a multiple of what a workgroup takes at a time
-  uint32_t splits;      // parts at most; the last takes what is left
+  uint32_t part_tiles;  // 32-token tiles of a part, at most unless there are `splits` of them
+  uint32_t splits;      // parts at most
   uint32_t wide;        // decode kernel: one workgroup of as many waves as a CU holds instead of parts
+  uint32_t least_rows;  // of the sequences that the launch is for
+  uint32_t most_rows;
   uint64_t partials;    // byte offsets in the workspace
   uint64_t statistics;
 };
@@ -84,9 +86,24 @@ __device__ __forceinline__ TileRange tile_range(const FerruleHipKvAttentionArgs 
   return t;
 }
 
+// A launch for the sequences of few rows leaves the others to its sibling, and the other way round.
+__device__ __forceinline__ bool for_others(const KvSequence &s, const SplitPlan &plan) {
+  return s.rows < plan.least_rows || s.rows > plan.most_rows;
+}
+
 // How many parts a range has.
 __device__ __forceinline__ uint32_t parts_of(uint32_t count, const SplitPlan &plan) {
   return max(1u, min((count + plan.part_tiles - 1u) / plan.part_tiles, plan.splits));
+}
+
+// Part `split` of them, all as long as the others (the last may be shorter, or empty): a long one behind a short one at
+// every other workgroup would leave half of the XCDs, which take workgroups in turn, with the long ones.
+struct PartRange {
+  uint32_t begin, end;
+};
+__device__ __forceinline__ PartRange part_of(uint32_t count, uint32_t parts, uint32_t split) {
+  const uint32_t length = (count + parts - 1u) / parts;
+  return PartRange{min(split * length, count), min((split + 1u) * length, count)};
 }
 
 template <uint32_t D>
@@ -474,7 +491,7 @@ __global__ __launch_bounds__(WAVES * 64u, kDecodeOccupancy<D>) void kv_attention
   const KvSequence s = kv_sequence(a.query_indptr, a.sequence_lengths, b, a.rows, a.max_query_length);
   if (s.bad && blockIdx.x == 0u && threadIdx.x == 0u) kv_report(a.error);
   const uint32_t first_row = row_tile * kTileRows;
-  if (first_row >= s.rows * group) return;
+  if (first_row >= s.rows * group || for_others(s, plan)) return;
   const uint32_t last_row = min(first_row + kTileRows, s.rows * group) - 1u;
   const int32_t low = s.position + static_cast<int32_t>(first_row / group);
   const int32_t high = s.position + static_cast<int32_t>(last_row / group);
@@ -482,8 +499,8 @@ __global__ __launch_bounds__(WAVES * 64u, kDecodeOccupancy<D>) void kv_attention
   if (high >= static_cast<int32_t>(a.max_pages * a.page_tokens) && threadIdx.x == 0u) kv_report(a.error);
   const uint32_t parts = parts_of(range.count, plan);
   if (split >= parts) return;
-  const uint32_t begin = split * plan.part_tiles;
-  const uint32_t end = split + 1u == parts ? range.count : begin + plan.part_tiles;
+  const PartRange part = part_of(range.count, parts, split);
+  const uint32_t begin = part.begin, end = part.end;
   const bool whole = parts == 1u;  // no join
 
   const PackedRow mine = packed_row(a, s, kv_head, group, first_row + i);
@@ -744,15 +761,15 @@ __global__ __launch_bounds__(WAVES * 64u, (Rows<D, NQ, WAVES, SHARES>::kOccupanc
   if (s.bad && blockIdx.x == 0u && threadIdx.x == 0u) kv_report(a.error);
   const uint32_t first_row = row_tile * R::kRows;
   const uint32_t all_rows = s.rows * group;
-  if (first_row >= all_rows) return;
+  if (first_row >= all_rows || for_others(s, plan)) return;
   const uint32_t last_row = min(first_row + R::kRows, all_rows) - 1u;
   const int32_t high = s.position + static_cast<int32_t>(last_row / group);
   const TileRange range = tile_range(a, s.position + static_cast<int32_t>(first_row / group), high);
   if (high >= static_cast<int32_t>(a.max_pages * a.page_tokens) && threadIdx.x == 0u) kv_report(a.error);
   const uint32_t parts = parts_of(range.count, plan);
   if (split >= parts) return;
-  const uint32_t begin = split * plan.part_tiles;
-  const uint32_t end = split + 1u == parts ? range.count : begin + plan.part_tiles;
+  const PartRange part = part_of(range.count, parts, split);
+  const uint32_t begin = part.begin, end = part.end;
   const bool whole = parts == 1u;
 
   // the wave's own rows
@@ -1081,7 +1098,7 @@ __device__ __forceinline__ Joined joined_row(const FerruleHipKvAttentionArgs &a,
   const uint32_t kv_head = item % a.kv_heads, r = item / a.kv_heads;
   Joined j;
   j.parts = 0u;
-  if (r < s.rows * group) {
+  if (r < s.rows * group && !for_others(s, plan)) {
     const uint32_t first_row = r / plan.tile_rows * plan.tile_rows;
     const uint32_t last_row = min(first_row + plan.tile_rows, s.rows * group) - 1u;
     j.parts = parts_of(tile_range(a, s.position + static_cast<int32_t>(first_row / group),
@@ -1230,13 +1247,12 @@ uint32_t rows_of_workgroup(const FerruleHipKvAttentionArgs &a) {
 
 // How the token ranges are cut: into parts of equal length, so that sequences of different lengths give
 // workgroups of the same work.
-SplitPlan plan_splits(const FerruleHipKvAttentionArgs &a) {
-  const uint32_t tiles = rows_of_workgroup(a);
+SplitPlan plan_splits(const FerruleHipKvAttentionArgs &a, uint32_t tiles, uint64_t segments) {
   SplitPlan plan = {};
   plan.tile_rows = tiles == 0u ? kTileRows : tiles;
   plan.page_shift = static_cast<uint32_t>(__builtin_ctz(a.page_tokens));
+  plan.most_rows = 0xffffffffu;
   const uint64_t range = token_tiles(a, plan.tile_rows);
-  const uint64_t segments = segments_of(a, plan.tile_rows);
   // Decode: about a thousand parts, which the card holds at once (64 sequences of 8192 tokens, 8 heads: 99 us, with
   // 2048 parts 112).  Rows: no more than fill it once, and parts long enough to pay for their f32 partials
   // (4 x 512 rows over 8192 tokens: 244 us, with 512 parts 285).
@@ -1259,9 +1275,58 @@ SplitPlan plan_splits(const FerruleHipKvAttentionArgs &a) {
   return plan;
 }
 
+// One launch, or two.  A few rows over a long range need many workgroups for their range, and in a kernel for many rows
+// they would keep one at work long after the others (63 rows over 8192 tokens each and 512 over as many: 1890 us, in
+// two launches 200): where a batch can hold both, each launch takes its own sequences.
+struct Plans {
+  SplitPlan plan;
+  bool both;
+  SplitPlan few;
+  FerruleHipKvAttentionArgs few_sizes;  // the arguments with the bound of the few rows
+};
+
+uint64_t parts_size(const FerruleHipKvAttentionArgs &a, const SplitPlan &plan) {
+  const uint64_t values = plan.splits == 1u ? 0u : static_cast<uint64_t>(a.rows) * a.q_heads * plan.splits * a.head_dim * sizeof(float);
+  return (values + values / a.head_dim * 2u + 255u) & ~255ull;  // statistics are two floats for head_dim values
+}
+
+Plans plans_of(const FerruleHipKvAttentionArgs &a) {
+  Plans p = {};
+  const uint32_t tiles = rows_of_workgroup(a), tile_rows = tiles == 0u ? kTileRows : tiles, group = a.q_heads / a.kv_heads;
+  uint64_t segments = segments_of(a, tile_rows);
+  if (tiles != 0u && a.batch > 1u) {
+    const uint32_t limit = (a.head_dim == 512u ? 16u : 32u) / group, few = limit == 0u ? 1u : limit;
+    p.few_sizes = a;
+    p.few_sizes.max_query_length = few;
+    const uint32_t few_tiles = rows_of_workgroup(p.few_sizes);
+    p.both = few_tiles < tiles && few < row_bound(a) && token_tiles(a, kTileRows) > kShortRange &&
+             a.rows <= static_cast<uint64_t>(a.batch - 1u) * a.max_query_length + few;
+    if (p.both) {
+      p.few = plan_splits(p.few_sizes, few_tiles, segments_of(p.few_sizes, few_tiles == 0u ? kTileRows : few_tiles));
+      p.few.most_rows = few;
+      // as many sequences as it takes to have all rows
+      const uint64_t sequences = (a.rows + a.max_query_length - 1ull) / a.max_query_length;
+      segments = (static_cast<uint64_t>(a.rows) * group / tile_rows + sequences) * a.kv_heads;
+    }
+  }
+  p.plan = plan_splits(a, tiles, segments);
+  if (p.both) {
+    p.plan.least_rows = p.few.most_rows + 1u;
+    const uint64_t behind = parts_size(a, p.plan);
+    p.few.partials += behind;
+    p.few.statistics += behind;
+  }
+  return p;
+}
+
 uint64_t workspace_size(const FerruleHipKvAttentionArgs &a) {
-  const SplitPlan plan = plan_splits(a);  // statistics are two floats for head_dim values
-  return plan.statistics + plan.statistics / a.head_dim * 2u;
+  const Plans p = plans_of(a);
+  return parts_size(a, p.plan) + (p.both ? parts_size(a, p.few) : 0u);
+}
+
+bool grid_fits(const FerruleHipKvAttentionArgs &a, const SplitPlan &plan) {
+  const uint64_t workgroups = static_cast<uint64_t>(row_tiles(a, plan.tile_rows)) * a.kv_heads * plan.splits;
+  return workgroups <= 0x7fffffull && (plan.splits == 1u || static_cast<uint64_t>(row_bound(a)) * a.q_heads <= 0x7fffffull);
 }
 
 // Scalar fields; validate() looks at the rest.
@@ -1278,9 +1343,9 @@ FerruleHipStatus validate_shape(const FerruleHipKvAttentionArgs &a) {
   // packed rows of a sequence count in 32 bits, and so do the threads of a grid's x (at most 512 to a workgroup)
   const uint64_t items = static_cast<uint64_t>(row_bound(a)) * a.q_heads;
   if (a.batch > 65535u || items > 0x0fffffffull) return FERRULE_HIP_UNSUPPORTED;
-  const SplitPlan plan = plan_splits(a);
-  const uint64_t workgroups = static_cast<uint64_t>(row_tiles(a, plan.tile_rows)) * a.kv_heads * plan.splits;
-  return workgroups > 0x7fffffull || (plan.splits > 1u && items > 0x7fffffull) ? FERRULE_HIP_UNSUPPORTED : FERRULE_HIP_SUCCESS;
+  const Plans p = plans_of(a);
+  const bool fits = grid_fits(a, p.plan) && (!p.both || grid_fits(p.few_sizes, p.few));
+  return fits ? FERRULE_HIP_SUCCESS : FERRULE_HIP_UNSUPPORTED;
 }
 
 FerruleHipStatus validate(const FerruleHipKvAttentionArgs &a) {
@@ -1304,10 +1369,9 @@ FerruleHipStatus validate(const FerruleHipKvAttentionArgs &a) {
 }
 
 template <uint32_t D>
-void launch(const FerruleHipKvAttentionArgs &a, hipStream_t stream) {
-  const SplitPlan plan = plan_splits(a);
-  const dim3 grid(row_tiles(a, plan.tile_rows) * a.kv_heads * plan.splits, a.batch);
-  switch (rows_of_workgroup(a)) {
+void launch(const FerruleHipKvAttentionArgs &a, const FerruleHipKvAttentionArgs &sizes, const SplitPlan &plan, hipStream_t stream) {
+  const dim3 grid(row_tiles(sizes, plan.tile_rows) * a.kv_heads * plan.splits, a.batch);
+  switch (rows_of_workgroup(sizes)) {
     case 0:
       if constexpr (D <= 256u) {
         if (plan.wide != 0u) {
@@ -1331,7 +1395,7 @@ void launch(const FerruleHipKvAttentionArgs &a, hipStream_t stream) {
       break;
   }
   if (plan.splits > 1u) {
-    const uint32_t items = row_bound(a) * a.q_heads;
+    const uint32_t items = row_bound(sizes) * a.q_heads;
     if (plan.splits <= kFewParts) {
       constexpr uint32_t kRows = 256u / (D / 4u);
       kv_attention_join_few_kernel<D><<<dim3((items + kRows - 1u) / kRows, a.batch), 256, 0, stream>>>(a, plan);
@@ -1339,6 +1403,13 @@ void launch(const FerruleHipKvAttentionArgs &a, hipStream_t stream) {
       kv_attention_join_kernel<D><<<dim3(items, a.batch), 256, 0, stream>>>(a, plan);
     }
   }
+}
+
+template <uint32_t D>
+void launch(const FerruleHipKvAttentionArgs &a, hipStream_t stream) {
+  const Plans p = plans_of(a);
+  launch<D>(a, a, p.plan, stream);
+  if (p.both) launch<D>(a, p.few_sizes, p.few, stream);
 }
 
 }  // namespace

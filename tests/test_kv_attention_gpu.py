@@ -230,3 +230,38 @@ def test_windows_beyond_31_bits_are_refused(ctx):  # noqa: F811
     for kw in (dict(window=2 ** 31), dict(window=2 ** 32 + 5), dict(window=5, sinks=2 ** 32)):
         with pytest.raises(ValueError):
             _attend(ctx, host, batch, q, 0.1, **kw)
+
+
+MIXED = [  # new rows, lengths, kv heads, group, head size, window, sinks
+    ([300, 1, 1, 3, 40, 1], [2500, 3000, 40, 2200, 2100, 1], 1, 2, 128, 0, 0), ([1, 70, 0, 2], [4000, 2100, 0, 600], 2, 4, 64, 0, 0),
+    ([100, 1, 2], [2300, 2700, 2048], 1, 4, 256, 0, 0), ([40, 1, 1], [2200, 2300, 50], 1, 8, 512, 0, 0),
+    ([150, 1, 5, 1], [2600, 2600, 2600, 90], 1, 8, 128, 2100, 3), ([200, 1, 1], [2400, 2400, 3], 1, 40, 64, 0, 0),
+]
+
+
+@pytest.mark.parametrize("types", ["bf16", "f32"])
+@pytest.mark.parametrize("new,lengths,heads,group,d,window,sinks", MIXED)
+def test_sequences_of_few_and_of_many_rows_in_one_batch(ctx, new, lengths, heads, group, d, window, sinks, types):  # noqa: F811
+    rng = np.random.default_rng(101 + d)
+    batch, host, q = _case(rng, new, lengths, 64, heads, group, d)
+    want, bound = K.attention_reference(host, batch, q, 0.09, window, sinks, f32_output=types == "f32")
+    t = torch.float32 if types == "f32" else torch.bfloat16
+    K.check_attention(_attend(ctx, host, batch, q, 0.09, window, sinks, t, t), want, bound)
+
+
+def test_a_batch_without_a_bound_of_its_query_lengths(ctx):  # noqa: F811
+    """Decode rows and a bound that would allow one sequence all of them; and rows behind the last sequence."""
+    rng = np.random.default_rng(103)
+    new, lengths = [1] * 9 + [0, 2], rng.integers(1, 2600, 11).tolist()
+    batch, host, q = _case(rng, new, lengths, 64, 2, 4, 128)
+    want, bound = K.attention_reference(host, batch, q, 0.09)
+    q = np.concatenate([q, np.ones((5, 8, 128), np.float32)])
+    qd = torch.from_numpy(q).bfloat16().cuda()
+    out = torch.full_like(qd, 9.0)
+    dev = batch.device(rows=batch.total + 5, max_query_length=batch.total + 5)
+    ws = ctx.kv_cache_attention_workspace(host.device(), dev, 8)
+    ws.fill_(255)
+    ctx.kv_cache_attention_into(host.device(), dev, qd, out, 0.09, workspace=ws)
+    got = out.float().cpu().numpy()
+    assert (got[batch.total:] == 9).all()
+    K.check_attention(got[:batch.total], want, bound)
