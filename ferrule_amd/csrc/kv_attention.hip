@@ -57,6 +57,8 @@ struct SplitPlan {
   uint32_t part_tiles;  // 32-token tiles of a part, at most unless there are `splits` of them
   uint32_t splits;      // parts at most
   uint32_t wide;        // decode kernel: one workgroup of as many waves as a CU holds instead of parts
+  uint32_t find;        // rows kernel: workgroups are numbered by tile, not by sequence and tile
+  uint32_t by_row;      // join: a workgroup for each of the rows there are, which looks for its sequence
   uint32_t least_rows;  // of the sequences that the launch is for
   uint32_t most_rows;
   uint64_t partials;    // byte offsets in the workspace
@@ -89,6 +91,49 @@ __device__ __forceinline__ TileRange tile_range(const FerruleHipKvAttentionArgs 
 // A launch for the sequences of few rows leaves the others to its sibling, and the other way round.
 __device__ __forceinline__ bool for_others(const KvSequence &s, const SplitPlan &plan) {
   return s.rows < plan.least_rows || s.rows > plan.most_rows;
+}
+
+// A tile of rows of some sequence.
+struct RowTile {
+  uint32_t b;
+  uint32_t tile;
+  bool there;
+};
+
+// Tile t of all that the sequences of the launch have, in their order, by the same rules as kv_sequence.  Workgroups
+// without a tile would not only take time: workgroups go to the shader engines in turn, so their pattern decides which
+// of those get the others (8 chunks of 200 to 600 rows in a grid for 600 each: 246 us, here 198; with the sequences
+// faster than the tiles, chunks of 2000, 100, 50 and 20 rows took 1536 us and take 625 here).
+template <uint32_t ROWS>
+__device__ __forceinline__ RowTile find_tile(const FerruleHipKvAttentionArgs &a, const SplitPlan &plan, uint32_t t, uint32_t lane,
+                                             bool report) {
+  const int32_t *indptr = global_ptr<const int32_t>(a.query_indptr), *lengths = global_ptr<const int32_t>(a.sequence_lengths);
+  RowTile r = {0u, 0u, false};
+  for (uint32_t from = 0u; from < a.batch; from += 64u) {
+    const uint32_t l = from + lane;
+    uint32_t tiles = 0u;
+    if (l < a.batch) {
+      const KvSequence s = kv_sequence_of(indptr[l], indptr[l + 1u], lengths[l], a.rows, a.max_query_length);
+      if (report && s.bad) kv_report(a.error);
+      if (!for_others(s, plan)) tiles = (s.rows * (a.q_heads / a.kv_heads) + ROWS - 1u) / ROWS;
+    }
+    uint32_t end = tiles;
+#pragma unroll
+    for (uint32_t step = 1u; step < 64u; step *= 2u) {
+      const uint32_t below = static_cast<uint32_t>(__shfl_up(static_cast<int>(end), step, 64));
+      end += lane >= step ? below : 0u;
+    }
+    const uint64_t behind = __ballot(end > t);
+    if (behind != 0u && !r.there) {
+      const uint32_t at = static_cast<uint32_t>(__ffsll(static_cast<unsigned long long>(behind))) - 1u;
+      r.b = from + at;
+      r.tile = t - static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(end - tiles), static_cast<int>(at)));
+      r.there = true;
+      if (!report) break;
+    }
+    t -= r.there ? 0u : static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(end), 63));
+  }
+  return r;
 }
 
 // How many parts a range has.
@@ -486,10 +531,12 @@ __global__ __launch_bounds__(WAVES * 64u, kDecodeOccupancy<D>) void kv_attention
   const uint32_t b = blockIdx.y;
   const uint32_t split = blockIdx.x % plan.splits;
   const uint32_t kv_head = blockIdx.x / plan.splits % a.kv_heads;
-  const uint32_t row_tile = blockIdx.x / plan.splits / a.kv_heads;
+  // the tile of rows is last in the order of workgroups: those that a sequence does not have are at the end, in nobody's
+  // way (63 rows and 4 in one sequence, 8192 tokens each, 8 heads: 138 -> 97 us)
+  const uint32_t row_tile = blockIdx.z;
   const uint32_t group = a.q_heads / a.kv_heads;
   const KvSequence s = kv_sequence(a.query_indptr, a.sequence_lengths, b, a.rows, a.max_query_length);
-  if (s.bad && blockIdx.x == 0u && threadIdx.x == 0u) kv_report(a.error);
+  if (s.bad && blockIdx.x == 0u && blockIdx.z == 0u && threadIdx.x == 0u) kv_report(a.error);
   const uint32_t first_row = row_tile * kTileRows;
   if (first_row >= s.rows * group || for_others(s, plan)) return;
   const uint32_t last_row = min(first_row + kTileRows, s.rows * group) - 1u;
@@ -751,17 +798,21 @@ __global__ __launch_bounds__(WAVES * 64u, (Rows<D, NQ, WAVES, SHARES>::kOccupanc
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t i = lane & 15u, g = lane >> 4;
   const uint32_t share = wave % SHARES, first_unit = share * R::kShareUnits, first_chunk = share * R::kShareChunks;
-  const uint32_t b = blockIdx.y;
   const uint32_t split = blockIdx.x % plan.splits;
   const uint32_t kv_head = blockIdx.x / plan.splits % a.kv_heads;
-  const uint32_t tiles = gridDim.x / plan.splits / a.kv_heads;
-  const uint32_t row_tile = tiles - 1u - blockIdx.x / plan.splits / a.kv_heads;  // the longest causal ranges first
   const uint32_t group = a.q_heads / a.kv_heads;
+  RowTile at = {blockIdx.y, blockIdx.x / plan.splits / a.kv_heads, true};
+  if (plan.find != 0u) {
+    at = find_tile<R::kRows>(a, plan, at.tile, lane, blockIdx.x == 0u && wave == 0u);
+    if (!at.there) return;
+  }
+  const uint32_t b = __builtin_amdgcn_readfirstlane(at.b), row_tile = __builtin_amdgcn_readfirstlane(at.tile);
   const KvSequence s = kv_sequence(a.query_indptr, a.sequence_lengths, b, a.rows, a.max_query_length);
-  if (s.bad && blockIdx.x == 0u && threadIdx.x == 0u) kv_report(a.error);
-  const uint32_t first_row = row_tile * R::kRows;
+  if (plan.find == 0u && s.bad && blockIdx.x == 0u && threadIdx.x == 0u) kv_report(a.error);
   const uint32_t all_rows = s.rows * group;
-  if (first_row >= all_rows || for_others(s, plan)) return;
+  const uint32_t tiles = (all_rows + R::kRows - 1u) / R::kRows;
+  if (row_tile >= tiles || for_others(s, plan)) return;
+  const uint32_t first_row = (tiles - 1u - row_tile) * R::kRows;  // the longest causal ranges first
   const uint32_t last_row = min(first_row + R::kRows, all_rows) - 1u;
   const int32_t high = s.position + static_cast<int32_t>(last_row / group);
   const TileRange range = tile_range(a, s.position + static_cast<int32_t>(first_row / group), high);
@@ -1087,6 +1138,20 @@ __global__ __launch_bounds__(WAVES * 64u, (Rows<D, NQ, WAVES, SHARES>::kOccupanc
   }
 }
 
+// The last sequence whose rows start at `row` or before it.
+__device__ __forceinline__ uint32_t sequence_of(const FerruleHipKvAttentionArgs &a, uint32_t row) {
+  uint32_t low = 0u, high = a.batch - 1u;
+  while (low < high) {
+    const uint32_t middle = (low + high + 1u) / 2u;
+    if (global_ptr<const int32_t>(a.query_indptr)[middle] <= static_cast<int32_t>(row)) {
+      low = middle;
+    } else {
+      high = middle - 1u;
+    }
+  }
+  return low;
+}
+
 // The row and the number of parts of the threads that join one (row, query head); 0: written already.
 struct Joined {
   PackedRow row;
@@ -1115,9 +1180,19 @@ constexpr uint32_t kFewParts = 8;
 template <uint32_t D>
 __global__ __launch_bounds__(256) void kv_attention_join_few_kernel(FerruleHipKvAttentionArgs a, SplitPlan plan) {
   constexpr uint32_t kQuads = D / 4u;
-  const KvSequence s = kv_sequence(a.query_indptr, a.sequence_lengths, blockIdx.y, a.rows, a.max_query_length);
   const uint32_t quad = threadIdx.x % kQuads;
-  const Joined j = joined_row(a, plan, s, (blockIdx.x * 256u + threadIdx.x) / kQuads);
+  uint32_t item = (blockIdx.x * 256u + threadIdx.x) / kQuads;
+  KvSequence s;
+  if (plan.by_row == 0u) {
+    s = kv_sequence(a.query_indptr, a.sequence_lengths, blockIdx.y, a.rows, a.max_query_length);
+  } else {  // a lane's own
+    const uint32_t row = item / a.q_heads, b = sequence_of(a, row);
+    const int32_t *indptr = global_ptr<const int32_t>(a.query_indptr), *lengths = global_ptr<const int32_t>(a.sequence_lengths);
+    s = kv_sequence_of(indptr[b], indptr[b + 1u], lengths[b], a.rows, a.max_query_length);
+    if (row < s.row) return;
+    item -= s.row * a.q_heads;
+  }
+  const Joined j = joined_row(a, plan, s, item);
   if (j.parts == 0u) return;
   const float2 *statistics = global_ptr<const float2>(a.workspace + plan.statistics) + j.row.index * plan.splits;
   const f32x4_t *partials = reinterpret_cast<const f32x4_t *>(global_ptr<const float>(a.workspace + plan.partials)) +
@@ -1155,8 +1230,14 @@ __global__ __launch_bounds__(256) void kv_attention_join_kernel(FerruleHipKvAtte
   constexpr uint32_t kQuads = D / 4u, kLanes = 256u / kQuads;
   __shared__ float wave_top[kWaves], wave_sums[kWaves];
   __shared__ __align__(16) f32x4_t added[256];
-  const KvSequence s = kv_sequence(a.query_indptr, a.sequence_lengths, blockIdx.y, a.rows, a.max_query_length);
-  const Joined j = joined_row(a, plan, s, blockIdx.x);
+  uint32_t b = blockIdx.y, item = blockIdx.x;
+  if (plan.by_row != 0u) b = __builtin_amdgcn_readfirstlane(sequence_of(a, item / a.q_heads));
+  const KvSequence s = kv_sequence(a.query_indptr, a.sequence_lengths, b, a.rows, a.max_query_length);
+  if (plan.by_row != 0u) {
+    if (item / a.q_heads < s.row) return;
+    item -= s.row * a.q_heads;  // joined_row leaves out what is behind the sequence's last row
+  }
+  const Joined j = joined_row(a, plan, s, item);
   if (j.parts == 0u) return;
   const float2 *statistics = global_ptr<const float2>(a.workspace + plan.statistics) + j.row.index * plan.splits;
   const f32x4_t *partials = reinterpret_cast<const f32x4_t *>(global_ptr<const float>(a.workspace + plan.partials)) +
@@ -1214,12 +1295,14 @@ uint64_t token_tiles(const FerruleHipKvAttentionArgs &a, uint32_t tile_rows) {
 constexpr uint32_t kSegments = 256;   // CUs
 constexpr uint32_t kShortRange = 64;  // tiles that eight waves take without parts
 
-// Tiles of rows of all heads, at most: the longest sequence's for every sequence, or what all rows make.
-uint64_t segments_of(const FerruleHipKvAttentionArgs &a, uint32_t tile_rows) {
+// Tiles of rows of one head, at most: the longest sequence's for every sequence, or what all rows make.
+uint64_t found_tiles(const FerruleHipKvAttentionArgs &a, uint32_t tile_rows) {
   const uint64_t each = static_cast<uint64_t>(a.batch) * row_tiles(a, tile_rows);
   const uint64_t all = static_cast<uint64_t>(a.rows) * (a.q_heads / a.kv_heads) / tile_rows + a.batch;
-  return (each < all ? each : all) * a.kv_heads;
+  return each < all ? each : all;
 }
+
+uint64_t segments_of(const FerruleHipKvAttentionArgs &a, uint32_t tile_rows) { return found_tiles(a, tile_rows) * a.kv_heads; }
 
 // Which kernel: packed rows of a workgroup of kv_attention_rows_kernel, 0 for kv_attention_decode_kernel.
 // The latter reads and expands the range once for every 16 rows.  Two tiles of 16 are worth that everywhere but at heads
@@ -1252,6 +1335,7 @@ SplitPlan plan_splits(const FerruleHipKvAttentionArgs &a, uint32_t tiles, uint64
   plan.tile_rows = tiles == 0u ? kTileRows : tiles;
   plan.page_shift = static_cast<uint32_t>(__builtin_ctz(a.page_tokens));
   plan.most_rows = 0xffffffffu;
+  plan.find = tiles != 0u && a.batch > 1u && row_tiles(a, plan.tile_rows) > 1u;
   const uint64_t range = token_tiles(a, plan.tile_rows);
   // Decode: about a thousand parts, which the card holds at once (64 sequences of 8192 tokens, 8 heads: 99 us, with
   // 2048 parts 112).  Rows: no more than fill it once, and parts long enough to pay for their f32 partials
@@ -1271,6 +1355,8 @@ SplitPlan plan_splits(const FerruleHipKvAttentionArgs &a, uint32_t tiles, uint64
   plan.part_tiles = static_cast<uint32_t>(part < 0x40000000u ? part : 0x40000000u);
   plan.splits = static_cast<uint32_t>(splits);
   if (plan.splits == 1u) return plan;
+  // a workgroup for every row that a sequence might have takes time, also where there is none
+  plan.by_row = static_cast<uint64_t>(a.batch) * row_bound(a) > 2ull * a.rows && static_cast<uint64_t>(a.rows) * a.q_heads <= 0x7fffffull;
   plan.statistics = static_cast<uint64_t>(a.rows) * a.q_heads * plan.splits * a.head_dim * sizeof(float);
   return plan;
 }
@@ -1302,7 +1388,9 @@ Plans plans_of(const FerruleHipKvAttentionArgs &a) {
     p.both = few_tiles < tiles && few < row_bound(a) && token_tiles(a, kTileRows) > kShortRange &&
              a.rows <= static_cast<uint64_t>(a.batch - 1u) * a.max_query_length + few;
     if (p.both) {
-      p.few = plan_splits(p.few_sizes, few_tiles, segments_of(p.few_sizes, few_tiles == 0u ? kTileRows : few_tiles));
+      // sized for one row each
+      const uint32_t few_rows = few_tiles == 0u ? kTileRows : few_tiles;
+      p.few = plan_splits(p.few_sizes, few_tiles, static_cast<uint64_t>(a.batch) * a.kv_heads * ((group + few_rows - 1u) / few_rows));
       p.few.most_rows = few;
       // as many sequences as it takes to have all rows
       const uint64_t sequences = (a.rows + a.max_query_length - 1ull) / a.max_query_length;
@@ -1324,9 +1412,17 @@ uint64_t workspace_size(const FerruleHipKvAttentionArgs &a) {
   return parts_size(a, p.plan) + (p.both ? parts_size(a, p.few) : 0u);
 }
 
+dim3 grid_of(const FerruleHipKvAttentionArgs &a, const SplitPlan &plan) {
+  const uint32_t tiles = row_tiles(a, plan.tile_rows), each = a.kv_heads * plan.splits;
+  if (plan.find != 0u) return dim3(static_cast<uint32_t>(found_tiles(a, plan.tile_rows)) * each);
+  if (plan.tile_rows == kTileRows) return dim3(each, a.batch, tiles);
+  return dim3(tiles * each, a.batch);  // one sequence or one tile
+}
+
 bool grid_fits(const FerruleHipKvAttentionArgs &a, const SplitPlan &plan) {
-  const uint64_t workgroups = static_cast<uint64_t>(row_tiles(a, plan.tile_rows)) * a.kv_heads * plan.splits;
-  return workgroups <= 0x7fffffull && (plan.splits == 1u || static_cast<uint64_t>(row_bound(a)) * a.q_heads <= 0x7fffffull);
+  const uint64_t tiles = plan.find != 0u ? found_tiles(a, plan.tile_rows) : row_tiles(a, plan.tile_rows);
+  return tiles * a.kv_heads * plan.splits <= 0x7fffffull &&
+         (plan.splits == 1u || static_cast<uint64_t>(row_bound(a)) * a.q_heads <= 0x7fffffull);
 }
 
 // Scalar fields; validate() looks at the rest.
@@ -1370,7 +1466,7 @@ FerruleHipStatus validate(const FerruleHipKvAttentionArgs &a) {
 
 template <uint32_t D>
 void launch(const FerruleHipKvAttentionArgs &a, const FerruleHipKvAttentionArgs &sizes, const SplitPlan &plan, hipStream_t stream) {
-  const dim3 grid(row_tiles(sizes, plan.tile_rows) * a.kv_heads * plan.splits, a.batch);
+  const dim3 grid = grid_of(sizes, plan);
   switch (rows_of_workgroup(sizes)) {
     case 0:
       if constexpr (D <= 256u) {
@@ -1395,12 +1491,12 @@ void launch(const FerruleHipKvAttentionArgs &a, const FerruleHipKvAttentionArgs 
       break;
   }
   if (plan.splits > 1u) {
-    const uint32_t items = row_bound(sizes) * a.q_heads;
+    const uint32_t items = (plan.by_row != 0u ? a.rows : row_bound(sizes)) * a.q_heads, sequences = plan.by_row != 0u ? 1u : a.batch;
     if (plan.splits <= kFewParts) {
       constexpr uint32_t kRows = 256u / (D / 4u);
-      kv_attention_join_few_kernel<D><<<dim3((items + kRows - 1u) / kRows, a.batch), 256, 0, stream>>>(a, plan);
+      kv_attention_join_few_kernel<D><<<dim3((items + kRows - 1u) / kRows, sequences), 256, 0, stream>>>(a, plan);
     } else {
-      kv_attention_join_kernel<D><<<dim3(items, a.batch), 256, 0, stream>>>(a, plan);
+      kv_attention_join_kernel<D><<<dim3(items, sequences), 256, 0, stream>>>(a, plan);
     }
   }
 }

@@ -28,11 +28,8 @@ __device__ __forceinline__ int32_t kv_uniform(uint64_t address, uint64_t index) 
   return reinterpret_cast<constant_t *>(static_cast<uintptr_t>(address))[index];
 }
 
-__device__ __forceinline__ KvSequence kv_sequence(uint64_t query_indptr, uint64_t sequence_lengths, uint32_t b,
-                                                  uint32_t rows, uint32_t max_query_length) {
-  const int32_t first = kv_uniform(query_indptr, b);
-  const int32_t last = kv_uniform(query_indptr, b + 1u);
-  const int32_t length = kv_uniform(sequence_lengths, b);
+__device__ __forceinline__ KvSequence kv_sequence_of(int32_t first, int32_t last, int32_t length, uint32_t rows,
+                                                     uint32_t max_query_length) {
   KvSequence s;
   const int32_t row = min(max(first, 0), static_cast<int32_t>(rows));
   const int32_t end = min(max(last, row), static_cast<int32_t>(rows));
@@ -42,6 +39,12 @@ __device__ __forceinline__ KvSequence kv_sequence(uint64_t query_indptr, uint64_
   s.bad = row != first || end != last || length < 0 || s.rows > max_query_length;
   if (s.rows > max_query_length) s.rows = max_query_length;  // the rows that the grid covers
   return s;
+}
+
+__device__ __forceinline__ KvSequence kv_sequence(uint64_t query_indptr, uint64_t sequence_lengths, uint32_t b,
+                                                  uint32_t rows, uint32_t max_query_length) {
+  return kv_sequence_of(kv_uniform(query_indptr, b), kv_uniform(query_indptr, b + 1u), kv_uniform(sequence_lengths, b), rows,
+                        max_query_length);
 }
 
 // What one wave wrote to LDS, read by its other lanes: the wave's LDS operations run in order, only
