@@ -265,3 +265,40 @@ def test_a_batch_without_a_bound_of_its_query_lengths(ctx):  # noqa: F811
     got = out.float().cpu().numpy()
     assert (got[batch.total:] == 9).all()
     K.check_attention(got[:batch.total], want, bound)
+
+
+@pytest.mark.parametrize("d,longest", [(64, 300), (128, 300), (64, 2400), (512, 300)])
+def test_tiles_of_more_sequences_than_a_wave_has_lanes(ctx, d, longest):  # noqa: F811
+    """90 sequences, few of them with many rows, the first and the last ones among those; rows behind the last sequence."""
+    rng = np.random.default_rng(107 + d)
+    new = rng.integers(0, 4, 90)
+    new[[0, 5, 63, 64, 88]] = 70, 33, 90, 41, 65
+    lengths = new + rng.integers(0, 60, 90)
+    lengths[[5, 70]] = longest, longest - 7
+    batch, host, q = _case(rng, new.tolist(), lengths.tolist(), 32, 1, 2, d)
+    want, bound = K.attention_reference(host, batch, q, 0.09)
+    qd = torch.from_numpy(np.concatenate([q, np.ones((3, 2, d), np.float32)])).bfloat16().cuda()
+    out = torch.full_like(qd, 9.0)
+    flag = torch.zeros(1, dtype=torch.int32, device="cuda")
+    ctx.kv_cache_attention_into(host.device(), batch.device(rows=batch.total + 3), qd, out, 0.09, error=flag)
+    got = out.float().cpu().numpy()
+    assert (got[batch.total:] == 9).all() and flag.item() == 0
+    K.check_attention(got[:batch.total], want, bound)
+
+
+@pytest.mark.parametrize("indptr,lengths,most", [
+    ((0, 200, 100, 300), (200, 50, 300), 300), ((-5, 100, 400, 900), (100, 300, 500), 300), ((0, 100, 200, 300), (-7, 2 ** 31 - 1, 300), 300),
+    ((0, 100, 200, 300), (100, 100, 100), 40)])
+@pytest.mark.parametrize("longest", [300, 9000])
+def test_bad_indices_of_many_rows_stay_inside_the_tensors(ctx, indptr, lengths, most, longest):  # noqa: F811
+    from ferrule_amd.provider import HipKvBatch
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    cache = K.HostCache(30, 32, 1, 64).random(np.random.default_rng(5), 124, 128).device()
+    table = torch.arange(30, dtype=torch.int32, device="cuda").view(3, 10)
+    batch = HipKvBatch(i32(*indptr), i32(*lengths), table, 300, most, longest)
+    guard = torch.full((304, 4, 64), 3.0, device="cuda")
+    q = torch.ones((300, 4, 64), device="cuda")
+    flag = torch.zeros(1, dtype=torch.int32, device="cuda")
+    ctx.kv_cache_attention_into(cache, batch, q, guard[2:302], 0.1, error=flag)
+    torch.cuda.synchronize()
+    assert (guard[:2] == 3).all() and (guard[302:] == 3).all() and flag.item() == 1
