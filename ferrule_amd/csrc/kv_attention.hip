@@ -22,7 +22,7 @@
 // 2^16 in the rows kernel; a wave-uniform branch): weights of that size cost a 32-bit sum nothing, and most steps
 // rescale nothing.
 //
-// Three kernels.  kv_attention_decode_kernel has 16 rows of which each wave takes its own tokens, four waves or
+// Two kernels, and two that join.  kv_attention_decode_kernel has 16 rows of which each wave takes its own tokens, four waves or
 // eight, so that the cache is read once and in as many places as possible; its bound is memory.
 // kv_attention_rows_kernel has 64 to 256 rows, its waves share the tokens and the expanded values; its bounds are
 // the matrix pipe and, for heads of 64, the exponentials beside it.  Where rows leave CUs idle, the tokens of a
@@ -30,7 +30,7 @@
 // a fixed order by the join kernels.
 //   64 sequences of 8192 tokens, 8 heads of 128 for 8 query heads each: 99 us, 5.8 TB/s
 //   the same with heads of 64: 55 us, 5.3 TB/s; 4096 tokens, heads of 256: 100 us, 5.7 TB/s
-//   64 x 8192 tokens of one 512-wide row for 16 heads: 97 us, for 64 heads 157 us (the cache is 0.29 GB)
+//   64 x 8192 tokens of one 512-wide row for 16 heads: 97 us, for 64 heads 134 us (the cache is 0.29 GB)
 //   a prompt of 8192 tokens, 32 heads of 128: 490-505 us, 1.1 PFLOP/s (a large bf16 matrix product: 1.2)
 //   heads of 64: 315-350 us, 0.82; 4096 tokens, 16 heads of 256: 153 us, 0.9; 1024 tokens, 64 of 512: 131 us, 0.53
 #include <hip/hip_runtime.h>
@@ -1362,8 +1362,8 @@ SplitPlan plan_splits(const FerruleHipKvAttentionArgs &a, uint32_t tiles, uint64
 }
 
 // One launch, or two.  A few rows over a long range need many workgroups for their range, and in a kernel for many rows
-// they would keep one at work long after the others (63 rows over 8192 tokens each and 512 over as many: 1890 us, in
-// two launches 200): where a batch can hold both, each launch takes its own sequences.
+// they would keep one at work long after the others (63 rows over 8192 tokens each and 512 over as many, 64 heads:
+// 1890 us, in two launches 260): where a batch can hold both, each launch takes its own sequences.
 struct Plans {
   SplitPlan plan;
   bool both;
