@@ -1304,6 +1304,11 @@ uint64_t found_tiles(const FerruleHipKvAttentionArgs &a, uint32_t tile_rows) {
 
 uint64_t segments_of(const FerruleHipKvAttentionArgs &a, uint32_t tile_rows) { return found_tiles(a, tile_rows) * a.kv_heads; }
 
+// Rows that are most of what they see: their ranges differ.
+bool rows_of_prompts(const FerruleHipKvAttentionArgs &a) {
+  return 2ull * a.max_query_length > kTileTokens * token_tiles(a, 64u);
+}
+
 // Which kernel: packed rows of a workgroup of kv_attention_rows_kernel, 0 for kv_attention_decode_kernel.
 // The latter reads and expands the range once for every 16 rows.  Two tiles of 16 are worth that everywhere but at heads
 // of 512 (64 sequences of 4096 tokens, 32 rows: heads of 128 48 us, rows kernel 81; heads of 512 89 and 73), four where
@@ -1322,9 +1327,13 @@ uint32_t rows_of_workgroup(const FerruleHipKvAttentionArgs &a) {
   // Nor are there enough steps in a short range to pay for the larger start (16 prompts of 256 tokens: 37, 32, 29).
   const uint64_t range = token_tiles(a, 64u);
   const uint64_t total = static_cast<uint64_t>(a.rows) * a.q_heads;
-  const bool prompts = 2ull * a.max_query_length > kTileTokens * range;
+  // And few workgroups of few steps, whatever their tiles, leave most CUs idle (12 x 270 rows of one head over a window of
+  // 574: heads of 64 33 us with 256 rows, 18.6 with 64; of 128 33 and 21).
   uint32_t tile = a.head_dim == 256u || rows <= 128u ? 128u : 256u;
-  while (tile > 64u && (range < 16u || (prompts && total < 512u * tile))) tile /= 2u;
+  while (tile > 64u && (range < 16u || (rows_of_prompts(a) && total < 512u * tile) ||
+                        segments_of(a, tile) * (range / 16u) < kSegments)) {
+    tile /= 2u;
+  }
   return tile;
 }
 
@@ -1338,12 +1347,15 @@ SplitPlan plan_splits(const FerruleHipKvAttentionArgs &a, uint32_t tiles, uint64
   plan.find = tiles != 0u && a.batch > 1u && row_tiles(a, plan.tile_rows) > 1u;
   const uint64_t range = token_tiles(a, plan.tile_rows);
   // Decode: about a thousand parts, which the card holds at once (64 sequences of 8192 tokens, 8 heads: 99 us, with
-  // 2048 parts 112).  Rows: no more than fill it once, and parts long enough to pay for their f32 partials
-  // (4 x 512 rows over 8192 tokens: 244 us, with 512 parts 285).
-  const uint64_t target = tiles == 0u ? 1024u : 256u;
-  const uint64_t least = tiles == 0u ? 2u * kWaves : 16u;
+  // 2048 parts 112).  Rows: no more than fill it once, one workgroup of eight waves or two of four to a CU, and parts
+  // long enough to pay for their f32 partials (4 x 512 rows over 8192 tokens: heads of 128 244 us, with 512 parts 285;
+  // heads of 64 191 us, with 256 parts 231; 100 rows of 2 heads over 4000 tokens: 19 us, with parts of 16 and more 31).
+  const uint32_t tile_waves = a.head_dim == 512u || (a.head_dim == 256u && tiles == 128u) || (a.head_dim == 128u && tiles == 256u) ? 8u : 4u;
+  const uint64_t target = tiles == 0u ? 1024u : tile_waves == 8u ? 256u : 512u;
+  const uint64_t least = tiles != 0u && rows_of_prompts(a) ? 16u : 8u;
   uint64_t part = (segments * range + target - 1u) / target;
   part = part < least ? least : part;
+  if (tiles != 0u && 2u * range < 3u * part && range <= kShortRange) part = range;  // not for a little more than one part
   // A range of a few steps of eight waves is not worth a second launch while there are CUs for all segments (32
   // sequences of 8 heads of 256: 1000 tokens 25.3 -> 17.3 us, 2000 tokens 34.6 -> 26.8).  At 512 values eight waves
   // would have half of the registers that the kernel needs (1 sequence of 500 tokens: 17.9 -> 30.8 us).
