@@ -196,7 +196,8 @@ def test_value_blocks_beyond_the_range_of_f32_count_as_nan(ctx, new, d):  # noqa
 
 @pytest.mark.parametrize("n,length,heads,group,d,window,sinks", [
     (2100, 2100, 1, 64, 64, 0, 0), (2100, 2300, 2, 32, 128, 0, 0), (1100, 1100, 2, 32, 256, 0, 0), (2200, 2200, 1, 64, 128, 900, 7),
-    (1030, 1030, 4, 16, 128, 0, 0), (600, 600, 1, 64, 512, 0, 0)])
+    (1030, 1030, 4, 16, 128, 0, 0), (600, 600, 1, 64, 512, 0, 0), (2100, 2100, 1, 64, 64, 700, 3), (1100, 1100, 1, 64, 256, 600, 1),
+    (1100, 1100, 1, 64, 128, 600, 40), (1100, 1200, 1, 64, 64, 530, 0), (300, 300, 1, 64, 512, 128, 4)])
 def test_prompts_of_many_rows_equal_float64(ctx, n, length, heads, group, d, window, sinks):  # noqa: F811
     """Enough rows for the largest workgroups.  The reference is float64 on the GPU over the values that the read operator
     gives back (exact), the bound that of tests/kv_helpers.py."""
@@ -302,3 +303,29 @@ def test_bad_indices_of_many_rows_stay_inside_the_tensors(ctx, indptr, lengths, 
     ctx.kv_cache_attention_into(cache, batch, q, guard[2:302], 0.1, error=flag)
     torch.cuda.synchronize()
     assert (guard[:2] == 3).all() and (guard[302:] == 3).all() and flag.item() == 1
+
+
+@pytest.mark.parametrize("broken", [False, True])
+@pytest.mark.parametrize("new,length,group,d", [(270, 700, 1, 64), (100, 700, 1, 64), (50, 300, 1, 64), (270, 700, 1, 128), (100, 700, 1, 128),
+                                                (50, 300, 1, 128), (100, 700, 1, 256), (50, 300, 1, 256), (50, 300, 2, 512)])
+def test_every_tile_of_rows_under_a_distant_bound_of_the_lengths(ctx, new, length, group, d, broken):  # noqa: F811
+    """The bound makes the tiles as large as the rows allow.  Broken: some values are NaN, what is behind the last token
+    and on unused pages cannot be held in f32."""
+    rng = np.random.default_rng(109 + d)
+    batch, host, q = _case(rng, [new, 3], [length, 90], 64, 1, group, d)
+    if broken:
+        for b, j, block in ((0, length - new // 2, d // 32 - 1), (1, 89, 0)):
+            code, scale = host.get(*_place(batch, b, j, 0), 1)
+            scale = scale.copy()
+            scale[block] = 255
+            host.put(*_place(batch, b, j, 0), 1, code, scale)
+        keep = K.HostCache(batch.pages, 64, 1, d, fill=0xf7)
+        keep.arrays[1][:] = keep.arrays[3][:] = 254
+        for b, n in ((0, length), (1, 90)):
+            for j in range(n):
+                for which in (0, 1):
+                    keep.put(*_place(batch, b, j, 0), which, *host.get(*_place(batch, b, j, 0), which))
+        host = keep
+    want, bound = K.attention_reference(host, batch, q, 0.1)
+    assert np.isnan(want).any() == broken
+    K.check_attention(_attend(ctx, host, batch, q, 0.1, max_sequence_length=200000), want, bound)
