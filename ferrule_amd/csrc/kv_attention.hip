@@ -51,6 +51,8 @@ constexpr uint32_t kTileTokens = 32; // tokens of one step
 constexpr float kLargest = 65536.0f; // rows kernel: sum of a lane's weights of one step that moves the maximum
 constexpr float kLazy = 8.0f;        // how far (in powers of two) scores may exceed the running maximum
 
+constexpr uint32_t kEveryRow = 0xffffffffu;
+
 struct SplitPlan {
   uint32_t tile_rows;   // packed rows of a workgroup
   uint32_t page_shift;  // log2 of page_tokens
@@ -60,7 +62,7 @@ struct SplitPlan {
   uint32_t find;        // rows kernel: workgroups are numbered by tile, not by sequence and tile
   uint32_t by_row;      // join: a workgroup for each of the rows there are, which looks for its sequence
   uint32_t least_rows;  // of the sequences that the launch is for
-  uint32_t most_rows;
+  uint32_t most_rows;   // kEveryRow: no bound
   uint64_t partials;    // byte offsets in the workspace
   uint64_t statistics;
 };
@@ -459,20 +461,21 @@ __device__ __forceinline__ Place place_at(const FerruleHipKvAttentionArgs &a, co
 struct PackedRow {
   uint64_t q;       // offset of its values in q
   uint64_t output;  // and in the output
-  uint64_t index;   // row * q_heads + head
+  uint64_t index;   // of its partials: row * q_heads + head
   int32_t position;
   bool live;
 };
 
-__device__ __forceinline__ PackedRow packed_row(const FerruleHipKvAttentionArgs &a, const KvSequence &s, uint32_t kv_head,
-                                                uint32_t group, uint32_t r) {
+// Launches for sequences of few rows count those, most_rows to a sequence: of all rows' partials few would be used.
+__device__ __forceinline__ PackedRow packed_row(const FerruleHipKvAttentionArgs &a, const SplitPlan &plan, const KvSequence &s,
+                                                uint32_t b, uint32_t kv_head, uint32_t group, uint32_t r) {
   PackedRow p;
   const uint32_t row = r / group, head = kv_head * group + r % group;
   p.live = row < s.rows;
   const uint64_t at = s.row + static_cast<uint64_t>(p.live ? row : 0u);
   p.q = at * a.q_row_stride + head * a.q_head_stride;
   p.output = at * a.output_row_stride + head * a.output_head_stride;
-  p.index = at * a.q_heads + head;
+  p.index = (plan.most_rows == kEveryRow ? at : static_cast<uint64_t>(b) * plan.most_rows + row) * a.q_heads + head;
   p.position = s.position + static_cast<int32_t>(row);
   return p;
 }
@@ -550,7 +553,7 @@ __global__ __launch_bounds__(WAVES * 64u, kDecodeOccupancy<D>) void kv_attention
   const uint32_t begin = part.begin, end = part.end;
   const bool whole = parts == 1u;  // no join
 
-  const PackedRow mine = packed_row(a, s, kv_head, group, first_row + i);
+  const PackedRow mine = packed_row(a, plan, s, b, kv_head, group, first_row + i);
   // a short range is a chain of memory latencies: the page number, then everything else at once
   bool bad = false;  // a page number outside the cache
   int32_t next_page = 0;
@@ -715,7 +718,7 @@ __global__ __launch_bounds__(WAVES * 64u, kDecodeOccupancy<D>) void kv_attention
 #pragma unroll
   for (uint32_t w = 0; w < WAVES; ++w) own_top = fmaxf(own_top, top_of[w][i]);
   const float keep = part_weight(top, own_top);
-  const PackedRow target = packed_row(a, s, kv_head, group, first_row + row_out);
+  const PackedRow target = packed_row(a, plan, s, b, kv_head, group, first_row + row_out);
   const bool seen_any = total != 0.0f;  // NaN too
   const float norm = whole ? (seen_any ? 1.0f / total : 0.0f) : 1.0f;
 #pragma unroll
@@ -831,7 +834,7 @@ __global__ __launch_bounds__(WAVES * 64u, (Rows<D, NQ, WAVES, SHARES>::kOccupanc
   uint64_t row_q[NQ];
 #pragma unroll
   for (uint32_t n = 0; n < NQ; ++n) {
-    const PackedRow row = packed_row(a, s, kv_head, group, wave_row + 16u * n + i);
+    const PackedRow row = packed_row(a, plan, s, b, kv_head, group, wave_row + 16u * n + i);
     position[n] = row.position;
     from[n] = a.window == 0u ? static_cast<int32_t>(0x80000000u) : row.position - static_cast<int32_t>(a.window - 1u);
     row_q[n] = row.q;
@@ -1111,7 +1114,7 @@ __global__ __launch_bounds__(WAVES * 64u, (Rows<D, NQ, WAVES, SHARES>::kOccupanc
 
 #pragma unroll
   for (uint32_t n = 0; n < NQ; ++n) {
-    const PackedRow row = packed_row(a, s, kv_head, group, wave_row + 16u * n + i);
+    const PackedRow row = packed_row(a, plan, s, b, kv_head, group, wave_row + 16u * n + i);
     const float total = row_sum(sum[n]);
     if (!row.live) continue;
     const float norm = whole ? (total != 0.0f ? 1.0f / total : 0.0f) : 1.0f;
@@ -1158,7 +1161,7 @@ struct Joined {
   uint32_t parts;
 };
 __device__ __forceinline__ Joined joined_row(const FerruleHipKvAttentionArgs &a, const SplitPlan &plan, const KvSequence &s,
-                                             uint32_t item) {
+                                             uint32_t b, uint32_t item) {
   const uint32_t group = a.q_heads / a.kv_heads;
   const uint32_t kv_head = item % a.kv_heads, r = item / a.kv_heads;
   Joined j;
@@ -1170,7 +1173,7 @@ __device__ __forceinline__ Joined joined_row(const FerruleHipKvAttentionArgs &a,
                                   s.position + static_cast<int32_t>(last_row / group)).count, plan);
     if (j.parts == 1u) j.parts = 0u;
   }
-  j.row = packed_row(a, s, kv_head, group, j.parts != 0u ? r : 0u);
+  j.row = packed_row(a, plan, s, b, kv_head, group, j.parts != 0u ? r : 0u);
   return j;
 }
 
@@ -1182,17 +1185,19 @@ __global__ __launch_bounds__(256) void kv_attention_join_few_kernel(FerruleHipKv
   constexpr uint32_t kQuads = D / 4u;
   const uint32_t quad = threadIdx.x % kQuads;
   uint32_t item = (blockIdx.x * 256u + threadIdx.x) / kQuads;
+  uint32_t b = blockIdx.y;
   KvSequence s;
   if (plan.by_row == 0u) {
-    s = kv_sequence(a.query_indptr, a.sequence_lengths, blockIdx.y, a.rows, a.max_query_length);
+    s = kv_sequence(a.query_indptr, a.sequence_lengths, b, a.rows, a.max_query_length);
   } else {  // a lane's own
-    const uint32_t row = item / a.q_heads, b = sequence_of(a, row);
+    const uint32_t row = item / a.q_heads;
+    b = sequence_of(a, row);
     const int32_t *indptr = global_ptr<const int32_t>(a.query_indptr), *lengths = global_ptr<const int32_t>(a.sequence_lengths);
     s = kv_sequence_of(indptr[b], indptr[b + 1u], lengths[b], a.rows, a.max_query_length);
     if (row < s.row) return;
     item -= s.row * a.q_heads;
   }
-  const Joined j = joined_row(a, plan, s, item);
+  const Joined j = joined_row(a, plan, s, b, item);
   if (j.parts == 0u) return;
   const float2 *statistics = global_ptr<const float2>(a.workspace + plan.statistics) + j.row.index * plan.splits;
   const f32x4_t *partials = reinterpret_cast<const f32x4_t *>(global_ptr<const float>(a.workspace + plan.partials)) +
@@ -1237,7 +1242,7 @@ __global__ __launch_bounds__(256) void kv_attention_join_kernel(FerruleHipKvAtte
     if (item / a.q_heads < s.row) return;
     item -= s.row * a.q_heads;  // joined_row leaves out what is behind the sequence's last row
   }
-  const Joined j = joined_row(a, plan, s, item);
+  const Joined j = joined_row(a, plan, s, b, item);
   if (j.parts == 0u) return;
   const float2 *statistics = global_ptr<const float2>(a.workspace + plan.statistics) + j.row.index * plan.splits;
   const f32x4_t *partials = reinterpret_cast<const f32x4_t *>(global_ptr<const float>(a.workspace + plan.partials)) +
@@ -1339,11 +1344,11 @@ uint32_t rows_of_workgroup(const FerruleHipKvAttentionArgs &a) {
 
 // How the token ranges are cut: into parts of equal length, so that sequences of different lengths give
 // workgroups of the same work.
-SplitPlan plan_splits(const FerruleHipKvAttentionArgs &a, uint32_t tiles, uint64_t segments) {
+SplitPlan plan_splits(const FerruleHipKvAttentionArgs &a, uint32_t tiles, uint64_t segments, uint64_t held_rows) {
   SplitPlan plan = {};
   plan.tile_rows = tiles == 0u ? kTileRows : tiles;
   plan.page_shift = static_cast<uint32_t>(__builtin_ctz(a.page_tokens));
-  plan.most_rows = 0xffffffffu;
+  plan.most_rows = kEveryRow;
   plan.find = tiles != 0u && a.batch > 1u && row_tiles(a, plan.tile_rows) > 1u;
   const uint64_t range = token_tiles(a, plan.tile_rows);
   // Decode: about a thousand parts, which the card holds at once (64 sequences of 8192 tokens, 8 heads: 99 us, with
@@ -1369,7 +1374,7 @@ SplitPlan plan_splits(const FerruleHipKvAttentionArgs &a, uint32_t tiles, uint64
   if (plan.splits == 1u) return plan;
   // a workgroup for every row that a sequence might have takes time, also where there is none
   plan.by_row = static_cast<uint64_t>(a.batch) * row_bound(a) > 2ull * a.rows && static_cast<uint64_t>(a.rows) * a.q_heads <= 0x7fffffull;
-  plan.statistics = static_cast<uint64_t>(a.rows) * a.q_heads * plan.splits * a.head_dim * sizeof(float);
+  plan.statistics = held_rows * a.q_heads * plan.splits * a.head_dim * sizeof(float);
   return plan;
 }
 
@@ -1383,9 +1388,10 @@ struct Plans {
   FerruleHipKvAttentionArgs few_sizes;  // the arguments with the bound of the few rows
 };
 
+// Bytes of what the parts leave: their values, and two floats of statistics for head_dim of them.
 uint64_t parts_size(const FerruleHipKvAttentionArgs &a, const SplitPlan &plan) {
-  const uint64_t values = plan.splits == 1u ? 0u : static_cast<uint64_t>(a.rows) * a.q_heads * plan.splits * a.head_dim * sizeof(float);
-  return (values + values / a.head_dim * 2u + 255u) & ~255ull;  // statistics are two floats for head_dim values
+  const uint64_t values = plan.statistics - plan.partials;
+  return (values + values / a.head_dim * 2u + 255u) & ~255ull;
 }
 
 Plans plans_of(const FerruleHipKvAttentionArgs &a) {
@@ -1402,14 +1408,15 @@ Plans plans_of(const FerruleHipKvAttentionArgs &a) {
     if (p.both) {
       // sized for one row each
       const uint32_t few_rows = few_tiles == 0u ? kTileRows : few_tiles;
-      p.few = plan_splits(p.few_sizes, few_tiles, static_cast<uint64_t>(a.batch) * a.kv_heads * ((group + few_rows - 1u) / few_rows));
+      p.few = plan_splits(p.few_sizes, few_tiles, static_cast<uint64_t>(a.batch) * a.kv_heads * ((group + few_rows - 1u) / few_rows),
+                          static_cast<uint64_t>(a.batch) * few);
       p.few.most_rows = few;
       // as many sequences as it takes to have all rows
       const uint64_t sequences = (a.rows + a.max_query_length - 1ull) / a.max_query_length;
       segments = (static_cast<uint64_t>(a.rows) * group / tile_rows + sequences) * a.kv_heads;
     }
   }
-  p.plan = plan_splits(a, tiles, segments);
+  p.plan = plan_splits(a, tiles, segments, a.rows);
   if (p.both) {
     p.plan.least_rows = p.few.most_rows + 1u;
     const uint64_t behind = parts_size(a, p.plan);

@@ -175,3 +175,17 @@ def test_batches_beyond_31_bits_are_refused():
     for more in ((2 ** 31, 1, 1), (1, 2 ** 32 + 1, 1), (1, 1, 2 ** 32)):
         with pytest.raises(ValueError):
             HipKvBatch(i32(2), i32(1), i32(1, 4), *more)
+
+
+def test_the_workspace_of_a_prompt_beside_a_long_decode_row_stays_small():
+    lib = abi.load()
+    size = lambda **kw: lib.ferrule_hip_kv_attention_workspace_size(C.byref(_attention_args(**kw)))  # noqa: E731
+    mixed = dict(batch=2, rows=8193, q_heads=64, kv_heads=8, max_query_length=8192, max_pages=1024, page_count=2048,
+                 max_sequence_length=65536)
+    # parts of a decode launch hold four rows a sequence, at most 1024 of 16 packed rows in two tiles
+    assert 0 < size(**mixed) <= 2 * 1024 * 16 * (128 + 2) * 4 + 512 * 256 * (128 + 2) * 4
+    for d in abi.KV_HEAD_DIMS:
+        for rows, batch, longest in ((1, 1, 65536), (64, 64, 8192), (600, 3, 60000), (8192, 4, 8192), (4000, 200, 30000)):
+            got = size(batch=batch, rows=rows, q_heads=64, kv_heads=8, head_dim=d, max_query_length=max(1, rows // 2), max_pages=1024,
+                       page_count=2048, max_sequence_length=longest)
+            assert got <= 600 << 20, (d, rows, batch, longest, got)
