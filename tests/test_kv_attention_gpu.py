@@ -329,3 +329,43 @@ def test_every_tile_of_rows_under_a_distant_bound_of_the_lengths(ctx, new, lengt
     want, bound = K.attention_reference(host, batch, q, 0.1)
     assert np.isnan(want).any() == broken
     K.check_attention(_attend(ctx, host, batch, q, 0.1, max_sequence_length=200000), want, bound)
+
+
+def test_a_captured_mixed_step_follows_new_row_counts(ctx):  # noqa: F811
+    """Captured with bounds; between the replays the rows move from one sequence to another, eager work in between."""
+    from ferrule_amd.provider import HipArtifactOperatorContext, HipKvBatch
+    rng = np.random.default_rng(113)
+    rows, heads, group, d = 64, 2, 4, 128
+    cache = K.HostCache(300, 64, heads, d).random(rng, 124, 128).device()
+    put = lambda t, v: t.copy_(torch.tensor(v, dtype=torch.int32))  # noqa: E731
+    indptr, lengths = torch.zeros(4, dtype=torch.int32, device="cuda"), torch.ones(3, dtype=torch.int32, device="cuda")
+    table = torch.arange(300, dtype=torch.int32, device="cuda").view(3, 100)
+    batch = HipKvBatch(indptr, lengths, table, rows, rows, 5000)
+    q = torch.randn((rows, heads * group, d), device="cuda").bfloat16()
+    out = torch.full_like(q, 9.0)
+    stream = torch.cuda.Stream()
+    side = HipArtifactOperatorContext(0, stream)
+    ws = side.kv_cache_attention_workspace(cache, batch, heads * group)
+    run = lambda who, o, **kw: who.kv_cache_attention_into(cache, batch, q, o, 0.09, **kw)  # noqa: E731
+    put(indptr, [0, 62, 63, 64])
+    put(lengths, [3000, 4000, 1])
+    torch.cuda.synchronize()
+    run(side, out, workspace=ws)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        run(side, out, workspace=ws)
+    for starts, tokens in (([0, 62, 63, 64], [3000, 4000, 1]), ([0, 1, 2, 64], [5000, 700, 62]), ([0, 3, 40, 44], [2500, 4800, 2600]),
+                           ([0, 0, 1, 1], [0, 5000, 10])):
+        put(indptr, starts)
+        put(lengths, tokens)
+        ws.fill_(255)
+        out.fill_(9.0)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        want = torch.full_like(q, 9.0)
+        run(ctx, want)
+        torch.cuda.synchronize()
+        same = torch.equal(out, want) and bool((out[starts[-1]:] == 9).all()) and not bool((out[:starts[-1]] == 9).all(-1).any())
+        assert same, starts
