@@ -58,7 +58,7 @@ struct SplitPlan {
   uint32_t page_shift;  // log2 of page_tokens
   uint32_t part_tiles;  // 32-token tiles of a part, at most unless there are `splits` of them
   uint32_t splits;      // parts at most
-  uint32_t wide;        // decode kernel: one workgroup of as many waves as a CU holds instead of parts
+  uint32_t wide;        // decode kernel: workgroups of eight waves instead of parts, 1, or 2 with half of the values each
   uint32_t find;        // rows kernel: workgroups are numbered by tile, not by sequence and tile
   uint32_t by_row;      // join: a workgroup for each of the rows there are, which looks for its sequence
   uint32_t least_rows;  // of the sequences that the launch is for
@@ -514,17 +514,20 @@ __device__ __forceinline__ void store(uint64_t output, uint64_t at, bool f32, co
 // of equal length), a step ahead; what a wave has in flight, 4.25 KB at heads of 128, times 16 waves is 68 KB a CU.
 // Heads of 256 and 512 have too many query terms for registers: one copy in LDS serves the four waves, and of a step's
 // values four 16-byte pieces are in flight at a time (16 heads on a row of 512: 157 -> 100 us).
+// Over a short range, eight waves, and two workgroups of them where there are CUs for it (COLUMNS = 2): both make the
+// scores, each multiplies half of the values, whose expansion is half of a step's vector work.
 // One sequence of 1000 tokens, 8 heads of 128 for 8 query heads each: 9.3 us, of which 5 are a single step's chain of
 // launch, table, cache and join; the others are a step's arithmetic, about 0.9 us for two waves of a SIMD (loads two,
 // three or four steps ahead change nothing).
 template <uint32_t D>
 constexpr uint32_t kDecodeOccupancy = D <= 128u ? 4u : D == 256u ? 2u : 1u;  // waves per SIMD that the registers allow
-template <uint32_t D, uint32_t WAVES>
+template <uint32_t D, uint32_t WAVES, uint32_t COLUMNS>
 __global__ __launch_bounds__(WAVES * 64u, kDecodeOccupancy<D>) void kv_attention_decode_kernel(FerruleHipKvAttentionArgs a, SplitPlan plan) {
   using C = Core<D>;
   constexpr uint32_t kPitch = 128u + 4u;  // floats of a row in LDS
   constexpr bool kShared = D >= 256u;     // query terms in LDS
-  constexpr uint32_t kRing = C::kUnits < 4u ? C::kUnits : 4u;
+  constexpr uint32_t kUnits = C::kUnits / COLUMNS, kWidth = D / COLUMNS;  // of the values, the workgroup's
+  constexpr uint32_t kRing = kUnits < 4u ? kUnits : 4u;
   __shared__ __align__(16) typename std::conditional<kShared, typename C::SharedQuery, uint32_t>::type shared;
   __shared__ __align__(16) float joined[WAVES][kTileRows][kPitch];
   __shared__ float top_of[WAVES][kTileRows], sum_of[WAVES][kTileRows];
@@ -534,6 +537,9 @@ __global__ __launch_bounds__(WAVES * 64u, kDecodeOccupancy<D>) void kv_attention
   const uint32_t b = blockIdx.y;
   const uint32_t split = blockIdx.x % plan.splits;
   const uint32_t kv_head = blockIdx.x / plan.splits % a.kv_heads;
+  // 0 where COLUMNS is 1; taken from the grid there too at the sizes that have both (as a constant it costs heads of 128
+  // three registers more, which spill: 64 x 8192 tokens 80 -> 86 us)
+  const uint32_t first_unit = D == 128u || D == 256u ? blockIdx.x / plan.splits / a.kv_heads * kUnits : 0u;
   // the tile of rows is last in the order of workgroups: those that a sequence does not have are at the end, in nobody's
   // way (63 rows and 4 in one sequence, 8192 tokens each, 8 heads: 138 -> 97 us)
   const uint32_t row_tile = blockIdx.z;
@@ -575,7 +581,7 @@ __global__ __launch_bounds__(WAVES * 64u, kDecodeOccupancy<D>) void kv_attention
   auto load_ring = [&](const Place &p) {
 #pragma unroll
     for (uint32_t u = 0; u < kRing; ++u) {
-      C::template load_piece<true>(v_payload + p.payload, v_scales + p.scales, u, offset, ring[u], ring_scale[u]);
+      C::template load_piece<true>(v_payload + p.payload, v_scales + p.scales, first_unit + u, offset, ring[u], ring_scale[u]);
     }
   };
   C::template load_keys<true>(k_payload + next_place.payload, k_scales + next_place.scales, offset, keys);
@@ -611,9 +617,10 @@ __global__ __launch_bounds__(WAVES * 64u, kDecodeOccupancy<D>) void kv_attention
   const int32_t sinks = a.window == 0u ? 0 : static_cast<int32_t>(a.sinks);
   const float factor = a.softmax_scale * 1.44269504088896341f;
 
-  f32x4_t out[C::kColumns];
+  constexpr uint32_t kColumns = kWidth / 16u;
+  f32x4_t out[kColumns];
 #pragma unroll
-  for (uint32_t c = 0; c < C::kColumns; ++c) out[c] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+  for (uint32_t c = 0; c < kColumns; ++c) out[c] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
   float top = -INFINITY, base = 0.0f, sum = 0.0f;  // base = top, or 0 while the row has seen nothing
   uint32_t nan_units = 0u;
 
@@ -653,7 +660,7 @@ __global__ __launch_bounds__(WAVES * 64u, kDecodeOccupancy<D>) void kv_attention
       base = next;
       sum *= keep;
 #pragma unroll
-      for (uint32_t c = 0; c < C::kColumns; ++c) out[c] *= keep;
+      for (uint32_t c = 0; c < kColumns; ++c) out[c] *= keep;
     }
     float w[8];
 #pragma unroll
@@ -663,18 +670,18 @@ __global__ __launch_bounds__(WAVES * 64u, kDecodeOccupancy<D>) void kv_attention
 #pragma unroll
     for (int e = 0; e < 8; ++e) weight[e] = static_cast<__bf16>(w[e]);
     bool nan = false;
-    if constexpr (C::kUnits <= 2u) {
+    if constexpr (kUnits <= 2u) {
 #pragma unroll
-      for (uint32_t u = 0; u < C::kUnits; ++u) nan |= C::has_nan(ring_scale[u]);
+      for (uint32_t u = 0; u < kUnits; ++u) nan |= C::has_nan(ring_scale[u]);
       if (__any(nan)) {
 #pragma unroll
-        for (uint32_t u = 0; u < C::kUnits; ++u) ring_scale[u] = C::without_nan(ring_scale[u]);
+        for (uint32_t u = 0; u < kUnits; ++u) ring_scale[u] = C::without_nan(ring_scale[u]);
       }
     }
 #pragma unroll
-    for (uint32_t u = 0; u < C::kUnits; ++u) {
+    for (uint32_t u = 0; u < kUnits; ++u) {
       u32x4_t operand[4];
-      if constexpr (C::kUnits <= 2u) {
+      if constexpr (kUnits <= 2u) {
         C::expand(ring[u], ring_scale[u], operand);
       } else {
         nan |= C::has_nan(ring_scale[u % kRing]);
@@ -684,16 +691,16 @@ __global__ __launch_bounds__(WAVES * 64u, kDecodeOccupancy<D>) void kv_attention
       for (uint32_t e = 0; e < 4u; ++e) {
         out[4u * u + e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, operand[e]), weight, out[4u * u + e], 0, 0, 0);
       }
-      if constexpr (C::kUnits > 2u) {
+      if constexpr (kUnits > 2u) {
         __builtin_amdgcn_sched_barrier(0);  // one piece's operands at a time
-        const Place &source = u + kRing < C::kUnits ? here : next_place;
-        C::template load_piece<true>(v_payload + source.payload, v_scales + source.scales, (u + kRing) % C::kUnits, offset,
+        const Place &source = u + kRing < kUnits ? here : next_place;
+        C::template load_piece<true>(v_payload + source.payload, v_scales + source.scales, first_unit + (u + kRing) % kUnits, offset,
                                      ring[u % kRing], ring_scale[u % kRing]);
       }
     }
-    if constexpr (C::kUnits <= 2u) load_ring(next_place);
+    if constexpr (kUnits <= 2u) load_ring(next_place);
     const bool nan_blocks = __any(nan);
-    if (nan_blocks && here.valid) nan_units |= C::nan_units(v_scales + here.scales, start, mine.position, from, sinks, g);
+    if (nan_blocks && here.valid) nan_units |= C::nan_units(v_scales + here.scales, start, mine.position, from, sinks, g, first_unit, kUnits);
   }
 
   if (bad && lane == 0u) kv_report(a.error);
@@ -722,10 +729,10 @@ __global__ __launch_bounds__(WAVES * 64u, kDecodeOccupancy<D>) void kv_attention
   const bool seen_any = total != 0.0f;  // NaN too
   const float norm = whole ? (seen_any ? 1.0f / total : 0.0f) : 1.0f;
 #pragma unroll
-  for (uint32_t c = 0; c < (D + 127u) / 128u; ++c) {
+  for (uint32_t c = 0; c < (kWidth + 127u) / 128u; ++c) {
     if (c != 0u) __syncthreads();
 #pragma unroll
-    for (uint32_t u = 0; u < (D < 128u ? 1u : 2u); ++u) {
+    for (uint32_t u = 0; u < (kWidth < 128u ? 1u : 2u); ++u) {
 #pragma unroll
       for (uint32_t e4 = 0; e4 < 4u; ++e4) {
         f32x4_t o;
@@ -737,7 +744,7 @@ __global__ __launch_bounds__(WAVES * 64u, kDecodeOccupancy<D>) void kv_attention
       }
     }
     __syncthreads();
-    if (target.live && d_out < D) {
+    if (target.live && d_out < kWidth) {
       float x[kPiece] = {};
 #pragma unroll
       for (uint32_t w = 0; w < WAVES; ++w) {
@@ -746,7 +753,7 @@ __global__ __launch_bounds__(WAVES * 64u, kDecodeOccupancy<D>) void kv_attention
       }
 #pragma unroll
       for (uint32_t e = 0; e < kPiece; ++e) x[e] *= norm;
-      const uint32_t d = c * 128u + d_out;
+      const uint32_t d = first_unit * 64u + c * 128u + d_out;
       if (whole) {
         store<kPiece>(a.output, target.output + d, (a.flags & FERRULE_HIP_KV_ATTENTION_OUTPUT_F32) != 0u, x);
       } else {
@@ -1365,7 +1372,7 @@ SplitPlan plan_splits(const FerruleHipKvAttentionArgs &a, uint32_t tiles, uint64
   // sequences of 8 heads of 256: 1000 tokens 25.3 -> 17.3 us, 2000 tokens 34.6 -> 26.8).  At 512 values eight waves
   // would have half of the registers that the kernel needs (1 sequence of 500 tokens: 17.9 -> 30.8 us).
   if (tiles == 0u && a.head_dim <= 256u && part < range && range <= kShortRange && segments <= kSegments) {
-    plan.wide = 1u;
+    plan.wide = a.head_dim > 64u && 2u * segments <= kSegments ? 2u : 1u;
     part = range;
   }
   uint64_t splits = (range + part - 1u) / part;
@@ -1434,7 +1441,7 @@ uint64_t workspace_size(const FerruleHipKvAttentionArgs &a) {
 dim3 grid_of(const FerruleHipKvAttentionArgs &a, const SplitPlan &plan) {
   const uint32_t tiles = row_tiles(a, plan.tile_rows), each = a.kv_heads * plan.splits;
   if (plan.find != 0u) return dim3(static_cast<uint32_t>(found_tiles(a, plan.tile_rows)) * each);
-  if (plan.tile_rows == kTileRows) return dim3(each, a.batch, tiles);
+  if (plan.tile_rows == kTileRows) return dim3(plan.wide == 2u ? 2u * each : each, a.batch, tiles);
   return dim3(tiles * each, a.batch);  // one sequence or one tile
 }
 
@@ -1489,12 +1496,18 @@ void launch(const FerruleHipKvAttentionArgs &a, const FerruleHipKvAttentionArgs 
   switch (rows_of_workgroup(sizes)) {
     case 0:
       if constexpr (D <= 256u) {
-        if (plan.wide != 0u) {
-          kv_attention_decode_kernel<D, 8><<<grid, 512, 0, stream>>>(a, plan);
+        if (plan.wide == 1u) {
+          kv_attention_decode_kernel<D, 8, 1><<<grid, 512, 0, stream>>>(a, plan);
           break;
         }
       }
-      kv_attention_decode_kernel<D, kWaves><<<grid, 256, 0, stream>>>(a, plan);
+      if constexpr (D == 128u || D == 256u) {
+        if (plan.wide == 2u) {
+          kv_attention_decode_kernel<D, 8, 2><<<grid, 512, 0, stream>>>(a, plan);
+          break;
+        }
+      }
+      kv_attention_decode_kernel<D, kWaves, 1><<<grid, 256, 0, stream>>>(a, plan);
       break;
     case 64:
       if constexpr (D == 512u) kv_attention_rows_kernel<D, 1, 8, 2><<<grid, 512, 0, stream>>>(a, plan);
