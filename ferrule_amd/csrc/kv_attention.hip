@@ -59,6 +59,7 @@ struct SplitPlan {
   uint32_t part_tiles;  // 32-token tiles of a part, at most unless there are `splits` of them
   uint32_t splits;      // parts at most
   uint32_t wide;        // decode kernel: workgroups of eight waves instead of parts, 1, or 2 with half of the values each
+  uint32_t inner;       // decode kernel: tiles of rows are neighbours in the order of workgroups
   uint32_t find;        // rows kernel: workgroups are numbered by tile, not by sequence and tile
   uint32_t by_row;      // join: a workgroup for each of the rows there are, which looks for its sequence
   uint32_t least_rows;  // of the sequences that the launch is for
@@ -516,9 +517,9 @@ __device__ __forceinline__ void store(uint64_t output, uint64_t at, bool f32, co
 // values four 16-byte pieces are in flight at a time (16 heads on a row of 512: 157 -> 100 us).
 // Over a short range, eight waves, and two workgroups of them where there are CUs for it (COLUMNS = 2): both make the
 // scores, each multiplies half of the values, whose expansion is half of a step's vector work.
-// One sequence of 1000 tokens, 8 heads of 128 for 8 query heads each: 9.3 us, of which 5 are a single step's chain of
-// launch, table, cache and join; the others are a step's arithmetic, about 0.9 us for two waves of a SIMD (loads two,
-// three or four steps ahead change nothing).
+// One sequence of 1000 tokens, 8 heads of 128 for 8 query heads each: 8.1 us (9.3 with one workgroup), of which 5 are a
+// single step's chain of launch, table, cache and join; the others are a step's arithmetic, 0.7 us for two waves of a
+// SIMD (loads two, three or four steps ahead change nothing).
 template <uint32_t D>
 constexpr uint32_t kDecodeOccupancy = D <= 128u ? 4u : D == 256u ? 2u : 1u;  // waves per SIMD that the registers allow
 template <uint32_t D, uint32_t WAVES, uint32_t COLUMNS>
@@ -539,10 +540,13 @@ __global__ __launch_bounds__(WAVES * 64u, kDecodeOccupancy<D>) void kv_attention
   const uint32_t kv_head = blockIdx.x / plan.splits % a.kv_heads;
   // 0 where COLUMNS is 1; taken from the grid there too at the sizes that have both (as a constant it costs heads of 128
   // three registers more, which spill: 64 x 8192 tokens 80 -> 86 us)
-  const uint32_t first_unit = D == 128u || D == 256u ? blockIdx.x / plan.splits / a.kv_heads * kUnits : 0u;
+  const uint32_t outer = blockIdx.x / plan.splits / a.kv_heads;
+  const uint32_t first_unit = (D == 128u || D == 256u) && plan.wide == 2u ? outer * kUnits : 0u;
   // the tile of rows is last in the order of workgroups: those that a sequence does not have are at the end, in nobody's
-  // way (63 rows and 4 in one sequence, 8192 tokens each, 8 heads: 138 -> 97 us)
-  const uint32_t row_tile = blockIdx.z;
+  // way (63 rows and 4 in one sequence, 8192 tokens each, 8 heads: 138 -> 97 us).  Where every sequence has all of them,
+  // they are neighbours, which share keys and values while those are in the cache (16 x 4 rows over 8192 tokens, 8 x 8
+  // heads: 57 -> 48 us; over a short range it costs 8 %).
+  const uint32_t row_tile = plan.inner != 0u ? outer : blockIdx.z;
   const uint32_t group = a.q_heads / a.kv_heads;
   const KvSequence s = kv_sequence(a.query_indptr, a.sequence_lengths, b, a.rows, a.max_query_length);
   if (s.bad && blockIdx.x == 0u && blockIdx.z == 0u && threadIdx.x == 0u) kv_report(a.error);
@@ -1375,6 +1379,8 @@ SplitPlan plan_splits(const FerruleHipKvAttentionArgs &a, uint32_t tiles, uint64
     plan.wide = a.head_dim > 64u && 2u * segments <= kSegments ? 2u : 1u;
     part = range;
   }
+  plan.inner = tiles == 0u && range > kShortRange && row_tiles(a, kTileRows) > 1u &&
+               a.rows == static_cast<uint64_t>(a.batch) * a.max_query_length;
   uint64_t splits = (range + part - 1u) / part;
   plan.part_tiles = static_cast<uint32_t>(part < 0x40000000u ? part : 0x40000000u);
   plan.splits = static_cast<uint32_t>(splits);
@@ -1441,6 +1447,7 @@ uint64_t workspace_size(const FerruleHipKvAttentionArgs &a) {
 dim3 grid_of(const FerruleHipKvAttentionArgs &a, const SplitPlan &plan) {
   const uint32_t tiles = row_tiles(a, plan.tile_rows), each = a.kv_heads * plan.splits;
   if (plan.find != 0u) return dim3(static_cast<uint32_t>(found_tiles(a, plan.tile_rows)) * each);
+  if (plan.inner != 0u) return dim3(tiles * each, a.batch);
   if (plan.tile_rows == kTileRows) return dim3(plan.wide == 2u ? 2u * each : each, a.batch, tiles);
   return dim3(tiles * each, a.batch);  // one sequence or one tile
 }
