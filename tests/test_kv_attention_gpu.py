@@ -369,3 +369,20 @@ def test_a_captured_mixed_step_follows_new_row_counts(ctx):  # noqa: F811
         torch.cuda.synchronize()
         same = torch.equal(out, want) and bool((out[starts[-1]:] == 9).all()) and not bool((out[:starts[-1]] == 9).all(-1).any())
         assert same, starts
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_short_ranges_of_most_of_the_card(ctx, d):  # noqa: F811
+    """140 segments: eight waves to each, and no second workgroup; one of the values' blocks is NaN."""
+    rng = np.random.default_rng(127 + d)
+    lengths = rng.integers(1, 30, 70)
+    lengths[[0, 33, 69]] = 500, 290, 321
+    batch, host, q = _case(rng, [1] * 70, lengths.tolist(), 32, 2, 3, d)
+    code, scale = host.get(*_place(batch, 33, 100, 1), 1)
+    scale = scale.copy()
+    scale[d // 32 - 1] = 255
+    host.put(*_place(batch, 33, 100, 1), 1, code, scale)
+    for window, sinks in ((0, 0), (310, 2)):
+        want, bound = K.attention_reference(host, batch, q, 0.1, window, sinks)
+        assert np.isnan(want).any()
+        K.check_attention(_attend(ctx, host, batch, q, 0.1, window, sinks), want, bound)
