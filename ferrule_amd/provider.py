@@ -1093,9 +1093,11 @@ class HipArtifactOperatorContext:
 
     # -- MXFP4 key/value cache ------------------------------------------------------
     def kv_cache(self, page_count: int, page_tokens: int, kv_heads: int, head_dim: int) -> HipKvCache:
-        """A new cache on this context's device; every byte zero."""
-        arrays = (torch.zeros(shape, dtype=torch.uint8, device=self.device)
-                  for shape in kv_cache_shapes(page_count, page_tokens, kv_heads, head_dim))
+        """A new cache on this context's device, every byte zero; its memory belongs to the context's stream, where the
+        operators that follow find it filled."""
+        with torch.cuda.stream(self.stream):
+            arrays = [torch.zeros(shape, dtype=torch.uint8, device=self.device)
+                      for shape in kv_cache_shapes(page_count, page_tokens, kv_heads, head_dim)]
         return HipKvCache(page_tokens, kv_heads, head_dim, *arrays)
 
     # A decode step's operators take the GPU a few microseconds, so their host side is kept short: argument blocks are
