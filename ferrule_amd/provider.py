@@ -1190,15 +1190,19 @@ class HipArtifactOperatorContext:
             batch.batch, batch.rows, q_heads, cache.kv_heads, cache.head_dim, cache.page_tokens, cache.page_count,
             batch.max_pages, batch.max_query_length, longest, window, sinks, flags, softmax_scale, *tensors)
 
+    def _kv_workspace(self, args: abi.KvAttentionArgs, cache: HipKvCache) -> torch.Tensor:
+        size = self.lib.ferrule_hip_kv_attention_workspace_size(C.byref(args))
+        with torch.cuda.stream(self.stream):           # the block is reused in this stream's order
+            return torch.empty(size, dtype=torch.uint8, device=cache.device)
+
     def kv_cache_attention_workspace(self, cache: HipKvCache, batch: HipKvBatch, q_heads: int, window: int = 0,
                                      sinks: int = 0) -> torch.Tensor:
         """The scratch that ``kv_cache_attention_into`` needs for batches of this shape (uint8, possibly
-        empty).  It belongs to one call at a time: keep one per stream, and one per captured graph that
-        may replay while another runs."""
+        empty), memory of the context's stream.  It belongs to one call at a time: keep one per stream, and one
+        per captured graph that may replay while another runs."""
         index = self._check_kv(cache, batch, None)
         args = self._kv_attention_args(cache, batch, q_heads, window, sinks)
-        size = self.lib.ferrule_hip_kv_attention_workspace_size(C.byref(args))
-        return torch.empty(size, dtype=torch.uint8, device=cache.device)
+        return self._kv_workspace(args, cache)
 
     def kv_cache_attention_into(self, cache: HipKvCache, batch: HipKvBatch, q: torch.Tensor, out: torch.Tensor,
                                 softmax_scale: float, window: int = 0, sinks: int = 0,
@@ -1221,9 +1225,7 @@ class HipArtifactOperatorContext:
         if batch.rows == 0 or batch.batch == 0:
             return out
         if workspace is None:
-            size = self.lib.ferrule_hip_kv_attention_workspace_size(C.byref(a))
-            with torch.cuda.stream(self.stream):       # the block is reused in this stream's order
-                workspace = torch.empty(size, dtype=torch.uint8, device=cache.device)
+            workspace = self._kv_workspace(a, cache)
         elif workspace.dtype != torch.uint8 or workspace.get_device() != index or not workspace.is_contiguous():
             raise ValueError("HIP KV attention workspace must be contiguous uint8 on the device")
         a.workspace, a.workspace_bytes = _ptr(workspace), workspace.numel()

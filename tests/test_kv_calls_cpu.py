@@ -37,3 +37,16 @@ def test_a_new_cache_is_filled_on_the_contexts_stream(monkeypatch):
     cache = ctx.kv_cache(3, 64, 2, 128)
     assert taken == ["side"] * 4
     assert all(not t.any() for t in (cache.k_payload, cache.k_scales, cache.v_payload, cache.v_scales))
+
+
+@pytest.mark.parametrize("length", [0, 5000])
+def test_the_workspace_of_a_side_context_belongs_to_its_stream(monkeypatch, length):
+    """Also where it is empty: the allocator hands a block out again in the order of the stream that it was taken on."""
+    ctx, taken = _host_context(monkeypatch, "side")
+    monkeypatch.setattr(ctx, "_check_kv", lambda *_: 0, raising=False)
+    cache = P.HipKvCache(64, 8, 128, *(torch.empty(s, dtype=torch.uint8) for s in P.kv_cache_shapes(90, 64, 8, 128)))
+    i32 = lambda *shape: torch.zeros(shape, dtype=torch.int32)  # noqa: E731
+    batch = P.HipKvBatch(i32(2), i32(1), i32(1, 90), 1, 1, length)
+    del taken[:]
+    workspace = ctx.kv_cache_attention_workspace(cache, batch, 64)
+    assert taken == ["side"] and (workspace.numel() > 0) == (length > 0)

@@ -35,3 +35,25 @@ def test_rows_appended_at_once_to_a_new_cache_of_a_side_context_stay(ctx):  # no
     for far, here in zip((cache.k_payload, cache.k_scales, cache.v_payload, cache.v_scales),
                          (small.k_payload, small.k_scales, small.v_payload, small.v_scales)):
         assert torch.equal(far[-2:], here) and not far[:-2].any()
+
+
+def test_a_workspace_dropped_after_its_call_is_not_handed_out_while_it_is_in_use(ctx):  # noqa: F811
+    """A split decode step on a side stream whose workspace nobody keeps; torch's own stream takes blocks of that size and
+    fills them at once."""
+    from ferrule_amd.provider import HipArtifactOperatorContext
+    rng = np.random.default_rng(131)
+    batch, host, q = _case(rng, [1, 1], [6000, 2000], 64, 2, 8, 128)
+    cache, dev = host.device(), batch.device()
+    qd = torch.from_numpy(q).bfloat16().cuda()
+    want = ctx.kv_cache_attention_into(cache, dev, qd, torch.empty_like(qd), 0.09)
+    size = ctx.kv_cache_attention_workspace(cache, dev, 16).numel()
+    assert size > 0
+    side = HipArtifactOperatorContext(0, torch.cuda.Stream())
+    outs = [torch.empty_like(qd) for _ in range(8)]
+    torch.cuda.synchronize()
+    for out in outs:
+        side.kv_cache_attention_into(cache, dev, qd, out, 0.09, workspace=side.kv_cache_attention_workspace(cache, dev, 16))
+        torch.full((size,), 255, dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+    same = [torch.equal(out, want) for out in outs]
+    assert all(same), same
