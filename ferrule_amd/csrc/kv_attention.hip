@@ -1489,6 +1489,11 @@ FerruleHipStatus validate(const FerruleHipKvAttentionArgs &a) {
       a.sequence_lengths == 0u || a.page_table == 0u || ((a.query_indptr | a.sequence_lengths | a.page_table | a.error) & 3u)) {
     return FERRULE_HIP_INVALID_ARGUMENT;
   }
+  // Two workgroups may read a query row of which each writes half of the output, and rows behind a sequence's last read
+  // its first: the output is elsewhere.  What shows that it is not without a look at every row:
+  if (a.q == a.output || (a.rows > 1u && a.output_row_stride == 0u) || (a.q_heads > 1u && a.output_head_stride == 0u)) {
+    return FERRULE_HIP_INVALID_ARGUMENT;
+  }
   if (status != FERRULE_HIP_SUCCESS) return status;
   const uint64_t needed = workspace_size(a);
   if (needed != 0u && (a.workspace == 0u || (a.workspace & 255u) != 0u || a.workspace_bytes < needed)) {

@@ -162,6 +162,42 @@ class HipKvBatch:
         self.pointers = (_ptr(query_indptr), _ptr(sequence_lengths), _ptr(page_table))
 
 
+def _kv_rows_repeat(shape: tuple[int, int, int], strides: tuple[int, ...]) -> bool:
+    """Whether some value of a row tensor [rows, heads, values] stands in memory twice."""
+    (rows, heads, d), (s, t) = shape, strides[:2]
+    if (rows == 1 or s >= (heads - 1) * t + d) and (heads == 1 or t >= d):
+        return False                                    # heads inside their row
+    if (heads == 1 or t >= (rows - 1) * s + d) and (rows == 1 or s >= d):
+        return False                                    # rows inside their head
+    if (rows > 1 and s < d) or (heads > 1 and t < d):
+        return True
+    return _kv_starts(rows, heads, s, t).diff().amin().item() < d
+
+
+def _kv_starts(rows: int, heads: int, s: int, t: int) -> torch.Tensor:
+    return (torch.arange(rows)[:, None] * s + torch.arange(heads) * t).flatten().sort().values
+
+
+def _kv_rows_meet(shape: tuple[int, int, int], p0: int, strides0: tuple[int, ...], size0: int, p1: int,
+                  strides1: tuple[int, ...], size1: int) -> bool:
+    """Whether two row tensors of one shape at addresses p0 and p1, of size0 and size1 bytes a value, share a byte."""
+    rows, heads, d = shape
+    s0, t0, s1, t1, w0, w1 = strides0[0] * size0, strides0[1] * size0, strides1[0] * size1, strides1[1] * size1, d * size0, d * size1
+    r0, r1 = (heads - 1) * t0 + w0, (heads - 1) * t1 + w1      # extents of a row
+    if p0 + (rows - 1) * s0 + r0 <= p1 or p1 + (rows - 1) * s1 + r1 <= p0:
+        return False
+    # views of one buffer, side by side in every period of it: a row, a head, a head of a row, a row of a head
+    h0, h1 = (rows - 1) * s0 + w0, (rows - 1) * s1 + w1
+    for period, other, first, second in ((s0, s1, r0, r1), (t0, t1, h0, h1), *(((t0, t1, w0, w1),) if t0 and not (s0 % t0 or s1 % t0) else ()),
+                                         *(((s0, s1, w0, w1),) if s0 and not (t0 % s0 or t1 % s0) else ())):
+        if period == other != 0 and first <= (p1 - p0) % period <= period - second:
+            return False
+    starts = _kv_starts(rows, heads, s0, t0) + p0
+    against = _kv_starts(rows, heads, s1, t1) + p1
+    last = torch.searchsorted(starts, against + w1) - 1        # the last row of a head that starts in front of the other's end
+    return bool(((last >= 0) & (starts[last.clamp(min=0)] + w0 > against)).any())
+
+
 def validate_dsv4_router_token_ids(token_ids, hash_rows: int) -> list[int]:
     """context.rs:1861-1891: every id must address a row of the hash table."""
     token_ids = [int(t) for t in token_ids]
@@ -1212,7 +1248,7 @@ class HipArtifactOperatorContext:
         ``q`` and ``out`` are BF16 or f32 [rows, q_heads, head_dim] (f32 queries are rounded to BF16), head h
         reads key/value head h // (q_heads // kv_heads), and the row at position p sees position j when
         ``j <= p and (window == 0 or p - j < window or j < sinks)``.  A row that sees nothing writes
-        zeros.  Without ``workspace`` one is taken from torch's allocator for the call."""
+        zeros.  ``out`` shares no byte with ``q``.  Without ``workspace`` one is taken from torch's allocator for the call."""
         index = self._check_kv(cache, batch, error)
         q_heads = q.shape[1] if q.dim() == 3 else 0
         shape = (batch.rows, q_heads, cache.head_dim)
@@ -1224,6 +1260,9 @@ class HipArtifactOperatorContext:
                                     q.data_ptr(), out.data_ptr(), *cache.pointers, *batch.pointers, _ptr(error))
         if batch.rows == 0 or batch.batch == 0:
             return out
+        if _kv_rows_repeat(shape, os) or _kv_rows_meet(shape, a.q, qs, q.element_size(), a.output, os, out.element_size()):
+            raise ValueError("HIP KV attention writes every output row once and none over a query row: "
+                             f"output strides {os}, {a.output - a.q} bytes behind the queries with strides {qs}")
         if workspace is None:
             workspace = self._kv_workspace(a, cache)
         elif workspace.dtype != torch.uint8 or workspace.get_device() != index or not workspace.is_contiguous():

@@ -957,6 +957,9 @@ int32_t ferrule_hip_kv_cache_read_launch(const FerruleHipKvCacheArgs *args);
  * are divided by their sum at the end and may be 2^16 large until then: values of 2^90 and more can
  * overflow, and a block of values with a scale byte of 253 or more, whose largest values f32 cannot
  * hold, counts as a block of NaN.
+ * The output is not written over the queries: several workgroups read a query row, and one may write while
+ * another still reads.  INVALID_ARGUMENT for equal addresses and for an output whose rows or heads have no
+ * stride; other overlaps are the caller's to avoid.
  * `max_sequence_length`, a bound of the L_b, sizes the split of long sequences over workgroups and
  * nothing else.  Workspace: ferrule_hip_kv_attention_workspace_size bytes (may be 0), 256-byte
  * aligned, used by this call alone until it has completed. */
@@ -980,7 +983,7 @@ typedef struct FerruleHipKvAttentionArgs {
   uint64_t output_row_stride;
   uint64_t output_head_stride;
   uint64_t q;                 /* [rows, q_heads, head_dim] */
-  uint64_t output;            /* [rows, q_heads, head_dim] */
+  uint64_t output;            /* [rows, q_heads, head_dim]; shares no byte with q or the cache */
   uint64_t k_payload;
   uint64_t k_scales;
   uint64_t v_payload;

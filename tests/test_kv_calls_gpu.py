@@ -57,3 +57,37 @@ def test_a_workspace_dropped_after_its_call_is_not_handed_out_while_it_is_in_use
     torch.cuda.synchronize()
     same = [torch.equal(out, want) for out in outs]
     assert all(same), same
+
+
+@pytest.mark.parametrize("new,lengths,d", [([1], [1000], 128), ([3, 1], [700, 90], 256), ([40], [200], 64), ([1, 1], [6000, 100], 512)])
+def test_outputs_over_the_queries_are_refused_and_beside_them_in_one_buffer_are_not(ctx, new, lengths, d):  # noqa: F811
+    from ferrule_amd.provider import ProviderError
+    rng = np.random.default_rng(137)
+    batch, host, q = _case(rng, new, lengths, 64, 2, 4, d)
+    cache, dev, rows, heads = host.device(), batch.device(), batch.total, 8
+    qd = torch.from_numpy(q).bfloat16().cuda()
+    want = ctx.kv_cache_attention_into(cache, dev, qd, torch.empty_like(qd), 0.09)
+
+    def views(buffer, type_q, type_o, split):
+        b = torch.zeros(buffer, dtype=torch.uint8, device="cuda").view(*buffer[:-1], -1)
+        first, second = split(b)
+        first, second = first.view(type_q), second.view(type_o)
+        return first.copy_(qd), second
+
+    half, full = torch.bfloat16, torch.float32
+    for kind in (half, full):
+        size = 2 if kind is half else 4
+        for first, second in (views((rows, 2, heads, size * d), kind, kind, lambda b: (b[:, 0], b[:, 1])),
+                              views((rows, heads, 2, size * d), kind, kind, lambda b: (b[:, :, 1], b[:, :, 0])),
+                              views((2, rows, heads, size * d), kind, kind, lambda b: (b[1], b[0])),
+                              views((heads, rows, 2, size * d), kind, kind, lambda b: (b[:, :, 0].transpose(0, 1), b[:, :, 1].transpose(0, 1)))):
+            ctx.kv_cache_attention_into(cache, dev, first, second, 0.09)
+            assert torch.equal(first.bfloat16(), qd) and torch.equal(second.bfloat16(), want)
+    n, shift = qd.numel(), heads // 2 * d                         # half a row
+    flat = torch.zeros(n + shift, dtype=half, device="cuda")
+    front, back = flat[:n].view_as(qd), flat[shift:].view_as(qd)
+    wide = torch.zeros((rows, heads, 2 * d), dtype=half, device="cuda")
+    for a, b in ((front, front), (front, back), (back, front), (wide[..., :d], wide[..., d // 2:d // 2 + d]),
+                 (qd, torch.empty((1, 1, d), dtype=half, device="cuda").expand(rows, heads, d))):
+        with pytest.raises((ValueError, ProviderError)):
+            ctx.kv_cache_attention_into(cache, dev, a, b, 0.09)
