@@ -305,10 +305,19 @@ FerruleHipStatus validate(const FerruleHipKvCacheArgs &a) {
   return FERRULE_HIP_SUCCESS;
 }
 
+// Rows that read writes stand once each; this is what shows it without a look at every row.
+FerruleHipStatus validate_read(const FerruleHipKvCacheArgs &a) {
+  const FerruleHipStatus status = validate(a);
+  if (status == FERRULE_HIP_INVALID_ARGUMENT || a.batch == 0u || a.rows == 0u) return status;
+  const bool rows = a.rows > 1u && (a.key_row_stride == 0u || a.value_row_stride == 0u);
+  const bool heads = a.kv_heads > 1u && (a.key_head_stride == 0u || a.value_head_stride == 0u);
+  return rows || heads || a.keys == a.values ? FERRULE_HIP_INVALID_ARGUMENT : status;
+}
+
 template <template <typename, uint32_t> class Launch>
 FerruleHipStatus dispatch(const FerruleHipKvCacheArgs *args) {
   if (args == nullptr) return FERRULE_HIP_INVALID_ARGUMENT;
-  const FerruleHipStatus status = validate(*args);
+  const FerruleHipStatus status = Launch<float, 64>::check(*args);
   if (status != FERRULE_HIP_SUCCESS || args->batch == 0u || args->rows == 0u) return status;
   const FerruleHipKvCacheArgs &a = *args;
   hipStream_t stream = reinterpret_cast<hipStream_t>(static_cast<uintptr_t>(a.stream));
@@ -335,6 +344,7 @@ FerruleHipStatus dispatch(const FerruleHipKvCacheArgs *args) {
 
 template <typename T, uint32_t D>
 struct Append {
+  static FerruleHipStatus check(const FerruleHipKvCacheArgs &a) { return validate(a); }
   // eight tokens and up to 128 values each
   static uint32_t waves_per_tile(uint32_t head_dim) { return 4u * ((head_dim + 127u) / 128u); }
   static void run(const FerruleHipKvCacheArgs &a, dim3 grid, hipStream_t stream) {
@@ -343,6 +353,7 @@ struct Append {
 };
 template <typename T, uint32_t D>
 struct Read {
+  static FerruleHipStatus check(const FerruleHipKvCacheArgs &a) { return validate_read(a); }
   static uint32_t waves_per_tile(uint32_t) { return 2u; }  // keys and values
   static void run(const FerruleHipKvCacheArgs &a, dim3 grid, hipStream_t stream) {
     kv_read_kernel<T, D><<<grid, 256, 0, stream>>>(a);
@@ -359,7 +370,7 @@ extern "C" int32_t ferrule_hip_kv_cache_append_launch(const FerruleHipKvCacheArg
   return ferrule_hip::dispatch<ferrule_hip::Append>(args);
 }
 extern "C" int32_t ferrule_hip_kv_cache_read_can_implement(const FerruleHipKvCacheArgs *args) {
-  return args == nullptr ? FERRULE_HIP_INVALID_ARGUMENT : ferrule_hip::validate(*args);
+  return args == nullptr ? FERRULE_HIP_INVALID_ARGUMENT : ferrule_hip::validate_read(*args);
 }
 extern "C" int32_t ferrule_hip_kv_cache_read_launch(const FerruleHipKvCacheArgs *args) {
   return ferrule_hip::dispatch<ferrule_hip::Read>(args);

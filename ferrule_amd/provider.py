@@ -1174,17 +1174,24 @@ class HipArtifactOperatorContext:
         self.kernel_launches += 1
 
     def _kv_cache_args(self, cache: HipKvCache, batch: HipKvBatch, k: torch.Tensor, v: torch.Tensor,
-                       error: torch.Tensor | None, index: int) -> abi.KvCacheArgs:
-        shape = (batch.rows, cache.kv_heads, cache.head_dim)
+                       error: torch.Tensor | None, index: int, written: bool) -> abi.KvCacheArgs:
+        rows, heads, d = shape = (batch.rows, cache.kv_heads, cache.head_dim)
         ks = self._check_kv_rows("keys", k, shape, index)
         vs = self._check_kv_rows("values", v, shape, index)
         dtype = k.dtype
         if dtype is not v.dtype:
             raise ValueError("HIP KV keys and values share one type")
+        kp, vp, kind, size = k.data_ptr(), v.data_ptr(), abi.KV_BF16, 2
+        if dtype is torch.float32:
+            kind, size = abi.KV_F32, 4
+        # the usual case in a few comparisons: heads inside their rows, one tensor behind the other
+        if written and not (ks == vs and ks[0] >= heads * ks[1] and ks[1] >= d and abs(vp - kp) >= rows * size * ks[0]) and \
+                (_kv_rows_repeat(shape, ks) or _kv_rows_repeat(shape, vs) or _kv_rows_meet(shape, kp, ks, size, vp, vs, size)):
+            raise ValueError(f"HIP KV cache read writes every row once: strides {ks} and {vs}, {vp - kp} bytes apart")
         return abi.KvCacheArgs(
-            batch.batch, batch.rows, cache.kv_heads, cache.head_dim, cache.page_tokens, cache.page_count, batch.max_pages,
-            batch.max_query_length, abi.KV_BF16 if dtype is torch.bfloat16 else abi.KV_F32, 0, ks[0], ks[1], vs[0], vs[1],
-            k.data_ptr(), v.data_ptr(), *cache.pointers, *batch.pointers, _ptr(error))
+            batch.batch, rows, heads, d, cache.page_tokens, cache.page_count, batch.max_pages,
+            batch.max_query_length, kind, 0, ks[0], ks[1], vs[0], vs[1],
+            kp, vp, *cache.pointers, *batch.pointers, 0 if error is None else error.data_ptr())
 
     def kv_cache_append(self, cache: HipKvCache, batch: HipKvBatch, k: torch.Tensor, v: torch.Tensor,
                         error: torch.Tensor | None = None) -> None:
@@ -1199,19 +1206,19 @@ class HipArtifactOperatorContext:
             return
         self._kv_launch("KV cache append", self.lib.ferrule_hip_kv_cache_append_can_implement,
                         self.lib.ferrule_hip_kv_cache_append_launch,
-                        self._kv_cache_args(cache, batch, k, v, error, index), index)
+                        self._kv_cache_args(cache, batch, k, v, error, index, False), index)
 
     def kv_cache_read_into(self, cache: HipKvCache, batch: HipKvBatch, k: torch.Tensor, v: torch.Tensor,
                            error: torch.Tensor | None = None) -> None:
         """The cache's values at the batch's positions into BF16 or f32 [rows, kv_heads, head_dim], exact
         in either type.  To read positions s..e of a sequence give it e - s rows and length e.  A row
-        without a valid place reads as zeros and sets ``error``."""
+        without a valid place reads as zeros and sets ``error``.  ``k`` and ``v`` share no byte."""
         index = self._check_kv(cache, batch, error)
         if batch.rows == 0 or batch.batch == 0:
             return
         self._kv_launch("KV cache read", self.lib.ferrule_hip_kv_cache_read_can_implement,
                         self.lib.ferrule_hip_kv_cache_read_launch,
-                        self._kv_cache_args(cache, batch, k, v, error, index), index)
+                        self._kv_cache_args(cache, batch, k, v, error, index, True), index)
 
     def _kv_attention_args(self, cache: HipKvCache, batch: HipKvBatch, q_heads: int, window: int, sinks: int,
                            flags: int = 0, softmax_scale: float = 1.0, *tensors) -> abi.KvAttentionArgs:
@@ -1254,15 +1261,21 @@ class HipArtifactOperatorContext:
         shape = (batch.rows, q_heads, cache.head_dim)
         qs = self._check_kv_rows("queries", q, shape, index)
         os = self._check_kv_rows("output", out, shape, index)
-        flags = (abi.KV_ATTENTION_QUERY_F32 if q.dtype is torch.float32 else 0) | \
-            (abi.KV_ATTENTION_OUTPUT_F32 if out.dtype is torch.float32 else 0)
+        flags, q_size, o_size, qp, op = 0, 2, 2, q.data_ptr(), out.data_ptr()
+        if q.dtype is torch.float32:
+            flags, q_size = abi.KV_ATTENTION_QUERY_F32, 4
+        if out.dtype is torch.float32:
+            flags, o_size = flags | abi.KV_ATTENTION_OUTPUT_F32, 4
         a = self._kv_attention_args(cache, batch, q_heads, window, sinks, flags, softmax_scale, qs[0], qs[1], os[0], os[1],
-                                    q.data_ptr(), out.data_ptr(), *cache.pointers, *batch.pointers, _ptr(error))
+                                    qp, op, *cache.pointers, *batch.pointers, _ptr(error))
         if batch.rows == 0 or batch.batch == 0:
             return out
-        if _kv_rows_repeat(shape, os) or _kv_rows_meet(shape, a.q, qs, q.element_size(), a.output, os, out.element_size()):
+        # the usual case in a few comparisons: heads inside their rows, one tensor behind the other
+        if not (os == qs and os[0] >= q_heads * os[1] and os[1] >= shape[2] and
+                abs(op - qp) >= batch.rows * os[0] * (o_size if op < qp else q_size)) and \
+                (_kv_rows_repeat(shape, os) or _kv_rows_meet(shape, qp, qs, q_size, op, os, o_size)):
             raise ValueError("HIP KV attention writes every output row once and none over a query row: "
-                             f"output strides {os}, {a.output - a.q} bytes behind the queries with strides {qs}")
+                             f"output strides {os}, {op - qp} bytes behind the queries with strides {qs}")
         if workspace is None:
             workspace = self._kv_workspace(a, cache)
         elif workspace.dtype != torch.uint8 or workspace.get_device() != index or not workspace.is_contiguous():

@@ -932,9 +932,12 @@ typedef struct FerruleHipKvCacheArgs {
 /* append: quantises the batch's rows and writes them at their positions; a row without a valid
  * place is dropped.  A page that one call writes belongs to one sequence and stands once in its table.
  * read: the cache's values at the rows' positions (exact in either type); a row without a valid
- * place reads as zeros.  To read positions [s, e) of a sequence pass n_b = e - s and L_b = e.
- * INVALID_ARGUMENT for a bad block, UNSUPPORTED for a head_dim outside the supported set; a block
- * with rows == 0 or batch == 0 is a successful no-op. */
+ * place reads as zeros.  To read positions [s, e) of a sequence pass n_b = e - s and L_b = e.  Its rows of keys
+ * and of values share no byte: INVALID_ARGUMENT for equal addresses and for rows or heads without a stride,
+ * other overlaps are the caller's to avoid (append reads its rows, which may stand anywhere).
+ * INVALID_ARGUMENT for a bad block, UNSUPPORTED for a head_dim outside the supported set and for a grid
+ * (tiles of 32 of max_query_length rows, kv_heads, pieces of 128 values) of 2^24 workgroups and more or
+ * 65536 sequences; a block with rows == 0 or batch == 0 is a successful no-op. */
 int32_t ferrule_hip_kv_cache_append_can_implement(const FerruleHipKvCacheArgs *args);
 int32_t ferrule_hip_kv_cache_append_launch(const FerruleHipKvCacheArgs *args);
 int32_t ferrule_hip_kv_cache_read_can_implement(const FerruleHipKvCacheArgs *args);

@@ -97,3 +97,62 @@ def test_shared_bytes_of_row_tensors_are_found_exactly():
         twice.append(len(set(a)) != len(a))
         assert P._kv_rows_repeat(shape, first[1]) == twice[-1], (shape, first)
     assert 400 < sum(answers) < 3600 and 400 < sum(twice) < 3600
+
+
+def _cache_args(**kw):
+    a = dict(batch=2, rows=10, kv_heads=2, head_dim=128, page_tokens=64, page_count=9, max_pages=4, max_query_length=7,
+             value_type=abi.KV_BF16, key_row_stride=256, key_head_stride=128, value_row_stride=256, value_head_stride=128,
+             keys=0x100000, values=0x200000, k_payload=0x3000, k_scales=0x4000, v_payload=0x5000, v_scales=0x6000,
+             query_indptr=0x7000, sequence_lengths=0x8000, page_table=0x9000)
+    return abi.KvCacheArgs(**{**a, **kw})
+
+
+def test_row_tensors_that_read_and_attention_may_write_are_told_from_those_that_they_may_not(monkeypatch):
+    """The Python entries' answers, before any call into the library, are those of the bytes."""
+    ctx, _ = _host_context(monkeypatch, None)
+    monkeypatch.setattr(ctx, "_check_kv", lambda *_: -1, raising=False)
+    cache = P.HipKvCache(64, 2, 64, *(torch.empty(s, dtype=torch.uint8) for s in P.kv_cache_shapes(3, 64, 2, 64)))
+    i32 = lambda *shape: torch.zeros(shape, dtype=torch.int32)  # noqa: E731
+    memory = torch.zeros(1 << 14, dtype=torch.uint8)
+    launched = []
+    monkeypatch.setattr(ctx, "_kv_launch", lambda *_: launched.append(True), raising=False)
+    rng, answers = random.Random(5), []
+    for _ in range(1500):
+        n, attention = rng.randint(1, 4), rng.random() < 0.5
+        batch = P.HipKvBatch(i32(2), i32(1), i32(1, 3), n)
+        heads = rng.choice((2, 4)) if attention else 2
+        types = [rng.choice((torch.bfloat16, torch.float32))] * 2
+        if attention and rng.random() < 0.3:
+            types[1] = rng.choice((torch.bfloat16, torch.float32))
+        tensors, places, strides = [], [], None
+        for t in types:
+            size = 2 if t is torch.bfloat16 else 4
+            if strides is None or rng.random() < 0.4:
+                strides = rng.choice((64 * heads, 64 * heads, 128 * heads, 64, 0)), rng.choice((64, 64, 128, 64 * n, 0))
+            base = 16 * rng.randint(0, 160)
+            tensors.append(torch.as_strided(memory.view(t), (n, heads, 64), (*strides, 1), base // size))
+            places.append(_bytes((n, heads, 64), base, strides, size))
+        bad = bool(set(places[0]) & set(places[1])) or any(len(set(p)) < len(p) for p in (places[1:] if attention else places))
+        answers.append(bad)
+        del launched[:]
+        with (pytest.raises(ValueError) if bad else contextlib.nullcontext()):
+            if attention:
+                ctx.kv_cache_attention_into(cache, batch, *tensors, 0.1, workspace=memory)
+            else:
+                ctx.kv_cache_read_into(cache, batch, *tensors)
+        assert bool(launched) != bad, (places, types)
+    assert 300 < sum(answers) < 1400
+
+
+def test_read_refuses_one_place_for_keys_and_values_and_append_does_not():
+    lib = abi.load()
+    can, launch = lib.ferrule_hip_kv_cache_read_can_implement, lib.ferrule_hip_kv_cache_read_launch
+    append = lib.ferrule_hip_kv_cache_append_can_implement
+    assert can(C.byref(_cache_args())) == abi.SUCCESS
+    one = dict(rows=1, batch=1, max_query_length=1, key_row_stride=0, value_row_stride=0)
+    assert can(C.byref(_cache_args(**one))) == abi.SUCCESS
+    assert can(C.byref(_cache_args(**one, kv_heads=1, key_head_stride=0, value_head_stride=0))) == abi.SUCCESS
+    for bad in (dict(values=0x100000), dict(key_row_stride=0), dict(value_row_stride=0), dict(key_head_stride=0), dict(value_head_stride=0)):
+        assert can(C.byref(_cache_args(**bad))) == abi.INVALID_ARGUMENT, bad
+        assert launch(C.byref(_cache_args(**bad))) == abi.INVALID_ARGUMENT, bad
+        assert append(C.byref(_cache_args(**bad))) == abi.SUCCESS, bad               # what is only read may stand twice

@@ -91,3 +91,21 @@ def test_outputs_over_the_queries_are_refused_and_beside_them_in_one_buffer_are_
                  (qd, torch.empty((1, 1, d), dtype=half, device="cuda").expand(rows, heads, d))):
         with pytest.raises((ValueError, ProviderError)):
             ctx.kv_cache_attention_into(cache, dev, a, b, 0.09)
+
+
+def test_read_into_one_place_is_refused_and_side_by_side_is_not(ctx):  # noqa: F811
+    from ferrule_amd.provider import ProviderError
+    rng = np.random.default_rng(139)
+    batch, host, _ = _case(rng, [40, 7], [90, 7], 32, 2, 1, 128)
+    cache, dev, n = host.device(), batch.device(), batch.total
+    want = [torch.empty((n, 2, 128), dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    ctx.kv_cache_read_into(cache, dev, *want)
+    for both in (torch.empty((n, 2, 2, 128), dtype=torch.bfloat16, device="cuda"), torch.empty((n, 2, 2, 128), device="cuda")):
+        for k, v in ((both[:, 0], both[:, 1]), (both[:, :, 1], both[:, :, 0])):
+            ctx.kv_cache_read_into(cache, dev, k, v)
+            assert torch.equal(k.bfloat16(), want[0]) and torch.equal(v.bfloat16(), want[1])
+    k, v = want
+    for pair in ((k, k), (k, k.view(-1)[:128].view(1, 1, 128).expand(n, 2, 128)), (v[:1].expand(n, 2, 128), k),
+                 (both[:, 0, :1].expand(n, 2, 128), both[:, 1])):
+        with pytest.raises((ValueError, ProviderError)):
+            ctx.kv_cache_read_into(cache, dev, *pair)
