@@ -64,6 +64,7 @@ struct SplitPlan {
   uint32_t by_row;      // join: a workgroup for each of the rows there are, which looks for its sequence
   uint32_t least_rows;  // of the sequences that the launch is for
   uint32_t most_rows;   // kEveryRow: no bound
+  uint32_t held_rows;   // rows for which a sequence has partials in the workspace, 0: they stand in the order of all rows
   uint64_t partials;    // byte offsets in the workspace
   uint64_t statistics;
 };
@@ -467,7 +468,8 @@ struct PackedRow {
   bool live;
 };
 
-// Launches for sequences of few rows count those, most_rows to a sequence: of all rows' partials few would be used.
+// Launches for sequences of few rows, and of fewer than the row tensors hold, have partials for those, held_rows to a
+// sequence: of all rows' partials few would be used.
 __device__ __forceinline__ PackedRow packed_row(const FerruleHipKvAttentionArgs &a, const SplitPlan &plan, const KvSequence &s,
                                                 uint32_t b, uint32_t kv_head, uint32_t group, uint32_t r) {
   PackedRow p;
@@ -476,7 +478,7 @@ __device__ __forceinline__ PackedRow packed_row(const FerruleHipKvAttentionArgs 
   const uint64_t at = s.row + static_cast<uint64_t>(p.live ? row : 0u);
   p.q = at * a.q_row_stride + head * a.q_head_stride;
   p.output = at * a.output_row_stride + head * a.output_head_stride;
-  p.index = (plan.most_rows == kEveryRow ? at : static_cast<uint64_t>(b) * plan.most_rows + row) * a.q_heads + head;
+  p.index = (plan.held_rows == 0u ? at : static_cast<uint64_t>(b) * plan.held_rows + row) * a.q_heads + head;
   p.position = s.position + static_cast<int32_t>(row);
   return p;
 }
@@ -1355,11 +1357,12 @@ uint32_t rows_of_workgroup(const FerruleHipKvAttentionArgs &a) {
 
 // How the token ranges are cut: into parts of equal length, so that sequences of different lengths give
 // workgroups of the same work.
-SplitPlan plan_splits(const FerruleHipKvAttentionArgs &a, uint32_t tiles, uint64_t segments, uint64_t held_rows) {
+SplitPlan plan_splits(const FerruleHipKvAttentionArgs &a, uint32_t tiles, uint64_t segments, uint32_t held_rows) {
   SplitPlan plan = {};
   plan.tile_rows = tiles == 0u ? kTileRows : tiles;
   plan.page_shift = static_cast<uint32_t>(__builtin_ctz(a.page_tokens));
   plan.most_rows = kEveryRow;
+  plan.held_rows = held_rows;
   plan.find = tiles != 0u && a.batch > 1u && row_tiles(a, plan.tile_rows) > 1u;
   const uint64_t range = token_tiles(a, plan.tile_rows);
   // Decode: about a thousand parts, which the card holds at once (64 sequences of 8192 tokens, 8 heads: 99 us, with
@@ -1387,7 +1390,9 @@ SplitPlan plan_splits(const FerruleHipKvAttentionArgs &a, uint32_t tiles, uint64
   if (plan.splits == 1u) return plan;
   // a workgroup for every row that a sequence might have takes time, also where there is none
   plan.by_row = static_cast<uint64_t>(a.batch) * row_bound(a) > 2ull * a.rows && static_cast<uint64_t>(a.rows) * a.q_heads <= 0x7fffffull;
-  plan.statistics = held_rows * a.q_heads * plan.splits * a.head_dim * sizeof(float);
+  // segments times parts are fewer than twice `target`: far below 2^64 bytes
+  const uint64_t held = held_rows == 0u ? a.rows : static_cast<uint64_t>(a.batch) * held_rows;
+  plan.statistics = held * a.q_heads * plan.splits * a.head_dim * sizeof(float);
   return plan;
 }
 
@@ -1421,15 +1426,15 @@ Plans plans_of(const FerruleHipKvAttentionArgs &a) {
     if (p.both) {
       // sized for one row each
       const uint32_t few_rows = few_tiles == 0u ? kTileRows : few_tiles;
-      p.few = plan_splits(p.few_sizes, few_tiles, static_cast<uint64_t>(a.batch) * a.kv_heads * ((group + few_rows - 1u) / few_rows),
-                          static_cast<uint64_t>(a.batch) * few);
+      p.few = plan_splits(p.few_sizes, few_tiles, static_cast<uint64_t>(a.batch) * a.kv_heads * ((group + few_rows - 1u) / few_rows), few);
       p.few.most_rows = few;
       // as many sequences as it takes to have all rows
       const uint64_t sequences = (a.rows + a.max_query_length - 1ull) / a.max_query_length;
       segments = (static_cast<uint64_t>(a.rows) * group / tile_rows + sequences) * a.kv_heads;
     }
   }
-  p.plan = plan_splits(a, tiles, segments, a.rows);
+  // row tensors may hold more rows than the sequences have
+  p.plan = plan_splits(a, tiles, segments, static_cast<uint64_t>(a.batch) * row_bound(a) < a.rows ? row_bound(a) : 0u);
   if (p.both) {
     p.plan.least_rows = p.few.most_rows + 1u;
     const uint64_t behind = parts_size(a, p.plan);

@@ -156,3 +156,19 @@ def test_read_refuses_one_place_for_keys_and_values_and_append_does_not():
         assert can(C.byref(_cache_args(**bad))) == abi.INVALID_ARGUMENT, bad
         assert launch(C.byref(_cache_args(**bad))) == abi.INVALID_ARGUMENT, bad
         assert append(C.byref(_cache_args(**bad))) == abi.SUCCESS, bad               # what is only read may stand twice
+
+
+@pytest.mark.parametrize("d", abi.KV_HEAD_DIMS)
+def test_rows_behind_the_last_sequence_take_no_workspace(d):
+    """A row tensor may be longer than what its sequences can have; also by so much that bytes would not count in 64 bits."""
+    lib = abi.load()
+    size = lambda **kw: lib.ferrule_hip_kv_attention_workspace_size(C.byref(_attention_args(head_dim=d, **kw)))  # noqa: E731
+    for q_heads, batch, most, length in ((64, 1, 1, 65536), (8, 3, 2, 30000), (64, 2, 100, 9000), (2048, 1, 1, 1 << 24)):
+        shape = dict(q_heads=q_heads, batch=batch, max_query_length=most, max_pages=1 << 19, max_sequence_length=length)
+        least = size(rows=batch * most, **shape)
+        assert least > 0
+        for rows in (batch * most + 1, 100000, 0x7fffffff):
+            assert size(rows=rows, **shape) <= least, (rows, shape)
+            # and the launch is content with that much
+            args = _attention_args(head_dim=d, rows=rows, workspace_bytes=least, **shape)
+            assert lib.ferrule_hip_kv_attention_can_implement(C.byref(args)) == abi.SUCCESS

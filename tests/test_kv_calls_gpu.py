@@ -109,3 +109,26 @@ def test_read_into_one_place_is_refused_and_side_by_side_is_not(ctx):  # noqa: F
                  (both[:, 0, :1].expand(n, 2, 128), both[:, 1])):
         with pytest.raises((ValueError, ProviderError)):
             ctx.kv_cache_read_into(cache, dev, *pair)
+
+
+@pytest.mark.parametrize("new,lengths,heads,group,d,most", [
+    ([1], [9000], 1, 8, 128, 1), ([2, 1, 2], [3000, 700, 5000], 2, 4, 64, 2), ([1, 0, 1], [6000, 0, 40], 1, 16, 512, 1),
+    ([40, 33], [2500, 4000], 1, 2, 128, 45), ([20, 1], [3000, 4000], 1, 8, 256, 20)])
+@pytest.mark.parametrize("behind", [1, 300])
+def test_partials_of_row_tensors_longer_than_their_sequences_stay_in_the_workspace(ctx, new, lengths, heads, group, d, most, behind):  # noqa: F811
+    """Split ranges; the workspace is what the entry asks for, and what stands behind it stays as it was."""
+    rng = np.random.default_rng(149 + d)
+    batch, host, q = _case(rng, new, lengths, 64, heads, group, d)
+    want, bound = K.attention_reference(host, batch, q, 0.09)
+    rows = len(new) * most + behind
+    qd = torch.ones((rows, heads * group, d), dtype=torch.bfloat16, device="cuda")
+    qd[:batch.total].copy_(torch.from_numpy(q))
+    out = torch.full_like(qd, 9.0)
+    cache, dev = host.device(), batch.device(rows=rows, max_query_length=most)
+    size = ctx.kv_cache_attention_workspace(cache, dev, heads * group).numel()
+    assert size > 0
+    memory = torch.full((size + 4096,), 129, dtype=torch.uint8, device="cuda")
+    ctx.kv_cache_attention_into(cache, dev, qd, out, 0.09, workspace=memory[:size])
+    got = out.float().cpu().numpy()
+    assert (got[batch.total:] == 9).all() and (memory[size:] == 129).all()
+    K.check_attention(got[:batch.total], want, bound)
