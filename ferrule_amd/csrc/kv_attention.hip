@@ -1327,6 +1327,9 @@ bool rows_of_prompts(const FerruleHipKvAttentionArgs &a) {
   return 2ull * a.max_query_length > kTileTokens * token_tiles(a, 64u);
 }
 
+// Packed rows that are the decode kernel's over any range.
+uint32_t few_packed(const FerruleHipKvAttentionArgs &a) { return a.head_dim == 512u ? 16u : 32u; }
+
 // Which kernel: packed rows of a workgroup of kv_attention_rows_kernel, 0 for kv_attention_decode_kernel.
 // The latter reads and expands the range once for every 16 rows.  Two tiles of 16 are worth that everywhere but at heads
 // of 512 (64 sequences of 4096 tokens, 32 rows: heads of 128 48 us, rows kernel 81; heads of 512 89 and 73), four where
@@ -1336,7 +1339,7 @@ bool rows_of_prompts(const FerruleHipKvAttentionArgs &a) {
 uint32_t rows_of_workgroup(const FerruleHipKvAttentionArgs &a) {
   const uint64_t rows = packed_rows(a);
   const bool wide = a.head_dim == 512u;
-  if (rows <= (wide ? 16u : 32u)) return 0u;
+  if (rows <= few_packed(a)) return 0u;
   if (rows <= 64u && segments_of(a, kTileRows) <= kSegments && token_tiles(a, kTileRows) <= (wide ? 2u * kWaves : kShortRange)) return 0u;
   if (rows <= 64u || a.head_dim == 512u) return 64u;
   // A workgroup of more rows reads and expands the tokens less often (a prompt of 8192 tokens, 32 heads of 128: 506 us
@@ -1355,6 +1358,18 @@ uint32_t rows_of_workgroup(const FerruleHipKvAttentionArgs &a) {
   return tile;
 }
 
+// Parts of all ranges together.
+// Decode: about a thousand parts, which the card holds at once (64 sequences of 8192 tokens, 8 heads: 99 us, with
+// 2048 parts 112).  Rows: no more than fill it once, one workgroup of eight waves or two of four to a CU, and parts
+// long enough to pay for their f32 partials (4 x 512 rows over 8192 tokens: heads of 128 244 us, with 512 parts 285;
+// heads of 64 191 us, with 256 parts 231; 100 rows of 2 heads over 4000 tokens: 19 us, with parts of 16 and more 31).
+uint32_t target_parts(uint32_t head_dim, uint32_t tiles) {
+  if (tiles == 0u) return 1024u;
+  const bool eight_waves = head_dim == 512u || (head_dim == 256u && tiles == 128u) || (head_dim == 128u && tiles == 256u);
+  return eight_waves ? 256u : 512u;
+}
+constexpr uint32_t kLeastPart = 8;  // tiles
+
 // How the token ranges are cut: into parts of equal length, so that sequences of different lengths give
 // workgroups of the same work.
 SplitPlan plan_splits(const FerruleHipKvAttentionArgs &a, uint32_t tiles, uint64_t segments, uint32_t held_rows) {
@@ -1365,13 +1380,8 @@ SplitPlan plan_splits(const FerruleHipKvAttentionArgs &a, uint32_t tiles, uint64
   plan.held_rows = held_rows;
   plan.find = tiles != 0u && a.batch > 1u && row_tiles(a, plan.tile_rows) > 1u;
   const uint64_t range = token_tiles(a, plan.tile_rows);
-  // Decode: about a thousand parts, which the card holds at once (64 sequences of 8192 tokens, 8 heads: 99 us, with
-  // 2048 parts 112).  Rows: no more than fill it once, one workgroup of eight waves or two of four to a CU, and parts
-  // long enough to pay for their f32 partials (4 x 512 rows over 8192 tokens: heads of 128 244 us, with 512 parts 285;
-  // heads of 64 191 us, with 256 parts 231; 100 rows of 2 heads over 4000 tokens: 19 us, with parts of 16 and more 31).
-  const uint32_t tile_waves = a.head_dim == 512u || (a.head_dim == 256u && tiles == 128u) || (a.head_dim == 128u && tiles == 256u) ? 8u : 4u;
-  const uint64_t target = tiles == 0u ? 1024u : tile_waves == 8u ? 256u : 512u;
-  const uint64_t least = tiles != 0u && rows_of_prompts(a) ? 16u : 8u;
+  const uint64_t target = target_parts(a.head_dim, tiles);
+  const uint64_t least = tiles != 0u && rows_of_prompts(a) ? 2u * kLeastPart : kLeastPart;
   uint64_t part = (segments * range + target - 1u) / target;
   part = part < least ? least : part;
   if (tiles != 0u && 2u * range < 3u * part && range <= kShortRange) part = range;  // not for a little more than one part
@@ -1417,7 +1427,7 @@ Plans plans_of(const FerruleHipKvAttentionArgs &a) {
   const uint32_t tiles = rows_of_workgroup(a), tile_rows = tiles == 0u ? kTileRows : tiles, group = a.q_heads / a.kv_heads;
   uint64_t segments = segments_of(a, tile_rows);
   if (tiles != 0u && a.batch > 1u) {
-    const uint32_t limit = (a.head_dim == 512u ? 16u : 32u) / group, few = limit == 0u ? 1u : limit;
+    const uint32_t limit = few_packed(a) / group, few = limit == 0u ? 1u : limit;
     p.few_sizes = a;
     p.few_sizes.max_query_length = few;
     const uint32_t few_tiles = rows_of_workgroup(p.few_sizes);
@@ -1444,9 +1454,63 @@ Plans plans_of(const FerruleHipKvAttentionArgs &a) {
   return p;
 }
 
+// What the block itself takes.
 uint64_t workspace_size(const FerruleHipKvAttentionArgs &a) {
   const Plans p = plans_of(a);
   return parts_size(a, p.plan) + (p.both ? parts_size(a, p.few) : 0u);
+}
+
+// A launch of smaller bounds can take more: fewer rows are cut into more parts.  What a program asks for once at its
+// largest bounds has to hold for all of them, so it is an upper bound that grows with each.
+//
+// With n tiles of rows to a key/value head a range has at most ceil(t / n) parts, t = ceil(target / kv_heads), and one
+// where n >= t.  The largest n * ceil(t / n) of n = 1 .. most < t: an n of s parts is at most (t - 1) / (s - 1), so
+// that n * s <= (t - 1) * s / (s - 1), which falls with s.
+uint64_t most_parts(uint64_t most, uint64_t t) {
+  if (t <= 1u || most == 0u) return 0u;
+  if (most >= t) most = t - 1u;
+  const uint64_t s = (t + most - 1u) / most, here = most * s, fewer = (t - 1u) * (s + 1u) / s;
+  return here > fewer ? here : fewer;
+}
+
+// (row, query head)s times parts in a launch of any smaller bounds: up to `tiles` tiles of rows a head, each with `per`
+// packed rows at most, `held` (row, query head)s in all, ranges of up to `range` tiles.
+uint64_t most_partials(const FerruleHipKvAttentionArgs &a, uint32_t target, uint64_t tiles, uint64_t per, uint64_t held, uint64_t range) {
+  const uint64_t t = (target + a.kv_heads - 1u) / a.kv_heads, splits = (range + kLeastPart - 1u) / kLeastPart;
+  if (t <= 1u || splits <= 1u) return 0u;
+  const uint64_t by_parts = a.kv_heads * per * most_parts(tiles, t);
+  const uint64_t cut = a.kv_heads * per * (t - 1u), by_range = (held < cut ? held : cut) * splits;
+  return by_parts < by_range ? by_parts : by_range;
+}
+
+uint64_t workspace_bound(const FerruleHipKvAttentionArgs &a) {
+  const uint32_t group = a.q_heads / a.kv_heads, limit = few_packed(a) / group, few = limit == 0u ? 1u : limit;
+  const uint64_t packed = packed_rows(a), all = static_cast<uint64_t>(a.batch) * row_bound(a), rows = all < a.rows ? all : a.rows;
+  const bool both = a.batch > 1u && packed > few_packed(a) && few < row_bound(a) && token_tiles(a, kTileRows) > kShortRange;
+  uint64_t most = 0u, beside = 0u;  // of the launch for all sequences, or for those of many rows; of the one for few rows beside that
+  const uint32_t kinds[] = {kTileRows, 64u, 128u, 256u};
+  for (const uint32_t tile : kinds) {
+    // whether rows_of_workgroup has this tile for so many packed rows or fewer
+    const auto reaches = [&](uint64_t count) {
+      return tile == kTileRows || (tile == 64u && count > few_packed(a)) || (tile == 128u && count > 64u && a.head_dim < 512u) ||
+             (tile == 256u && count > 128u && a.head_dim < 256u);
+    };
+    const uint32_t target = target_parts(a.head_dim, tile == kTileRows ? 0u : tile);
+    if (reaches(packed)) {
+      // beside a launch for few rows, tiles are counted by all rows
+      const uint64_t tiles = tile == kTileRows ? found_tiles(a, tile) : rows * group / tile + a.batch;
+      const uint64_t partials = most_partials(a, target, tiles, packed < tile ? packed : tile, rows * a.q_heads, token_tiles(a, tile));
+      most = most > partials ? most : partials;
+    }
+    if (both && reaches(few * group)) {  // tiles are counted for one row of each sequence
+      const uint64_t each = (group + tile - 1u) / tile, sequences = a.batch;
+      const uint64_t partials = most_partials(a, target, sequences * each, (few * group + each - 1u) / each, sequences * few * a.q_heads,
+                                              token_tiles(a, tile));
+      beside = beside > partials ? beside : partials;
+    }
+  }
+  const uint64_t bytes = (a.head_dim + 2u) * sizeof(float);
+  return ((most * bytes + 255u) & ~255ull) + ((beside * bytes + 255u) & ~255ull);
 }
 
 dim3 grid_of(const FerruleHipKvAttentionArgs &a, const SplitPlan &plan) {
@@ -1563,7 +1627,7 @@ void launch(const FerruleHipKvAttentionArgs &a, hipStream_t stream) {
 extern "C" uint64_t ferrule_hip_kv_attention_workspace_size(const FerruleHipKvAttentionArgs *args) {
   using namespace ferrule_hip;
   if (args == nullptr || args->batch == 0u || args->rows == 0u || validate_shape(*args) != FERRULE_HIP_SUCCESS) return 0u;
-  return workspace_size(*args);
+  return workspace_bound(*args);
 }
 
 extern "C" int32_t ferrule_hip_kv_attention_can_implement(const FerruleHipKvAttentionArgs *args) {

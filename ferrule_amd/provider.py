@@ -1240,9 +1240,10 @@ class HipArtifactOperatorContext:
 
     def kv_cache_attention_workspace(self, cache: HipKvCache, batch: HipKvBatch, q_heads: int, window: int = 0,
                                      sinks: int = 0) -> torch.Tensor:
-        """The scratch that ``kv_cache_attention_into`` needs for batches of this shape (uint8, possibly
-        empty), memory of the context's stream.  It belongs to one call at a time: keep one per stream, and one
-        per captured graph that may replay while another runs."""
+        """The scratch that ``kv_cache_attention_into`` needs for this batch and for every one whose sequences, rows
+        and bounds of the lengths are no more (uint8, possibly empty), memory of the context's stream; asked
+        for without a window it serves every window.  It belongs to one call at a time: keep one per stream, and
+        one per captured graph that may replay while another runs."""
         index = self._check_kv(cache, batch, None)
         args = self._kv_attention_args(cache, batch, q_heads, window, sinks)
         return self._kv_workspace(args, cache)

@@ -965,7 +965,10 @@ int32_t ferrule_hip_kv_cache_read_launch(const FerruleHipKvCacheArgs *args);
  * stride; other overlaps are the caller's to avoid.
  * `max_sequence_length`, a bound of the L_b, sizes the split of long sequences over workgroups and
  * nothing else.  Workspace: ferrule_hip_kv_attention_workspace_size bytes (may be 0), 256-byte
- * aligned, used by this call alone until it has completed. */
+ * aligned, used by this call alone until it has completed.  The size holds for every block with the same
+ * q_heads, kv_heads, head_dim, window and sinks whose batch, rows, max_query_length and max_sequence_length
+ * are no larger, and one asked for with window 0 holds for any window and sinks: ask once, for the largest
+ * bounds.  (A block itself may take less than that; fewer rows are cut into more parts.) */
 typedef struct FerruleHipKvAttentionArgs {
   uint32_t batch;
   uint32_t rows;

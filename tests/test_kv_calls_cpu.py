@@ -172,3 +172,49 @@ def test_rows_behind_the_last_sequence_take_no_workspace(d):
             # and the launch is content with that much
             args = _attention_args(head_dim=d, rows=rows, workspace_bytes=least, **shape)
             assert lib.ferrule_hip_kv_attention_can_implement(C.byref(args)) == abi.SUCCESS
+
+
+def _smaller(rng, most):
+    """A block with no larger a bound than `most`."""
+    log = lambda n: min(n, max(1, round(n ** rng.random())))  # noqa: E731
+    pick = lambda n: rng.choice((n, log(n), rng.randint(1, n)))  # noqa: E731
+    return dict(batch=pick(most["batch"]), rows=pick(most["rows"]), max_query_length=pick(most["max_query_length"]),
+                max_sequence_length=pick(most["max_sequence_length"]))
+
+
+@pytest.mark.parametrize("seed", range(8))
+@pytest.mark.parametrize("d", abi.KV_HEAD_DIMS)
+def test_a_workspace_sized_by_the_largest_bounds_holds_every_smaller_block(d, seed):
+    lib = abi.load()
+    can, sizes = lib.ferrule_hip_kv_attention_can_implement, lib.ferrule_hip_kv_attention_workspace_size
+    rng = random.Random(1000 * d + seed)
+    split = 0
+    for _ in range(60):
+        group, kv_heads = rng.choice((1, 2, 3, 4, 5, 8, 16, 24, 40, 64, 100, 128)), rng.choice((1, 2, 3, 4, 6, 8, 16))
+        window, sinks = rng.choice(((0, 0), (0, 0), (rng.randint(1, 9000), rng.choice((0, 4, 40)))))
+        fixed = dict(q_heads=group * kv_heads, kv_heads=kv_heads, head_dim=d, max_pages=2048)
+        most = dict(batch=rng.choice((1, 2, 5, 17, 64, 100, 300)), rows=rng.choice((1, 3, 64, 100, 700, 2048, 8193)),
+                    max_query_length=rng.choice((1, 2, 5, 33, 64, 300, 2048, 8192)), max_sequence_length=rng.choice((1, 600, 4000, 8192, 60000, 131072)))
+        size = sizes(C.byref(_attention_args(**fixed, **most, window=window, sinks=sinks)))
+        for _ in range(60):
+            small = _smaller(rng, most)
+            less = sizes(C.byref(_attention_args(**fixed, **small, window=window, sinks=sinks)))
+            assert less <= size, (fixed, most, small, window, sinks)
+            # sized without a window it holds for every window
+            narrow = (window, sinks) if window else rng.choice(((0, 0), (rng.randint(1, 9000), rng.choice((0, 4, 40)))))
+            block = dict(fixed, **small, window=narrow[0], sinks=narrow[1], workspace=0x300000 if size else 0)
+            assert can(C.byref(_attention_args(**block, workspace_bytes=size))) == abi.SUCCESS, (block, most, size)
+            split += can(C.byref(_attention_args(**block, workspace_bytes=0))) != abi.SUCCESS
+    assert split > 300                                          # of the smaller blocks need some
+
+
+def test_the_workspace_of_the_largest_bounds_is_not_much_larger_than_what_a_block_needs():
+    lib = abi.load()
+    size = lambda **kw: lib.ferrule_hip_kv_attention_workspace_size(C.byref(_attention_args(max_pages=2048, **kw)))  # noqa: E731
+    decode = dict(rows=1, max_query_length=1, q_heads=64, kv_heads=8, max_sequence_length=8192)
+    # 1024 parts of eight heads, and one more for each row
+    for batch in (32, 64, 100, 1024):
+        assert 0 < size(**dict(decode, batch=batch, rows=batch)) <= 2 * 1024 * 8 * (128 + 2) * 4
+    assert size(**dict(decode, batch=1, max_sequence_length=200)) == 0       # one part
+    prompt = dict(batch=1, rows=8192, max_query_length=8192, q_heads=32, kv_heads=8, max_sequence_length=8192)
+    assert 0 < size(**prompt) <= 2 * 256 * 256 * (128 + 2) * 4

@@ -132,3 +132,30 @@ def test_partials_of_row_tensors_longer_than_their_sequences_stay_in_the_workspa
     got = out.float().cpu().numpy()
     assert (got[batch.total:] == 9).all() and (memory[size:] == 129).all()
     K.check_attention(got[:batch.total], want, bound)
+
+
+@pytest.mark.parametrize("d,group", [(64, 8), (128, 8), (256, 4), (512, 16)])
+def test_one_workspace_of_the_largest_bounds_serves_every_smaller_step(ctx, d, group):  # noqa: F811
+    """Asked for once; steps of fewer sequences, rows and tokens, with windows and without, decode rows beside a prompt."""
+    from ferrule_amd.provider import HipKvBatch
+    rng = np.random.default_rng(151 + d)
+    heads, page, longest = 2, 64, 9000
+    most = HipKvBatch(_i32(*range(65)), _i32(*[longest] * 64), torch.zeros((64, 141), dtype=torch.int32, device="cuda"), 700, 600, longest)
+    cache = K.HostCache(900, page, heads, d).random(rng, 124, 128).device()
+    size = ctx.kv_cache_attention_workspace(cache, most, heads * group).numel()
+    memory = torch.full((size + 4096,), 129, dtype=torch.uint8, device="cuda")
+    cut = 0
+    for new, lengths in (([1], [9000]), ([1] * 5, [8000, 3, 700, 2500, 9000]), ([1] * 33, [2100] * 33), ([1] * 64, [4000] * 64), ([600], [600]),
+                         ([300], [8000]), ([64, 1, 3], [64, 9000, 5000]), ([500, 1, 1, 1], [5000, 40, 9000, 6000]), ([2] * 17, [5000] * 17)):
+        table = torch.from_numpy(rng.integers(0, 900, (len(new), 141)).astype(np.int32)).cuda()
+        starts = np.concatenate([[0], np.cumsum(new)]).tolist()
+        dev = HipKvBatch(_i32(*starts), _i32(*lengths), table, sum(new), max(new), max(lengths))
+        q = torch.randn((sum(new), heads * group, d), device="cuda").bfloat16()
+        for window, sinks in ((0, 0), (700, 4), (8000, 0)):
+            memory[:size] = 255
+            got = ctx.kv_cache_attention_into(cache, dev, q, torch.empty_like(q), 0.09, window, sinks, workspace=memory[:size])
+            cut += not bool((memory[:size] == 255).all())
+            want = ctx.kv_cache_attention_into(cache, dev, q, torch.empty_like(q), 0.09, window, sinks)
+            same = torch.equal(got, want) and bool(torch.isfinite(got).all()) and bool((memory[size:] == 129).all())
+            assert same, (new, lengths, window)
+    assert cut >= 8                                             # steps that used it
