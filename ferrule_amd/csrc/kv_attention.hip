@@ -1438,6 +1438,7 @@ Plans plans_of(const FerruleHipKvAttentionArgs &a) {
       const uint32_t few_rows = few_tiles == 0u ? kTileRows : few_tiles;
       p.few = plan_splits(p.few_sizes, few_tiles, static_cast<uint64_t>(a.batch) * a.kv_heads * ((group + few_rows - 1u) / few_rows), few);
       p.few.most_rows = few;
+      p.few.inner = 0u;  // the sequences of many rows have no tile in it, so not every sequence has all of them
       // as many sequences as it takes to have all rows
       const uint64_t sequences = (a.rows + a.max_query_length - 1ull) / a.max_query_length;
       segments = (static_cast<uint64_t>(a.rows) * group / tile_rows + sequences) * a.kv_heads;

@@ -159,3 +159,28 @@ def test_one_workspace_of_the_largest_bounds_serves_every_smaller_step(ctx, d, g
             same = torch.equal(got, want) and bool(torch.isfinite(got).all()) and bool((memory[size:] == 129).all())
             assert same, (new, lengths, window)
     assert cut >= 8                                             # steps that used it
+
+
+@pytest.mark.parametrize("new,lengths,heads,group,d,window,sinks", [
+    # 17 to 32 packed rows over more than 2048 tokens: both tiles of every sequence, ragged, in several heads
+    ([3, 3, 3], [2500, 4100, 2070], 3, 8, 128, 0, 0), ([5, 5], [2600, 5000], 2, 5, 64, 0, 0), ([4, 4, 4, 4], [2300, 40, 4, 3000], 2, 8, 128, 2200, 3),
+    ([2, 2, 2], [2200, 2900, 700], 2, 16, 256, 0, 0), ([32, 32], [2400, 3300], 3, 1, 64, 2250, 40), ([2, 2], [2700, 2100], 4, 9, 256, 2090, 5),
+    # bounds that fit the rows though no sequence has so many: 16 = 4 * 4 rows, 24 = 3 * 8
+    ([13, 1, 1, 1], [2500, 4000, 2600, 50], 2, 8, 128, 0, 0), ([20, 3, 1], [2600, 2400, 3000], 2, 4, 64, 2300, 4),
+    # as many rows as sequences times the bound, not all of them there
+    ([3, 1, 2], [2500, 2600, 4000], 2, 8, 128, 0, 0)])
+@pytest.mark.parametrize("types", ["bf16", "f32"])
+def test_two_tiles_of_few_rows_in_every_order_of_workgroups(ctx, new, lengths, heads, group, d, window, sinks, types):  # noqa: F811
+    rng = np.random.default_rng(157 + d)
+    batch, host, q = _case(rng, new, lengths, 64, heads, group, d)
+    want, bound = K.attention_reference(host, batch, q, 0.09, window, sinks, f32_output=types == "f32")
+    t = torch.float32 if types == "f32" else torch.bfloat16
+    K.check_attention(_attend(ctx, host, batch, q, 0.09, window, sinks, t, t), want, bound)
+    rows = len(new) * max(new)                                  # padded to the bound
+    qd = torch.ones((rows, heads * group, d), dtype=t, device="cuda")
+    qd[:batch.total].copy_(torch.from_numpy(q))
+    out = torch.full_like(qd, 9.0)
+    ctx.kv_cache_attention_into(host.device(), batch.device(rows=rows), qd, out, 0.09, window=window, sinks=sinks)
+    got = out.float().cpu().numpy()
+    assert (got[batch.total:] == 9).all()
+    K.check_attention(got[:batch.total], want, bound)
