@@ -558,7 +558,7 @@ __global__ __launch_bounds__(WAVES * 64u, kDecodeOccupancy<D>) void kv_attention
   const int32_t low = s.position + static_cast<int32_t>(first_row / group);
   const int32_t high = s.position + static_cast<int32_t>(last_row / group);
   const TileRange range = tile_range(a, low, high);
-  if (high >= static_cast<int32_t>(a.max_pages * a.page_tokens) && threadIdx.x == 0u) kv_report(a.error);
+  if ((low < 0 || high >= static_cast<int32_t>(a.max_pages * a.page_tokens)) && threadIdx.x == 0u) kv_report(a.error);
   const uint32_t parts = parts_of(range.count, plan);
   if (split >= parts) return;
   const PartRange part = part_of(range.count, parts, split);
@@ -831,8 +831,9 @@ __global__ __launch_bounds__(WAVES * 64u, (Rows<D, NQ, WAVES, SHARES>::kOccupanc
   const uint32_t first_row = (tiles - 1u - row_tile) * R::kRows;  // the longest causal ranges first
   const uint32_t last_row = min(first_row + R::kRows, all_rows) - 1u;
   const int32_t high = s.position + static_cast<int32_t>(last_row / group);
-  const TileRange range = tile_range(a, s.position + static_cast<int32_t>(first_row / group), high);
-  if (high >= static_cast<int32_t>(a.max_pages * a.page_tokens) && threadIdx.x == 0u) kv_report(a.error);
+  const int32_t low = s.position + static_cast<int32_t>(first_row / group);
+  const TileRange range = tile_range(a, low, high);
+  if ((low < 0 || high >= static_cast<int32_t>(a.max_pages * a.page_tokens)) && threadIdx.x == 0u) kv_report(a.error);
   const uint32_t parts = parts_of(range.count, plan);
   if (split >= parts) return;
   const PartRange part = part_of(range.count, parts, split);

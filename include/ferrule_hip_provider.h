@@ -896,8 +896,9 @@ int32_t ferrule_hip_hc_producer_launch(const FerruleHipHcProducerArgs *args);
  *   page_table [batch][max_pages]  the page of position p is page_table[b][p / page_tokens]
  * `rows` is how many rows the row tensors hold; rows behind query_indptr[batch] are not touched.
  * `max_query_length` is an upper bound of the n_b (it sizes the grid).  A page number outside
- * [0, page_count), a position outside the table, rows beyond `rows` or `max_query_length` are never
- * followed; whoever meets one stores 1 to `error` (int32 [1], may be 0; the caller clears it). */
+ * [0, page_count), a position before 0 or behind the table, rows beyond `rows` or `max_query_length` are
+ * never followed; each operator that meets one stores 1 to `error` (int32 [1], may be 0; the caller clears
+ * it).  A sequence with nothing to do has n_b = 0. */
 #define FERRULE_HIP_KV_F32 0u
 #define FERRULE_HIP_KV_BF16 1u
 
@@ -952,8 +953,8 @@ int32_t ferrule_hip_kv_cache_read_launch(const FerruleHipKvCacheArgs *args);
  *   j <= p and (window == 0 or p - j < window or j < sinks),
  * i.e. causal, or the last `window` positions and the first `sinks`.  The rows' own keys and values
  * are in the cache already (append first).  A row that sees nothing (a position before 0, every
- * visible page invalid) writes zeros; keys and values at positions that a row does not see do not
- * reach it, whatever they hold.
+ * visible page invalid; both are reported) writes zeros; keys and values at positions that a row does
+ * not see do not reach it, whatever they hold.
  * Arithmetic: q enters rounded to BF16 (exact for BF16, and for the f32 rows of the FP8 projections,
  * which hold BF16 values); scores, softmax statistics and sums are f32; the softmax weights are
  * rounded to BF16 before they multiply the values.  Sums are formed in a fixed order, over weights that

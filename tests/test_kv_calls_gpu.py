@@ -184,3 +184,26 @@ def test_two_tiles_of_few_rows_in_every_order_of_workgroups(ctx, new, lengths, h
     got = out.float().cpu().numpy()
     assert (got[batch.total:] == 9).all()
     K.check_attention(got[:batch.total], want, bound)
+
+
+@pytest.mark.parametrize("new,lengths,heads,group,d", [
+    # one token a sequence, verification rows, and rows for each of the kernels; over short ranges and split ones
+    ([1, 2, 1], [40, 1, 300], 2, 4, 128), ([1, 1], [9, 0], 1, 8, 64), ([2, 3], [5000, 2], 1, 4, 256), ([1, 4], [300, 3], 1, 16, 512),
+    ([90, 40], [60, 300], 1, 2, 64), ([270, 3], [269, 3], 1, 1, 128), ([150], [1], 1, 1, 256), ([60, 1], [40, 1], 1, 2, 512),
+    ([40, 1, 2], [2500, 4000, 1], 1, 8, 128)])
+def test_rows_in_front_of_position_0_are_reported_by_all_three_operators(ctx, new, lengths, heads, group, d):  # noqa: F811
+    rng = np.random.default_rng(163 + d)
+    for short in (True, False):
+        tokens = lengths if short else [max(n, length) for n, length in zip(new, lengths)]
+        batch, host, q = _case(rng, new, tokens, 32, heads, group, d)
+        want, bound = K.attention_reference(host, batch, q, 0.1)
+        cache, dev = host.device(), batch.device()
+        rows = torch.ones((batch.total, heads, d), device="cuda")
+        qd = torch.from_numpy(q).cuda()
+        out = torch.full_like(qd, 9.0)
+        flags = [torch.zeros(1, dtype=torch.int32, device="cuda") for _ in range(3)]
+        ctx.kv_cache_attention_into(cache, dev, qd, out, 0.1, error=flags[0])
+        ctx.kv_cache_read_into(cache, dev, torch.empty_like(rows), torch.empty_like(rows), flags[1])
+        ctx.kv_cache_append(cache, dev, rows, rows, flags[2])
+        K.check_attention(out.cpu().numpy(), want, bound)
+        assert [f.item() for f in flags] == [int(short)] * 3
