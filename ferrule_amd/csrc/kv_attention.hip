@@ -1554,9 +1554,9 @@ FerruleHipStatus validate(const FerruleHipKvAttentionArgs &a) {
   if (status == FERRULE_HIP_INVALID_ARGUMENT) return status;
   const uint32_t q_bytes = (a.flags & FERRULE_HIP_KV_ATTENTION_QUERY_F32) ? 4u : 2u;
   const uint32_t o_bytes = (a.flags & FERRULE_HIP_KV_ATTENTION_OUTPUT_F32) ? 4u : 2u;
-  if (!kv_rows_aligned(a.q, a.q_row_stride, a.q_head_stride, q_bytes) ||
-      !kv_rows_aligned(a.output, a.output_row_stride, a.output_head_stride, o_bytes) || !kv_aligned16(a.k_payload) ||
-      !kv_aligned16(a.k_scales) || !kv_aligned16(a.v_payload) || !kv_aligned16(a.v_scales) || a.query_indptr == 0u ||
+  if (!kv_rows_aligned(a.q, a.rows, a.q_row_stride, a.q_heads, a.q_head_stride, q_bytes) ||
+      !kv_rows_aligned(a.output, a.rows, a.output_row_stride, a.q_heads, a.output_head_stride, o_bytes) ||
+      !kv_aligned16(a.k_payload) || !kv_aligned16(a.k_scales) || !kv_aligned16(a.v_payload) || !kv_aligned16(a.v_scales) || a.query_indptr == 0u ||
       a.sequence_lengths == 0u || a.page_table == 0u || ((a.query_indptr | a.sequence_lengths | a.page_table | a.error) & 3u)) {
     return FERRULE_HIP_INVALID_ARGUMENT;
   }

@@ -90,9 +90,10 @@ struct KvLayout {
 inline bool kv_aligned16(uint64_t p) { return p != 0u && (p & 15u) == 0u; }
 inline bool kv_head_dim_supported(uint32_t d) { return d == 64u || d == 128u || d == 256u || d == 512u; }
 inline bool kv_page_tokens_valid(uint32_t p) { return p >= 32u && p <= 1024u && (p & (p - 1u)) == 0u; }
-// a strided row tensor: every row of every head on 16 bytes
-inline bool kv_rows_aligned(uint64_t base, uint64_t row_stride, uint64_t head_stride, uint32_t value_bytes) {
-  return kv_aligned16(base) && (row_stride * value_bytes) % 16u == 0u && (head_stride * value_bytes) % 16u == 0u;
+// a strided row tensor: every row of every head on 16 bytes (a stride that takes nothing anywhere may be any)
+inline bool kv_rows_aligned(uint64_t base, uint32_t rows, uint64_t row_stride, uint32_t heads, uint64_t head_stride, uint32_t value_bytes) {
+  return kv_aligned16(base) && (rows == 1u || (row_stride * value_bytes) % 16u == 0u) &&
+         (heads == 1u || (head_stride * value_bytes) % 16u == 0u);
 }
 
 }  // namespace ferrule_hip

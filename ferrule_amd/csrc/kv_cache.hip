@@ -290,9 +290,9 @@ FerruleHipStatus validate(const FerruleHipKvCacheArgs &a) {
     return FERRULE_HIP_INVALID_ARGUMENT;
   }
   const uint32_t bytes = a.value_type == FERRULE_HIP_KV_BF16 ? 2u : 4u;
-  if (!kv_rows_aligned(a.keys, a.key_row_stride, a.key_head_stride, bytes) ||
-      !kv_rows_aligned(a.values, a.value_row_stride, a.value_head_stride, bytes) || !kv_aligned16(a.k_payload) ||
-      !kv_aligned16(a.k_scales) || !kv_aligned16(a.v_payload) || !kv_aligned16(a.v_scales) || a.query_indptr == 0u ||
+  if (!kv_rows_aligned(a.keys, a.rows, a.key_row_stride, a.kv_heads, a.key_head_stride, bytes) ||
+      !kv_rows_aligned(a.values, a.rows, a.value_row_stride, a.kv_heads, a.value_head_stride, bytes) ||
+      !kv_aligned16(a.k_payload) || !kv_aligned16(a.k_scales) || !kv_aligned16(a.v_payload) || !kv_aligned16(a.v_scales) || a.query_indptr == 0u ||
       a.sequence_lengths == 0u || a.page_table == 0u || ((a.query_indptr | a.sequence_lengths | a.page_table | a.error) & 3u)) {
     return FERRULE_HIP_INVALID_ARGUMENT;
   }

@@ -914,7 +914,7 @@ typedef struct FerruleHipKvCacheArgs {
   uint32_t value_type;        /* FERRULE_HIP_KV_*: type of keys and values */
   uint32_t reserved;          /* 0 */
   uint64_t key_row_stride;    /* in values; a row's head_dim values are consecutive and every */
-  uint64_t key_head_stride;   /* row of a head starts on 16 bytes */
+  uint64_t key_head_stride;   /* row of a head starts on 16 bytes (one row or head: any stride) */
   uint64_t value_row_stride;
   uint64_t value_head_stride;
   uint64_t keys;              /* [rows, kv_heads, head_dim] */

@@ -218,3 +218,19 @@ def test_the_workspace_of_the_largest_bounds_is_not_much_larger_than_what_a_bloc
     assert size(**dict(decode, batch=1, max_sequence_length=200)) == 0       # one part
     prompt = dict(batch=1, rows=8192, max_query_length=8192, q_heads=32, kv_heads=8, max_sequence_length=8192)
     assert 0 < size(**prompt) <= 2 * 256 * 256 * (128 + 2) * 4
+
+
+def test_a_stride_that_nothing_takes_may_be_any():
+    """One row, or one head: every row that there is stands on 16 bytes."""
+    lib = abi.load()
+    row = dict(batch=1, rows=1, max_query_length=1)
+    can = lib.ferrule_hip_kv_cache_append_can_implement
+    assert can(C.byref(_cache_args(**row, key_row_stride=577, value_row_stride=3))) == abi.SUCCESS
+    assert can(C.byref(_cache_args(kv_heads=1, key_head_stride=577, value_head_stride=1))) == abi.SUCCESS
+    for bad in (dict(row, key_head_stride=577), dict(row, kv_heads=1, keys=0x100008), dict(kv_heads=1, value_row_stride=577)):
+        assert can(C.byref(_cache_args(**bad))) == abi.INVALID_ARGUMENT, bad
+    can = lib.ferrule_hip_kv_attention_can_implement
+    assert can(C.byref(_attention_args(**row, q_row_stride=577, output_row_stride=1))) == abi.SUCCESS
+    assert can(C.byref(_attention_args(q_heads=1, kv_heads=1, q_head_stride=577, output_head_stride=1))) == abi.SUCCESS
+    for bad in (dict(row, q_head_stride=577), dict(row, output_head_stride=129), dict(q_heads=1, kv_heads=1, output_row_stride=577)):
+        assert can(C.byref(_attention_args(**bad))) == abi.INVALID_ARGUMENT, bad

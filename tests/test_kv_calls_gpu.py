@@ -207,3 +207,25 @@ def test_rows_in_front_of_position_0_are_reported_by_all_three_operators(ctx, ne
         ctx.kv_cache_append(cache, dev, rows, rows, flags[2])
         K.check_attention(out.cpu().numpy(), want, bound)
         assert [f.item() for f in flags] == [int(short)] * 3
+
+
+def test_one_row_with_a_stride_off_16_bytes(ctx):  # noqa: F811
+    """A projection's single row of an odd width: keys, values and queries are views of it."""
+    rng = np.random.default_rng(167)
+    batch, host, _ = _case(rng, [1], [90], 32, 2, 4, 64)
+    cache, dev, width = host.device(), batch.device(), 12 * 64 + 1
+    row = torch.randn(width, device="cuda").bfloat16()
+    view = lambda first, heads: torch.as_strided(row, (1, heads, 64), (width, 64, 1), 64 * first)  # noqa: E731
+    ctx.kv_cache_append(cache, dev, view(0, 2), view(2, 2))
+    k, v = (torch.as_strided(torch.empty(130, dtype=torch.bfloat16, device="cuda"), (1, 2, 64), (129, 64, 1)) for _ in range(2))
+    ctx.kv_cache_read_into(cache, dev, k, v)
+    out = torch.as_strided(torch.empty(520, dtype=torch.bfloat16, device="cuda"), (1, 8, 64), (519, 64, 1))
+    ctx.kv_cache_attention_into(cache, dev, view(4, 8), out, 0.1)
+    x = row.float().cpu().numpy()
+    for h in range(2):
+        for which in (0, 1):
+            at = 64 * (2 * which + h)
+            host.put(batch.table[0, 2], h, 89 - 64, which, *K.quantise(x[at:at + 64]))
+            assert np.array_equal((k, v)[which][0, h].float().cpu().numpy(), host.value(batch.table[0, 2], h, 89 - 64, which).astype(np.float32))
+    want, bound = K.attention_reference(host, batch, x[256:768].reshape(1, 8, 64), 0.1)
+    K.check_attention(out.float().cpu().numpy(), want, bound)
