@@ -490,23 +490,18 @@ __device__ __forceinline__ uint32_t bf16_pair(float x, float y) {  // to nearest
 // N consecutive values of a row
 template <uint32_t N>
 __device__ __forceinline__ void store(uint64_t output, uint64_t at, bool f32, const float (&x)[N]) {
-  static_assert(N == 2u || N == 4u || N == 8u, "whole stores");
+  static_assert(N == 4u || N == 8u, "whole stores");
   if (f32) {
     float *dst = global_ptr<float>(output) + at;
-    if constexpr (N == 2u) {
-      *reinterpret_cast<float2 *>(dst) = make_float2(x[0], x[1]);
-    } else {
 #pragma unroll
-      for (uint32_t q = 0; q < N / 4u; ++q) {
-        reinterpret_cast<f32x4_t *>(dst)[q] = f32x4_t{x[4u * q], x[4u * q + 1u], x[4u * q + 2u], x[4u * q + 3u]};
-      }
+    for (uint32_t q = 0; q < N / 4u; ++q) {
+      reinterpret_cast<f32x4_t *>(dst)[q] = f32x4_t{x[4u * q], x[4u * q + 1u], x[4u * q + 2u], x[4u * q + 3u]};
     }
   } else {
     uint16_t *dst = global_ptr<uint16_t>(output) + at;
     uint32_t w[N / 2u];
 #pragma unroll
     for (uint32_t e = 0; e < N / 2u; ++e) w[e] = bf16_pair(x[2u * e], x[2u * e + 1u]);
-    if constexpr (N == 2u) *reinterpret_cast<uint32_t *>(dst) = w[0];
     if constexpr (N == 4u) *reinterpret_cast<uint2 *>(dst) = make_uint2(w[0], w[1]);
     if constexpr (N == 8u) *reinterpret_cast<u32x4_t *>(dst) = u32x4_t{w[0], w[1], w[2], w[3]};
   }
@@ -794,9 +789,9 @@ struct Rows {
   static constexpr uint32_t kOwn = kPieces / WAVES;                     // of them, a wave's
   static constexpr uint32_t kSub = kPieces / kUnits;                    // 32-token tiles of a step
   static constexpr bool kAhead = WAVES == 8u;  // the next tile's scores are made before this one's weights
-  static constexpr uint32_t kInner = kAhead || D >= 512u || NQ >= 4u ? 1u : kSub < 2u ? 1u : 2u;  // tiles between two looks at the maximum
+  static constexpr uint32_t kInner = kAhead || NQ >= 4u || kSub < 2u ? 1u : 2u;  // tiles between two looks at the maximum
   static constexpr uint32_t kRows = 16u * NQ * WAVES / SHARES;
-  static constexpr uint32_t kOccupancy = WAVES * 64u == 512u ? 2u : D >= 512u ? 1u : 2u;  // waves per SIMD
+  static constexpr uint32_t kOccupancy = 2u;  // waves per SIMD: one workgroup of eight waves on a CU, or two of four
 };
 
 template <uint32_t D, uint32_t NQ, uint32_t WAVES, uint32_t SHARES>
