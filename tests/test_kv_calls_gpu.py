@@ -229,3 +229,35 @@ def test_one_row_with_a_stride_off_16_bytes(ctx):  # noqa: F811
             assert np.array_equal((k, v)[which][0, h].float().cpu().numpy(), host.value(batch.table[0, 2], h, 89 - 64, which).astype(np.float32))
     want, bound = K.attention_reference(host, batch, x[256:768].reshape(1, 8, 64), 0.1)
     K.check_attention(out.float().cpu().numpy(), want, bound)
+
+
+def test_offsets_of_scale_bytes_beyond_32_bits(ctx):  # noqa: F811
+    """Scale arrays of more than 4 GiB (and so payloads of more than 64), the sequence on the last pages; nothing is filled."""
+    from ferrule_amd.provider import HipKvBatch, HipKvCache, kv_cache_shapes
+    heads, d, page = 8, 64, 1024
+    pages = (1 << 32) // (heads * page * d // 32) + 3
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < 150 << 30:
+        pytest.skip("needs 150 GiB of GPU memory")
+    cache = HipKvCache(page, heads, d, *(torch.empty(s, dtype=torch.uint8, device="cuda") for s in kv_cache_shapes(pages, page, heads, d)))
+    assert cache.k_scales.numel() > 1 << 32 and cache.v_scales.numel() > 1 << 32
+    small = ctx.kv_cache(2, page, heads, d)
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(7)
+    n = page + 40
+    k, v, q = (torch.randn((n, heads, d), generator=gen, device="cuda").bfloat16() for _ in range(3))
+    outs = []
+    for held, table in ((cache, _i32(pages - 1, pages - 2)), (small, _i32(1, 0))):
+        batch = HipKvBatch(_i32(0, n), _i32(n), table.view(1, 2), n)
+        ctx.kv_cache_append(held, batch, k, v)
+        kd, vd, rows = (torch.empty_like(k) for _ in range(3))
+        ctx.kv_cache_read_into(held, batch, kd, vd)
+        ctx.kv_cache_attention_into(held, batch, q, rows, 0.1)
+        last = HipKvBatch(_i32(0, 1), _i32(n), table.view(1, 2), 1)
+        one = ctx.kv_cache_attention_into(held, last, q[-1:], torch.empty_like(q[-1:]), 0.1)
+        outs.append((kd, vd, rows, one))
+    same = [torch.equal(a, b) and bool(torch.isfinite(a).all()) for a, b in zip(*outs)]
+    del cache
+    torch.cuda.empty_cache()
+    assert all(same), same
+    assert ((outs[0][0] - k).abs() <= 1).all() and ((outs[0][1] - v).abs() <= 1).all() and k.abs().max().item() < 6 > v.abs().max().item()
