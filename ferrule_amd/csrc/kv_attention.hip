@@ -28,11 +28,14 @@
 // the matrix pipe and, for heads of 64, the exponentials beside it.  Where rows leave CUs idle, the tokens of a
 // tile are cut into parts of equal length for several workgroups, and (maximum, sum, O) of the parts are joined in
 // a fixed order by the join kernels.
-//   64 sequences of 8192 tokens, 8 heads of 128 for 8 query heads each: 99 us, 5.8 TB/s
-//   the same with heads of 64: 55 us, 5.3 TB/s; 4096 tokens, heads of 256: 100 us, 5.7 TB/s
-//   64 x 8192 tokens of one 512-wide row for 16 heads: 97 us, for 64 heads 134 us (the cache is 0.29 GB)
-//   a prompt of 8192 tokens, 32 heads of 128: 490-505 us, 1.1 PFLOP/s (a large bf16 matrix product: 1.2)
-//   heads of 64: 315-350 us, 0.82; 4096 tokens, 16 heads of 256: 153 us, 0.9; 1024 tokens, 64 of 512: 131 us, 0.53
+//   64 sequences of 8192 tokens, 8 heads of 128 for 8 query heads each: 102 us, 5.6 TB/s
+//   the same with heads of 64: 59 us, 4.8 TB/s; 4096 tokens, heads of 256: 101 us, 5.6 TB/s
+//   64 x 8192 tokens of one 512-wide row for 16 heads: 89 us, for 64 heads 124 us (the cache is 0.29 GB)
+//   a prompt of 8192 tokens, 32 heads of 128: 470-480 us, 1.16 PFLOP/s (a large bf16 matrix product: 1.2)
+//   heads of 64: 316 us, 0.87; 4096 tokens, 16 heads of 256: 145 us, 0.95; 1024 tokens, 64 of 512: 124 us, 0.55
+// Here and below, unless a case of perf/operators.py is named (whose sequences are ragged): sequences of equal length on
+// shuffled pages, between events over launches one after the other through the Python entry; "a, with .. b" is the same
+// source with that one rule changed, "took a of what .. takes" a step's gain when it was made.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -106,8 +109,8 @@ struct RowTile {
 
 // Tile t of all that the sequences of the launch have, in their order, by the same rules as kv_sequence.  Workgroups
 // without a tile would not only take time: workgroups go to the shader engines in turn, so their pattern decides which
-// of those get the others (8 chunks of 200 to 600 rows in a grid for 600 each: 246 us, here 198; with the sequences
-// faster than the tiles, chunks of 2000, 100, 50 and 20 rows took 1536 us and take 625 here).
+// of those get the others (8 chunks of 200 to 600 rows in a grid for 600 each took 1.24 times what they take here, chunks of
+// 2000, 100, 50 and 20 rows with the sequences faster than the tiles 2.5 times).
 template <uint32_t ROWS>
 __device__ __forceinline__ RowTile find_tile(const FerruleHipKvAttentionArgs &a, const SplitPlan &plan, uint32_t t, uint32_t lane,
                                              bool report) {
@@ -508,13 +511,15 @@ __device__ __forceinline__ void store(uint64_t output, uint64_t at, bool f32, co
 }
 
 // Few rows: 16 of them, the token tiles shared out over the WAVES waves.  Keys and values go from memory to registers
-// with loads that leave no line behind (decode of 64 x 8192 tokens, 8 heads of 128: 117 -> 99 us with those and parts
-// of equal length), a step ahead; what a wave has in flight, 4.25 KB at heads of 128, times 16 waves is 68 KB a CU.
+// with loads that leave no line behind (decode of 64 x 8192 tokens, 8 heads of 128: with those and parts of equal length
+// it took 0.85 of the time), a step ahead; what a wave has in flight, 4.25 KB at heads of 128, times 16 waves is 68 KB a CU.
 // Heads of 256 and 512 have too many query terms for registers: one copy in LDS serves the four waves, and of a step's
-// values four 16-byte pieces are in flight at a time (16 heads on a row of 512: 157 -> 100 us).
+// values four 16-byte pieces are in flight at a time (16 heads on a row of 512 took 0.64 of the time).
+// At heads of 512 that leaves 244 registers and 136 accumulation registers a lane, one wave per SIMD: nothing runs while a
+// step waits for its loads.
 // Over a short range, eight waves, and two workgroups of them where there are CUs for it (COLUMNS = 2): both make the
 // scores, each multiplies half of the values, whose expansion is half of a step's vector work.
-// One sequence of 1000 tokens, 8 heads of 128 for 8 query heads each: 8.1 us (9.3 with one workgroup), of which 5 are a
+// One sequence of 1000 tokens, 8 heads of 128 for 8 query heads each: 8.4 us (9.7 with one workgroup), of which 5 are a
 // single step's chain of launch, table, cache and join; the others are a step's arithmetic, 0.7 us for two waves of a
 // SIMD (loads two, three or four steps ahead change nothing).
 template <uint32_t D>
@@ -536,13 +541,13 @@ __global__ __launch_bounds__(WAVES * 64u, kDecodeOccupancy<D>) void kv_attention
   const uint32_t split = blockIdx.x % plan.splits;
   const uint32_t kv_head = blockIdx.x / plan.splits % a.kv_heads;
   // 0 where COLUMNS is 1; taken from the grid there too at the sizes that have both (as a constant it costs heads of 128
-  // three registers more, which spill: 64 x 8192 tokens 80 -> 86 us)
+  // three registers more, which spill: the case decode_batch 80 -> 86 us)
   const uint32_t outer = blockIdx.x / plan.splits / a.kv_heads;
   const uint32_t first_unit = (D == 128u || D == 256u) && plan.wide == 2u ? outer * kUnits : 0u;
   // the tile of rows is last in the order of workgroups: those that a sequence does not have are at the end, in nobody's
-  // way (63 rows and 4 in one sequence, 8192 tokens each, 8 heads: 138 -> 97 us).  Where every sequence has all of them,
-  // they are neighbours, which share keys and values while those are in the cache (16 x 4 rows over 8192 tokens, 8 x 8
-  // heads: 57 -> 48 us; over a short range it costs 8 %).
+  // way (63 sequences of one row and one of four, 8192 tokens each, 8 heads, took 0.7 of the time).  Where every sequence
+  // has all of them, they are neighbours, which share keys and values while those are in the cache (16 x 4 rows over 8192
+  // tokens, 8 x 8 heads: 53 us, the other order 59; over a short range it costs 8 %).
   const uint32_t row_tile = plan.inner != 0u ? outer : blockIdx.z;
   const uint32_t group = a.q_heads / a.kv_heads;
   const KvSequence s = kv_sequence(a.query_indptr, a.sequence_lengths, b, a.rows, a.max_query_length);
@@ -627,7 +632,7 @@ __global__ __launch_bounds__(WAVES * 64u, kDecodeOccupancy<D>) void kv_attention
 
   for (uint32_t v = begin + wave; v < end; v += WAVES) {
     // keys and values are loaded one step ahead, as soon as the registers of this step's are free; two or
-    // three steps ahead at 3 or 2 waves per SIMD took as long (64 x 8192 tokens, 8 heads: 112, 110, 122 us)
+    // three steps ahead at 3 or 2 waves per SIMD took 0.98 and 1.09 of the time (64 x 8192 tokens, 8 heads of 128)
     const Place here = next_place;
     next_place = place_at<D>(a, plan, range, kv_head, v + WAVES, end, next_page, bad);
     next_page = page_of(a, plan, range, b, v + 2u * WAVES, end);
@@ -773,13 +778,15 @@ __global__ __launch_bounds__(WAVES * 64u, kDecodeOccupancy<D>) void kv_attention
 // one step ahead of their use; keys are read by every wave, from cache, as they stand.  One barrier per step.
 // Heads of 128 take 256 rows in eight waves: per 32 tokens and 16 rows the matrix pipe is busy for 256 cycles, the
 // vector pipe for about 230 (8 exponentials of 16 cycles each, and their sums, conversions and address steps): 41 %
-// and 52 % busy by the counters, at 2.1 GHz.  Heads of 64 halve the first and not the second, and are bound by it.
+// and 50 % busy by the counters, at 2.1 GHz.  Heads of 64 halve the first and not the second: 32 % and 54 %.
 // Eight waves have the next tile's scores made before this one's weights, so that neither waits for the other (heads of
-// 256, 128 rows, 4 x 512 rows over 8192 tokens, 32 heads: 534 -> 438 us; a prompt of 4096 tokens, heads of 128: 146 ->
-// 142 us; four waves gain nothing).  At heads of 512 a wave's accumulators alone are half of the registers, so that only four waves of 16 rows
+// 256, 128 rows, chunks of 512 rows took 0.82 of the time; a prompt of 4096 tokens, heads of 128, 0.97; four waves gain
+// nothing).  At heads of 512 a wave's accumulators alone are half of the registers, so that only four waves of 16 rows
 // would stand on a CU, one for a SIMD: instead SHARES = 2 waves have the same 16 rows, each half of the values, and
-// add up their halves of the scores in LDS (4 x 512 rows over 4096 tokens, 64 heads: 1160 -> 890 us; four shares of
-// 32 rows 996).
+// add up their halves of the scores in LDS (chunks of 512 rows for 64 heads took 0.77 of the time, four shares of 32 rows
+// 0.86; 4 x 512 rows over 4096 tokens take 1330 us, 0.77 PFLOP/s).
+// <128, 2, 8, 1> and <64, 4, 4, 1> keep 8 and 9 registers in scratch memory, stored in front of their loops and loaded
+// behind them.
 template <uint32_t D, uint32_t NQ, uint32_t WAVES, uint32_t SHARES>
 struct Rows {
   static constexpr uint32_t kUnits = D / 64u;
@@ -1330,24 +1337,24 @@ uint32_t few_packed(const FerruleHipKvAttentionArgs &a) { return a.head_dim == 5
 
 // Which kernel: packed rows of a workgroup of kv_attention_rows_kernel, 0 for kv_attention_decode_kernel.
 // The latter reads and expands the range once for every 16 rows.  Two tiles of 16 are worth that everywhere but at heads
-// of 512 (64 sequences of 4096 tokens, 32 rows: heads of 128 48 us, rows kernel 81; heads of 512 89 and 73), four where
-// every tile has a CU and a range is so short that it needs no parts (16 sequences, 4 heads, 64 rows over a window of
-// 1024: heads of 64 12 us, rows kernel 19, of 256 16 and 32; at 512 over 128 tokens 15-18 and 17-21, but over 256 tokens
-// 39 and 26).
+// of 512 (64 sequences of 4096 tokens, 32 query heads to each: 4 heads of 128 55 us, rows kernel 66, of 64 32 and 44, of
+// 256 90 and 112; one of 512 79 and 66), four where every tile has a CU and a range is so short that it needs no parts
+// (16 sequences, 4 heads, 64 rows over a window of 1024: the rows kernel took 1.6 times as long at heads of 64, twice as
+// long at 256; at 512 over 128 tokens 1.15 times, but over 256 tokens 0.67).
 uint32_t rows_of_workgroup(const FerruleHipKvAttentionArgs &a) {
   const uint64_t rows = packed_rows(a);
   const bool wide = a.head_dim == 512u;
   if (rows <= few_packed(a)) return 0u;
   if (rows <= 64u && segments_of(a, kTileRows) <= kSegments && token_tiles(a, kTileRows) <= (wide ? 2u * kWaves : kShortRange)) return 0u;
   if (rows <= 64u || a.head_dim == 512u) return 64u;
-  // A workgroup of more rows reads and expands the tokens less often (a prompt of 8192 tokens, 32 heads of 128: 506 us
-  // with 256 rows, 543 with 128, 645 with 64).  But the ranges of a prompt's rows differ, and cutting them costs more
-  // than it gives: two workgroups for a CU even them out (2048 tokens: 66, 60 and 61 us; 512 tokens: 28, 24 and 16.6).
-  // Nor are there enough steps in a short range to pay for the larger start (16 prompts of 256 tokens: 37, 32, 29).
+  // A workgroup of more rows reads and expands the tokens less often (a prompt of 8192 tokens, 32 heads of 128: 473 us
+  // with 256 rows, 504 with 128, 600 with 64).  But the ranges of a prompt's rows differ, and cutting them costs more
+  // than it gives: two workgroups for a CU even them out (2048 tokens: 64, 58 and 54 us; 512 tokens: 24 with 256, 15 with 64).
+  // Nor are there enough steps in a short range to pay for the larger start (16 prompts of 256 tokens: 41 and 37).
   const uint64_t range = token_tiles(a, 64u);
   const uint64_t total = static_cast<uint64_t>(a.rows) * a.q_heads;
   // And few workgroups of few steps, whatever their tiles, leave most CUs idle (12 x 270 rows of one head over a window of
-  // 574: heads of 64 33 us with 256 rows, 18.6 with 64; of 128 33 and 21).
+  // 574: heads of 64 29 us with 256 rows, 14 with 64; of 128 31 and 18).
   uint32_t tile = a.head_dim == 256u || rows <= 128u ? 128u : 256u;
   while (tile > 64u && (range < 16u || (rows_of_prompts(a) && total < 512u * tile) ||
                         segments_of(a, tile) * (range / 16u) < kSegments)) {
@@ -1357,10 +1364,12 @@ uint32_t rows_of_workgroup(const FerruleHipKvAttentionArgs &a) {
 }
 
 // Parts of all ranges together.
-// Decode: about a thousand parts, which the card holds at once (64 sequences of 8192 tokens, 8 heads: 99 us, with
-// 2048 parts 112).  Rows: no more than fill it once, one workgroup of eight waves or two of four to a CU, and parts
-// long enough to pay for their f32 partials (4 x 512 rows over 8192 tokens: heads of 128 244 us, with 512 parts 285;
-// heads of 64 191 us, with 256 parts 231; 100 rows of 2 heads over 4000 tokens: 19 us, with parts of 16 and more 31).
+// Decode: 1024, which the card holds at once up to heads of 128 (64 sequences of 8192 tokens, 8 heads of 128: 101 us, with
+// 2048 parts 109, with 512 98).  At 256 it holds 512 of them and at 512 values 256, so that 1024 take two rounds and four:
+// 512 parts are faster there (4096 tokens, 8 heads of 256: 100 and 92 us; 16 heads on a row of 512: 89 and 72; 64 heads
+// the same).  Rows: no more than fill it once, one workgroup of eight waves or two of four to a CU, and parts long enough
+// to pay for their f32 partials (4 x 512 rows over 8192 tokens: 8 x 4 heads of 128 227 us, with 512 parts 260; of 64
+// 167 us, with 256 parts 200; 100 rows of 2 heads over 4000 tokens took 0.6 of what parts of 16 tiles and more took).
 uint32_t target_parts(uint32_t head_dim, uint32_t tiles) {
   if (tiles == 0u) return 1024u;
   const bool eight_waves = head_dim == 512u || (head_dim == 256u && tiles == 128u) || (head_dim == 128u && tiles == 256u);
@@ -1384,8 +1393,9 @@ SplitPlan plan_splits(const FerruleHipKvAttentionArgs &a, uint32_t tiles, uint64
   part = part < least ? least : part;
   if (tiles != 0u && 2u * range < 3u * part && range <= kShortRange) part = range;  // not for a little more than one part
   // A range of a few steps of eight waves is not worth a second launch while there are CUs for all segments (32
-  // sequences of 8 heads of 256: 1000 tokens 25.3 -> 17.3 us, 2000 tokens 34.6 -> 26.8).  At 512 values eight waves
-  // would have half of the registers that the kernel needs (1 sequence of 500 tokens: 17.9 -> 30.8 us).
+  // sequences of 8 heads of 256: 1000 tokens 15.4 us, in parts 24; 2000 tokens 26 and 33).  At 512 values eight waves
+  // with all of the values each would have half of the registers that they need (1 sequence of 500 tokens: 1.7 times the
+  // time); halves of the values, as at 128 and 256, are not built there.
   if (tiles == 0u && a.head_dim <= 256u && part < range && range <= kShortRange && segments <= kSegments) {
     plan.wide = a.head_dim > 64u && 2u * segments <= kSegments ? 2u : 1u;
     part = range;
@@ -1405,8 +1415,8 @@ SplitPlan plan_splits(const FerruleHipKvAttentionArgs &a, uint32_t tiles, uint64
 }
 
 // One launch, or two.  A few rows over a long range need many workgroups for their range, and in a kernel for many rows
-// they would keep one at work long after the others (63 rows over 8192 tokens each and 512 over as many, 64 heads:
-// 1890 us, in two launches 260): where a batch can hold both, each launch takes its own sequences.
+// they would keep one at work long after the others (63 sequences of a row and one of 512 rows, 8192 tokens each, 64
+// heads: seven times what two launches take): where a batch can hold both, each launch takes its own sequences.
 struct Plans {
   SplitPlan plan;
   bool both;
