@@ -175,7 +175,7 @@ def _kv_rows_repeat(shape: tuple[int, int, int], strides: tuple[int, ...]) -> bo
 
 
 def _kv_starts(rows: int, heads: int, s: int, t: int) -> torch.Tensor:
-    return (torch.arange(rows)[:, None] * s + torch.arange(heads) * t).flatten().sort().values
+    return (torch.arange(rows, device="cpu")[:, None] * s + torch.arange(heads, device="cpu") * t).flatten().sort().values
 
 
 def _kv_rows_meet(shape: tuple[int, int, int], p0: int, strides0: tuple[int, ...], size0: int, p1: int,
@@ -1129,11 +1129,14 @@ class HipArtifactOperatorContext:
 
     # -- MXFP4 key/value cache ------------------------------------------------------
     def kv_cache(self, page_count: int, page_tokens: int, kv_heads: int, head_dim: int) -> HipKvCache:
-        """A new cache on this context's device, every byte zero; its memory belongs to the context's stream, where the
-        operators that follow find it filled."""
-        with torch.cuda.stream(self.stream):
+        """A new cache on this context's device, every byte zero; its memory belongs to the context's stream.  Operators
+        that follow on that stream, or on torch's current one, find it filled."""
+        stream, current = self.stream, torch.cuda.current_stream(self.device)
+        with torch.cuda.stream(stream):
             arrays = [torch.zeros(shape, dtype=torch.uint8, device=self.device)
                       for shape in kv_cache_shapes(page_count, page_tokens, kv_heads, head_dim)]
+        if stream != current:
+            current.wait_stream(stream)
         return HipKvCache(page_tokens, kv_heads, head_dim, *arrays)
 
     # A decode step's operators take the GPU a few microseconds, so their host side is kept short: argument blocks are

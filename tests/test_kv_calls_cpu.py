@@ -34,9 +34,29 @@ def _host_context(monkeypatch, own_stream):
     return ctx, taken
 
 
-def test_a_new_cache_is_filled_on_the_contexts_stream(monkeypatch):
+class _Stream:
+    """torch's current stream, which keeps what it waited for."""
+
+    def __init__(self, waited):
+        self.waited = waited
+
+    def wait_stream(self, other):
+        self.waited.append(other)
+
+
+def test_a_new_cache_is_filled_on_the_contexts_stream_and_torchs_waits_for_it(monkeypatch):
+    """Whoever writes to it next finds it filled: the context's operators, and torch on its current stream."""
     ctx, taken = _host_context(monkeypatch, "side")
+    waited = []
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda *_: _Stream(waited))
     cache = ctx.kv_cache(3, 64, 2, 128)
+    assert waited == ["side"]
+    del waited[:]
+    ctx._stream = own = torch.cuda.current_stream()
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda *_: own)
+    ctx.kv_cache(3, 64, 2, 128)
+    assert waited == [] and taken[4:] == [own] * 4
+    del taken[4:]
     assert taken == ["side"] * 4
     assert all(not t.any() for t in (cache.k_payload, cache.k_scales, cache.v_payload, cache.v_scales))
 

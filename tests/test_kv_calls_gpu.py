@@ -261,3 +261,15 @@ def test_offsets_of_scale_bytes_beyond_32_bits(ctx):  # noqa: F811
     torch.cuda.empty_cache()
     assert all(same), same
     assert ((outs[0][0] - k).abs() <= 1).all() and ((outs[0][1] - v).abs() <= 1).all() and k.abs().max().item() < 6 > v.abs().max().item()
+
+
+def test_bytes_copied_at_once_into_a_new_cache_of_a_side_context_stay():
+    """On torch's own stream, with nothing waited for; the cache is large, so that its fill takes a while."""
+    from ferrule_amd.provider import HipArtifactOperatorContext
+    side = HipArtifactOperatorContext(0, torch.cuda.Stream())
+    cache = side.kv_cache(4096, 64, 16, 256)
+    for t in (cache.v_scales, cache.k_scales, cache.v_payload, cache.k_payload):
+        t[-1].fill_(77)
+    torch.cuda.synchronize()
+    for t in (cache.v_scales, cache.k_scales, cache.v_payload, cache.k_payload):
+        assert (t[-1] == 77).all() and not t[:-1].any()
