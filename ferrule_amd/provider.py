@@ -1259,7 +1259,8 @@ class HipArtifactOperatorContext:
         ``q`` and ``out`` are BF16 or f32 [rows, q_heads, head_dim] (f32 queries are rounded to BF16), head h
         reads key/value head h // (q_heads // kv_heads), and the row at position p sees position j when
         ``j <= p and (window == 0 or p - j < window or j < sinks)``.  A row that sees nothing writes
-        zeros (and one in front of position 0 sets ``error``).  ``out`` shares no byte with ``q``.  Without ``workspace`` one is taken from torch's allocator for the call."""
+        zeros (and one in front of position 0 sets ``error``).  ``out`` shares no byte with ``q``.  Without
+        ``workspace`` one is taken from torch's allocator for the call."""
         index = self._check_kv(cache, batch, error)
         q_heads = q.shape[1] if q.dim() == 3 else 0
         shape = (batch.rows, q_heads, cache.head_dim)
